@@ -24,8 +24,10 @@ LIB_NAME = "libcpab_b200.so"
 LIB_PATH = os.path.join(OUT_DIR, LIB_NAME)
 OBJ_DIR = os.path.join(HERE, "_build")
 
-SOURCES = ["integrate.cu", "warp.cu", "basis.cu", "resample.cu", "capi.cu", "noalloc.cu"]
-HEADERS = ["cpab_device.cuh", "integrate_body.cuh", "launch.h", "resample_device.cuh"]
+SOURCES = ["integrate.cu", "warp.cu", "basis.cu", "resample.cu", "capi.cu", "noalloc.cu",
+           "recurrence.cu", "norm.cu", "adamw.cu"]
+HEADERS = ["cpab_device.cuh", "integrate_body.cuh", "launch.h", "resample_device.cuh",
+           "sequence.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -85,32 +87,47 @@ def build(force=False, verbose=False, extra_flags=(), out=None):
 
 EXT_NAME = "_cpab_ext"
 EXT_PATH = os.path.join(OUT_DIR, EXT_NAME + ".so")
-EXT_SRC = os.path.join(CSRC, "torch_ext.cpp")
+EXT_SOURCES = ["torch_ext.cpp", "sequence_ext.cpp"]
 
 
 def build_ext(force=False, verbose=False):
-    """Compile the C++ autograd node (csrc/torch_ext.cpp, host code only) into
-    cpab/_cpab_ext.so against this Python's torch, linked to libcpab_b200.so
-    (found next to it at run time).  Returns its path."""
+    """Compile the C++ autograd nodes (csrc/torch_ext.cpp and
+    csrc/sequence_ext.cpp, host code only) into cpab/_cpab_ext.so against this
+    Python's torch, linked to libcpab_b200.so (found next to it at run time).
+    Returns its path."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
     lib = build(verbose=verbose)
-    if not (force or _mtime(EXT_PATH) < max(_mtime(EXT_SRC), _mtime(lib), _mtime(__file__),
-                                           _mtime(os.path.join(INCLUDE, "cpab_b200.h")))):
-        return EXT_PATH
+    srcs = [os.path.join(CSRC, f) for f in EXT_SOURCES]
+    dep_time = max(_mtime(__file__), _mtime(os.path.join(INCLUDE, "cpab_b200.h")))
     cuda_home = cpp_extension.CUDA_HOME or "/usr/local/cuda"
     incs = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], INCLUDE,
                                             os.path.join(cuda_home, "include")]
     libdirs = cpp_extension.library_paths()
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    objs, procs = [], []
+    for src in srcs:
+        obj = os.path.join(OBJ_DIR, os.path.basename(src).replace(".cpp", ".o"))
+        objs.append(obj)
+        if force or _mtime(obj) < max(_mtime(src), dep_time):
+            cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-c", src, "-o", obj,
+                    "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi, "-DTORCH_EXTENSION_NAME=" + EXT_NAME,
+                    "-DTORCH_API_INCLUDE_EXTENSION_H", "-Wno-deprecated-declarations"]
+                   + ["-I" + i for i in incs])
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            procs.append((cmd, subprocess.Popen(cmd)))
+    failed = [cmd for cmd, p in procs if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    if not force and _mtime(EXT_PATH) >= max(_mtime(lib), *[_mtime(o) for o in objs]):
+        return EXT_PATH
     tmp = EXT_PATH + ".tmp"
-    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", EXT_SRC, "-o", tmp,
-            "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi, "-DTORCH_EXTENSION_NAME=" + EXT_NAME,
-            "-DTORCH_API_INCLUDE_EXTENSION_H", "-Wno-deprecated-declarations"]
-           + ["-I" + i for i in incs] + ["-L" + d for d in libdirs]
+    cmd = (["g++", "-shared", *objs, "-o", tmp] + ["-L" + d for d in libdirs]
            + ["-L" + OUT_DIR, "-lcpab_b200", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
               "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
     if verbose:

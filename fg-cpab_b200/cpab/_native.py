@@ -48,10 +48,32 @@ _SIGNATURES = {
                        _c_int, _c_int, _p, _c_int, _p, _p, _p, _p],
     "cpab_b200_warp_backward": [_c_int, _p, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _p,
                                 _c_int, _c_int, _p, _c_int, _p, _p, _p, _p, _p, _p],
+    "cpab_b200_gated_scan": [_c_int, _p, _c_i64, _c_i64, _p, _c_i64, _c_i64, _c_i64, _c_i64,
+                             _c_i64, _p, _p, _p, _p, _p, _p],
+    "cpab_b200_gated_scan_backward": [_c_int, _p, _c_i64, _c_i64, _p, _c_i64, _c_i64, _c_i64,
+                                      _c_i64, _c_i64, _p, _p, _p, _p, _p, _c_i64, _c_i64, _p,
+                                      _c_i64, _c_i64, _p, _p],
+    "cpab_b200_gated_scan_step": [_c_int, _p, _c_i64, _p, _c_i64, _c_i64, _c_i64, _p, _c_i64, _p,
+                                  _p, _p],
+    "cpab_b200_rms_norm": [_c_int, _c_int, _c_int, _p, _c_i64, _p, _c_i64, _p, _c_i64, _c_i64,
+                           _c_float, _p, _p, _p, _p],
+    "cpab_b200_rms_norm_quantized": [_c_int, _c_int, _c_int, _p, _c_i64, _p, _c_i64, _p, _c_i64,
+                                     _c_i64, _c_float, _p, _p, _p, _p],
+    "cpab_b200_rms_norm_backward": [_c_int, _c_int, _c_int, _p, _c_i64, _p, _p, _c_i64, _c_i64,
+                                    _p, _p, _p, _p, _p, _p, _p],
+    "cpab_b200_adamw": [_p, _c_int, ctypes.c_uint32, _p, _p],
 }
 
-EXPORTS = tuple(_SIGNATURES) + ("cpab_b200_version", "cpab_b200_max_steps",
-                                "cpab_b200_last_error")
+# Entry points that return something else than a status.
+_OTHERS = {
+    "cpab_b200_version": (ctypes.c_int, []),
+    "cpab_b200_max_steps": (ctypes.c_int, []),
+    "cpab_b200_last_error": (ctypes.c_char_p, []),
+    "cpab_b200_gated_scan_chunk": (ctypes.c_int, []),
+    "cpab_b200_rms_norm_workspace": (_c_i64, [_c_int, _c_i64, _c_i64]),
+}
+
+EXPORTS = tuple(_SIGNATURES) + tuple(_OTHERS)
 
 _lib = None
 
@@ -73,9 +95,9 @@ def lib():
             fn = getattr(L, name)
             fn.argtypes = args
             fn.restype = ctypes.c_int
-        L.cpab_b200_version.restype = ctypes.c_int
-        L.cpab_b200_max_steps.restype = ctypes.c_int
-        L.cpab_b200_last_error.restype = ctypes.c_char_p
+        for name, (res, args) in _OTHERS.items():
+            getattr(L, name).restype = res
+            getattr(L, name).argtypes = args
         _lib = L
     return _lib
 
@@ -440,3 +462,269 @@ def backward_chain(ndim, nc, points, batched, As, n_stages, grad_out, stage_poin
             n_theta, _ptr(grad_out), _ptr(stage_points), int(nstepsolver), int(adaptive),
             _ptr(moments), _ptr(gp), _stream(As.device)))
     return moments, gp
+
+
+# ---------------------------------------------------------------------------
+# Operators of the sequence networks.
+# ---------------------------------------------------------------------------
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _dtype(t, name):
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    return code
+
+
+def _like(t, x, name, dtype, shape):
+    if t.device != x.device:
+        raise RuntimeError("%s is on %s, x on %s" % (name, t.device, x.device))
+    if t.dtype != dtype:
+        raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+
+
+def _cuda(x):
+    if not x.is_cuda:
+        raise RuntimeError("x must be a CUDA tensor (no CPU path)")
+    _dtype(x, "x")
+
+
+def _adjacent(t):
+    """t with the last axis' elements adjacent in memory."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def check_scan(x, gate, h0, lengths):
+    _cuda(x)
+    if x.dim() != 3:
+        raise ValueError("x must be [B, T, D], got %s" % (tuple(x.shape),))
+    if gate is not None:
+        _like(gate, x, "gate", x.dtype, x.shape)
+    elif x.shape[2] % 2:
+        raise ValueError("x without a gate must be [B, T, 2 D], got %s" % (tuple(x.shape),))
+    D = x.shape[2] if gate is not None else x.shape[2] // 2
+    if h0 is not None:
+        _like(h0, x, "h0", torch.float32, (x.shape[0], D))
+    if lengths is not None:
+        _like(lengths, x, "lengths", torch.int32, (x.shape[0],))
+
+
+def _scan_input(x, gate):
+    """(tensors to keep alive, B, T, D, the C arguments of x and gate)."""
+    xa = _adjacent(x)
+    sx = (xa.stride(0), xa.stride(1))
+    if gate is not None:
+        ga = _adjacent(gate)
+        return (xa, ga), x.shape[0], x.shape[1], x.shape[2], (
+            _ptr(xa), *sx, _ptr(ga), ga.stride(0), ga.stride(1))
+    D = x.shape[2] // 2
+    return (xa,), x.shape[0], x.shape[1], D, (_ptr(xa), *sx, _ptr(xa) + D * x.element_size(), *sx)
+
+
+def _contiguous(t):
+    return t.contiguous() if t is not None else None
+
+
+def gated_scan(x, gate, h0, lengths, keep):
+    """(h, last, states or None); states only when `keep` (for the backward)."""
+    alive, B, T, D, args = _scan_input(x, gate)
+    f32 = dict(device=x.device, dtype=torch.float32)
+    h = torch.empty((B, T, D), device=x.device, dtype=x.dtype)
+    last = torch.empty((B, D), **f32)
+    c = lib().cpab_b200_gated_scan_chunk()
+    states = torch.empty((B, (T + c - 1) // c, D), **f32) if keep else None
+    h0, lengths = _contiguous(h0), _contiguous(lengths)
+    with _on(x.device):
+        _check(lib().cpab_b200_gated_scan(
+            _dtype(x, "x"), *args, B, T, D, _ptr(lengths), _ptr(h0), _ptr(h), _ptr(last),
+            _ptr(states), _stream(x.device)))
+    return h, last, states
+
+
+def gated_scan_backward(x, gate, lengths, states, dh, dlast, want_h0):
+    """(grad_x, grad_gate or None, grad_h0 or None)."""
+    alive, B, T, D, args = _scan_input(x, gate)
+    dx = torch.empty((B, T, D if gate is not None else 2 * D), device=x.device, dtype=x.dtype)
+    dg = torch.empty((B, T, D), device=x.device, dtype=x.dtype) if gate is not None else None
+    dgp = _ptr(dg) if dg is not None else _ptr(dx) + D * x.element_size()
+    dgs = dg if dg is not None else dx
+    dh0 = torch.empty((B, D), device=x.device, dtype=torch.float32) if want_h0 else None
+    dh, dlast, lengths = _contiguous(dh), _contiguous(dlast), _contiguous(lengths)
+    with _on(x.device):
+        _check(lib().cpab_b200_gated_scan_backward(
+            _dtype(x, "x"), *args, B, T, D, _ptr(lengths), _ptr(states), _ptr(dh), _ptr(dlast),
+            _ptr(dx), dx.stride(0), dx.stride(1), dgp, dgs.stride(0), dgs.stride(1), _ptr(dh0),
+            _stream(x.device)))
+    return dx, dg, dh0
+
+
+def gated_scan_step(x, gate, state, slots):
+    _cuda(x)
+    if x.dim() != 2:
+        raise ValueError("x must be [B, D], got %s" % (tuple(x.shape),))
+    if gate is not None:
+        _like(gate, x, "gate", x.dtype, x.shape)
+    elif x.shape[1] % 2:
+        raise ValueError("x without a gate must be [B, 2 D], got %s" % (tuple(x.shape),))
+    B, D = x.shape[0], x.shape[1] if gate is not None else x.shape[1] // 2
+    if state.dim() != 2 or (slots is None and state.shape[0] != B):
+        raise ValueError("state must be [rows, D] (rows = B without slots), got %s"
+                         % (tuple(state.shape),))
+    _like(state, x, "state", torch.float32, (state.shape[0], D))
+    if not state.is_contiguous():
+        raise ValueError("state must be contiguous (it is updated in place)")
+    if slots is not None:
+        _like(slots, x, "slots", torch.int32, (B,))
+    xa = _adjacent(x)
+    ga = _adjacent(gate) if gate is not None else None
+    slots = _contiguous(slots)
+    h = torch.empty((B, D), device=x.device, dtype=x.dtype)
+    gp = _ptr(ga) if ga is not None else _ptr(xa) + D * x.element_size()
+    with _on(x.device):
+        _check(lib().cpab_b200_gated_scan_step(
+            _dtype(x, "x"), _ptr(xa), xa.stride(0), gp, (ga if ga is not None else xa).stride(0), B,
+            D, _ptr(slots), state.shape[0], _ptr(state), _ptr(h), _stream(x.device)))
+    return h
+
+
+def check_norm(x, weight, residual):
+    _cuda(x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must be [..., D] with D > 0, got %s" % (tuple(x.shape),))
+    for t, name, shape in ((weight, "weight", (x.shape[-1],)), (residual, "residual", x.shape)):
+        if t is not None:
+            if t.dtype not in (torch.float32, x.dtype):
+                raise TypeError("%s must be float32 or of x's type, got %s" % (name, t.dtype))
+            _like(t, x, name, t.dtype, shape)
+
+
+def _rows(t):
+    if t is None:
+        return None
+    return _adjacent(t if t.dim() == 2 else t.reshape(t.numel() // t.shape[-1], t.shape[-1]))
+
+
+def _norm_args(x, weight, residual, eps):
+    """(tensors to keep alive, the C arguments up to eps)."""
+    xr, rr, w = _rows(x), _rows(residual), weight.contiguous()
+    s = residual if residual is not None else x
+    return (xr, rr, w), (
+        _dtype(x, "x"), _dtype(s, "residual"), _dtype(w, "weight"), _ptr(xr), xr.stride(0), _ptr(rr),
+        rr.stride(0) if rr is not None else 0, _ptr(w), xr.shape[0], xr.shape[1], eps)
+
+
+def rms_norm(x, weight, residual, eps, keep):
+    """(y, sum or None, rstd or None); rstd only when `keep` (for the backward)."""
+    alive, args = _norm_args(x, weight, residual, eps)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    s = torch.empty(x.shape, device=x.device, dtype=residual.dtype) if residual is not None else None
+    rstd = torch.empty(args[8], device=x.device, dtype=torch.float32) if keep else None
+    with _on(x.device):
+        _check(lib().cpab_b200_rms_norm(*args, _ptr(y), _ptr(s), _ptr(rstd), _stream(x.device)))
+    return y, s, rstd
+
+
+def rms_norm_quantized(x, weight, residual, eps):
+    """(q, scale) or (q, scale, sum)."""
+    alive, args = _norm_args(x, weight, residual, eps)
+    q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    s = torch.empty(x.shape, device=x.device, dtype=residual.dtype) if residual is not None else None
+    with _on(x.device):
+        _check(lib().cpab_b200_rms_norm_quantized(*args, _ptr(q), _ptr(scale), _ptr(s),
+                                                  _stream(x.device)))
+    return (q, scale) if s is None else (q, scale, s)
+
+
+def rms_norm_backward(s, weight, rstd, gy, gs, x_type, want_weight):
+    """(grad_x, grad_residual, grad_weight or None); the first two are one
+    tensor where their types are one."""
+    rows, w, gy, gs = _rows(s), weight.contiguous(), gy.contiguous(), _contiguous(gs)
+    n, D = rows.shape
+    dx = torch.empty(s.shape, device=s.device, dtype=x_type)
+    dres = torch.empty(s.shape, device=s.device, dtype=s.dtype) if s.dtype != x_type else None
+    dw = torch.empty_like(w) if want_weight else None
+    dt = _dtype(dx, "x")
+    work = (torch.empty(lib().cpab_b200_rms_norm_workspace(dt, n, D), device=s.device,
+                        dtype=torch.float32) if want_weight else None)
+    with _on(s.device):
+        _check(lib().cpab_b200_rms_norm_backward(
+            dt, _dtype(s, "residual"), _dtype(w, "weight"), _ptr(rows), rows.stride(0), _ptr(w),
+            _ptr(rstd), n, D, _ptr(gy), _ptr(gs), _ptr(dx), _ptr(dres), _ptr(work), _ptr(dw),
+            _stream(s.device)))
+    return dx, (dres if dres is not None else dx), dw
+
+
+def _dense(t):
+    """Whether t's elements fill their span of memory, in some order of its axes."""
+    span = 1
+    for stride, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != span:
+            return t.numel() == 0
+        span *= n
+    return True
+
+
+class _AdamWTensor(ctypes.Structure):
+    """cpab_adamw_tensor."""
+    _fields_ = ([(k, _p) for k in ("param", "grad", "exp_avg", "exp_avg_sq", "scales", "step",
+                                   "lr_device")]
+                + [("numel", _c_i64), ("dtype", ctypes.c_int32), ("state_bits", ctypes.c_int32)]
+                + [(k, ctypes.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")])
+
+
+def adamw(params, grads, exp_avgs, exp_avg_sqs, scales, steps, counts, hyper, lrs, seed, workspace):
+    """counts[g] tensors of group g one after another; hyper: each group's (lr,
+    beta1, beta2, eps, weight_decay) one after another; lrs: each group's
+    learning rate on the device, or None."""
+    device = params[0].device
+    if not params[0].is_cuda:
+        raise RuntimeError("params must be CUDA tensors (no CPU path)")
+    if not (len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(steps)) or \
+            len(scales) not in (0, len(params)):
+        raise ValueError("adamw: lists of different lengths")
+    table, alive, k = (_AdamWTensor * len(params))(), [], 0
+    for group, n in enumerate(counts):
+        for _ in range(n):
+            p, g, m, v, step = params[k], grads[k], exp_avgs[k], exp_avg_sqs[k], steps[k]
+            if any(t.device != device for t in (p, g, m, v, step)):
+                raise RuntimeError("adamw: tensor %d: all tensors must be on one device" % k)
+            if g.dtype != p.dtype:
+                raise TypeError("adamw: tensor %d: gradient of type %s for a parameter of type %s"
+                                % (k, g.dtype, p.dtype))
+            if v.dtype != m.dtype or m.dtype not in (torch.float32, torch.float8_e4m3fn):
+                raise TypeError("adamw: tensor %d: states must be float32, or both float8_e4m3fn" % k)
+            if step.dtype != torch.float32 or step.numel() != 1:
+                raise TypeError("adamw: tensor %d: step must be one float32" % k)
+            if not (g.shape == p.shape == m.shape == v.shape):
+                raise ValueError("adamw: tensor %d: parameter, gradient and states must have one "
+                                 "shape" % k)
+            alike = ((m.is_contiguous() and v.is_contiguous()) if p.is_contiguous() else
+                     m.stride() == p.stride() == v.stride())
+            if not _dense(p) or not alike:
+                raise ValueError("adamw: tensor %d: parameter and states must be dense and laid out "
+                                 "alike" % k)
+            if not (g.is_contiguous() if p.is_contiguous() else g.stride() == p.stride()):
+                g = torch.empty_like(p).copy_(g)
+                alive.append(g)
+            eight, sc = m.dtype == torch.float8_e4m3fn, None
+            if eight:
+                blocks = (p.numel() + 255) // 256
+                sc = scales[k] if scales else None
+                if sc is None or sc.device != device or sc.dtype != torch.float32 or \
+                        not sc.is_contiguous() or sc.numel() != 2 * blocks:
+                    raise ValueError("adamw: tensor %d: 8-bit states need float32 scales [%d, 2]"
+                                     % (k, blocks))
+            t = table[k]
+            t.param, t.grad, t.exp_avg, t.exp_avg_sq = _ptr(p), _ptr(g), _ptr(m), _ptr(v)
+            t.scales, t.step, t.lr_device = _ptr(sc), _ptr(step), _ptr(lrs[group])
+            t.numel, t.dtype, t.state_bits = p.numel(), _dtype(p, "a parameter"), 8 if eight else 32
+            t.lr, t.beta1, t.beta2, t.eps, t.weight_decay = hyper[5 * group:5 * group + 5]
+            k += 1
+    with _on(device):
+        _check(lib().cpab_b200_adamw(ctypes.byref(table), len(params), seed & 0xFFFFFFFF,
+                                     _ptr(workspace), _stream(device)))

@@ -303,8 +303,12 @@ Tensor transform(Tensor points, Tensor theta, std::vector<Tensor> basis, int64_t
 
 }  // namespace
 
+// The sequence-network operators (sequence_ext.cpp).
+void bind_sequence(pybind11::module &m);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.doc() = "transform_grid autograd node over libcpab_b200 (C++)";
+  m.doc() = "autograd nodes over libcpab_b200 (C++)";
+  bind_sequence(m);
   m.def("transform", &transform,
         "points, theta, basis (6 CSR tensors of B and B^T), d, dense, nc, nstepsolver, "
         "adaptive, order or None, compute_points_grad, batched -> transformed points");

@@ -5,10 +5,13 @@
  * piecewise-affine (CPA) velocity fields in 1D/2D/3D, runs the factorized
  * adjoint sweep that produces per-cell moments, projects the moments onto the
  * CPA basis (dtheta = B^T vec(M)) and resamples images/volumes on warped grids.
+ * It also holds the operators of the sequence networks that predict theta (a
+ * gated linear recurrence, a residual norm, an optimizer step).
  *
  * Conventions shared by every entry point:
- *   - All pointers are device pointers to contiguous fp32 / int32 arrays; the
- *     caller owns every buffer.  Nothing here allocates device memory.
+ *   - All pointers are device pointers to contiguous fp32 / int32 arrays unless
+ *     an entry point says otherwise; the caller owns every buffer.  Nothing
+ *     here allocates device memory.
  *   - Work is enqueued on `stream` (a cudaStream_t; NULL = legacy default
  *     stream) and is asynchronous with respect to the host.
  *   - The return value is CPAB_OK (0) or a negative cpab_status.  Argument
@@ -352,6 +355,130 @@ int cpab_b200_warp_backward(int ndim, const int32_t *nc, const int64_t *out_size
                             const float *stage_points, const float *grid_t,
                             const float *grad_out, float *moments, float *grad_data,
                             cpab_stream_t stream);
+
+/*
+ * Operators of the networks that predict theta from long signals and of their
+ * training.  Element types are a cpab_dtype; strides count elements and the
+ * innermost axis is contiguous.  The reference has no counterpart of these.
+ */
+typedef enum { CPAB_F32 = 0, CPAB_F16 = 1, CPAB_BF16 = 2 } cpab_dtype;
+
+/*
+ * Gated linear recurrence of B series of T samples of D channels,
+ *   h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = sigmoid(gate_t),
+ * from the state h0 ([B, D] float32, NULL: zeros).  x and gate are [B, T, D]
+ * with the given strides of series and samples (so both may be halves of one
+ * projection); h is [B, T, D] contiguous, of the same type; the state is
+ * float32 throughout.  lengths ([B] int32, NULL: all T; values outside [0, T]
+ * are taken as 0 or T): samples from a series' length on are not read and
+ * their h is 0.  h_last ([B, D] float32, may be NULL) receives the state after
+ * the last sample.  states ([B, ceil(T / c), D] float32 with c =
+ * cpab_b200_gated_scan_chunk(), may be NULL) receives the states that
+ * cpab_b200_gated_scan_backward needs.
+ */
+int cpab_b200_gated_scan(int dtype, const void *x, int64_t x_series, int64_t x_sample,
+                         const void *gate, int64_t gate_series, int64_t gate_sample, int64_t B,
+                         int64_t T, int64_t D, const int32_t *lengths, const float *h0, void *h,
+                         float *h_last, float *states, cpab_stream_t stream);
+
+/* Samples between two states kept by cpab_b200_gated_scan. */
+int cpab_b200_gated_scan_chunk(void);
+
+/*
+ * Gradient of cpab_b200_gated_scan: grad_x and grad_gate (shaped as x and
+ * gate, own strides), and grad_h0 ([B, D] float32, may be NULL) from grad_h
+ * ([B, T, D] contiguous, NULL: zeros) and grad_last ([B, D] float32, NULL:
+ * zeros).  The gradients of samples past a series' length are 0.
+ */
+int cpab_b200_gated_scan_backward(int dtype, const void *x, int64_t x_series, int64_t x_sample,
+                                  const void *gate, int64_t gate_series, int64_t gate_sample,
+                                  int64_t B, int64_t T, int64_t D, const int32_t *lengths,
+                                  const float *states, const void *grad_h, const float *grad_last,
+                                  void *grad_x, int64_t grad_x_series, int64_t grad_x_sample,
+                                  void *grad_gate, int64_t grad_gate_series,
+                                  int64_t grad_gate_sample, float *grad_h0, cpab_stream_t stream);
+
+/*
+ * One sample of B streams: state row slots[b] (slots NULL: row b) of the
+ * [rows, D] float32 table takes one step of the recurrence with x[b], gate[b]
+ * ([B, D], row strides given) and its new value, rounded, is h[b] ([B, D]
+ * contiguous).  A slot outside [0, rows) marks a stream without a sample: no
+ * state changes and its h is 0.  Slots in use must differ from one another.
+ */
+int cpab_b200_gated_scan_step(int dtype, const void *x, int64_t x_row, const void *gate,
+                              int64_t gate_row, int64_t B, int64_t D, const int32_t *slots,
+                              int64_t rows, float *state, void *h, cpab_stream_t stream);
+
+/*
+ * Root-mean-square norm with the residual's addition, per row of D <= 16384
+ * columns:
+ *   sum = x + residual (rounded to stream_dtype), y = sum * r * weight,
+ *   r = 1 / sqrt(mean(sum^2) + eps).
+ * x (row stride x_row) and y ([rows, D] contiguous) are of type dtype;
+ * residual (row stride residual_row) and sum ([rows, D] contiguous) of
+ * stream_dtype, which is dtype or CPAB_F32; weight [D] of dtype or CPAB_F32.
+ * residual NULL: sum is x, is not written, and stream_dtype must be dtype.
+ * rstd ([rows] float32, may be NULL) receives r for the gradient.
+ */
+int cpab_b200_rms_norm(int dtype, int stream_dtype, int weight_dtype, const void *x, int64_t x_row,
+                       const void *residual, int64_t residual_row, const void *weight, int64_t rows,
+                       int64_t D, float eps, void *y, void *sum, float *rstd, cpab_stream_t stream);
+
+/*
+ * cpab_b200_rms_norm with y in 8 bits: q ([rows, D] e4m3 codes) and one float32
+ * scale per row, y ~ q * scale, scale = max(max|y| / 448, 2^-126).
+ */
+int cpab_b200_rms_norm_quantized(int dtype, int stream_dtype, int weight_dtype, const void *x,
+                                 int64_t x_row, const void *residual, int64_t residual_row,
+                                 const void *weight, int64_t rows, int64_t D, float eps, uint8_t *q,
+                                 float *scale, void *sum, cpab_stream_t stream);
+
+/* Floats of the workspace of cpab_b200_rms_norm_backward. */
+int64_t cpab_b200_rms_norm_workspace(int dtype, int64_t rows, int64_t D);
+
+/*
+ * Gradient of cpab_b200_rms_norm.  sum (row stride sum_row) is the kept sum
+ * (x itself without a residual); grad_y [rows, D] of dtype, grad_sum [rows, D]
+ * of stream_dtype (the gradient that reaches sum directly; NULL: none), both
+ * contiguous.  grad_x [rows, D] of dtype; grad_residual [rows, D] of
+ * stream_dtype where that is not dtype (may be NULL; where the types are one,
+ * grad_x is the gradient of both and grad_residual must be NULL).
+ * grad_weight ([D] of weight_dtype, may be NULL) needs the workspace; its sum
+ * over rows runs in a fixed order.
+ */
+int cpab_b200_rms_norm_backward(int dtype, int stream_dtype, int weight_dtype, const void *sum,
+                                int64_t sum_row, const void *weight, const float *rstd,
+                                int64_t rows, int64_t D, const void *grad_y, const void *grad_sum,
+                                void *grad_x, void *grad_residual, float *workspace,
+                                void *grad_weight, cpab_stream_t stream);
+
+/* One tensor of cpab_b200_adamw (device pointers unless noted). */
+typedef struct {
+  void *param;            /* [numel] of dtype, updated                              */
+  const void *grad;       /* [numel] of dtype                                       */
+  void *exp_avg;          /* [numel] float32, or e4m3 codes of the first moment     */
+  void *exp_avg_sq;       /* [numel] float32, or e4m3 codes of the second's root    */
+  float *scales;          /* state_bits 8: [ceil(numel / 256), 2] (first moment, root) */
+  float *step;            /* steps taken so far; the call adds 1                    */
+  const float *lr_device; /* learning rate on the device, or NULL: lr               */
+  int64_t numel;
+  int32_t dtype;          /* cpab_dtype of param and grad                           */
+  int32_t state_bits;     /* 32 or 8                                                */
+  double lr, beta1, beta2, eps, weight_decay;
+} cpab_adamw_tensor;
+
+/*
+ * One AdamW step (decoupled weight decay, bias correction) over `count`
+ * tensors (an array in host memory), 256 of them a launch:
+ *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+ * in float32.  8-bit states are e4m3 codes of m and sqrt(v) times one float32
+ * scale per 256 elements, rounded stochastically by a hash of (seed, tensor's
+ * place, t, element).  workspace: one int32 on the device, 0 before the first
+ * call and left 0; calls that overlap on the GPU must not share it.
+ */
+int cpab_b200_adamw(const cpab_adamw_tensor *tensors, int count, uint32_t seed, int32_t *workspace,
+                    cpab_stream_t stream);
 
 #ifdef __cplusplus
 }

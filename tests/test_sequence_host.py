@@ -1,0 +1,163 @@
+"""Host-side checks of the sequence-network operators: the C ABI's refusals,
+the Python layer's argument errors (no GPU needed)."""
+import ctypes
+
+import pytest
+import torch
+
+from cpab import _ext, _native
+from cpab.optim import AdamW, adamw_
+from cpab.pytorch.norm import rms_norm, rms_norm_quantized
+from cpab.pytorch.recurrence import gated_scan, gated_scan_step
+
+P = ctypes.c_void_p(4096)  # never dereferenced: validation fails first
+
+
+def err():
+    return _native.lib().cpab_b200_last_error().decode()
+
+
+def call(fn, base, **kw):
+    a = list(base)
+    for i, v in kw.items():
+        a[int(i[1:])] = v
+    return fn(*a)
+
+
+def test_scan_entry_points_validate():
+    L = _native.lib()
+    # dtype, x, strides, gate, strides, B, T, D, lengths, h0, h, last, states, stream
+    ok = [2, P, 64, 8, P, 64, 8, 2, 8, 8, None, None, P, P, P, None]
+    f = L.cpab_b200_gated_scan
+    assert call(f, ok, a0=3) == -1 and "dtype" in err()
+    assert call(f, ok, a1=None) == -1 and "null" in err()
+    assert call(f, ok, a4=None) == -1
+    assert call(f, ok, a7=-1) == -1 and "negative" in err()
+    assert call(f, ok, a8=1 << 31) == -4 and "2^31" in err()
+    assert call(f, ok, a7=1 << 20, a9=1 << 11) == -4 and "2^30" in err()
+    assert call(f, ok, a12=None) == -1 and "output" in err()
+    assert call(f, ok, a7=0) == 0 and err() == ""
+    assert call(f, ok, a8=0, a13=None) == 0            # no samples, no state wanted
+    # ..., lengths, states, grad_h, grad_last, grad_x, strides, grad_gate, strides, grad_h0, stream
+    okb = [2, P, 64, 8, P, 64, 8, 2, 8, 8, None, P, P, P, P, 64, 8, P, 64, 8, P, None]
+    g = L.cpab_b200_gated_scan_backward
+    assert call(g, okb, a11=None) == -1 and "states" in err()
+    assert call(g, okb, a14=None) == -1 and call(g, okb, a17=None) == -1
+    assert call(g, okb, a0=-1) == -1
+    assert call(g, okb, a9=0) == 0
+    # dtype, x, row, gate, row, B, D, slots, rows, state, h, stream
+    oks = [0, P, 8, P, 8, 2, 8, None, 2, P, P, None]
+    s = L.cpab_b200_gated_scan_step
+    assert call(s, oks, a8=1) == -1 and "state rows" in err()
+    assert call(s, oks, a9=None) == -1 and call(s, oks, a10=None) == -1
+    assert call(s, oks, a5=0) == 0
+    assert L.cpab_b200_gated_scan_chunk() > 0
+
+
+def test_norm_entry_points_validate():
+    L = _native.lib()
+    # dtype, stream, weight, x, row, residual, row, w, rows, D, eps, y, sum, rstd, stream
+    ok = [2, 2, 0, P, 8, P, 8, P, 4, 8, 1e-6, P, P, P, None]
+    f = L.cpab_b200_rms_norm
+    assert call(f, ok, a0=7) == -1 and "types" in err()
+    assert call(f, ok, a1=1) == -1 and call(f, ok, a2=1) == -1
+    assert call(f, ok, a9=0) == -1 and "shape" in err()
+    assert call(f, ok, a9=16385) == -4 and "16384" in err()
+    assert call(f, ok, a10=-1.0) == -1 and "eps" in err()
+    assert call(f, ok, a10=float("nan")) == -1
+    assert call(f, ok, a12=None) == -1 and "null" in err()
+    assert call(f, ok, a8=1 << 31) == -4
+    assert call(f, ok, a8=0) == 0 and err() == ""
+    # ..., eps, q, scale, sum, stream
+    okq = [2, 2, 0, P, 8, P, 8, P, 4, 8, 1e-6, P, P, P, None]
+    q = L.cpab_b200_rms_norm_quantized
+    assert call(q, okq, a11=None) == -1 and call(q, okq, a12=None) == -1
+    assert call(q, okq, a13=None) == -1 and call(q, okq, a9=-3) == -1
+    # dtype, stream, weight, sum, row, w, rstd, rows, D, gy, gs, gx, gres, work, gw, stream
+    okb = [2, 2, 0, P, 8, P, P, 4, 8, P, P, P, None, P, P, None]
+    b = L.cpab_b200_rms_norm_backward
+    assert call(b, okb, a13=None) == -1 and "workspace" in err()
+    assert call(b, okb, a12=P) == -1 and "grad_residual" in err()
+    assert call(b, okb, a9=None) == -1 and call(b, okb, a6=None) == -1
+    assert L.cpab_b200_rms_norm_workspace(2, 100, 64) >= 64
+    assert L.cpab_b200_rms_norm_workspace(9, 100, 64) == 0
+
+
+def test_adamw_entry_point_validates():
+    L = _native.lib()
+    t = (_native._AdamWTensor * 1)()
+
+    def one(**kw):
+        base = dict(param=4096, grad=4096, exp_avg=4096, exp_avg_sq=4096, scales=None, step=4096,
+                    lr_device=None, numel=8, dtype=0, state_bits=32, lr=1e-3, beta1=0.9, beta2=0.999,
+                    eps=1e-8, weight_decay=0.0)
+        for k, v in {**base, **kw}.items():
+            setattr(t[0], k, v)
+        return L.cpab_b200_adamw(ctypes.byref(t), 1, 0, P, None)
+
+    assert one(dtype=5) == -1 and "dtype" in err()
+    assert one(numel=-1) == -1 and "negative" in err()
+    assert one(numel=(1 << 40) + 1) == -4
+    assert one(step=None) == -1 and one(grad=None) == -1 and "null" in err()
+    assert one(state_bits=16) == -1 and "bits" in err()
+    assert one(state_bits=8) == -1 and "scales" in err()
+    assert one(beta1=1.0) == -1 and "betas" in err()
+    assert one(beta2=float("nan")) == -1
+    assert one(eps=-1.0) == -1
+    assert L.cpab_b200_adamw(None, 1, 0, P, None) == -1
+    assert L.cpab_b200_adamw(ctypes.byref(t), 1, 0, None, None) == -1
+    assert L.cpab_b200_adamw(ctypes.byref(t), -1, 0, P, None) == -1
+    assert L.cpab_b200_adamw(None, 0, 0, P, None) == 0 and err() == ""
+
+
+@pytest.fixture(params=["ext", "python"])
+def path(request):
+    if request.param == "python":
+        with _ext.python_path():
+            yield
+    else:
+        assert _ext.module() is not None
+        yield
+
+
+def test_cpu_tensors_are_refused(path):
+    x, w = torch.randn(2, 3, 4), torch.ones(4)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        gated_scan(x, x)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        gated_scan_step(x[0], x[0], torch.zeros(3, 4))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        rms_norm(x, w)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        rms_norm_quantized(x, w)
+    p, s = torch.zeros(4), torch.zeros(())
+    with pytest.raises(RuntimeError, match="CUDA"):
+        adamw_([p], [p], [p], [p], [s], lr=1e-3)
+
+
+def test_whole_number_arguments_and_gradients_are_checked():
+    x = torch.randn(2, 3, 4)
+    with pytest.raises(TypeError, match="lengths"):
+        gated_scan(x, x, lengths=torch.ones(2))
+    with pytest.raises(TypeError, match="slots"):
+        gated_scan_step(x[0], x[0], torch.zeros(3, 4), slots=torch.ones(3))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        gated_scan_step(x[0].clone().requires_grad_(True), x[0], torch.zeros(3, 4))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        rms_norm_quantized(x, torch.ones(4, requires_grad=True))
+
+
+def test_adamw_checks_its_options():
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1e-8), dict(weight_decay=-0.1),
+                dict(state_bits=16)):
+        with pytest.raises(ValueError):
+            AdamW(p, **bad)
+    q = torch.zeros(3)
+    with pytest.raises(ValueError, match="lengths"):
+        adamw_([q], [q, q], [q], [q], [q], lr=1e-3)
+    with pytest.raises(ValueError, match="lr"):
+        adamw_([q], [q], [q], [q], [q], lr=torch.tensor(1e-3))
+    opt = AdamW(p)
+    opt.step()                                         # no gradients: nothing to do
+    assert p[0] not in opt.state or not opt.state[p[0]]
