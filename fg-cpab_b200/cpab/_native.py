@@ -49,10 +49,10 @@ _SIGNATURES = {
     "cpab_b200_warp_backward": [_c_int, _p, _p, _p, _p, _p, _c_int, _c_int, _c_int, _c_int, _p,
                                 _c_int, _c_int, _p, _c_int, _p, _p, _p, _p, _p, _p],
     "cpab_b200_gated_scan": [_c_int, _p, _c_i64, _c_i64, _p, _c_i64, _c_i64, _c_i64, _c_i64,
-                             _c_i64, _p, _p, _p, _p, _p, _p],
+                             _c_i64, _p, _p, _p, _p, _p, _p, _p],
     "cpab_b200_gated_scan_backward": [_c_int, _p, _c_i64, _c_i64, _p, _c_i64, _c_i64, _c_i64,
                                       _c_i64, _c_i64, _p, _p, _p, _p, _p, _c_i64, _c_i64, _p,
-                                      _c_i64, _c_i64, _p, _p],
+                                      _c_i64, _c_i64, _p, _p, _p],
     "cpab_b200_gated_scan_step": [_c_int, _p, _c_i64, _p, _c_i64, _c_i64, _c_i64, _p, _c_i64, _p,
                                   _p, _p],
     "cpab_b200_rms_norm": [_c_int, _c_int, _c_int, _p, _c_i64, _p, _c_i64, _p, _c_i64, _c_i64,
@@ -70,6 +70,7 @@ _OTHERS = {
     "cpab_b200_max_steps": (ctypes.c_int, []),
     "cpab_b200_last_error": (ctypes.c_char_p, []),
     "cpab_b200_gated_scan_chunk": (ctypes.c_int, []),
+    "cpab_b200_gated_scan_workspace": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
     "cpab_b200_rms_norm_workspace": (_c_i64, [_c_int, _c_i64, _c_i64]),
 }
 
@@ -529,6 +530,11 @@ def _contiguous(t):
     return t.contiguous() if t is not None else None
 
 
+def _scan_workspace(x, B, T, D):
+    n = lib().cpab_b200_gated_scan_workspace(_dtype(x, "x"), B, T, D)
+    return torch.empty(n, device=x.device, dtype=torch.float32)
+
+
 def gated_scan(x, gate, h0, lengths, keep):
     """(h, last, states or None); states only when `keep` (for the backward)."""
     alive, B, T, D, args = _scan_input(x, gate)
@@ -539,9 +545,10 @@ def gated_scan(x, gate, h0, lengths, keep):
     states = torch.empty((B, (T + c - 1) // c, D), **f32) if keep else None
     h0, lengths = _contiguous(h0), _contiguous(lengths)
     with _on(x.device):
+        work = _scan_workspace(x, B, T, D)
         _check(lib().cpab_b200_gated_scan(
             _dtype(x, "x"), *args, B, T, D, _ptr(lengths), _ptr(h0), _ptr(h), _ptr(last),
-            _ptr(states), _stream(x.device)))
+            _ptr(states), _ptr(work), _stream(x.device)))
     return h, last, states
 
 
@@ -555,10 +562,11 @@ def gated_scan_backward(x, gate, lengths, states, dh, dlast, want_h0):
     dh0 = torch.empty((B, D), device=x.device, dtype=torch.float32) if want_h0 else None
     dh, dlast, lengths = _contiguous(dh), _contiguous(dlast), _contiguous(lengths)
     with _on(x.device):
+        work = _scan_workspace(x, B, T, D)
         _check(lib().cpab_b200_gated_scan_backward(
             _dtype(x, "x"), *args, B, T, D, _ptr(lengths), _ptr(states), _ptr(dh), _ptr(dlast),
             _ptr(dx), dx.stride(0), dx.stride(1), dgp, dgs.stride(0), dgs.stride(1), _ptr(dh0),
-            _stream(x.device)))
+            _ptr(work), _stream(x.device)))
     return dx, dg, dh0
 
 

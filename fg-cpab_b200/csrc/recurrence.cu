@@ -7,12 +7,16 @@
 // (1 - a = sigmoid(-z) keeps its relative precision as a -> 1).
 //
 // A step (a, b): h -> a h + b; two steps compose to (a2 a1, a2 b1 + b2), which
-// is associative.  A block owns a tile of channels of one series and walks it
-// stage by stage; within a stage each thread reads a segment of kSteps samples
-// of its channels, composes them, and the segments' compositions are scanned
-// over the warp (shuffles) and the block (shared memory) to give each segment
-// the state it starts from; a second pass over the registers writes the
-// segment's states.  Every input is read once and every output written once.
+// is associative.  A block owns a tile of channels of one piece of a series and
+// walks it stage by stage: cp.async brings the next stages into shared memory,
+// each thread reads a segment of kSteps samples of its channels from there and
+// composes them, and the segments' compositions are scanned over the warp
+// (shuffles) and the block (shared memory) to give each segment the state it
+// starts from; a second pass over the registers writes the segment's states.
+//
+// A series is one piece where there are tiles enough to fill the GPU.  Else a
+// kernel before composes every kSpan samples, and a block begins at the state
+// that the spans before its own piece lead to.
 //
 // The gradient runs the same way from the last sample back:
 //   delta_t = dh_t + c_{t+1},  c_t = a_t delta_t
@@ -20,17 +24,22 @@
 // with h_{t-1} recomputed in float32 from the states that the forward keeps at
 // the start of every kChunk samples (reading the rounded output instead would
 // cost more bytes and lose the difference h_{t-1} - x_t where it is small).
+#include <type_traits>
+
 #include "sequence.cuh"
 
 namespace cpab {
 namespace {
 
-constexpr int kChunk = 64;    // samples between two kept states
-constexpr int kWarps = 8;     // warps of a full block
-constexpr int kFwdSteps = 16; // samples of a thread's segment (divide kChunk)
+constexpr int kChunk = 64;     // samples between two kept states
+constexpr int kFwdSteps = 16;  // samples of a thread's segment (divide kChunk)
 constexpr int kBwdSteps = 8;
+constexpr int kSpan = 512;     // samples composed together where a series is cut into pieces
 static_assert(kChunk % kFwdSteps == 0 && kChunk % kBwdSteps == 0, "states start segments");
-static_assert((kWarps * kBwdSteps) % kChunk == 0, "a full block's stage starts on a kept state");
+// Warps of a full block with 2^log2 lanes along the channels: a stage has 8
+// segments.
+__host__ __device__ constexpr int warps_of(int log2) { return log2 == 4 ? 4 : 2; }
+static_assert((8 * kBwdSteps) % kChunk == 0, "a full block's stage starts on a kept state");
 
 struct ScanArgs {
   const void *x, *gate;
@@ -46,272 +55,668 @@ struct ScanArgs {
   void *grad_x, *grad_gate;
   int64_t dxb, dxt, dgb, dgt;
   float *grad_h0;           // [B, D] or null
-  int lanes;                // lanes of a warp that lie along the channels (a power of two)
+  int aligned;              // every row of a tile starts on 16 bytes
+  int words;                // inputs' and outputs' rows start on words
+  int64_t x_end, gate_end, grad_h_end;  // bytes from a tensor's start to its end
+  int ring;                 // stages in shared memory
   int64_t tiles;            // channel tiles of a series
+  int64_t piece;            // samples of a piece of a series (of kSpan, if more than one)
+  int pieces;
+  float2 *totals;           // [B, ceil(T / kSpan), D]: compositions of spans (pieces > 1)
 };
+
+// The channels a lane holds: a 32-bit word's worth.
+template <int V>
+struct Lane {
+  float v[V];
+  __device__ __forceinline__ float operator[](int i) const { return v[i]; }
+  __device__ __forceinline__ void set(int i, float f) { v[i] = f; }
+};
+template <int V>
+__device__ __forceinline__ Lane<V> fma(Lane<V> a, Lane<V> b, Lane<V> c) {
+  Lane<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = fmaf(a.v[i], b.v[i], c.v[i]);
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Lane<V> operator*(Lane<V> a, Lane<V> b) {
+  Lane<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = a.v[i] * b.v[i];
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Lane<V> operator+(Lane<V> a, Lane<V> b) {
+  Lane<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = a.v[i] + b.v[i];
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Lane<V> all(float f) {
+  Lane<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.set(i, f);
+  return r;
+}
+
+// Words of shared or global memory as float32 channels and back.
+__device__ __forceinline__ Lane<1> unpack(uint32_t w, float) { return {{__uint_as_float(w)}}; }
+__device__ __forceinline__ Lane<2> unpack(uint32_t w, __nv_bfloat16) {
+  return {{__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)}};
+}
+__device__ __forceinline__ Lane<2> unpack(uint32_t w, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  return {{f.x, f.y}};
+}
+__device__ __forceinline__ uint32_t pack(Lane<1> a, float) { return __float_as_uint(a[0]); }
+__device__ __forceinline__ uint32_t pack(Lane<2> a, __nv_bfloat16) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a[0], a[1]);
+  return *reinterpret_cast<const uint32_t *>(&p);
+}
+__device__ __forceinline__ uint32_t pack(Lane<2> a, __half) {
+  const __half2 p = __floats2half2_rn(a[0], a[1]);
+  return *reinterpret_cast<const uint32_t *>(&p);
+}
+// +inf in every element: the gate of a sample that is none (a = 1, 1 - a = 0).
+__device__ __forceinline__ uint32_t closed_gate(float) { return 0x7F800000u; }
+__device__ __forceinline__ uint32_t closed_gate(__nv_bfloat16) { return 0x7F807F80u; }
+__device__ __forceinline__ uint32_t closed_gate(__half) { return 0x7C007C00u; }
 
 // a = sigmoid(z) and f = 1 - a = sigmoid(-z) from e = exp(-z), by the hardware's
 // approximate exponential and reciprocal (2 and 1 units in the last place).
 // f = e / (1 + e) keeps its relative precision as a -> 1; where e > 1, 1 - a
 // loses none and is right for e = inf too.
-__device__ __forceinline__ void gate_of(float z, float &a, float &f) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.0f + e));
-  f = e > 1.0f ? 1.0f - a : e * a;
+template <int V>
+__device__ __forceinline__ void gate_of(Lane<V> z, Lane<V> &a, Lane<V> &f) {
+  const Lane<V> t = z * all<V>(-1.4426950408889634f);
+  Lane<V> e;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t[i]));
+    e.set(i, r);
+  }
+  const Lane<V> d = e + all<V>(1.0f);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d[i]));
+    a.set(i, r);
+  }
+  f = e * a;
+  const Lane<V> g = fma(a, all<V>(-1.0f), all<V>(1.0f));
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (e[i] > 1.0f) f.set(i, g[i]);
 }
 
-// Inclusive scan of (A, H) over a warp's segments: lanes `lanes` apart hold
-// consecutive segments.
-template <int VEC>
-__device__ __forceinline__ void warp_compose(float (&A)[VEC], float (&H)[VEC], int lanes, int lane) {
-  for (int o = lanes; o < 32; o <<= 1) {
+__device__ __forceinline__ uint32_t shared_address(const void *p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+// One input: a tile's samples of a series.
+template <typename T>
+struct Rows {
+  const T *first;           // sample 0, the tile's first channel
+  int64_t stride;           // of samples, in elements
+  const char *begin, *end;  // of the whole tensor
+  uint32_t fill;            // the value of a sample that is none
+};
+
+// A stage in shared memory: a row per sample, `kPitch` words of it, and a gap of
+// a row after each segment of L, which keeps a warp's segments on different
+// banks.  Rows that start on 16 bytes lie there from word 0 on.  Of others the
+// 16-byte pieces of memory that hold them are copied as they are, so a row
+// starts at byte (address & 15).
+template <int L, int LOG2, bool ALIGNED>
+struct Stage {
+  static constexpr int kPitch = (1 << LOG2) + (ALIGNED ? 0 : 4);
+  static constexpr int kCopies = kPitch / 4;  // of 16 bytes, per row
+  __host__ __device__ static constexpr int words(int samples) { return (samples + samples / L) * kPitch; }
+  __device__ static __forceinline__ int row(int r) { return (r + r / L) * kPitch; }
+};
+
+// Copies samples s0 .. s0 + rows - 1 of a tile to `to`.  Nothing is read of
+// samples from `len` on nor outside the tensor.
+template <typename T, int L, int LOG2, bool ALIGNED>
+__device__ __forceinline__ void copy_stage(uint32_t *to, const Rows<T> &in, int s0, int rows, int len, int channels) {
+  using S = Stage<L, LOG2, ALIGNED>;
+  constexpr int V = 4 / sizeof(T);
+  const uint4 fill = make_uint4(in.fill, in.fill, in.fill, in.fill);
+  if (ALIGNED) {
+    const int step = blockDim.x / S::kCopies, word = (threadIdx.x % S::kCopies) * 4;
+    int r = threadIdx.x / S::kCopies;
+    const T *src = in.first + (int64_t)(s0 + r) * in.stride + word * V;
+    if (s0 + rows <= len && channels >= V << LOG2) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      const float pa = __shfl_up_sync(~0u, A[v], o), ph = __shfl_up_sync(~0u, H[v], o);
-      if (lane >= o) {
-        H[v] = fmaf(A[v], ph, H[v]);
-        A[v] *= pa;
+      for (int k = 0; k < L / 4; ++k, r += step, src += step * in.stride)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address(to + S::row(r) + word)),
+                     "l"(src));
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < L / 4; ++k, r += step, src += step * in.stride) {
+      uint32_t *dst = to + S::row(r) + word;
+      if (s0 + r < len && word * V < channels) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address(dst)), "l"(src));
+      } else {
+        *reinterpret_cast<uint4 *>(dst) = fill;
       }
+    }
+    return;
+  }
+  for (int q = threadIdx.x; q < rows * S::kCopies; q += blockDim.x) {
+    const int r = q / S::kCopies, piece = q % S::kCopies;
+    uint32_t *dst = to + S::row(r) + piece * 4;
+    if (s0 + r >= len) {
+      *reinterpret_cast<uint4 *>(dst) = fill;
+      continue;
+    }
+    const char *row = reinterpret_cast<const char *>(in.first + (int64_t)(s0 + r) * in.stride);
+    const char *src = reinterpret_cast<const char *>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15) + piece * 16;
+    const char *row_end = row + channels * (int)sizeof(T);
+    if (src >= row_end) continue;
+    if (src >= in.begin && src + 16 <= in.end) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address(dst)), "l"(src));
+    } else {  // the tensor's first or last bytes: its elements one by one
+      for (int i = 0; i < 16; i += (int)sizeof(T))
+        if (src + i >= row && src + i < row_end)
+          reinterpret_cast<T *>(dst)[i / sizeof(T)] = *reinterpret_cast<const T *>(src + i);
     }
   }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kWarps * 32) k_scan(ScanArgs p) {
-  constexpr int L = kFwdSteps;
-  __shared__ float2 total[2][kWarps][32][VEC];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int sub = lane / p.lanes, cl = lane % p.lanes, subs = 32 / p.lanes;
-  const int64_t b = blockIdx.x / p.tiles;
-  const int64_t d = ((blockIdx.x % p.tiles) * p.lanes + cl) * VEC;
-  const bool on = d < p.D;
-  int64_t len = p.T;
-  if (p.lengths != nullptr) len = min(max((int64_t)p.lengths[b], (int64_t)0), p.T);
-  const T *x = static_cast<const T *>(p.x) + b * p.xb + d;
+template <typename T>
+__device__ __forceinline__ Rows<T> rows_of(const void *tensor, int64_t at, int64_t stride, int64_t bytes, uint32_t fill) {
+  const char *begin = static_cast<const char *>(tensor);
+  return {static_cast<const T *>(tensor) + at, stride, begin, begin + bytes, fill};
+}
+
+// A lane's word of each of L consecutive samples, from sample t0 of a tile and
+// row r of its stage on.
+template <typename T, int L, int LOG2, bool ALIGNED>
+struct Words {
+  const uint32_t *row;
+  int at, step;             // of the row's start, as bytes beyond a multiple of 16
+  __device__ __forceinline__ Words(const uint32_t *stage, int r, int cl, const Rows<T> &in, int t0) {
+    row = stage + Stage<L, LOG2, ALIGNED>::row(r) + cl;
+    if (!ALIGNED) {
+      at = (int)(reinterpret_cast<uintptr_t>(in.first + t0 * in.stride) & 15);
+      step = (int)(in.stride * (int64_t)sizeof(T)) & 15;
+    }
+  }
+  __device__ __forceinline__ uint32_t operator[](int i) const {
+    const uint32_t *w = row + i * Stage<L, LOG2, ALIGNED>::kPitch;
+    if (ALIGNED) return *w;
+    const int m = (at + i * step) & 15;
+    w += m >> 2;
+    if (sizeof(T) == 4) return *w;
+    return __funnelshift_r(w[0], w[1], (m & 2) * 8);
+  }
+};
+
+// Stores a lane's channels of one sample: as a word, or of 16-bit elements
+// whose pairs do not lie on words the first `n`.
+template <bool WORDS, typename T, int V>
+__device__ __forceinline__ void store_lane(T *row, Lane<V> v, int n) {
+  const uint32_t w = pack(v, T{});
+  if (WORDS || V == 1) {
+    *reinterpret_cast<uint32_t *>(row) = w;
+  } else {
+    unsigned short *q = reinterpret_cast<unsigned short *>(row);
+    q[0] = (unsigned short)w;
+    if (n > 1) q[1] = (unsigned short)(w >> 16);
+  }
+}
+
+template <int V>
+__device__ __forceinline__ Lane<V> load_state(const float *row, int64_t d, int64_t D) {
+  Lane<V> r = all<V>(0.0f);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (d + i < D) r.set(i, row[d + i]);
+  return r;
+}
+template <int V>
+__device__ __forceinline__ void store_state(float *row, int64_t d, int64_t D, Lane<V> v) {
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (d + i < D) row[d + i] = v[i];
+}
+
+template <int V>
+__device__ __forceinline__ Lane<V> shuffle_up(Lane<V> v, int o) {
+  Lane<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.set(i, __shfl_up_sync(~0u, v[i], o));
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Lane<V> shuffle_down(Lane<V> v, int o) {
+  Lane<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.set(i, __shfl_down_sync(~0u, v[i], o));
+  return r;
+}
+
+// A composition of steps: state -> A state + H.
+template <int V>
+struct Step {
+  Lane<V> A, H;
+};
+template <int V>
+__device__ __forceinline__ void put(float2 *at, Lane<V> A, Lane<V> H) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) at[i] = make_float2(A[i], H[i]);
+}
+template <int V>
+__device__ __forceinline__ Step<V> get(const float2 *at) {
+  Step<V> s;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    s.A.set(i, at[i].x);
+    s.H.set(i, at[i].y);
+  }
+  return s;
+}
+
+// Where a thread stands.
+template <int L, int LOG2, int V>
+struct Place {
+  static constexpr int kLanes = 1 << LOG2, kSubs = 32 >> LOG2;
+  int lane, warp, sub, cl, seg;
+  int64_t b, d;          // series; first channel of the lane
+  int channels;          // of the tile
+  int len, stage;
+  int piece, first, end; // the block's samples; from len on there are none
+  int live;              // stages that have some
+  __device__ __forceinline__ Place(const ScanArgs &p) {
+    lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    sub = lane >> LOG2, cl = lane & (kLanes - 1), seg = warp * kSubs + sub;
+    // neighbouring blocks: neighbouring channels
+    const int64_t c = blockIdx.x / p.tiles, d0 = (blockIdx.x % p.tiles) * (kLanes * V);
+    b = c / p.pieces;
+    piece = (int)(c % p.pieces);
+    d = d0 + cl * V;
+    channels = (int)min((int64_t)(kLanes * V), p.D - d0);
+    len = (int)p.T;
+    if (p.lengths != nullptr) len = min(max(p.lengths[b], 0), len);
+    stage = (int)(blockDim.x >> 5) * kSubs * L;
+    first = (int)(piece * p.piece);
+    end = (int)min((piece + 1) * p.piece, p.T);
+    live = len > first ? (min(len, end) - first + stage - 1) / stage : 0;
+  }
+};
+
+__device__ __forceinline__ void wait_for_stage(int ring) {
+  if (ring == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  else if (ring == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else if (ring == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else asm volatile("cp.async.wait_group 3;" ::: "memory");
+  __syncthreads();
+}
+
+// The compositions of spans of kSpan samples: forward (A, H) with the state
+// after one A state + H, for the gradient (A, R) with c at its first sample
+// A c + R.  A block takes a span of 32 lanes' channels, a warp a part of it.
+constexpr int kTotalWarps = 8, kTotalSteps = kSpan / kTotalWarps;
+
+template <typename T>
+__device__ __forceinline__ uint32_t load_word(const T *row, int n, bool words) {
+  if (sizeof(T) == 4 || words) return *reinterpret_cast<const uint32_t *>(row);
+  const unsigned short *q = reinterpret_cast<const unsigned short *>(row);
+  return q[0] | (n > 1 ? (uint32_t)q[1] << 16 : 0u);
+}
+
+template <typename T, bool BACK>
+__global__ void __launch_bounds__(kTotalWarps * 32) k_scan_totals(const __grid_constant__ ScanArgs p) {
+  constexpr int L = 16, V = 4 / sizeof(T);
+  static_assert(kTotalSteps % L == 0, "a warp's part of a span is read L samples at a time");
+  asm volatile("griddepcontrol.launch_dependents;");
+  __shared__ float2 total[kTotalWarps][32][V];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t tiles = (p.D + 32 * V - 1) / (32 * V), spans = (p.T + kSpan - 1) / kSpan;
+  const int64_t c = blockIdx.x / tiles, d = (blockIdx.x % tiles) * (32 * V) + lane * V;
+  const int64_t b = c / spans, span = c % spans;
+  const int n = (int)min(p.D - d, (int64_t)V);
+  int len = (int)p.T;
+  if (p.lengths != nullptr) len = min(max(p.lengths[b], 0), len);
+  // u: what is added per sample, f x or dh
+  const T *u = BACK ? static_cast<const T *>(p.grad_h) + b * p.T * p.D + d
+                    : static_cast<const T *>(p.x) + b * p.xb + d;
+  const int64_t ut = BACK ? p.D : p.xt;
   const T *g = static_cast<const T *>(p.gate) + b * p.gb + d;
-  T *h = static_cast<T *>(p.h) + b * p.T * p.D + d;
-  const int64_t chunks = (p.T + kChunk - 1) / kChunk;
-
-  float carry[VEC];
+  const int first = (int)(span * kSpan) + warp * kTotalSteps;
+  const bool any = n > 0 && (!BACK || p.grad_h != nullptr);
+  Lane<V> A = all<V>(1.0f), H = all<V>(0.0f);
+#pragma unroll 1
+  for (int k = 0; k < kTotalSteps; k += L) {
+    const int t0 = first + (BACK ? kTotalSteps - L - k : k);
+    if (t0 >= len) continue;
+    uint32_t gw[L], uw[L];
+    const T *gr = g + t0 * p.gt, *ur = u + t0 * ut;
 #pragma unroll
-  for (int v = 0; v < VEC; ++v)
-    carry[v] = on && p.h0 != nullptr ? p.h0[b * p.D + d + v] : 0.0f;
-
-  const int64_t stage = (int64_t)warps * subs * L;
-  int buf = 0;
-  for (int64_t s0 = 0; s0 < p.T; s0 += stage, buf ^= 1) {
-    const int64_t t0 = s0 + (int64_t)(warp * subs + sub) * L;
-    float a[L][VEC], in[L][VEC];
-    float A[VEC], H[VEC];
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const bool live = on && t0 + i < len;
-      Pack<T, VEC> xv{}, gv{};
-      if (live) {
-        xv = *reinterpret_cast<const Pack<T, VEC> *>(x + (t0 + i) * p.xt);
-        gv = *reinterpret_cast<const Pack<T, VEC> *>(g + (t0 + i) * p.gt);
-      }
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        float f;
-        gate_of(to_f32(gv.v[v]), a[i][v], f);
-        in[i][v] = live ? f * to_f32(xv.v[v]) : 0.0f;
-        if (!live) a[i][v] = 1.0f;
-      }
+    for (int i = 0; i < L; ++i, gr += p.gt, ur += ut) {
+      gw[i] = closed_gate(T{});
+      uw[i] = 0u;
+      if (n > 0 && t0 + i < len) gw[i] = load_word(gr, n, p.words);
+      if (any && t0 + i < len) uw[i] = load_word(ur, n, p.words);
     }
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      A[v] = 1.0f;
-      H[v] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-        H[v] = fmaf(a[i][v], H[v], in[i][v]);
-        A[v] *= a[i][v];
-      }
-    }
-    warp_compose(A, H, p.lanes, lane);
-    if (sub == subs - 1) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) total[buf][warp][cl][v] = make_float2(A[v], H[v]);
-    }
-    __syncthreads();
-    float state[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      const float ea = __shfl_up_sync(~0u, A[v], p.lanes), eh = __shfl_up_sync(~0u, H[v], p.lanes);
-      float c = carry[v], start = 0.0f;
-      for (int w = 0; w < warps; ++w) {
-        if (w == warp) start = c;
-        const float2 q = total[buf][w][cl][v];
-        c = fmaf(q.x, c, q.y);
-      }
-      carry[v] = c;
-      state[v] = sub > 0 ? fmaf(ea, start, eh) : start;
-    }
-    if (on && p.states != nullptr && t0 < p.T && t0 % kChunk == 0) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v)
-        p.states[(b * chunks + t0 / kChunk) * p.D + d + v] = state[v];
-    }
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      Pack<T, VEC> hv;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        state[v] = fmaf(a[i][v], state[v], in[i][v]);
-        hv.v[v] = from_f32<T>(t0 + i < len ? state[v] : 0.0f);
-      }
-      if (on && t0 + i < p.T) *reinterpret_cast<Pack<T, VEC> *>(h + (t0 + i) * p.D) = hv;
+    for (int k = 0; k < L; ++k) {
+      const int i = BACK ? L - 1 - k : k;
+      Lane<V> a, f;
+      gate_of(unpack(gw[i], T{}), a, f);
+      H = BACK ? a * (H + unpack(uw[i], T{})) : fma(a, H, f * unpack(uw[i], T{}));
+      A = A * a;
     }
   }
-  if (on && p.last != nullptr && warp == 0 && sub == 0) {
+  put(total[warp][lane], A, H);
+  __syncthreads();
+  if (warp != 0 || n <= 0) return;
+  A = all<V>(1.0f), H = all<V>(0.0f);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) p.last[b * p.D + d + v] = carry[v];
+  for (int k = 0; k < kTotalWarps; ++k) {
+    const Step<V> q = get<V>(total[BACK ? kTotalWarps - 1 - k : k][lane]);
+    H = fma(q.A, H, q.H);
+    A = A * q.A;
   }
+  float2 *to = p.totals + (b * spans + span) * p.D + d;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i < n) to[i] = make_float2(A[i], H[i]);
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kWarps * 32) k_scan_backward(ScanArgs p) {
-  constexpr int L = kBwdSteps;
-  __shared__ float4 total[2][kWarps][32][VEC];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int sub = lane / p.lanes, cl = lane % p.lanes, subs = 32 / p.lanes;
-  const int64_t b = blockIdx.x / p.tiles;
-  const int64_t d = ((blockIdx.x % p.tiles) * p.lanes + cl) * VEC;
-  const bool on = d < p.D;
-  int64_t len = p.T;
-  if (p.lengths != nullptr) len = min(max((int64_t)p.lengths[b], (int64_t)0), p.T);
-  const T *x = static_cast<const T *>(p.x) + b * p.xb + d;
-  const T *g = static_cast<const T *>(p.gate) + b * p.gb + d;
-  const T *dh = static_cast<const T *>(p.grad_h) + b * p.T * p.D + d;
-  T *dx = static_cast<T *>(p.grad_x) + b * p.dxb + d;
-  T *dg = static_cast<T *>(p.grad_gate) + b * p.dgb + d;
-  const int64_t chunks = (p.T + kChunk - 1) / kChunk;
-
-  float carry[VEC];  // c of the first sample after the stage
+// A lane's state at the start of its piece from the spans before it (forward),
+// or its c after the piece from those after it (gradient).  The block's
+// segments compose a part each; `total` is shared memory of kWarps * kSubs.
+template <int V, bool BACK, typename At>
+__device__ __forceinline__ Lane<V> through_spans(const ScanArgs &p, const At &at, float2 (*total)[V], int mine,
+                                                 Lane<V> c) {
+  if (p.pieces == 1) return c;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int all_spans = (int)((p.T + kSpan - 1) / kSpan), each = (int)(p.piece / kSpan);
+  const int from = BACK ? min((at.piece + 1) * each, all_spans) : 0;
+  const int count = BACK ? all_spans - from : at.piece * each;
+  const int segments = (int)(blockDim.x >> 5) * At::kSubs, share = (count + segments - 1) / segments;
+  const int lo = min(at.seg * share, count), hi = min(lo + share, count);
+  Lane<V> A = all<V>(1.0f), H = all<V>(0.0f);
+  const float2 *q = p.totals + (at.b * all_spans + from) * p.D + at.d;
+#pragma unroll 4
+  for (int k = 0; k < hi - lo; ++k) {
+    const float2 *row = q + (int64_t)(BACK ? hi - 1 - k : lo + k) * p.D;
 #pragma unroll
-  for (int v = 0; v < VEC; ++v)
-    carry[v] = on && p.grad_last != nullptr ? p.grad_last[b * p.D + d + v] : 0.0f;
+    for (int i = 0; i < V; ++i)
+      if (i < mine) {
+        const float2 t = row[i];
+        H.set(i, fmaf(t.x, H[i], t.y));
+        A.set(i, A[i] * t.x);
+      }
+  }
+  put(total[at.seg * At::kLanes + at.cl], A, H);
+  __syncthreads();
+  for (int k = 0; k < segments; ++k) {
+    const Step<V> t = get<V>(total[(BACK ? segments - 1 - k : k) * At::kLanes + at.cl]);
+    c = fma(t.A, c, t.H);
+  }
+  __syncthreads();
+  return c;
+}
 
-  const int64_t stage = (int64_t)warps * subs * L;
-  int buf = 0;
-  for (int64_t s0 = (p.T - 1) / stage * stage; s0 >= 0; s0 -= stage, buf ^= 1) {
-    const int64_t t0 = s0 + (int64_t)(warp * subs + sub) * L;
-    float a[L][VEC], f[L][VEC], xs[L][VEC], gr[L][VEC];
+template <typename T, int LOG2, bool ALIGNED>
+__global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_scan(const __grid_constant__ ScanArgs p) {
+  constexpr int L = kFwdSteps, V = 4 / sizeof(T), kWarps = warps_of(LOG2);
+  using At = Place<L, LOG2, V>;
+  extern __shared__ uint4 ring_memory[];
+  __shared__ float2 warp_total[kWarps][At::kLanes][V], span_total[kWarps * 32][V];
+  const At at(p);
+  const int mine = at.channels - at.cl * V;  // channels of this lane, if positive
+  const bool on = mine > 0;
+  const int64_t d0 = at.d - at.cl * V;
+  const Rows<T> x = rows_of<T>(p.x, at.b * p.xb + d0, p.xt, p.x_end, 0u);
+  const Rows<T> g = rows_of<T>(p.gate, at.b * p.gb + d0, p.gt, p.gate_end, closed_gate(T{}));
+  T *h = static_cast<T *>(p.h) + at.b * p.T * p.D + at.d;
+  const int64_t chunks = (p.T + kChunk - 1) / kChunk;
+  const int words = Stage<L, LOG2, ALIGNED>::words(at.stage);  // of one tensor's stage
+  uint32_t *ring = reinterpret_cast<uint32_t *>(ring_memory);
+
+  auto fetch = [&](int k, int slot) {
+    if (k < at.live) {
+      uint32_t *to = ring + slot * 2 * words;
+      const int s0 = at.first + k * at.stage;
+      copy_stage<T, L, LOG2, ALIGNED>(to, x, s0, at.stage, at.len, at.channels);
+      copy_stage<T, L, LOG2, ALIGNED>(to + words, g, s0, at.stage, at.len, at.channels);
+    }
+    asm volatile("cp.async.commit_group;");
+  };
+  for (int k = 0; k < p.ring; ++k) fetch(k, k);
+
+  for (int k = threadIdx.x; k < kWarps * At::kLanes; k += blockDim.x)  // warps that are not there
+    put(warp_total[k >> LOG2][k & (At::kLanes - 1)], all<V>(1.0f), all<V>(0.0f));
+  Lane<V> carry = all<V>(0.0f);
+  if (p.h0 != nullptr) carry = load_state<V>(p.h0 + at.b * p.D, at.d, p.D);
+  carry = through_spans<V, false>(p, at, span_total, mine, carry);
+
+  int slot = 0;
+  for (int k = 0; k < at.live; ++k) {
+    const int t0 = at.first + k * at.stage + at.seg * L;
+    wait_for_stage(p.ring);
+    const uint32_t *here = ring + slot * 2 * words;
+    const Words<T, L, LOG2, ALIGNED> xs(here, at.seg * L, at.cl, x, t0), gs(here + words, at.seg * L, at.cl, g, t0);
+    Lane<V> a[L], in[L], A = all<V>(1.0f), H = all<V>(0.0f);
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      const bool live = on && t0 + i < len;
-      Pack<T, VEC> xv{}, gv{}, dv{};
-      if (live) {
-        xv = *reinterpret_cast<const Pack<T, VEC> *>(x + (t0 + i) * p.xt);
-        gv = *reinterpret_cast<const Pack<T, VEC> *>(g + (t0 + i) * p.gt);
-        if (p.grad_h != nullptr)
-          dv = *reinterpret_cast<const Pack<T, VEC> *>(dh + (t0 + i) * p.D);
-      }
+      Lane<V> f;
+      gate_of(unpack(gs[i], T{}), a[i], f);
+      in[i] = f * unpack(xs[i], T{});
+      H = fma(a[i], H, in[i]);
+      A = A * a[i];
+    }
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        gate_of(to_f32(gv.v[v]), a[i][v], f[i][v]);
-        xs[i][v] = to_f32(xv.v[v]);
-        gr[i][v] = to_f32(dv.v[v]);
-        if (!live) {
-          a[i][v] = 1.0f;
-          f[i][v] = 0.0f;
-        }
+    for (int o = At::kLanes; o < 32; o <<= 1) {
+      const Lane<V> pa = shuffle_up(A, o), ph = shuffle_up(H, o);
+      if (at.lane >= o) {
+        H = fma(A, ph, H);
+        A = A * pa;
       }
     }
-    // (A, H): the segment's samples forward; (A, R): c at its first sample is
-    // A c_next + R.
-    float A[VEC], H[VEC], R[VEC], base[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      A[v] = 1.0f;
-      H[v] = R[v] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-        H[v] = fmaf(a[i][v], H[v], f[i][v] * xs[i][v]);
-        A[v] *= a[i][v];
-        R[v] = a[L - 1 - i][v] * (R[v] + gr[L - 1 - i][v]);
-      }
-      base[v] = on ? p.states[(b * chunks + s0 / kChunk) * p.D + d + v] : 0.0f;
-    }
-    // Scans over the warp's segments: forward ones up, backward ones down.
-    float Af[VEC], Ab[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) Af[v] = Ab[v] = A[v];
-    for (int o = p.lanes; o < 32; o <<= 1) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float pa = __shfl_up_sync(~0u, Af[v], o), ph = __shfl_up_sync(~0u, H[v], o);
-        const float na = __shfl_down_sync(~0u, Ab[v], o), nr = __shfl_down_sync(~0u, R[v], o);
-        if (lane >= o) {
-          H[v] = fmaf(Af[v], ph, H[v]);
-          Af[v] *= pa;
-        }
-        if (lane + o < 32) {
-          R[v] = fmaf(Ab[v], nr, R[v]);
-          Ab[v] *= na;
-        }
-      }
-    }
-    // The warp's totals: A and H from its last segment, R from its first.
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      const float r0 = __shfl_sync(~0u, R[v], cl);
-      if (sub == subs - 1) total[buf][warp][cl][v] = make_float4(Af[v], H[v], r0, 0.0f);
-    }
+    if (at.sub == At::kSubs - 1) put(warp_total[at.warp][at.cl], A, H);
     __syncthreads();
-    float state[VEC], c[VEC];
+    fetch(k + p.ring, slot);
+    slot = slot + 1 == p.ring ? 0 : slot + 1;
+    Lane<V> start = carry;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      const float ea = __shfl_up_sync(~0u, Af[v], p.lanes), eh = __shfl_up_sync(~0u, H[v], p.lanes);
-      const float na = __shfl_down_sync(~0u, Ab[v], p.lanes), nr = __shfl_down_sync(~0u, R[v], p.lanes);
-      float s = base[v];
-      for (int w = 0; w < warp; ++w) {
-        const float4 q = total[buf][w][cl][v];
-        s = fmaf(q.x, s, q.y);
-      }
-      float r = carry[v], after = 0.0f;
-      for (int w = warps - 1; w >= 0; --w) {
-        if (w == warp) after = r;
-        const float4 q = total[buf][w][cl][v];
-        r = fmaf(q.x, r, q.z);
-      }
-      carry[v] = r;
-      state[v] = sub > 0 ? fmaf(ea, s, eh) : s;
-      c[v] = sub < subs - 1 ? fmaf(na, after, nr) : after;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == at.warp) start = carry;
+      const Step<V> q = get<V>(warp_total[w][at.cl]);
+      carry = fma(q.A, carry, q.H);
     }
+    Lane<V> state = start;
+    const Lane<V> ea = shuffle_up(A, At::kLanes), eh = shuffle_up(H, At::kLanes);
+    if (at.sub > 0) state = fma(ea, start, eh);
+    if (p.states != nullptr && t0 % kChunk == 0 && t0 < at.len)
+      store_state(p.states + (at.b * chunks + t0 / kChunk) * p.D, at.d, p.D, state);
+    auto write = [&](auto words) {
+      T *row = h + t0 * p.D;
+      if (t0 + L <= at.len) {
+#pragma unroll
+        for (int i = 0; i < L; ++i, row += p.D) {
+          state = fma(a[i], state, in[i]);
+          store_lane<words.value>(row, state, mine);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < L; ++i, row += p.D) {
+          state = fma(a[i], state, in[i]);
+          if (t0 + i < p.T) store_lane<words.value>(row, t0 + i < at.len ? state : all<V>(0.0f), mine);
+        }
+      }
+    };
+    if (on) {
+      if (p.words) write(std::true_type{});
+      else write(std::false_type{});
+    }
+  }
+  // Stages past the series' end: zeros.
+  for (int s0 = at.first + at.live * at.stage; s0 < at.end; s0 += at.stage) {
+    const int t0 = s0 + at.seg * L;
+    for (int i = 0; i < L; ++i)
+      if (on && t0 + i < at.end) store_lane<false>(h + (t0 + i) * p.D, all<V>(0.0f), mine);
+  }
+  if (p.last != nullptr && at.piece == p.pieces - 1 && at.warp == 0 && at.sub == 0)
+    store_state(p.last + at.b * p.D, at.d, p.D, carry);
+}
+
+template <typename T, int LOG2, bool ALIGNED>
+__global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_scan_backward(const __grid_constant__ ScanArgs p) {
+  constexpr int L = kBwdSteps, V = 4 / sizeof(T), kWarps = warps_of(LOG2);
+  using At = Place<L, LOG2, V>;
+  extern __shared__ uint4 ring_memory[];
+  __shared__ float2 up_total[kWarps][At::kLanes][V], down_total[kWarps][At::kLanes][V];
+  __shared__ float2 span_total[kWarps * 32][V];
+  const At at(p);
+  const int mine = at.channels - at.cl * V;  // channels of this lane, if positive
+  const bool on = mine > 0;
+  const int64_t d0 = at.d - at.cl * V;
+  const Rows<T> x = rows_of<T>(p.x, at.b * p.xb + d0, p.xt, p.x_end, 0u);
+  const Rows<T> g = rows_of<T>(p.gate, at.b * p.gb + d0, p.gt, p.gate_end, closed_gate(T{}));
+  const Rows<T> dh = rows_of<T>(p.grad_h, at.b * p.T * p.D + d0, p.D, p.grad_h_end, 0u);
+  T *dx = static_cast<T *>(p.grad_x) + at.b * p.dxb + at.d;
+  T *dg = static_cast<T *>(p.grad_gate) + at.b * p.dgb + at.d;
+  const int64_t chunks = (p.T + kChunk - 1) / kChunk;
+  const int words = Stage<L, LOG2, ALIGNED>::words(at.stage);
+  uint32_t *ring = reinterpret_cast<uint32_t *>(ring_memory);
+
+  // Stage k counts from the last one with samples back.
+  auto fetch = [&](int k, int slot) {
+    if (k < at.live) {
+      uint32_t *to = ring + slot * 3 * words;
+      const int s0 = at.first + (at.live - 1 - k) * at.stage;
+      copy_stage<T, L, LOG2, ALIGNED>(to, x, s0, at.stage, at.len, at.channels);
+      copy_stage<T, L, LOG2, ALIGNED>(to + words, g, s0, at.stage, at.len, at.channels);
+      copy_stage<T, L, LOG2, ALIGNED>(to + 2 * words, dh, s0, at.stage, p.grad_h != nullptr ? at.len : 0,
+                                      at.channels);
+    }
+    asm volatile("cp.async.commit_group;");
+  };
+  for (int k = 0; k < p.ring; ++k) fetch(k, k);
+
+  for (int k = threadIdx.x; k < kWarps * At::kLanes; k += blockDim.x) {
+    put(up_total[k >> LOG2][k & (At::kLanes - 1)], all<V>(1.0f), all<V>(0.0f));
+    put(down_total[k >> LOG2][k & (At::kLanes - 1)], all<V>(1.0f), all<V>(0.0f));
+  }
+  Lane<V> carry = all<V>(0.0f);  // c of the first sample after the stage
+  if (p.grad_last != nullptr) carry = load_state<V>(p.grad_last + at.b * p.D, at.d, p.D);
+  carry = through_spans<V, true>(p, at, span_total, mine, carry);
+
+  int slot = 0;
+  for (int k = 0; k < at.live; ++k) {
+    const int s0 = at.first + (at.live - 1 - k) * at.stage, t0 = s0 + at.seg * L;
+    Lane<V> base = load_state<V>(p.states + (at.b * chunks + s0 / kChunk) * p.D, at.d, p.D);
+    wait_for_stage(p.ring);
+    const uint32_t *here = ring + slot * 3 * words;
+    const Words<T, L, LOG2, ALIGNED> xs(here, at.seg * L, at.cl, x, t0), gs(here + words, at.seg * L, at.cl, g, t0);
+    const Words<T, L, LOG2, ALIGNED> ds(here + 2 * words, at.seg * L, at.cl, dh, t0);
+    Lane<V> a[L], f[L], xv[L], gr[L];
+    Lane<V> A = all<V>(1.0f), H = all<V>(0.0f), R = all<V>(0.0f);
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      gate_of(unpack(gs[i], T{}), a[i], f[i]);
+      xv[i] = unpack(xs[i], T{});
+      gr[i] = unpack(ds[i], T{});
+      H = fma(a[i], H, f[i] * xv[i]);
+      A = A * a[i];
+    }
+#pragma unroll
+    for (int i = L - 1; i >= 0; --i) R = a[i] * (R + gr[i]);
+    // Over the warp's segments: (Af, H) from the first on, (Ab, R) from the last back.
+    Lane<V> Af = A, Ab = A;
+#pragma unroll
+    for (int o = At::kLanes; o < 32; o <<= 1) {
+      const Lane<V> pa = shuffle_up(Af, o), ph = shuffle_up(H, o);
+      const Lane<V> na = shuffle_down(Ab, o), nr = shuffle_down(R, o);
+      if (at.lane >= o) {
+        H = fma(Af, ph, H);
+        Af = Af * pa;
+      }
+      if (at.lane + o < 32) {
+        R = fma(Ab, nr, R);
+        Ab = Ab * na;
+      }
+    }
+    if (at.sub == At::kSubs - 1) put(up_total[at.warp][at.cl], Af, H);
+    if (at.sub == 0) put(down_total[at.warp][at.cl], Ab, R);
+    __syncthreads();
+    fetch(k + p.ring, slot);
+    slot = slot + 1 == p.ring ? 0 : slot + 1;
+    Lane<V> after = carry;
+#pragma unroll
+    for (int w = kWarps - 1; w >= 0; --w) {
+      if (w == at.warp) after = carry;
+      const Step<V> q = get<V>(down_total[w][at.cl]);
+      carry = fma(q.A, carry, q.H);
+    }
+    {
+      Lane<V> c = base;
+#pragma unroll
+      for (int w = 0; w < kWarps - 1; ++w) {
+        const Step<V> q = get<V>(up_total[w][at.cl]);
+        c = fma(q.A, c, q.H);
+        if (w + 1 == at.warp) base = c;
+      }
+    }
+    Lane<V> state = base, c = after;
+    const Lane<V> ea = shuffle_up(Af, At::kLanes), eh = shuffle_up(H, At::kLanes);
+    const Lane<V> na = shuffle_down(Ab, At::kLanes), nr = shuffle_down(R, At::kLanes);
+    if (at.sub > 0) state = fma(ea, base, eh);
+    if (at.sub < At::kSubs - 1) c = fma(na, after, nr);
     // Forward once more for h_{t-1} - x_t, then back.
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float before = state[v];
-        state[v] = fmaf(a[i][v], before, f[i][v] * xs[i][v]);
-        xs[i][v] = before - xs[i][v];
-      }
+      const Lane<V> before = state;
+      state = fma(a[i], before, f[i] * xv[i]);
+      xv[i] = fma(xv[i], all<V>(-1.0f), before);
     }
+    auto write = [&](auto words) {
+      T *rx = dx + (t0 + L - 1) * p.dxt, *rg = dg + (t0 + L - 1) * p.dgt;
+      if (t0 + L <= at.len) {
 #pragma unroll
-    for (int i = L - 1; i >= 0; --i) {
-      Pack<T, VEC> dxv, dgv;
+        for (int i = L - 1; i >= 0; --i, rx -= p.dxt, rg -= p.dgt) {
+          const Lane<V> delta = gr[i] + c;
+          c = a[i] * delta;
+          store_lane<words.value>(rx, f[i] * delta, mine);
+          store_lane<words.value>(rg, c * xv[i] * f[i], mine);
+        }
+      } else {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float delta = gr[i][v] + c[v];
-        c[v] = a[i][v] * delta;
-        const bool live = t0 + i < len;
-        dxv.v[v] = from_f32<T>(live ? f[i][v] * delta : 0.0f);
-        dgv.v[v] = from_f32<T>(live ? c[v] * xs[i][v] * f[i][v] : 0.0f);
+        for (int i = L - 1; i >= 0; --i, rx -= p.dxt, rg -= p.dgt) {
+          const Lane<V> delta = gr[i] + c;
+          c = a[i] * delta;
+          if (t0 + i < p.T) {
+            const bool live = t0 + i < at.len;
+            store_lane<words.value>(rx, live ? f[i] * delta : all<V>(0.0f), mine);
+            store_lane<words.value>(rg, live ? c * xv[i] * f[i] : all<V>(0.0f), mine);
+          }
+        }
       }
-      if (on && t0 + i < p.T) {
-        *reinterpret_cast<Pack<T, VEC> *>(dx + (t0 + i) * p.dxt) = dxv;
-        *reinterpret_cast<Pack<T, VEC> *>(dg + (t0 + i) * p.dgt) = dgv;
-      }
+    };
+    if (on) {
+      if (p.words) write(std::true_type{});
+      else write(std::false_type{});
     }
   }
-  if (on && p.grad_h0 != nullptr && warp == 0 && sub == 0) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) p.grad_h0[b * p.D + d + v] = carry[v];
+  for (int s0 = at.first + at.live * at.stage; s0 < at.end; s0 += at.stage) {
+    const int t0 = s0 + at.seg * L;
+    for (int i = 0; i < L; ++i)
+      if (on && t0 + i < at.end) {
+        store_lane<false>(dx + (t0 + i) * p.dxt, all<V>(0.0f), mine);
+        store_lane<false>(dg + (t0 + i) * p.dgt, all<V>(0.0f), mine);
+      }
   }
+  if (p.grad_h0 != nullptr && at.piece == 0 && at.warp == 0 && at.sub == 0)
+    store_state(p.grad_h0 + at.b * p.D, at.d, p.D, carry);
 }
 
 // One sample of B streams whose states are rows of a table.
@@ -330,9 +735,9 @@ __global__ void k_scan_step(const T *x, int64_t xs, const T *gate, int64_t gs, i
     float *st = state + row * D + d;
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-      float a, f;
-      gate_of(to_f32(gv.v[v]), a, f);
-      const float s = fmaf(a, st[v], f * to_f32(xv.v[v]));
+      Lane<1> a, f;
+      gate_of(all<1>(to_f32(gv.v[v])), a, f);
+      const float s = fmaf(a[0], st[v], f[0] * to_f32(xv.v[v]));
       st[v] = s;
       out.v[v] = from_f32<T>(s);
     }
@@ -340,44 +745,91 @@ __global__ void k_scan_step(const T *x, int64_t xs, const T *gate, int64_t gs, i
   *reinterpret_cast<Pack<T, VEC> *>(h + b * D + d) = out;
 }
 
-// How a launch covers the series: as few lanes along the channels as hold
-// them, and no more warps than the samples fill.
+// How a launch covers the series.
 struct Shape {
-  int lanes, threads;
-  int64_t tiles;
+  int lanes_log2, threads, ring, smem;
+  int64_t tiles, piece, pieces;
 };
 
-Shape shape_of(int64_t T, int64_t D, int vec, int steps) {
+Shape shape_of(int64_t B, int64_t T, int64_t D, int vec, bool back, bool aligned) {
+  const int steps = back ? kBwdSteps : kFwdSteps, tensors = back ? 3 : 2;
   Shape s;
-  s.lanes = 1;
-  while (s.lanes < 32 && (int64_t)s.lanes * vec < D) s.lanes *= 2;
-  s.tiles = (D + (int64_t)s.lanes * vec - 1) / ((int64_t)s.lanes * vec);
+  // Rows of 64 bytes, of 32 for 8 lanes' channels.
+  s.lanes_log2 = D <= 8 * vec ? 3 : 4;
+  s.tiles = (D + ((int64_t)vec << s.lanes_log2) - 1) / ((int64_t)vec << s.lanes_log2);
+  auto stage_at = [&](int warps) { return (int64_t)warps * (32 >> s.lanes_log2) * steps; };
   int warps = 1;
-  while (warps < kWarps && (int64_t)warps * (32 / s.lanes) * steps < T) warps *= 2;
+  while (warps < warps_of(s.lanes_log2) && stage_at(warps) < T) warps *= 2;
   s.threads = warps * 32;
+  // One piece, or as many as give four blocks (what its registers hold) to
+  // each SM.  A block takes a unit of time per stage and some to begin, longer
+  // on an SM that waits for it alone; composing the spans reads as much again
+  // as two thirds (the gradient: two fifths) of what the main kernel moves.
+  const int64_t stage = stage_at(warps), stages = (T + stage - 1) / stage, sms = device_info().sm_count;
+  const int64_t tiles = B * s.tiles, spans = (T + kSpan - 1) / kSpan;
+  const int64_t full = 16 / warps_of(s.lanes_log2) * sms;
+  int64_t each = (spans * tiles + full - 1) / full;  // spans of a piece
+  const double share = (double)(tiles * stages) / (double)sms;
+  const int64_t fullest = (tiles + sms - 1) / sms;
+  const double whole = (double)fullest * (double)(stages + 1) * (fullest == 1 ? 1.4 : 1.0);
+  s.piece = stages * stage, s.pieces = 1;
+  if (spans > 1 && tiles < full && share * (back ? 1.4 : 1.67) + 8.0 < whole && each < spans) {
+    s.piece = each * kSpan;
+    s.pieces = (T + s.piece - 1) / s.piece;
+  }
+  const int64_t rounds = s.piece / stage;
+  const int ring = back ? 3 : 2;
+  s.ring = (int)(rounds < ring ? rounds : ring);
+  s.smem = (int)(s.ring * tensors * (stage + stage / steps) * ((1 << s.lanes_log2) + (aligned ? 0 : 4)) * 4);
   return s;
 }
 
-template <typename T>
-cudaError_t scan_as(ScanArgs a, int64_t B, bool pairs, cudaStream_t stream) {
-  const Shape s = shape_of(a.T, a.D, pairs ? 2 : 1, kFwdSteps);
-  a.lanes = s.lanes;
-  a.tiles = s.tiles;
-  const unsigned grid = (unsigned)(B * s.tiles);
-  if (pairs) k_scan<T, 2><<<grid, s.threads, 0, stream>>>(a);
-  else k_scan<T, 1><<<grid, s.threads, 0, stream>>>(a);
-  return cudaGetLastError();
+template <typename T, int LOG2, bool BACK, bool ALIGNED>
+cudaError_t scan_launch(const ScanArgs &a, const Shape &s, int64_t B, cudaStream_t stream) {
+  const auto kernel = BACK ? k_scan_backward<T, LOG2, ALIGNED> : k_scan<T, LOG2, ALIGNED>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t c{};
+  cudaLaunchAttribute attr{};
+  if (s.pieces > 1) {  // begins, and fetches its first stages, while the pieces are composed
+    const int64_t vec = 4 / sizeof(T), tiles = (a.D + 32 * vec - 1) / (32 * vec), spans = (a.T + kSpan - 1) / kSpan;
+    k_scan_totals<T, BACK><<<(unsigned)(B * spans * tiles), kTotalWarps * 32, 0, stream>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &attr, c.numAttrs = 1;
+  }
+  c.gridDim = dim3((unsigned)(B * s.pieces * s.tiles)), c.blockDim = dim3(s.threads);
+  c.dynamicSmemBytes = s.smem, c.stream = stream;
+  return cudaLaunchKernelEx(&c, kernel, a);
 }
 
-template <typename T>
-cudaError_t scan_backward_as(ScanArgs a, int64_t B, bool pairs, cudaStream_t stream) {
-  const Shape s = shape_of(a.T, a.D, pairs ? 2 : 1, kBwdSteps);
-  a.lanes = s.lanes;
-  a.tiles = s.tiles;
-  const unsigned grid = (unsigned)(B * s.tiles);
-  if (pairs) k_scan_backward<T, 2><<<grid, s.threads, 0, stream>>>(a);
-  else k_scan_backward<T, 1><<<grid, s.threads, 0, stream>>>(a);
-  return cudaGetLastError();
+template <typename T, bool BACK>
+cudaError_t scan_as(ScanArgs a, int64_t B, cudaStream_t stream) {
+  constexpr int V = 4 / sizeof(T);
+  const Shape s = shape_of(B, a.T, a.D, V, BACK, a.aligned);
+  a.tiles = s.tiles, a.piece = s.piece, a.pieces = (int)s.pieces, a.ring = s.ring;
+  if (a.aligned)
+    return s.lanes_log2 == 4 ? scan_launch<T, 4, BACK, true>(a, s, B, stream)
+                             : scan_launch<T, 3, BACK, true>(a, s, B, stream);
+  return s.lanes_log2 == 4 ? scan_launch<T, 4, BACK, false>(a, s, B, stream)
+                           : scan_launch<T, 3, BACK, false>(a, s, B, stream);
+}
+
+// Fills in what the kernels need to know of the inputs' and outputs' places.
+void set_places(ScanArgs &a, int64_t B, int e) {
+  auto rows_on = [&](int w) {
+    return a.D * e % w == 0 && aligned_to(a.x, a.xb, e, w) && aligned_to(a.x, a.xt, e, w) &&
+           aligned_to(a.gate, a.gb, e, w) && aligned_to(a.gate, a.gt, e, w) && aligned_to(a.grad_h, 0, e, w);
+  };
+  a.aligned = rows_on(16);
+  a.words = rows_on(4) && aligned_to(a.h, 0, e, 4) && aligned_to(a.grad_x, a.dxb, e, 4) &&
+            aligned_to(a.grad_x, a.dxt, e, 4) && aligned_to(a.grad_gate, a.dgb, e, 4) &&
+            aligned_to(a.grad_gate, a.dgt, e, 4);
+  a.x_end = ((B - 1) * a.xb + (a.T - 1) * a.xt + a.D) * e;
+  a.gate_end = ((B - 1) * a.gb + (a.T - 1) * a.gt + a.D) * e;
+  a.grad_h_end = B * a.T * a.D * e;
 }
 
 template <typename T>
@@ -395,10 +847,12 @@ cudaError_t step_as(const void *x, int64_t xs, const void *gate, int64_t gs, int
 }
 
 // Checks shared by the scan's two directions.
-int check_scan(const char *fn, int dtype, const void *x, const void *gate, int64_t B, int64_t T,
-               int64_t D) {
+int check_scan(const char *fn, int dtype, const void *x, int64_t x_series, int64_t x_sample,
+               const void *gate, int64_t gate_series, int64_t gate_sample, int64_t B, int64_t T, int64_t D) {
   if (!dtype_ok(dtype)) return report_error(CPAB_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
   if (B < 0 || T < 0 || D < 0) return report_error(CPAB_ERR_ARG, "%s: negative size", fn);
+  if (x_series < 0 || x_sample < 0 || gate_series < 0 || gate_sample < 0)
+    return report_error(CPAB_ERR_ARG, "%s: negative stride", fn);
   if (T >= (int64_t(1) << 31)) return report_error(CPAB_ERR_SIZE, "%s: T must be below 2^31", fn);
   if (D > 0 && B > (int64_t(1) << 30) / D)
     return report_error(CPAB_ERR_SIZE, "%s: B * D must not exceed 2^30", fn);
@@ -414,12 +868,20 @@ using namespace cpab;
 
 extern "C" int cpab_b200_gated_scan_chunk(void) { return kChunk; }
 
+extern "C" int64_t cpab_b200_gated_scan_workspace(int dtype, int64_t B, int64_t T, int64_t D) {
+  if (!dtype_ok(dtype) || B < 1 || T < 1 || D < 1 || T >= (int64_t(1) << 31) || B > (int64_t(1) << 30) / D)
+    return 0;
+  const int vec = 4 / dtype_size(dtype);
+  const bool cut = shape_of(B, T, D, vec, false, true).pieces > 1 || shape_of(B, T, D, vec, true, true).pieces > 1;
+  return cut ? 2 * B * D * ((T + kSpan - 1) / kSpan) : 2;
+}
+
 extern "C" int cpab_b200_gated_scan(int dtype, const void *x, int64_t x_series, int64_t x_sample,
                                     const void *gate, int64_t gate_series, int64_t gate_sample,
                                     int64_t B, int64_t T, int64_t D, const int32_t *lengths,
                                     const float *h0, void *h, float *h_last, float *states,
-                                    cpab_stream_t stream) {
-  const int st = check_scan("gated_scan", dtype, x, gate, B, T, D);
+                                    float *workspace, cpab_stream_t stream) {
+  const int st = check_scan("gated_scan", dtype, x, x_series, x_sample, gate, gate_series, gate_sample, B, T, D);
   if (st != CPAB_OK) return st;
   if (B == 0 || D == 0) return launch_status(cudaSuccess, "");
   if (T == 0) {  // no samples: the state is what it was
@@ -429,16 +891,16 @@ extern "C" int cpab_b200_gated_scan(int dtype, const void *x, int64_t x_series, 
                                        : cudaMemsetAsync(h_last, 0, bytes, stream), "gated_scan");
   }
   if (h == nullptr) return report_error(CPAB_ERR_ARG, "gated_scan: null output pointer");
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
+    return report_error(CPAB_ERR_ARG, "gated_scan: null or misaligned workspace");
   ScanArgs a{};
   a.x = x, a.gate = gate, a.xb = x_series, a.xt = x_sample, a.gb = gate_series, a.gt = gate_sample;
   a.T = T, a.D = D, a.lengths = lengths, a.h0 = h0, a.h = h, a.last = h_last, a.states = states;
-  const int e = dtype_size(dtype);
-  const bool pairs = D % 2 == 0 && aligned_to(x, x_series, e, 2 * e) && aligned_to(x, x_sample, e, 2 * e) &&
-                     aligned_to(gate, gate_series, e, 2 * e) && aligned_to(gate, gate_sample, e, 2 * e) &&
-                     aligned_to(h, 0, e, 2 * e);
-  const cudaError_t err = dtype == CPAB_F32   ? scan_as<float>(a, B, pairs, stream)
-                          : dtype == CPAB_F16 ? scan_as<__half>(a, B, pairs, stream)
-                                              : scan_as<__nv_bfloat16>(a, B, pairs, stream);
+  a.totals = reinterpret_cast<float2 *>(workspace);
+  set_places(a, B, dtype_size(dtype));
+  const cudaError_t err = dtype == CPAB_F32   ? scan_as<float, false>(a, B, stream)
+                          : dtype == CPAB_F16 ? scan_as<__half, false>(a, B, stream)
+                                              : scan_as<__nv_bfloat16, false>(a, B, stream);
   return launch_status(err, "gated_scan");
 }
 
@@ -447,8 +909,10 @@ extern "C" int cpab_b200_gated_scan_backward(
     int64_t gate_series, int64_t gate_sample, int64_t B, int64_t T, int64_t D,
     const int32_t *lengths, const float *states, const void *grad_h, const float *grad_last,
     void *grad_x, int64_t grad_x_series, int64_t grad_x_sample, void *grad_gate,
-    int64_t grad_gate_series, int64_t grad_gate_sample, float *grad_h0, cpab_stream_t stream) {
-  const int st = check_scan("gated_scan_backward", dtype, x, gate, B, T, D);
+    int64_t grad_gate_series, int64_t grad_gate_sample, float *grad_h0, float *workspace,
+    cpab_stream_t stream) {
+  const int st = check_scan("gated_scan_backward", dtype, x, x_series, x_sample, gate, gate_series, gate_sample, B, T,
+                            D);
   if (st != CPAB_OK) return st;
   if (B == 0 || D == 0) return launch_status(cudaSuccess, "");
   if (T == 0) {
@@ -460,22 +924,18 @@ extern "C" int cpab_b200_gated_scan_backward(
   }
   if (states == nullptr || grad_x == nullptr || grad_gate == nullptr)
     return report_error(CPAB_ERR_ARG, "gated_scan_backward: null states or gradient pointer");
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
+    return report_error(CPAB_ERR_ARG, "gated_scan_backward: null or misaligned workspace");
   ScanArgs a{};
   a.x = x, a.gate = gate, a.xb = x_series, a.xt = x_sample, a.gb = gate_series, a.gt = gate_sample;
   a.T = T, a.D = D, a.lengths = lengths, a.states = const_cast<float *>(states);
   a.grad_h = grad_h, a.grad_last = grad_last, a.grad_x = grad_x, a.grad_gate = grad_gate;
   a.dxb = grad_x_series, a.dxt = grad_x_sample, a.dgb = grad_gate_series, a.dgt = grad_gate_sample;
-  a.grad_h0 = grad_h0;
-  const int e = dtype_size(dtype);
-  const bool pairs = D % 2 == 0 && aligned_to(x, x_series, e, 2 * e) && aligned_to(x, x_sample, e, 2 * e) &&
-                     aligned_to(gate, gate_series, e, 2 * e) && aligned_to(gate, gate_sample, e, 2 * e) &&
-                     aligned_to(grad_h, 0, e, 2 * e) &&
-                     aligned_to(grad_x, grad_x_series, e, 2 * e) && aligned_to(grad_x, grad_x_sample, e, 2 * e) &&
-                     aligned_to(grad_gate, grad_gate_series, e, 2 * e) &&
-                     aligned_to(grad_gate, grad_gate_sample, e, 2 * e);
-  const cudaError_t err = dtype == CPAB_F32   ? scan_backward_as<float>(a, B, pairs, stream)
-                          : dtype == CPAB_F16 ? scan_backward_as<__half>(a, B, pairs, stream)
-                                              : scan_backward_as<__nv_bfloat16>(a, B, pairs, stream);
+  a.grad_h0 = grad_h0, a.totals = reinterpret_cast<float2 *>(workspace);
+  set_places(a, B, dtype_size(dtype));
+  const cudaError_t err = dtype == CPAB_F32   ? scan_as<float, true>(a, B, stream)
+                          : dtype == CPAB_F16 ? scan_as<__half, true>(a, B, stream)
+                                              : scan_as<__nv_bfloat16, true>(a, B, stream);
   return launch_status(err, "gated_scan_backward");
 }
 
@@ -483,7 +943,7 @@ extern "C" int cpab_b200_gated_scan_step(int dtype, const void *x, int64_t x_row
                                          int64_t gate_row, int64_t B, int64_t D,
                                          const int32_t *slots, int64_t rows, float *state, void *h,
                                          cpab_stream_t stream) {
-  const int st = check_scan("gated_scan_step", dtype, x, gate, B, 1, D);
+  const int st = check_scan("gated_scan_step", dtype, x, x_row, 0, gate, gate_row, 0, B, 1, D);
   if (st != CPAB_OK) return st;
   if (rows < 0 || (slots == nullptr && rows < B))
     return report_error(CPAB_ERR_ARG, "gated_scan_step: %lld state rows for %lld streams",

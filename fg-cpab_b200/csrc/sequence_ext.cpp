@@ -107,6 +107,10 @@ void check_scan(const Tensor &x, const Tensor &gate, const Tensor &h0, const Ten
   if (lengths.defined()) require(lengths, x, at::kInt, {x.size(0)}, "lengths");
 }
 
+Tensor scan_workspace(const ScanInput &s) {
+  return at::empty({cpab_b200_gated_scan_workspace(s.dtype, s.B, s.T, s.D)}, s.x.options().dtype(at::kFloat));
+}
+
 struct ScanOutput {
   Tensor h, last, states;
 };
@@ -122,9 +126,10 @@ ScanOutput scan_forward(const ScanInput &s, const Tensor &h0, const Tensor &leng
   }
   const Tensor start = h0.defined() ? h0.contiguous() : h0;
   const Tensor len = lengths.defined() ? lengths.contiguous() : lengths;
+  const Tensor work = scan_workspace(s);
   check(cpab_b200_gated_scan(s.dtype, s.xp, s.xb, s.xt, s.gp, s.gb, s.gt, s.B, s.T, s.D,
                              static_cast<const int32_t *>(ptr(len)), fptr(start), ptr_mut(o.h),
-                             fptr_mut(o.last), fptr_mut(o.states), stream_of(s.x)));
+                             fptr_mut(o.last), fptr_mut(o.states), fptr_mut(work), stream_of(s.x)));
   return o;
 }
 
@@ -160,10 +165,11 @@ class ScanFunction : public torch::autograd::Function<ScanFunction> {
     const Tensor &dg = gate.defined() ? dgate : dx;
     const Tensor dh0 = ctx->saved_data["want_h0"].toBool()
                            ? at::empty({s.B, s.D}, x.options().dtype(at::kFloat)) : Tensor();
+    const Tensor work = scan_workspace(s);
     check(cpab_b200_gated_scan_backward(
         s.dtype, s.xp, s.xb, s.xt, s.gp, s.gb, s.gt, s.B, s.T, s.D,
         static_cast<const int32_t *>(ptr(len)), fptr(states), ptr(dh), fptr(dlast), ptr_mut(dx),
-        dx.stride(0), dx.stride(1), dgp, dg.stride(0), dg.stride(1), fptr_mut(dh0), stream_of(x)));
+        dx.stride(0), dx.stride(1), dgp, dg.stride(0), dg.stride(1), fptr_mut(dh0), fptr_mut(work), stream_of(x)));
     return {dx, dgate, dh0, Tensor()};
   }
 };

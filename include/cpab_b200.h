@@ -374,15 +374,20 @@ typedef enum { CPAB_F32 = 0, CPAB_F16 = 1, CPAB_BF16 = 2 } cpab_dtype;
  * their h is 0.  h_last ([B, D] float32, may be NULL) receives the state after
  * the last sample.  states ([B, ceil(T / c), D] float32 with c =
  * cpab_b200_gated_scan_chunk(), may be NULL) receives the states that
- * cpab_b200_gated_scan_backward needs.
+ * cpab_b200_gated_scan_backward needs.  workspace: 8-byte aligned,
+ * cpab_b200_gated_scan_workspace floats.
  */
 int cpab_b200_gated_scan(int dtype, const void *x, int64_t x_series, int64_t x_sample,
                          const void *gate, int64_t gate_series, int64_t gate_sample, int64_t B,
                          int64_t T, int64_t D, const int32_t *lengths, const float *h0, void *h,
-                         float *h_last, float *states, cpab_stream_t stream);
+                         float *h_last, float *states, float *workspace, cpab_stream_t stream);
 
 /* Samples between two states kept by cpab_b200_gated_scan. */
 int cpab_b200_gated_scan_chunk(void);
+
+/* Floats of the workspace of cpab_b200_gated_scan and its backward on the
+ * current device (0 for sizes they refuse). */
+int64_t cpab_b200_gated_scan_workspace(int dtype, int64_t B, int64_t T, int64_t D);
 
 /*
  * Gradient of cpab_b200_gated_scan: grad_x and grad_gate (shaped as x and
@@ -396,7 +401,8 @@ int cpab_b200_gated_scan_backward(int dtype, const void *x, int64_t x_series, in
                                   const float *states, const void *grad_h, const float *grad_last,
                                   void *grad_x, int64_t grad_x_series, int64_t grad_x_sample,
                                   void *grad_gate, int64_t grad_gate_series,
-                                  int64_t grad_gate_sample, float *grad_h0, cpab_stream_t stream);
+                                  int64_t grad_gate_sample, float *grad_h0, float *workspace,
+                                  cpab_stream_t stream);
 
 /*
  * One sample of B streams: state row slots[b] (slots NULL: row b) of the

@@ -26,8 +26,8 @@ def call(fn, base, **kw):
 
 def test_scan_entry_points_validate():
     L = _native.lib()
-    # dtype, x, strides, gate, strides, B, T, D, lengths, h0, h, last, states, stream
-    ok = [2, P, 64, 8, P, 64, 8, 2, 8, 8, None, None, P, P, P, None]
+    # dtype, x, strides, gate, strides, B, T, D, lengths, h0, h, last, states, workspace, stream
+    ok = [2, P, 64, 8, P, 64, 8, 2, 8, 8, None, None, P, P, P, P, None]
     f = L.cpab_b200_gated_scan
     assert call(f, ok, a0=3) == -1 and "dtype" in err()
     assert call(f, ok, a1=None) == -1 and "null" in err()
@@ -36,14 +36,18 @@ def test_scan_entry_points_validate():
     assert call(f, ok, a8=1 << 31) == -4 and "2^31" in err()
     assert call(f, ok, a7=1 << 20, a9=1 << 11) == -4 and "2^30" in err()
     assert call(f, ok, a12=None) == -1 and "output" in err()
+    assert call(f, ok, a15=None) == -1 and "workspace" in err()
+    assert call(f, ok, a15=ctypes.c_void_p(4100)) == -1
     assert call(f, ok, a7=0) == 0 and err() == ""
     assert call(f, ok, a8=0, a13=None) == 0            # no samples, no state wanted
-    # ..., lengths, states, grad_h, grad_last, grad_x, strides, grad_gate, strides, grad_h0, stream
-    okb = [2, P, 64, 8, P, 64, 8, 2, 8, 8, None, P, P, P, P, 64, 8, P, 64, 8, P, None]
+    # ..., lengths, states, grad_h, grad_last, grad_x, strides, grad_gate, strides, grad_h0, workspace,
+    # stream
+    okb = [2, P, 64, 8, P, 64, 8, 2, 8, 8, None, P, P, P, P, 64, 8, P, 64, 8, P, P, None]
     g = L.cpab_b200_gated_scan_backward
     assert call(g, okb, a11=None) == -1 and "states" in err()
     assert call(g, okb, a14=None) == -1 and call(g, okb, a17=None) == -1
     assert call(g, okb, a0=-1) == -1
+    assert call(g, okb, a21=None) == -1 and "workspace" in err()
     assert call(g, okb, a9=0) == 0
     # dtype, x, row, gate, row, B, D, slots, rows, state, h, stream
     oks = [0, P, 8, P, 8, 2, 8, None, 2, P, P, None]
@@ -52,6 +56,8 @@ def test_scan_entry_points_validate():
     assert call(s, oks, a9=None) == -1 and call(s, oks, a10=None) == -1
     assert call(s, oks, a5=0) == 0
     assert L.cpab_b200_gated_scan_chunk() > 0
+    assert L.cpab_b200_gated_scan_workspace(2, 3, 100, 64) > 0
+    assert L.cpab_b200_gated_scan_workspace(2, 3, 1 << 31, 64) == 0
 
 
 def test_norm_entry_points_validate():
