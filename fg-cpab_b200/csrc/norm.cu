@@ -16,6 +16,8 @@
 // result every run; no atomics).
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "sequence.cuh"
 
 namespace cpab {
@@ -23,8 +25,10 @@ namespace {
 
 constexpr int kBlock = 256;        // threads of a block whose rows take fewer
 constexpr int kMost = 512;         // threads of a row at most
+constexpr int kResident = 768;     // threads of an SM that the gradient's registers leave room for
 constexpr int64_t kMaxWidth = 16384;
 constexpr float kE4m3Max = 448.0f;
+constexpr float kTiny = 1.17549435e-38f;  // 2^-126, the smallest scale
 
 struct NormArgs {
   const void *x, *res;
@@ -41,202 +45,393 @@ struct NormArgs {
   const void *dy, *gs;     // [rows, D]; gs null when none flows into s
   void *dx, *dres;         // dres null when dx's type is the stream's
   float *partial;          // [blocks, D]
-  int threads;             // of a row
+  int threads_log2;        // of a row
+  float inverse;           // 1 / D
 };
 
-// Sum (or maximum) over the `n` threads (a power of two) that share a row.
-template <bool MAX>
-__device__ __forceinline__ float over_row(float v, int n, float *shared) {
-  const int width = n < 32 ? n : 32;
-  for (int o = width / 2; o > 0; o >>= 1) {
-    const float u = __shfl_xor_sync(~0u, v, o);
-    if (MAX) asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(v), "f"(u));
-    else v += u;
+// Sum of `sum` (and maximum of `top`) over the 2^log2 threads that share a row.
+// `shared` is another half for every second row, so one barrier a row is enough.
+template <bool TOP>
+__device__ __forceinline__ void over_row(float &sum, float &top, int log2, float *shared) {
+  for (int o = log2 < 5 ? (1 << log2) >> 1 : 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(~0u, sum, o);
+    if (TOP) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
   }
-  if (n <= 32) return v;
-  const int warp = threadIdx.x >> 5, first = (threadIdx.x / n) * (n >> 5);
-  if ((threadIdx.x & 31) == 0) shared[warp] = v;
-  __syncthreads();
-  v = shared[first];
-  for (int k = 1; k < n >> 5; ++k) {
-    const float u = shared[first + k];
-    if (MAX) asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(v), "f"(u));
-    else v += u;
+  if (log2 <= 5) return;
+  constexpr int kWarps = kMost / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = 1 << (log2 - 5);
+  if (lane == 0) {
+    shared[warp] = sum;
+    if (TOP) shared[kWarps + warp] = top;
   }
   __syncthreads();
-  return v;
+  const int from = (warp & -warps) + (lane & (warps - 1));
+  sum = shared[from];
+  if (TOP) top = shared[kWarps + from];
+  for (int o = warps >> 1; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(~0u, sum, o);
+    if (TOP) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  }
 }
 
-// VEC consecutive elements as loaded: half the registers of their float32
-// values where T has 16 bits.
+// VEC consecutive elements as they lie in memory: words of one float32 or two
+// 16-bit elements (VEC 1: one element's bits).
 template <typename T, int VEC>
 struct Row {
-  static constexpr int N = sizeof(T) * VEC > 16 ? 16 / sizeof(T) : VEC;  // at most 16 bytes at a time
-  Pack<T, N> part[VEC / N];
-  __device__ __forceinline__ void load(const void *base, int64_t at) {
+  static constexpr int kPer = VEC == 1 ? 1 : 4 / (int)sizeof(T), kWords = VEC / kPer;
+  static constexpr int N = kWords > 4 ? 4 : kWords;  // words of an access
+  uint32_t w[kWords];
+  using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+
+  __device__ __forceinline__ void load(const T *at) {
+    if (VEC == 1) {
+      w[0] = *reinterpret_cast<const Bits *>(at);
+      return;
+    }
 #pragma unroll
-    for (int k = 0; k < VEC / N; ++k)
-      part[k] = *reinterpret_cast<const Pack<T, N> *>(static_cast<const T *>(base) + at + k * N);
+    for (int k = 0; k < kWords; k += N) {
+      const Pack<uint32_t, N> p = *reinterpret_cast<const Pack<uint32_t, N> *>(at + k * kPer);
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[k + i] = p.v[i];
+    }
   }
-  __device__ __forceinline__ float operator[](int i) const { return to_f32(part[i / N].v[i % N]); }
+  __device__ __forceinline__ void store(T *at) const {
+    if (VEC == 1) {
+      *reinterpret_cast<Bits *>(at) = (Bits)w[0];
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < kWords; k += N) {
+      Pack<uint32_t, N> p;
+#pragma unroll
+      for (int i = 0; i < N; ++i) p.v[i] = w[k + i];
+      *reinterpret_cast<Pack<uint32_t, N> *>(at + k * kPer) = p;
+    }
+  }
+  // Elements lo .. hi - 1 one by one, zeros around them.
+  __device__ __forceinline__ void load_some(const T *at, int lo, int hi) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i >= lo && i < hi) w[i / kPer] |= (uint32_t)reinterpret_cast<const Bits *>(at)[i] << (16 * (i % kPer));
+  }
+  __device__ __forceinline__ void store_some(T *at, int lo, int hi) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i >= lo && i < hi) reinterpret_cast<Bits *>(at)[i] = (Bits)(w[i / kPer] >> (16 * (i % kPer)));
+  }
+  __device__ __forceinline__ void zero_outside(int lo, int hi) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i < lo || i >= hi) w[i / kPer] &= kPer == 2 ? 0xFFFF0000u >> (16 * (i % 2)) : 0u;
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (VEC == 1) {
+      return unpack_pair<T>(w[0]).x;
+    } else {
+      return i % 2 ? unpack_pair<T>(w[i / 2]).y : unpack_pair<T>(w[i / 2]).x;
+    }
+  }
+  __device__ __forceinline__ void set(const float (&f)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+      else if constexpr (VEC == 1) w[0] = pack_pair<T>(f[0], 0.0f);
+      else w[i] = pack_pair<T>(f[2 * i], f[2 * i + 1]);
+    }
+  }
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_f32(const void *base, int64_t at, float (&out)[VEC]) {
+// The stream's new value x + residual, rounded to its type.
+template <typename T, typename S, int VEC>
+__device__ __forceinline__ void add_to(Row<S, VEC> &res, const Row<T, VEC> &x) {
+  if constexpr (sizeof(S) == 2) {
+#pragma unroll
+    for (int i = 0; i < Row<S, VEC>::kWords; ++i) res.w[i] = add_pair<S>(x.w[i], res.w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) res.w[i] = __float_as_uint(x[i] + res[i]);
+  }
+}
+
+// A thread's vector of a row: elements lo .. hi - 1 of the vector are columns
+// c + lo .. c + hi - 1 of the row (all of them, or with EDGE fewer at a row's
+// ends).
+struct Span {
+  int c, lo, hi;
+  __device__ __forceinline__ bool any() const { return hi > lo; }
+};
+
+// Where rows do not begin on a vector, all tensors' rows begin as many elements
+// (`shift`) after one, and the vectors that hold a row are taken as they lie:
+// those at its ends hold elements of the rows beside it too, which are masked.
+// Only past the last row there may be nothing to read.
+template <typename T, int VEC, bool EDGE>
+__device__ __forceinline__ void load_span(Row<T, VEC> &r, const T *row, const Span &s, bool last) {
+  if (!EDGE || (s.lo == 0 && s.hi == VEC)) {
+    r.load(row + s.c);
+  } else if (!last || s.hi == VEC) {
+    r.load(row + s.c);
+    r.zero_outside(s.lo, s.hi);
+  } else {
+    r.load_some(row + s.c, s.lo, s.hi);
+  }
+}
+
+template <typename T, int VEC, bool EDGE>
+__device__ __forceinline__ void store_span(T *row, const Span &s, const Row<T, VEC> &r) {
+  if (!EDGE || (s.lo == 0 && s.hi == VEC)) r.store(row + s.c);
+  else r.store_some(row + s.c, s.lo, s.hi);
+}
+
+template <typename T, int VEC, bool EDGE>
+__device__ __forceinline__ void store_span(T *row, const Span &s, const float (&in)[VEC]) {
   Row<T, VEC> r;
-  r.load(base, at);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) out[i] = r[i];
+  r.set(in);
+  store_span<T, VEC, EDGE>(row, s, r);
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void store_f32(void *base, int64_t at, const float (&in)[VEC]) {
-  constexpr int N = sizeof(T) * VEC > 16 ? 16 / sizeof(T) : VEC;
+template <typename T, int VEC, bool EDGE>
+__device__ __forceinline__ void load_weight(const NormArgs &p, const Span &s, float (&w)[VEC]) {
+  if (!EDGE) {
+    if (p.w_f32) {
+      Row<float, VEC> r;
+      r.load(static_cast<const float *>(p.w) + s.c);
 #pragma unroll
-  for (int k = 0; k < VEC; k += N) {
-    Pack<T, N> p;
+      for (int i = 0; i < VEC; ++i) w[i] = r[i];
+    } else {
+      Row<T, VEC> r;
+      r.load(static_cast<const T *>(p.w) + s.c);
 #pragma unroll
-    for (int i = 0; i < N; ++i) p.v[i] = from_f32<T>(in[k + i]);
-    *reinterpret_cast<Pack<T, N> *>(static_cast<T *>(base) + at + k) = p;
+      for (int i = 0; i < VEC; ++i) w[i] = r[i];
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    w[i] = 0.0f;
+    if (i >= s.lo && i < s.hi)
+      w[i] = p.w_f32 ? static_cast<const float *>(p.w)[s.c + i] : to_f32(static_cast<const T *>(p.w)[s.c + i]);
   }
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_weight(const NormArgs &p, int64_t at, float (&w)[VEC]) {
-  if (p.w_f32) load_f32<float, VEC>(p.w, at, w);
-  else load_f32<T, VEC>(p.w, at, w);
+// Vector v of a row of D columns that begins `shift` elements into one.
+template <int VEC, bool EDGE>
+__device__ __forceinline__ Span span_of(int v, int shift, int D) {
+  Span s;
+  s.c = v * VEC - (EDGE ? shift : 0);
+  s.lo = EDGE ? max(0, -s.c) : 0;
+  s.hi = EDGE ? max(0, min(VEC, D - s.c)) : (s.c < D ? VEC : 0);
+  return s;
 }
 
-// T: x and y; S: the stream.
-template <typename T, typename S, int VEC, int NV, bool QUANT>
-__global__ void __launch_bounds__(kMost) k_norm(NormArgs p) {
-  __shared__ float shared[kMost / 32];
-  const int n = p.threads, j = threadIdx.x % n;
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / n) + threadIdx.x / n;
-  const bool on = row < p.rows;
-  float v[NV][VEC];
-  float sum = 0.0f;
+// Weights of a thread's vectors, kept in registers where its rows all begin
+// alike and they fit, else read from the caches for every row.
+template <typename T, int VEC, int NV, bool EDGE, bool KEEP>
+struct Weights {
+  float kept[KEEP ? NV : 1][VEC];
+  __device__ __forceinline__ Weights(const NormArgs &p, int log2, int j, int shift) {
+    if (!KEEP) return;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int64_t c = (int64_t)(k * n + j) * VEC;
-    if (on && c < p.D) {
-      load_f32<T, VEC>(p.x, row * p.xs + c, v[k]);
-      if (p.res != nullptr) {
-        float r[VEC];
-        load_f32<S, VEC>(p.res, row * p.rs + c, r);
+    for (int k = 0; k < NV; ++k) load_weight<T, VEC, EDGE>(p, span_of<VEC, EDGE>((k << log2) + j, shift, (int)p.D), kept[k]);
+  }
+  __device__ __forceinline__ const float (&of(const NormArgs &p, int k, const Span &at))[VEC] {
+    if (!KEEP) load_weight<T, VEC, EDGE>(p, at, kept[0]);
+    return kept[KEEP ? k : 0];
+  }
+};
+
+// T: x and y; S: the stream.  With EDGE blocks stride over rows so that a
+// thread's rows have one shift.
+template <typename T, typename S, int VEC, int NV, bool QUANT, bool EDGE>
+__global__ void __launch_bounds__(kMost) k_norm(const __grid_constant__ NormArgs p) {
+  __shared__ float shared[2][2 * kMost / 32];
+  const int log2 = p.threads_log2, j = threadIdx.x & ((1 << log2) - 1), groups = blockDim.x >> log2;
+  const int D = (int)p.D;
+  int64_t row = (int64_t)blockIdx.x * groups + (threadIdx.x >> log2);
+  const int shift = EDGE ? (int)(row * p.D % VEC) : 0;
+  Weights<T, VEC, NV, EDGE, EDGE && NV * VEC <= 24> weights(p, log2, j, shift);
+  int half = 0;
+  // (as many rounds for each of the block's rows: the sums wait for one another)
+  for (int64_t first = (int64_t)blockIdx.x * groups; first < p.rows; first += (int64_t)gridDim.x * groups) {
+    const bool on = row < p.rows, last = row == p.rows - 1;
+    const T *x = static_cast<const T *>(p.x) + row * p.xs;
+    const S *res = static_cast<const S *>(p.res) + row * p.rs;
+    Row<S, VEC> v[QUANT ? 1 : NV];  // the stream as it is kept
+    float t[QUANT ? NV : 1][VEC];   // or times the weights
+    float sum = 0.0f, top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[k][i] = to_f32(from_f32<S>(v[k][i] + r[i]));
-        store_f32<S, VEC>(p.s, row * p.D + c, v[k]);
+    for (int k = 0; k < NV; ++k) {
+      const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
+      if (on && at.any()) {
+        Row<S, VEC> &s = v[QUANT ? 0 : k];
+        Row<T, VEC> in;
+        load_span<T, VEC, EDGE>(in, x, at, last);
+        if (p.res != nullptr) {
+          load_span<S, VEC, EDGE>(s, res, at, last);
+          add_to(s, in);
+          store_span<S, VEC, EDGE>(static_cast<S *>(p.s) + row * p.D, at, s);
+        } else if constexpr (sizeof(T) == sizeof(S)) {
+#pragma unroll
+          for (int i = 0; i < Row<S, VEC>::kWords; ++i) s.w[i] = in.w[i];
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum = fmaf(s[i], s[i], sum);
+        if (QUANT) {
+          const float (&w)[VEC] = weights.of(p, k, at);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            t[k][i] = s[i] * w[i];
+            top = fmaxf(top, fabsf(t[k][i]));
+          }
+        }
       }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) sum = fmaf(v[k][i], v[k][i], sum);
     }
-  }
-  const float mean = over_row<false>(sum, n, shared) / (float)p.D;
-  const float r = rsqrtf(mean + p.eps);
-  if (on && p.r != nullptr && j == 0) p.r[row] = r;
-  float top = 0.0f;
+    over_row<QUANT>(sum, top, log2, shared[half]);
+    half ^= 1;
+    const float r = rsqrtf(fmaf(sum, p.inverse, p.eps));
+    if (on && p.r != nullptr && j == 0) p.r[row] = r;
+    if (!QUANT) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int64_t c = (int64_t)(k * n + j) * VEC;
-    if (on && c < p.D) {
-      float w[VEC];
-      load_weight<T, VEC>(p, c, w);
+      for (int k = 0; k < NV; ++k) {
+        const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
+        if (on && at.any()) {
+          const float (&w)[VEC] = weights.of(p, k, at);
+          float y[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        v[k][i] = v[k][i] * r * w[i];
-        if (QUANT) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(fabsf(v[k][i])));
+          for (int i = 0; i < VEC; ++i) y[i] = v[k][i] * r * w[i];
+          store_span<T, VEC, EDGE>(static_cast<T *>(p.y) + row * p.D, at, y);
+        }
       }
-      if (!QUANT) store_f32<T, VEC>(p.y, row * p.D + c, v[k]);
-    }
-  }
-  if (!QUANT) return;
-  // Never zero: a row of zeros has codes 0, and a reader may divide by it.
-  float scale = over_row<true>(top, n, shared) * (1.0f / kE4m3Max);
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(scale) : "f"(scale), "f"(1.17549435e-38f));
-  if (on && j == 0) p.scale[row] = scale;
+    } else {
+      // y = t r: its codes are those of t over the largest |t|, so r (and its
+      // rounding) does not enter them.  The scale is never 0: a row of zeros
+      // has codes 0, and a reader may divide by it.  A NaN in the row is in r.
+      const float unit = top * (1.0f / kE4m3Max), scale = unit * r < kTiny ? kTiny : unit * r;
+      const bool usual = unit >= kTiny && scale > kTiny;  // (and so 1 / unit in float32's range)
+      const float factor = usual ? 1.0f / unit : r;
+      if (on && j == 0) p.scale[row] = scale;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int64_t c = (int64_t)(k * n + j) * VEC;
-    if (on && c < p.D) {
-      Pack<uint8_t, VEC> q;
+      for (int k = 0; k < NV; ++k) {
+        const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
+        if (on && at.any()) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        q.v[i] = __nv_cvt_float_to_fp8(v[k][i] / scale, __NV_SATFINITE, __NV_E4M3);
-      *reinterpret_cast<Pack<uint8_t, VEC> *>(p.q + row * p.D + c) = q;
+          for (int i = 0; i < VEC; ++i) t[k][i] *= factor;
+          if (!usual) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) t[k][i] /= scale;
+          }
+          uint8_t *q = p.q + row * p.D + at.c;
+          if (VEC > 1 && (!EDGE || (at.lo == 0 && at.hi == VEC))) {
+            using Codes = Pack<uint16_t, (VEC + 1) / 2>;
+            Codes c;
+#pragma unroll
+            for (int i = 0; i + 1 < VEC; i += 2)
+              c.v[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(t[k][i], t[k][i + 1]), __NV_SATFINITE, __NV_E4M3);
+            *reinterpret_cast<Codes *>(q) = c;
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+              if (i >= at.lo && i < at.hi) q[i] = __nv_cvt_float_to_fp8(t[k][i], __NV_SATFINITE, __NV_E4M3);
+          }
+        }
+      }
     }
+    row += (int64_t)gridDim.x * groups;
   }
 }
 
 // x here is the stream s as kept (x itself without a residual), of type S.
-template <typename T, typename S, int VEC, int NV>
-__global__ void __launch_bounds__(kMost) k_norm_backward(NormArgs p) {
-  __shared__ float shared[kMost / 32];
-  const int n = p.threads, j = threadIdx.x % n, group = threadIdx.x / n, groups = blockDim.x / n;
+// With t = dy r: dw = sum t s, ds = gs + t w - s (r^2 mean(t w s)).
+template <typename T, typename S, int VEC, int NV, bool EDGE, int BLOCK>
+__global__ void __launch_bounds__(BLOCK, NV * VEC <= 16 ? kResident / BLOCK : 512 / BLOCK)
+    k_norm_backward(const __grid_constant__ NormArgs p) {
+  // Of wide rows a thread holds too much to fetch gs early.
+  constexpr bool kLean = NV * VEC > 16;
+  extern __shared__ float sums[];  // [groups, D] where a block has several groups
+  __shared__ float shared[2][kMost / 32];
+  const int log2 = p.threads_log2, j = threadIdx.x & ((1 << log2) - 1), groups = BLOCK >> log2;
+  const int group = threadIdx.x >> log2, D = (int)p.D;
+  int64_t row = (int64_t)blockIdx.x * groups + group;
+  const int shift = EDGE ? (int)(row * p.D % VEC) : 0;
+  Weights<T, VEC, NV, EDGE, EDGE && NV * VEC <= 8> weights(p, log2, j, shift);
   float dw[NV][VEC];
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[k][i] = 0.0f;
+  int half = 0;
   for (int64_t first = (int64_t)blockIdx.x * groups; first < p.rows; first += (int64_t)gridDim.x * groups) {
-    const int64_t row = first + group;
-    const bool on = row < p.rows;
-    const float r = on ? p.r[row] : 0.0f;
-    Row<S, VEC> v[NV];
+    const bool on = row < p.rows, last = row == p.rows - 1;
+    const S *x = static_cast<const S *>(p.x) + row * p.xs, *gs = static_cast<const S *>(p.gs) + row * p.D;
+    const T *dy = static_cast<const T *>(p.dy) + row * p.D;
+    Row<S, VEC> v[NV], a[kLean ? 1 : NV];
     Row<T, VEC> g[NV];
-    float sum = 0.0f;
+    const float r = on ? p.r[row] : 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t)(k * n + j) * VEC;
-      if (on && c < p.D) {
-        v[k].load(p.x, row * p.xs + c);
-        g[k].load(p.dy, row * p.D + c);
+      const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
+      if (on && at.any()) {
+        load_span<S, VEC, EDGE>(v[k], x, at, last);
+        load_span<T, VEC, EDGE>(g[k], dy, at, last);
+        if (!kLean && p.gs != nullptr) load_span<S, VEC, EDGE>(a[k], gs, at, last);
       }
     }
+    float tw[NV][VEC];
+    float sum = 0.0f, none = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t)(k * n + j) * VEC;
-      if (on && c < p.D) {
-        float w[VEC];
-        load_weight<T, VEC>(p, c, w);
+      const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
+      if (on && at.any()) {
+        const float (&w)[VEC] = weights.of(p, k, at);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float gi = g[k][i], vi = v[k][i];
-          dw[k][i] = fmaf(gi, vi * r, dw[k][i]);
-          sum = fmaf(gi * w[i], vi, sum);
+          const float t = g[k][i] * r, s = v[k][i];
+          dw[k][i] = fmaf(t, s, dw[k][i]);
+          tw[k][i] = t * w[i];
+          sum = fmaf(tw[k][i], s, sum);
         }
       }
     }
-    const float m = over_row<false>(sum, n, shared) / (float)p.D * (r * r);
+    over_row<false>(sum, none, log2, shared[half]);
+    half ^= 1;
+    const float m = -sum * p.inverse * (r * r);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t)(k * n + j) * VEC;
-      if (on && c < p.D) {
-        float w[VEC], d[VEC];
-        load_weight<T, VEC>(p, c, w);
+      const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
+      if (on && at.any()) {
+        if (kLean && p.gs != nullptr) load_span<S, VEC, EDGE>(a[0], gs, at, last);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) d[i] = r * (g[k][i] * w[i] - v[k][i] * m);
+        for (int i = 0; i < VEC; ++i) tw[k][i] = fmaf(v[k][i], m, tw[k][i]);
         if (p.gs != nullptr) {
-          float a[VEC];
-          load_f32<S, VEC>(p.gs, row * p.D + c, a);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) d[i] += a[i];
+          for (int i = 0; i < VEC; ++i) tw[k][i] += a[kLean ? 0 : k][i];
         }
-        store_f32<T, VEC>(p.dx, row * p.D + c, d);
-        if (p.dres != nullptr) store_f32<S, VEC>(p.dres, row * p.D + c, d);
+        store_span<T, VEC, EDGE>(static_cast<T *>(p.dx) + row * p.D, at, tw[k]);
+        if (p.dres != nullptr) store_span<S, VEC, EDGE>(static_cast<S *>(p.dres) + row * p.D, at, tw[k]);
       }
     }
+    row += (int64_t)gridDim.x * groups;
   }
   if (p.partial == nullptr) return;
   // The block's groups hold the same columns: added one after another.
+  float *to = groups > 1 ? sums + group * D : p.partial + (int64_t)blockIdx.x * D;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int64_t c = (int64_t)(k * n + j) * VEC;
+    const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      if (c < p.D)
-        p.partial[((int64_t)blockIdx.x * groups + group) * p.D + c + i] = dw[k][i];
-    }
+    for (int i = 0; i < VEC; ++i)
+      if (i >= at.lo && i < at.hi) to[at.c + i] = dw[k][i];
+  }
+  if (groups == 1) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < D; c += BLOCK) {
+    float s = 0.0f;
+    for (int k = 0; k < groups; ++k) s += sums[k * D + c];
+    p.partial[(int64_t)blockIdx.x * D + c] = s;
   }
 }
 
@@ -258,91 +453,116 @@ __global__ void __launch_bounds__(1024) k_norm_weight(const float *partial, int6
 }
 
 // A row's vectors and threads: enough threads (a power of two) that each holds
-// at most `most` vectors.
+// at most `held` vectors; one more vector where rows begin inside one.
 struct Shape {
-  int threads, block;
+  int threads_log2, block, groups;
   int per;            // vectors a thread holds
 };
 
-Shape shape_of(int64_t D, int vec, int most) {
-  const int64_t vectors = (D + vec - 1) / vec;
+constexpr int kHeld = 3, kHeldBackward = 2;
+
+Shape shape_of(int64_t D, int vec, bool edge, int held) {
+  const int64_t vectors = (D + vec - 1 + (edge ? vec - 1 : 0)) / vec;
   Shape s;
-  s.threads = 1;
-  while (s.threads < kMost && (int64_t)s.threads * most < vectors) s.threads *= 2;
-  s.per = (int)((vectors + s.threads - 1) / s.threads);
-  s.block = s.threads < kBlock ? kBlock : s.threads;
+  s.threads_log2 = 0;
+  while (1 << s.threads_log2 < kMost && (int64_t)held << s.threads_log2 < vectors) ++s.threads_log2;
+  const int threads = 1 << s.threads_log2;
+  s.per = (int)((vectors + threads - 1) / threads);
+  s.block = threads < kBlock ? kBlock : threads;
+  s.groups = s.block / threads;
   return s;
 }
 
-constexpr int most_of(int vec) { return vec > 1 ? 2 : 4; }
-
-int64_t backward_rows(int64_t rows, const Shape &s) {
-  const int groups = s.block / s.threads;
-  const int64_t want = (rows + groups - 1) / groups;
-  const int64_t cap = 148 * 2;
-  return (want < cap ? want : cap) * groups;
+// Blocks for all rows; of the gradient as many as run at once (each keeps a sum
+// of the weight's gradient); with EDGE a few times as many, so that each keeps
+// its weights for some rows, and so many that a thread's next row begins where
+// its last one did.
+int64_t blocks_of(int64_t rows, const Shape &s, int vec, bool edge, bool resident) {
+  int64_t n = (rows + s.groups - 1) / s.groups;
+  const int64_t cap = (int64_t)device_info().sm_count * ((resident ? kResident : 4096) / s.block);
+  if ((resident || edge) && n > cap) n = cap;
+  if (edge && n * s.groups < rows) {
+    const int64_t step = s.groups >= vec ? 1 : vec / s.groups;
+    n = (n + step - 1) / step * step;
+  }
+  return n;
 }
 
-template <typename T, typename S, int VEC, int NV>
+template <typename T, typename S, int VEC, int NV, bool EDGE>
 cudaError_t norm_launch(const NormArgs &a, const Shape &s, bool quant, cudaStream_t stream) {
-  const int groups = s.block / s.threads;
-  const unsigned grid = (unsigned)((a.rows + groups - 1) / groups);
-  if (quant) k_norm<T, S, VEC, NV, true><<<grid, s.block, 0, stream>>>(a);
-  else k_norm<T, S, VEC, NV, false><<<grid, s.block, 0, stream>>>(a);
+  const unsigned grid = (unsigned)blocks_of(a.rows, s, VEC, EDGE, false);
+  if (quant) k_norm<T, S, VEC, NV, true, EDGE><<<grid, s.block, 0, stream>>>(a);
+  else k_norm<T, S, VEC, NV, false, EDGE><<<grid, s.block, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
-template <typename T, typename S, int VEC, int NV>
+template <typename T, typename S, int VEC, int NV, bool EDGE>
 cudaError_t norm_backward_launch(const NormArgs &a, const Shape &s, cudaStream_t stream) {
-  const unsigned grid = (unsigned)(backward_rows(a.rows, s) / (s.block / s.threads));
-  k_norm_backward<T, S, VEC, NV><<<grid, s.block, 0, stream>>>(a);
+  const unsigned grid = (unsigned)blocks_of(a.rows, s, VEC, EDGE, true);
+  const size_t smem = s.groups > 1 ? (size_t)s.groups * a.D * sizeof(float) : 0;
+  if (s.block == kBlock) k_norm_backward<T, S, VEC, NV, EDGE, kBlock><<<grid, kBlock, smem, stream>>>(a);
+  else k_norm_backward<T, S, VEC, NV, EDGE, kMost><<<grid, kMost, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
-// The kernel for s.per vectors a thread; kMaxWidth / kMost elements at most.
-template <typename T, typename S, int VEC>
+// The kernel for s.per vectors a thread; kMaxWidth / kMost elements at most
+// (and a vector more with EDGE).
+template <typename T, typename S, int VEC, bool EDGE>
 cudaError_t norm_vec(NormArgs a, bool quant, cudaStream_t stream) {
-  const Shape s = shape_of(a.D, VEC, most_of(VEC));
-  constexpr int kAll = (int)(kMaxWidth / kMost) / VEC;
-  a.threads = s.threads;
-  if (s.per <= 1) return norm_launch<T, S, VEC, 1>(a, s, quant, stream);
-  if (s.per <= 2) return norm_launch<T, S, VEC, 2>(a, s, quant, stream);
-  if (s.per <= 4) return norm_launch<T, S, VEC, 4>(a, s, quant, stream);
-  return norm_launch<T, S, VEC, kAll>(a, s, quant, stream);
+  const Shape s = shape_of(a.D, VEC, EDGE, kHeld);
+  constexpr int kAll = (int)(kMaxWidth / kMost) / VEC + (EDGE ? 1 : 0);
+  a.threads_log2 = s.threads_log2;
+  if (s.per <= 1) return norm_launch<T, S, VEC, 1, EDGE>(a, s, quant, stream);
+  if (s.per <= 2) return norm_launch<T, S, VEC, 2, EDGE>(a, s, quant, stream);
+  if (s.per <= 3) return norm_launch<T, S, VEC, 3, EDGE>(a, s, quant, stream);
+  if (s.per <= 4) return norm_launch<T, S, VEC, 4, EDGE>(a, s, quant, stream);
+  return norm_launch<T, S, VEC, kAll, EDGE>(a, s, quant, stream);
 }
 
-template <typename T, typename S, int VEC>
+template <typename T, typename S, int VEC, bool EDGE>
 cudaError_t norm_backward_vec(NormArgs a, cudaStream_t stream) {
-  const Shape s = shape_of(a.D, VEC, most_of(VEC));
-  constexpr int kAll = (int)(kMaxWidth / kMost) / VEC;
-  a.threads = s.threads;
-  if (s.per <= 1) return norm_backward_launch<T, S, VEC, 1>(a, s, stream);
-  if (s.per <= 2) return norm_backward_launch<T, S, VEC, 2>(a, s, stream);
-  if (s.per <= 4) return norm_backward_launch<T, S, VEC, 4>(a, s, stream);
-  return norm_backward_launch<T, S, VEC, kAll>(a, s, stream);
+  const Shape s = shape_of(a.D, VEC, EDGE, kHeldBackward);
+  constexpr int kAll = (int)(kMaxWidth / kMost) / VEC + (EDGE ? 1 : 0);
+  a.threads_log2 = s.threads_log2;
+  if (s.per <= 1) return norm_backward_launch<T, S, VEC, 1, EDGE>(a, s, stream);
+  if (s.per <= 2) return norm_backward_launch<T, S, VEC, 2, EDGE>(a, s, stream);
+  if (s.per <= 4) return norm_backward_launch<T, S, VEC, 4, EDGE>(a, s, stream);
+  return norm_backward_launch<T, S, VEC, kAll, EDGE>(a, s, stream);
 }
 
-// Elements a 16-byte access of T moves; rows that do not allow it go one
-// element at a time.
+// Elements a 16-byte access of T moves.
 template <typename T>
 constexpr int vec_of() { return 16 / (int)sizeof(T); }
 
+// How rows lie: all of them on vectors, all tensors' rows equally far from one,
+// or otherwise (one element at a time).
+enum Lie { kOnVectors, kShifted, kAnyhow };
+
 template <typename T, typename S>
-cudaError_t norm_as(const NormArgs &a, bool wide, bool quant, cudaStream_t stream) {
-  return wide ? norm_vec<T, S, vec_of<T>()>(a, quant, stream) : norm_vec<T, S, 1>(a, quant, stream);
+cudaError_t norm_as(const NormArgs &a, Lie lie, bool quant, cudaStream_t stream) {
+  if (lie == kOnVectors) return norm_vec<T, S, vec_of<T>(), false>(a, quant, stream);
+  if (lie == kShifted) return norm_vec<T, S, vec_of<T>(), true>(a, quant, stream);
+  return norm_vec<T, S, 1, false>(a, quant, stream);
 }
 
 template <typename T, typename S>
-cudaError_t norm_backward_as(const NormArgs &a, bool wide, cudaStream_t stream) {
-  return wide ? norm_backward_vec<T, S, vec_of<T>()>(a, stream) : norm_backward_vec<T, S, 1>(a, stream);
+cudaError_t norm_backward_as(const NormArgs &a, Lie lie, cudaStream_t stream) {
+  if (lie == kOnVectors) return norm_backward_vec<T, S, vec_of<T>(), false>(a, stream);
+  if (lie == kShifted) return norm_backward_vec<T, S, vec_of<T>(), true>(a, stream);
+  return norm_backward_vec<T, S, 1, false>(a, stream);
 }
 
-bool wide_rows(const NormArgs &a, int e, int f) {
+Lie lie_of(const NormArgs &a, int e, int f, int x_size) {
   const int vec = 16 / e;
-  return a.D % vec == 0 && aligned_to(a.x, a.xs, e, 16) && aligned_to(a.res, a.rs, f, 16) &&
-         aligned_to(a.w, 0, 4, 16) && aligned_to(a.y, 0, e, 16) && aligned_to(a.s, 0, f, 16) &&
-         aligned_to(a.q, 0, 1, vec) && aligned_to(a.dy, 0, e, 16) && aligned_to(a.gs, 0, f, 16) &&
-         aligned_to(a.dx, 0, e, 16) && aligned_to(a.dres, 0, f, 16);
+  // starts on vectors of `vec` elements, whatever a tensor's type
+  auto on = [&](const void *p, int size) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)(vec * size) == 0; };
+  const bool starts = on(a.x, x_size) && on(a.res, f) && on(a.y, e) && on(a.s, f) && on(a.q, 1) && on(a.dy, e) &&
+                      on(a.gs, f) && on(a.dx, e) && on(a.dres, f);
+  if (!starts) return kAnyhow;
+  const bool strides = (a.xs - a.D) % vec == 0 && (a.res == nullptr || (a.rs - a.D) % vec == 0);
+  if (!strides) return kAnyhow;
+  if (a.D % vec == 0) return aligned_to(a.w, 0, 4, 16) ? kOnVectors : kAnyhow;
+  return kShifted;
 }
 
 int check_norm(const char *fn, int dtype, int stream_dtype, int w_dtype, int64_t rows, int64_t D, float eps) {
@@ -368,15 +588,15 @@ cudaError_t by_type(int dtype, int stream_dtype, F32 f32, F16 f16, BF16 bf16, M1
 
 int forward(const char *fn, int dtype, int stream_dtype, int w_dtype, NormArgs a, bool quant,
             cudaStream_t stream) {
-  const bool wide = wide_rows(a, dtype_size(dtype), dtype_size(stream_dtype));
+  const Lie lie = lie_of(a, dtype_size(dtype), dtype_size(stream_dtype), dtype_size(dtype));
   a.w_f32 = w_dtype == CPAB_F32;
   using H = __half;
   using B = __nv_bfloat16;
-  return launch_status(by_type(dtype, stream_dtype, [&] { return norm_as<float, float>(a, wide, quant, stream); },
-                               [&] { return norm_as<H, H>(a, wide, quant, stream); },
-                               [&] { return norm_as<B, B>(a, wide, quant, stream); },
-                               [&] { return norm_as<H, float>(a, wide, quant, stream); },
-                               [&] { return norm_as<B, float>(a, wide, quant, stream); }),
+  return launch_status(by_type(dtype, stream_dtype, [&] { return norm_as<float, float>(a, lie, quant, stream); },
+                               [&] { return norm_as<H, H>(a, lie, quant, stream); },
+                               [&] { return norm_as<B, B>(a, lie, quant, stream); },
+                               [&] { return norm_as<H, float>(a, lie, quant, stream); },
+                               [&] { return norm_as<B, float>(a, lie, quant, stream); }),
                        fn);
 }
 
@@ -395,7 +615,7 @@ extern "C" int cpab_b200_rms_norm(int dtype, int stream_dtype, int weight_dtype,
   if (x == nullptr || weight == nullptr || y == nullptr || (residual != nullptr && sum == nullptr))
     return report_error(CPAB_ERR_ARG, "rms_norm: null pointer");
   NormArgs a{};
-  a.x = x, a.xs = x_row, a.res = residual, a.rs = residual_row, a.w = weight, a.rows = rows, a.D = D;
+  a.x = x, a.xs = x_row, a.res = residual, a.rs = residual_row, a.w = weight, a.rows = rows, a.D = D, a.inverse = 1.0f / (float)D;
   a.eps = eps, a.y = y, a.s = sum, a.r = rstd;
   return forward("rms_norm", dtype, stream_dtype, weight_dtype, a, false, stream);
 }
@@ -412,17 +632,20 @@ extern "C" int cpab_b200_rms_norm_quantized(int dtype, int stream_dtype, int wei
       (residual != nullptr && sum == nullptr))
     return report_error(CPAB_ERR_ARG, "rms_norm_quantized: null pointer");
   NormArgs a{};
-  a.x = x, a.xs = x_row, a.res = residual, a.rs = residual_row, a.w = weight, a.rows = rows, a.D = D;
+  a.x = x, a.xs = x_row, a.res = residual, a.rs = residual_row, a.w = weight, a.rows = rows, a.D = D, a.inverse = 1.0f / (float)D;
   a.eps = eps, a.q = q, a.scale = scale, a.s = sum;
   return forward("rms_norm_quantized", dtype, stream_dtype, weight_dtype, a, true, stream);
 }
 
 extern "C" int64_t cpab_b200_rms_norm_workspace(int dtype, int64_t rows, int64_t D) {
   if (!dtype_ok(dtype) || rows < 1 || D < 1 || D > kMaxWidth) return 0;
-  // The scalar and the vector kernel's blocks hold different numbers of rows.
-  const int64_t one = backward_rows(rows, shape_of(D, 1, most_of(1)));
-  const int64_t wide = backward_rows(rows, shape_of(D, 16 / dtype_size(dtype), most_of(16 / dtype_size(dtype))));
-  return (one > wide ? one : wide) * D;
+  const int vec = 16 / dtype_size(dtype);
+  int64_t most = 0;
+  for (const int64_t n : {blocks_of(rows, shape_of(D, 1, false, kHeldBackward), 1, false, true),
+                          blocks_of(rows, shape_of(D, vec, false, kHeldBackward), vec, false, true),
+                          blocks_of(rows, shape_of(D, vec, true, kHeldBackward), vec, true, true)})
+    most = n > most ? n : most;
+  return most * D;
 }
 
 extern "C" int cpab_b200_rms_norm_backward(int dtype, int stream_dtype, int weight_dtype,
@@ -446,21 +669,20 @@ extern "C" int cpab_b200_rms_norm_backward(int dtype, int stream_dtype, int weig
     return report_error(CPAB_ERR_ARG, "rms_norm_backward: grad_residual is grad_x where the types are one");
   NormArgs a{};
   a.x = sum, a.xs = sum_row, a.w = weight, a.w_f32 = weight_dtype == CPAB_F32;
-  a.r = const_cast<float *>(rstd), a.rows = rows, a.D = D, a.dy = grad_y, a.gs = grad_sum;
+  a.r = const_cast<float *>(rstd), a.rows = rows, a.D = D, a.inverse = 1.0f / (float)D, a.dy = grad_y, a.gs = grad_sum;
   a.dx = grad_x, a.dres = grad_residual, a.partial = grad_weight != nullptr ? workspace : nullptr;
   const int e = dtype_size(dtype), f = dtype_size(stream_dtype);
-  const bool wide = wide_rows(a, e, f) && aligned_to(sum, sum_row, f, 16);
+  const Lie lie = lie_of(a, e, f, f);
   using H = __half;
   using B = __nv_bfloat16;
-  const cudaError_t err = by_type(dtype, stream_dtype, [&] { return norm_backward_as<float, float>(a, wide, stream); },
-                            [&] { return norm_backward_as<H, H>(a, wide, stream); },
-                            [&] { return norm_backward_as<B, B>(a, wide, stream); },
-                            [&] { return norm_backward_as<H, float>(a, wide, stream); },
-                            [&] { return norm_backward_as<B, float>(a, wide, stream); });
+  const cudaError_t err = by_type(dtype, stream_dtype, [&] { return norm_backward_as<float, float>(a, lie, stream); },
+                            [&] { return norm_backward_as<H, H>(a, lie, stream); },
+                            [&] { return norm_backward_as<B, B>(a, lie, stream); },
+                            [&] { return norm_backward_as<H, float>(a, lie, stream); },
+                            [&] { return norm_backward_as<B, float>(a, lie, stream); });
   if (err != cudaSuccess || grad_weight == nullptr) return launch_status(err, "rms_norm_backward");
-  const int vec = wide ? 16 / e : 1;
-  const Shape s = shape_of(D, vec, most_of(vec));
-  const int64_t n = backward_rows(rows, s);
+  const int vec = lie == kAnyhow ? 1 : 16 / e;
+  const int64_t n = blocks_of(rows, shape_of(D, vec, lie == kShifted, kHeldBackward), vec, lie == kShifted, true);
   const unsigned grid = (unsigned)((D + 31) / 32);
   const dim3 block(32, 32);
   if (weight_dtype == CPAB_F32)

@@ -103,21 +103,15 @@ __device__ __forceinline__ Lane<V> all(float f) {
 
 // Words of shared or global memory as float32 channels and back.
 __device__ __forceinline__ Lane<1> unpack(uint32_t w, float) { return {{__uint_as_float(w)}}; }
-__device__ __forceinline__ Lane<2> unpack(uint32_t w, __nv_bfloat16) {
-  return {{__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)}};
-}
-__device__ __forceinline__ Lane<2> unpack(uint32_t w, __half) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+template <typename T>
+__device__ __forceinline__ Lane<2> unpack(uint32_t w, T) {
+  const float2 f = unpack_pair<T>(w);
   return {{f.x, f.y}};
 }
 __device__ __forceinline__ uint32_t pack(Lane<1> a, float) { return __float_as_uint(a[0]); }
-__device__ __forceinline__ uint32_t pack(Lane<2> a, __nv_bfloat16) {
-  const __nv_bfloat162 p = __floats2bfloat162_rn(a[0], a[1]);
-  return *reinterpret_cast<const uint32_t *>(&p);
-}
-__device__ __forceinline__ uint32_t pack(Lane<2> a, __half) {
-  const __half2 p = __floats2half2_rn(a[0], a[1]);
-  return *reinterpret_cast<const uint32_t *>(&p);
+template <typename T>
+__device__ __forceinline__ uint32_t pack(Lane<2> a, T) {
+  return pack_pair<T>(a[0], a[1]);
 }
 // +inf in every element: the gate of a sample that is none (a = 1, 1 - a = 0).
 __device__ __forceinline__ uint32_t closed_gate(float) { return 0x7F800000u; }

@@ -27,6 +27,44 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
+// The two 16-bit elements of a word as float32, and two values rounded to one.
+template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack_pair<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack_pair<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&p);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&p);
+}
+// The rounded sums of two words' elements (one rounding, as of the float32 sum).
+template <typename T>
+__device__ __forceinline__ uint32_t add_pair(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t add_pair<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 s = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&a),
+                                   *reinterpret_cast<const __nv_bfloat162 *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&s);
+}
+template <>
+__device__ __forceinline__ uint32_t add_pair<__half>(uint32_t a, uint32_t b) {
+  const __half2 s = __hadd2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+  return *reinterpret_cast<const uint32_t *>(&s);
+}
+
 // N consecutive elements moved by one access of N * sizeof(T) bytes (at most
 // 16), which is also the alignment it needs.
 template <typename T, int N>
