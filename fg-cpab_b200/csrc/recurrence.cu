@@ -179,7 +179,7 @@ __device__ __forceinline__ void copy_stage(uint32_t *to, const Rows<T> &in, int 
   using S = Stage<L, LOG2, ALIGNED>;
   constexpr int V = 4 / sizeof(T);
   const uint4 fill = make_uint4(in.fill, in.fill, in.fill, in.fill);
-  if (ALIGNED) {
+  if constexpr (ALIGNED) {
     const int step = blockDim.x / S::kCopies, word = (threadIdx.x % S::kCopies) * 4;
     int r = threadIdx.x / S::kCopies;
     const T *src = in.first + (int64_t)(s0 + r) * in.stride + word * V;
@@ -199,25 +199,25 @@ __device__ __forceinline__ void copy_stage(uint32_t *to, const Rows<T> &in, int 
         *reinterpret_cast<uint4 *>(dst) = fill;
       }
     }
-    return;
-  }
-  for (int q = threadIdx.x; q < rows * S::kCopies; q += blockDim.x) {
-    const int r = q / S::kCopies, piece = q % S::kCopies;
-    uint32_t *dst = to + S::row(r) + piece * 4;
-    if (s0 + r >= len) {
-      *reinterpret_cast<uint4 *>(dst) = fill;
-      continue;
-    }
-    const char *row = reinterpret_cast<const char *>(in.first + (int64_t)(s0 + r) * in.stride);
-    const char *src = reinterpret_cast<const char *>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15) + piece * 16;
-    const char *row_end = row + channels * (int)sizeof(T);
-    if (src >= row_end) continue;
-    if (src >= in.begin && src + 16 <= in.end) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address(dst)), "l"(src));
-    } else {  // the tensor's first or last bytes: its elements one by one
-      for (int i = 0; i < 16; i += (int)sizeof(T))
-        if (src + i >= row && src + i < row_end)
-          reinterpret_cast<T *>(dst)[i / sizeof(T)] = *reinterpret_cast<const T *>(src + i);
+  } else {
+    for (int q = threadIdx.x; q < rows * S::kCopies; q += blockDim.x) {
+      const int r = q / S::kCopies, piece = q % S::kCopies;
+      uint32_t *dst = to + S::row(r) + piece * 4;
+      if (s0 + r >= len) {
+        *reinterpret_cast<uint4 *>(dst) = fill;
+        continue;
+      }
+      const char *row = reinterpret_cast<const char *>(in.first + (int64_t)(s0 + r) * in.stride);
+      const char *src = reinterpret_cast<const char *>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)15) + piece * 16;
+      const char *row_end = row + channels * (int)sizeof(T);
+      if (src >= row_end) continue;
+      if (src >= in.begin && src + 16 <= in.end) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address(dst)), "l"(src));
+      } else {  // the tensor's first or last bytes: its elements one by one
+        for (int i = 0; i < 16; i += (int)sizeof(T))
+          if (src + i >= row && src + i < row_end)
+            reinterpret_cast<T *>(dst)[i / sizeof(T)] = *reinterpret_cast<const T *>(src + i);
+      }
     }
   }
 }
