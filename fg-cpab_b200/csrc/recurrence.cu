@@ -228,6 +228,35 @@ __device__ __forceinline__ Rows<T> rows_of(const void *tensor, int64_t at, int64
   return {static_cast<const T *>(tensor) + at, stride, begin, begin + bytes, fill};
 }
 
+// copy_stage for the stages of a full block whose rows start on 16 bytes and
+// are all there, with what a thread's addresses have in common kept.
+template <typename T, int L, int LOG2>
+struct Feed {
+  using S = Stage<L, LOG2, true>;
+  static constexpr int kThreads = warps_of(LOG2) * 32, kRows = kThreads / S::kCopies;  // rows copied at a time
+  static_assert(kRows % L == 0, "a thread's rows lie equally far apart in shared memory");
+  const char *src;          // the thread's first copy of the next stage
+  int64_t row_step, stage_step;
+  __device__ __forceinline__ Feed(const Rows<T> &in, int s0, int stage, int direction) {
+    constexpr int V = 4 / sizeof(T);
+    src = reinterpret_cast<const char *>(in.first + (int64_t)(s0 + (int)threadIdx.x / S::kCopies) * in.stride +
+                                         (threadIdx.x % S::kCopies) * 4 * V);
+    row_step = kRows * in.stride * (int64_t)sizeof(T);
+    stage_step = direction * (int64_t)stage * in.stride * (int64_t)sizeof(T);
+  }
+  // Bytes of the thread's first copy from the start of a stage in shared memory.
+  static __device__ __forceinline__ uint32_t place() {
+    return (S::row((int)threadIdx.x / S::kCopies) + (threadIdx.x % S::kCopies) * 4) * 4;
+  }
+  __device__ __forceinline__ void copy(uint32_t to) const {
+#pragma unroll
+    for (int k = 0; k < L / 4; ++k)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + k * (kRows + kRows / L) * S::kPitch * 4),
+                   "l"(src + k * row_step));
+  }
+  __device__ __forceinline__ void next() { src += stage_step; }
+};
+
 // A lane's word of each of L consecutive samples, from sample t0 of a tile and
 // row r of its stage on.
 template <typename T, int L, int LOG2, bool ALIGNED>
@@ -479,12 +508,22 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
   const int words = Stage<L, LOG2, ALIGNED>::words(at.stage);  // of one tensor's stage
   uint32_t *ring = reinterpret_cast<uint32_t *>(ring_memory);
 
+  const bool whole = ALIGNED && blockDim.x == kWarps * 32 && at.channels == At::kLanes * V;
+  Feed<T, L, LOG2> x_feed(x, at.first, at.stage, 1), g_feed(g, at.first, at.stage, 1);
+  const uint32_t place = shared_address(ring) + Feed<T, L, LOG2>::place();
   auto fetch = [&](int k, int slot) {
     if (k < at.live) {
-      uint32_t *to = ring + slot * 2 * words;
       const int s0 = at.first + k * at.stage;
-      copy_stage<T, L, LOG2, ALIGNED>(to, x, s0, at.stage, at.len, at.channels);
-      copy_stage<T, L, LOG2, ALIGNED>(to + words, g, s0, at.stage, at.len, at.channels);
+      if (whole && s0 + at.stage <= at.len) {
+        x_feed.copy(place + slot * 2 * words * 4);
+        g_feed.copy(place + (slot * 2 + 1) * words * 4);
+      } else {
+        uint32_t *to = ring + slot * 2 * words;
+        copy_stage<T, L, LOG2, ALIGNED>(to, x, s0, at.stage, at.len, at.channels);
+        copy_stage<T, L, LOG2, ALIGNED>(to + words, g, s0, at.stage, at.len, at.channels);
+      }
+      x_feed.next();
+      g_feed.next();
     }
     asm volatile("cp.async.commit_group;");
   };
@@ -496,6 +535,8 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
   if (p.h0 != nullptr) carry = load_state<V>(p.h0 + at.b * p.D, at.d, p.D);
   carry = through_spans<V, false>(p, at, span_total, mine, carry);
 
+  T *h_row = h + (int64_t)(at.first + at.seg * L) * p.D;
+  const int64_t h_stage = at.stage * p.D;
   int slot = 0;
   for (int k = 0; k < at.live; ++k) {
     const int t0 = at.first + k * at.stage + at.seg * L;
@@ -536,7 +577,7 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
     if (p.states != nullptr && t0 % kChunk == 0 && t0 < at.len)
       store_state(p.states + (at.b * chunks + t0 / kChunk) * p.D, at.d, p.D, state);
     auto write = [&](auto words) {
-      T *row = h + t0 * p.D;
+      T *row = h_row;
       if (t0 + L <= at.len) {
 #pragma unroll
         for (int i = 0; i < L; ++i, row += p.D) {
@@ -555,6 +596,7 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
       if (p.words) write(std::true_type{});
       else write(std::false_type{});
     }
+    h_row += h_stage;
   }
   // Stages past the series' end: zeros.
   for (int s0 = at.first + at.live * at.stage; s0 < at.end; s0 += at.stage) {
@@ -587,14 +629,27 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
   uint32_t *ring = reinterpret_cast<uint32_t *>(ring_memory);
 
   // Stage k counts from the last one with samples back.
+  const int s_last = at.first + (at.live - 1) * at.stage;
+  const bool whole = ALIGNED && blockDim.x == kWarps * 32 && at.channels == At::kLanes * V && p.grad_h != nullptr;
+  Feed<T, L, LOG2> x_feed(x, s_last, at.stage, -1), g_feed(g, s_last, at.stage, -1), d_feed(dh, s_last, at.stage, -1);
+  const uint32_t place = shared_address(ring) + Feed<T, L, LOG2>::place();
   auto fetch = [&](int k, int slot) {
     if (k < at.live) {
-      uint32_t *to = ring + slot * 3 * words;
-      const int s0 = at.first + (at.live - 1 - k) * at.stage;
-      copy_stage<T, L, LOG2, ALIGNED>(to, x, s0, at.stage, at.len, at.channels);
-      copy_stage<T, L, LOG2, ALIGNED>(to + words, g, s0, at.stage, at.len, at.channels);
-      copy_stage<T, L, LOG2, ALIGNED>(to + 2 * words, dh, s0, at.stage, p.grad_h != nullptr ? at.len : 0,
-                                      at.channels);
+      const int s0 = s_last - k * at.stage;
+      if (whole && s0 + at.stage <= at.len) {
+        x_feed.copy(place + slot * 3 * words * 4);
+        g_feed.copy(place + (slot * 3 + 1) * words * 4);
+        d_feed.copy(place + (slot * 3 + 2) * words * 4);
+      } else {
+        uint32_t *to = ring + slot * 3 * words;
+        copy_stage<T, L, LOG2, ALIGNED>(to, x, s0, at.stage, at.len, at.channels);
+        copy_stage<T, L, LOG2, ALIGNED>(to + words, g, s0, at.stage, at.len, at.channels);
+        copy_stage<T, L, LOG2, ALIGNED>(to + 2 * words, dh, s0, at.stage, p.grad_h != nullptr ? at.len : 0,
+                                        at.channels);
+      }
+      x_feed.next();
+      g_feed.next();
+      d_feed.next();
     }
     asm volatile("cp.async.commit_group;");
   };
@@ -608,10 +663,14 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
   if (p.grad_last != nullptr) carry = load_state<V>(p.grad_last + at.b * p.D, at.d, p.D);
   carry = through_spans<V, true>(p, at, span_total, mine, carry);
 
+  const float *base_row = p.states + (at.b * chunks + s_last / kChunk) * p.D;
+  T *dx_row = dx + (int64_t)(s_last + at.seg * L + L - 1) * p.dxt, *dg_row = dg + (int64_t)(s_last + at.seg * L + L - 1) * p.dgt;
+  const int64_t dx_stage = at.stage * p.dxt, dg_stage = at.stage * p.dgt;
   int slot = 0;
   for (int k = 0; k < at.live; ++k) {
-    const int s0 = at.first + (at.live - 1 - k) * at.stage, t0 = s0 + at.seg * L;
-    Lane<V> base = load_state<V>(p.states + (at.b * chunks + s0 / kChunk) * p.D, at.d, p.D);
+    const int t0 = s_last - k * at.stage + at.seg * L;
+    Lane<V> base = load_state<V>(base_row, at.d, p.D);
+    base_row -= at.stage / kChunk * p.D;
     wait_for_stage(p.ring);
     const uint32_t *here = ring + slot * 3 * words;
     const Words<T, L, LOG2, ALIGNED> xs(here, at.seg * L, at.cl, x, t0), gs(here + words, at.seg * L, at.cl, g, t0);
@@ -677,7 +736,7 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
       xv[i] = fma(xv[i], all<V>(-1.0f), before);
     }
     auto write = [&](auto words) {
-      T *rx = dx + (t0 + L - 1) * p.dxt, *rg = dg + (t0 + L - 1) * p.dgt;
+      T *rx = dx_row, *rg = dg_row;
       if (t0 + L <= at.len) {
 #pragma unroll
         for (int i = L - 1; i >= 0; --i, rx -= p.dxt, rg -= p.dgt) {
@@ -703,6 +762,8 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
       if (p.words) write(std::true_type{});
       else write(std::false_type{});
     }
+    dx_row -= dx_stage;
+    dg_row -= dg_stage;
   }
   for (int s0 = at.first + at.live * at.stage; s0 < at.end; s0 += at.stage) {
     const int t0 = s0 + at.seg * L;
