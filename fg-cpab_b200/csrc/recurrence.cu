@@ -423,12 +423,29 @@ __global__ void __launch_bounds__(kTotalWarps * 32) k_scan_totals(const __grid_c
     if (t0 >= len) continue;
     uint32_t gw[L], uw[L];
     const T *gr = g + t0 * p.gt, *ur = u + t0 * ut;
+    if (any && p.words && t0 + L <= len) {
 #pragma unroll
-    for (int i = 0; i < L; ++i, gr += p.gt, ur += ut) {
-      gw[i] = closed_gate(T{});
-      uw[i] = 0u;
-      if (n > 0 && t0 + i < len) gw[i] = load_word(gr, n, p.words);
-      if (any && t0 + i < len) uw[i] = load_word(ur, n, p.words);
+      for (int i = 0; i < L; ++i) {
+        gw[i] = *reinterpret_cast<const uint32_t *>(gr + i * p.gt);
+        uw[i] = *reinterpret_cast<const uint32_t *>(ur + i * ut);
+      }
+    } else if (sizeof(T) == 2 && any && n == V && t0 + L <= len) {
+      // a lane's second element by itself where pairs do not lie on words
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        const unsigned short *gh = reinterpret_cast<const unsigned short *>(gr + i * p.gt);
+        const unsigned short *uh = reinterpret_cast<const unsigned short *>(ur + i * ut);
+        gw[i] = gh[0] | (uint32_t)gh[V - 1] << 16;
+        uw[i] = uh[0] | (uint32_t)uh[V - 1] << 16;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < L; ++i, gr += p.gt, ur += ut) {
+        gw[i] = closed_gate(T{});
+        uw[i] = 0u;
+        if (n > 0 && t0 + i < len) gw[i] = load_word(gr, n, p.words);
+        if (any && t0 + i < len) uw[i] = load_word(ur, n, p.words);
+      }
     }
 #pragma unroll
     for (int k = 0; k < L; ++k) {
