@@ -52,10 +52,10 @@ def call(fn, *args):
     """fn(*args) of the extension; a failed C ABI call (the node's message
     starts with the library's name) raises the same error type as the
     Python path."""
-    from . import _native
     try:
         return fn(*args)
     except RuntimeError as e:
+        from . import _native
         first = str(e).split("\n", 1)[0]
         if first.startswith("libcpab_b200: "):
             raise _native.CpabNativeError(first[len("libcpab_b200: "):]) from None

@@ -116,18 +116,23 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             lists = {}
             for p in group["params"]:
-                if p.grad is None:
+                g = p.grad
+                if g is None:
                     continue
-                if p.grad.is_sparse:
+                if g.is_sparse:
                     raise RuntimeError("AdamW does not take sparse gradients")
-                s = self._state(p, group)
-                to = lists.setdefault(p.device, ([], [], [], [], [], []))
+                s = self.state[p]
+                if not s:
+                    s = self._state(p, group)
+                to = lists.get(p.device)
+                if to is None:
+                    to = lists[p.device] = ([], [], [], [], [], [])
+                scales = s.get("scales")
                 to[0].append(p)
-                to[1].append(p.grad)
+                to[1].append(g)
                 to[2].append(s["exp_avg"])
-                eight = "scales" in s
-                to[3].append(s["root_avg_sq"] if eight else s["exp_avg_sq"])
-                to[4].append(s["scales"] if eight else None)
+                to[3].append(s["exp_avg_sq"] if scales is None else s["root_avg_sq"])
+                to[4].append(scales)
                 to[5].append(s["step"])
             for device, to in lists.items():
                 scales = to[4] if any(t is not None for t in to[4]) else None
@@ -135,9 +140,10 @@ class AdamW(torch.optim.Optimizer):
                     (*to[:4], scales, to[5], group["lr"], group["betas"], group["eps"],
                      group["weight_decay"]))
         for device, groups in by_device.items():
-            if device not in self._workspace:
-                self._workspace[device] = torch.zeros(1, device=device, dtype=torch.int32)
-            _step(groups, self.seed, self._workspace[device])
+            workspace = self._workspace.get(device)
+            if workspace is None:
+                workspace = self._workspace[device] = torch.zeros(1, device=device, dtype=torch.int32)
+            _step(groups, self.seed, workspace)
         return loss
 
     def load_state_dict(self, state_dict):

@@ -52,7 +52,8 @@ def rms_norm_quantized(x, weight, residual=None, eps=1e-6):
     (q, scale, s) with a residual, where q [..., D] float8_e4m3fn and scale
     [...] float32 (one per row) stand for y ~ q * scale; scale =
     max(max|y| / 448, 2^-126), never 0.  No gradient."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                    or (residual is not None and residual.requires_grad)):
         raise RuntimeError("rms_norm_quantized has no gradient; call it under torch.no_grad()")
     ext = _ext.module()
     if ext is None:

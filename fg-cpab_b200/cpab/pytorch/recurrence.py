@@ -71,7 +71,8 @@ def gated_scan_step(x, gate, state, slots=None):
 
     Returns h [B, D] of x's type, the streams' new states.  No gradient."""
     slots = _int32(slots, "slots", state.shape[0])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, state)):
+    if torch.is_grad_enabled() and (x.requires_grad or state.requires_grad
+                                    or (gate is not None and gate.requires_grad)):
         raise RuntimeError("gated_scan_step has no gradient (its state is updated in place); "
                            "call it under torch.no_grad(), or use gated_scan")
     ext = _ext.module()

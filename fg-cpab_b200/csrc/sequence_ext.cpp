@@ -327,13 +327,21 @@ std::vector<Tensor> rms_norm_quantized(const Tensor &x, const Tensor &weight, co
 
 // ---- adamw ---------------------------------------------------------------------
 
+// Element i of a Python list of tensors (null where it is None and `maybe`),
+// read in place: a step's lists hold every tensor of a network.
+const Tensor *item(const pybind11::list &list, size_t i, const char *name, bool maybe = false) {
+  PyObject *o = PyList_GET_ITEM(list.ptr(), (Py_ssize_t)i);
+  if (maybe && o == Py_None) return nullptr;
+  TORCH_CHECK_TYPE(THPVariable_Check(o), "adamw: ", name, " ", i, " is no tensor");
+  return &THPVariable_Unpack(o);
+}
+
 // counts[g] tensors of group g one after another in the lists; hyper holds a
 // group's (lr, beta1, beta2, eps, weight_decay); lr_tensors a group's learning
-// rate on the device (undefined: hyper's).  scales is empty where every state
-// has 32 bits.
-void adamw(const std::vector<Tensor> &params, const std::vector<Tensor> &grads,
-           const std::vector<Tensor> &exp_avgs, const std::vector<Tensor> &exp_avg_sqs,
-           const std::vector<MaybeTensor> &scales, const std::vector<Tensor> &steps,
+// rate on the device (None: hyper's).  scales is empty where every state has
+// 32 bits.
+void adamw(const pybind11::list &params, const pybind11::list &grads, const pybind11::list &exp_avgs,
+           const pybind11::list &exp_avg_sqs, const pybind11::list &scales, const pybind11::list &steps,
            const std::vector<int64_t> &counts, const std::vector<double> &hyper,
            const std::vector<MaybeTensor> &lr_tensors, int64_t seed, const Tensor &workspace) {
   const size_t n = params.size();
@@ -341,7 +349,7 @@ void adamw(const std::vector<Tensor> &params, const std::vector<Tensor> &grads,
                         (scales.empty() || scales.size() == n),
                     "adamw: lists of different lengths");
   if (n == 0) return;
-  const at::Device device = params[0].device();
+  const at::Device device = item(params, 0, "parameter")->device();
   TORCH_CHECK(device.is_cuda(), "params must be CUDA tensors (no CPU path)");
   const c10::cuda::CUDAGuard guard(device);
   std::vector<cpab_adamw_tensor> list(n);
@@ -349,50 +357,51 @@ void adamw(const std::vector<Tensor> &params, const std::vector<Tensor> &grads,
   size_t k = 0;
   for (size_t g = 0; g < counts.size(); ++g) {
     for (int64_t i = 0; i < counts[g]; ++i, ++k) {
-      const Tensor &p = params[k], &m = exp_avgs[k], &v = exp_avg_sqs[k], &step = steps[k];
+      const Tensor &p = *item(params, k, "parameter"), &m = *item(exp_avgs, k, "first moment");
+      const Tensor &v = *item(exp_avg_sqs, k, "second moment"), &step = *item(steps, k, "step");
+      const Tensor *grad = item(grads, k, "gradient");
       const bool eight = m.scalar_type() == at::kFloat8_e4m3fn;
-      TORCH_CHECK(p.device() == device && grads[k].device() == device && m.device() == device &&
+      TORCH_CHECK(p.device() == device && grad->device() == device && m.device() == device &&
                       v.device() == device && step.device() == device,
                   "adamw: tensor ", k, ": all tensors must be on one device");
-      TORCH_CHECK_TYPE(grads[k].scalar_type() == p.scalar_type(), "adamw: tensor ", k, ": gradient of type ",
-                       grads[k].scalar_type(), " for a parameter of type ", p.scalar_type());
+      TORCH_CHECK_TYPE(grad->scalar_type() == p.scalar_type(), "adamw: tensor ", k, ": gradient of type ",
+                       grad->scalar_type(), " for a parameter of type ", p.scalar_type());
       TORCH_CHECK_TYPE(v.scalar_type() == m.scalar_type() && (eight || m.scalar_type() == at::kFloat),
                        "adamw: tensor ", k, ": states must be float32, or both float8_e4m3fn");
       TORCH_CHECK_TYPE(step.scalar_type() == at::kFloat && step.numel() == 1,
                        "adamw: tensor ", k, ": step must be one float32");
-      TORCH_CHECK_VALUE(grads[k].sizes() == p.sizes() && m.sizes() == p.sizes() && v.sizes() == p.sizes(),
+      TORCH_CHECK_VALUE(grad->sizes() == p.sizes() && m.sizes() == p.sizes() && v.sizes() == p.sizes(),
                         "adamw: tensor ", k, ": parameter, gradient and states must have one shape");
-      TORCH_CHECK_VALUE(p.is_non_overlapping_and_dense() &&
-                            (p.is_contiguous() ? m.is_contiguous() && v.is_contiguous()
-                                               : m.strides() == p.strides() && v.strides() == p.strides()),
+      const bool plain = p.is_contiguous();
+      TORCH_CHECK_VALUE(plain ? m.is_contiguous() && v.is_contiguous()
+                              : p.is_non_overlapping_and_dense() && m.strides() == p.strides() &&
+                                    v.strides() == p.strides(),
                         "adamw: tensor ", k, ": parameter and states must be dense and laid out alike");
-      Tensor grad = grads[k];
-      if (!(p.is_contiguous() ? grad.is_contiguous() : grad.strides() == p.strides())) {
-        grad = at::empty_like(p);
-        grad.copy_(grads[k]);
-        copies.push_back(grad);
+      if (!(plain ? grad->is_contiguous() : grad->strides() == p.strides())) {
+        copies.push_back(at::empty_like(p));
+        copies.back().copy_(*grad);
       }
+      const bool copied = !(plain ? grad->is_contiguous() : grad->strides() == p.strides());
       float *sc = nullptr;
       if (eight) {
         const int64_t blocks = (p.numel() + 255) / 256;
-        const Tensor given_scales = scales.empty() ? Tensor() : given(scales[k]);
-        TORCH_CHECK_VALUE(given_scales.defined() && given_scales.device() == device &&
-                              given_scales.scalar_type() == at::kFloat && given_scales.is_contiguous() &&
-                              given_scales.numel() == 2 * blocks,
+        const Tensor *t = scales.empty() ? nullptr : item(scales, k, "scales", true);
+        TORCH_CHECK_VALUE(t != nullptr && t->device() == device && t->scalar_type() == at::kFloat &&
+                              t->is_contiguous() && t->numel() == 2 * blocks,
                           "adamw: tensor ", k, ": 8-bit states need float32 scales [", blocks, ", 2]");
-        sc = fptr_mut(given_scales);
+        sc = fptr_mut(*t);
       }
       cpab_adamw_tensor &t = list[k];
-      t.param = ptr_mut(p), t.grad = ptr(grad), t.exp_avg = ptr_mut(m), t.exp_avg_sq = ptr_mut(v);
-      t.scales = sc, t.step = fptr_mut(step), t.numel = p.numel();
-      t.lr_device = fptr(given(lr_tensors[g]));
+      t.param = ptr_mut(p), t.grad = ptr(copied ? copies.back() : *grad), t.exp_avg = ptr_mut(m);
+      t.exp_avg_sq = ptr_mut(v), t.scales = sc, t.step = fptr_mut(step), t.numel = p.numel();
+      t.lr_device = lr_tensors[g].has_value() ? fptr(*lr_tensors[g]) : nullptr;
       t.dtype = dtype_of(p, "a parameter"), t.state_bits = eight ? 8 : 32;
       t.lr = hyper[5 * g], t.beta1 = hyper[5 * g + 1], t.beta2 = hyper[5 * g + 2], t.eps = hyper[5 * g + 3];
       t.weight_decay = hyper[5 * g + 4];
     }
   }
   check(cpab_b200_adamw(list.data(), (int)n, (uint32_t)seed, static_cast<int32_t *>(ptr_mut(workspace)),
-                        stream_of(params[0])));
+                        stream_of(*item(params, 0, "parameter"))));
 }
 
 }  // namespace
