@@ -19,8 +19,8 @@ SCALE_BLOCK = 256  # elements of an 8-bit state that share a scale
 def adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8,
            weight_decay=0.01, scales=None, seed=0, workspace=None):
     """One AdamW step over lists of CUDA tensors, in place.  params and grads
-    float32, float16 or bfloat16; steps: one float32 element each, the steps
-    taken so far, counted up by the call.  A parameter's states are both
+    float32, float16 or bfloat16; steps: one float32 element each (its own), the
+    steps taken so far, counted up by the call.  A parameter's states are both
     float32, or both float8_e4m3fn codes (exp_avg_sqs then holds those of the
     second moment's square root) with scales[i] float32 [ceil(numel / 256), 2]
     (columns: first moment, root).  lr: a number, or one float32 on the device

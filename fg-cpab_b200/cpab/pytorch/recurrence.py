@@ -31,6 +31,9 @@ def gated_scan(x, gate=None, h0=None, lengths=None):
     has lengths[b] samples; what x and gate hold after them is never read,
     h is 0 there and the state stays.
 
+    A NaN stays in its channel from its sample on; an infinity does too, as an
+    infinity or a NaN.
+
     Returns (h [B, T, D] of x's type, last [B, D] float32, the state after
     each series' last sample).  Differentiable (once) in x, gate and h0; any
     strides, without a copy where the channels are adjacent."""

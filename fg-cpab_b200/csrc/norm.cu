@@ -25,7 +25,10 @@ namespace {
 
 constexpr int kBlock = 256;        // threads of a block whose rows take fewer
 constexpr int kMost = 512;         // threads of a row at most
-constexpr int kResident = 768;     // threads of an SM that the gradient's registers leave room for
+// Threads of an SM that the gradient's registers leave room for, by the elements a
+// thread holds.  (32768x4096 bf16, 16 elements: 228 us at 512 threads, 192 at 768,
+// 225 at 1024; 65536x999 f32, 8 elements: 388, 296 and 260 us.)
+__host__ __device__ constexpr int resident_of(int elements) { return elements <= 8 ? 1024 : elements <= 16 ? 768 : 512; }
 constexpr int64_t kMaxWidth = 16384;
 constexpr float kE4m3Max = 448.0f;
 constexpr float kTiny = 1.17549435e-38f;  // 2^-126, the smallest scale
@@ -84,7 +87,6 @@ __device__ __forceinline__ void over_row(float &sum, float &top, int log2, float
 template <typename T, int VEC>
 struct Row {
   static constexpr int kPer = VEC == 1 ? 1 : 4 / (int)sizeof(T), kWords = VEC / kPer;
-  static constexpr int N = kWords > 4 ? 4 : kWords;  // words of an access (VEC > 1)
   uint32_t w[kWords];
   using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
 
@@ -92,6 +94,7 @@ struct Row {
     if constexpr (VEC == 1) {
       w[0] = *reinterpret_cast<const Bits *>(at);
     } else {
+      constexpr int N = kWords > 4 ? 4 : kWords;  // words of an access
 #pragma unroll
       for (int k = 0; k < kWords; k += N) {
         const Pack<uint32_t, N> p = *reinterpret_cast<const Pack<uint32_t, N> *>(at + k * kPer);
@@ -104,6 +107,7 @@ struct Row {
     if constexpr (VEC == 1) {
       *reinterpret_cast<Bits *>(at) = (Bits)w[0];
     } else {
+      constexpr int N = kWords > 4 ? 4 : kWords;
 #pragma unroll
       for (int k = 0; k < kWords; k += N) {
         Pack<uint32_t, N> p;
@@ -354,7 +358,7 @@ __global__ void __launch_bounds__(kMost, EDGE || QUANT || NV * VEC > 24 ? 2 : 3)
 // x here is the stream s as kept (x itself without a residual), of type S.
 // With t = dy r: dw = sum t s, ds = gs + t w - s (r^2 mean(t w s)).
 template <typename T, typename S, int VEC, int NV, bool EDGE, int BLOCK>
-__global__ void __launch_bounds__(BLOCK, NV * VEC <= 16 ? kResident / BLOCK : 512 / BLOCK)
+__global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
     k_norm_backward(const __grid_constant__ NormArgs p) {
   // Of wide rows a thread holds too much to fetch gs early.
   constexpr bool kLean = NV * VEC > 16;
@@ -486,11 +490,11 @@ Shape shape_of(int64_t D, int vec, bool edge, int held) {
 // its last one did.
 int64_t blocks_of(int64_t rows, const Shape &s, int vec, bool edge, bool resident) {
   int64_t n = (rows + s.groups - 1) / s.groups;
-  const int64_t cap = (int64_t)device_info().sm_count * ((resident ? kResident : 4096) / s.block);
+  const int64_t cap = (int64_t)device_info().sm_count * ((resident ? resident_of(s.per * vec) : 4096) / s.block);
   if ((resident || edge) && n > cap) n = cap;
   if (edge && n * s.groups < rows) {
-    const int64_t step = s.groups >= vec ? 1 : vec / s.groups;
-    n = (n + step - 1) / step * step;
+    const int64_t step = s.groups >= vec ? 1 : vec / s.groups;  // (divides no more than 16: n is not 0)
+    n = n / step * step;
   }
   return n;
 }
@@ -569,7 +573,11 @@ Lie lie_of(const NormArgs &a, int e, int f, int x_size) {
   const bool strides = (a.xs - a.D) % vec == 0 && (a.res == nullptr || (a.rs - a.D) % vec == 0);
   if (!strides) return kAnyhow;
   if (a.D % vec == 0) return aligned_to(a.w, 0, 4, 16) ? kOnVectors : kAnyhow;
-  return kShifted;
+  // One at a time what is narrower than 32 columns, where a vector's masks cost
+  // more (15 columns bf16: 241 against 488 us, 31: 234 and 302, the gradient 304
+  // and 322; 31 columns f32: 126 and 142, 166 and 226; but 95 columns bf16: 210
+  // and 148, 433 and 237, for 64 and 32 million elements).
+  return a.D < 32 ? kAnyhow : kShifted;
 }
 
 int check_norm(const char *fn, int dtype, int stream_dtype, int w_dtype, int64_t rows, int64_t D, float eps) {
@@ -621,6 +629,8 @@ extern "C" int cpab_b200_rms_norm(int dtype, int stream_dtype, int weight_dtype,
   if (rows == 0) return launch_status(cudaSuccess, "");
   if (x == nullptr || weight == nullptr || y == nullptr || (residual != nullptr && sum == nullptr))
     return report_error(CPAB_ERR_ARG, "rms_norm: null pointer");
+  if (residual == nullptr && stream_dtype != dtype)
+    return report_error(CPAB_ERR_ARG, "rms_norm: without a residual the stream is x, of x's type");
   NormArgs a{};
   a.x = x, a.xs = x_row, a.res = residual, a.rs = residual_row, a.w = weight, a.rows = rows, a.D = D, a.inverse = 1.0f / (float)D;
   a.eps = eps, a.y = y, a.s = sum, a.r = rstd;
@@ -638,6 +648,8 @@ extern "C" int cpab_b200_rms_norm_quantized(int dtype, int stream_dtype, int wei
   if (x == nullptr || weight == nullptr || q == nullptr || scale == nullptr ||
       (residual != nullptr && sum == nullptr))
     return report_error(CPAB_ERR_ARG, "rms_norm_quantized: null pointer");
+  if (residual == nullptr && stream_dtype != dtype)
+    return report_error(CPAB_ERR_ARG, "rms_norm_quantized: without a residual the stream is x, of x's type");
   NormArgs a{};
   a.x = x, a.xs = x_row, a.res = residual, a.rs = residual_row, a.w = weight, a.rows = rows, a.D = D, a.inverse = 1.0f / (float)D;
   a.eps = eps, a.q = q, a.scale = scale, a.s = sum;

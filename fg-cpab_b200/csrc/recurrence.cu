@@ -24,6 +24,18 @@
 // with h_{t-1} recomputed in float32 from the states that the forward keeps at
 // the start of every kChunk samples (reading the rounded output instead would
 // cost more bytes and lose the difference h_{t-1} - x_t where it is small).
+//
+// What bounds it.  In 16 bits the forward moves 6 and the gradient 10 bytes per
+// sample and channel, against 23 and 45 instructions (two of them the special
+// functions'): with tiles enough the blocks issue 72% and 75% of the time and
+// move 5.9 and 5.4 TB/s (64x512x2048 bf16: 69 and 123 us; a copy: 6.46 TB/s).
+// Tiles of 64-byte rows and blocks of 4 warps were the fastest of 32, 64 and 128
+// bytes (64x512x2048 forward 89, 75, 81 us when they were compared): two blocks
+// already fill an SM, so small ones share out evenly.  With few tiles the spread
+// over the SMs costs most (16x2048x1024: 512 tiles on 148 SMs, 41 and 71 us,
+// 5.0 and 4.8 TB/s); clusters of blocks that exchange their compositions stage
+// by stage were slower than composing the spans first (1x65536x512: 76 and 143
+// us with the best cluster sizes, 71 and 104 with spans).
 #include <type_traits>
 
 #include "sequence.cuh"
@@ -975,8 +987,11 @@ Shape shape_of(int64_t B, int64_t T, int64_t D, int vec, bool back, bool aligned
 template <typename T, int LOG2, bool BACK, bool ALIGNED>
 cudaError_t scan_launch(const ScanArgs &a, const Shape &s, int64_t B, cudaStream_t stream) {
   const auto kernel = BACK ? k_scan_backward<T, LOG2, ALIGNED> : k_scan<T, LOG2, ALIGNED>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem);
-  if (e != cudaSuccess) return e;
+  cudaError_t e = cudaSuccess;
+  if (s.smem > 44 * 1024) {  // (4 KB beside it are the kernel's own)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t c{};
   cudaLaunchAttribute attr{};
   if (s.pieces > 1) {  // begins, and fetches its first stages, while the pieces are composed
@@ -1047,7 +1062,7 @@ int check_scan(const char *fn, int dtype, const void *x, int64_t x_series, int64
   if (B < 0 || T < 0 || D < 0) return report_error(CPAB_ERR_ARG, "%s: negative size", fn);
   if (x_series < 0 || x_sample < 0 || gate_series < 0 || gate_sample < 0)
     return report_error(CPAB_ERR_ARG, "%s: negative stride", fn);
-  if (T >= (int64_t(1) << 31)) return report_error(CPAB_ERR_SIZE, "%s: T must be below 2^31", fn);
+  if (T > (int64_t(1) << 31) - 4096) return report_error(CPAB_ERR_SIZE, "%s: T must not exceed 2^31 - 4096", fn);
   if (D > 0 && B > (int64_t(1) << 30) / D)
     return report_error(CPAB_ERR_SIZE, "%s: B * D must not exceed 2^30", fn);
   if (B > 0 && T > 0 && D > 0 && (x == nullptr || gate == nullptr))
@@ -1063,7 +1078,7 @@ using namespace cpab;
 extern "C" int cpab_b200_gated_scan_chunk(void) { return kChunk; }
 
 extern "C" int64_t cpab_b200_gated_scan_workspace(int dtype, int64_t B, int64_t T, int64_t D) {
-  if (!dtype_ok(dtype) || B < 1 || T < 1 || D < 1 || T >= (int64_t(1) << 31) || B > (int64_t(1) << 30) / D)
+  if (!dtype_ok(dtype) || B < 1 || T < 1 || D < 1 || T > (int64_t(1) << 31) - 4096 || B > (int64_t(1) << 30) / D)
     return 0;
   const int vec = 4 / dtype_size(dtype);
   const bool cut = shape_of(B, T, D, vec, false, true).pieces > 1 || shape_of(B, T, D, vec, true, true).pieces > 1;

@@ -369,7 +369,7 @@ typedef enum { CPAB_F32 = 0, CPAB_F16 = 1, CPAB_BF16 = 2 } cpab_dtype;
  * from the state h0 ([B, D] float32, NULL: zeros).  x and gate are [B, T, D]
  * with the given strides of series and samples (so both may be halves of one
  * projection); h is [B, T, D] contiguous, of the same type; the state is
- * float32 throughout.  lengths ([B] int32, NULL: all T; values outside [0, T]
+ * float32 throughout.  T may be up to 2^31 - 4096, B * D up to 2^30.  lengths ([B] int32, NULL: all T; values outside [0, T]
  * are taken as 0 or T): samples from a series' length on are not read and
  * their h is 0.  h_last ([B, D] float32, may be NULL) receives the state after
  * the last sample.  states ([B, ceil(T / c), D] float32 with c =
@@ -465,7 +465,7 @@ typedef struct {
   void *exp_avg;          /* [numel] float32, or e4m3 codes of the first moment     */
   void *exp_avg_sq;       /* [numel] float32, or e4m3 codes of the second's root    */
   float *scales;          /* state_bits 8: [ceil(numel / 256), 2] (first moment, root) */
-  float *step;            /* steps taken so far; the call adds 1                    */
+  float *step;            /* steps taken so far, a tensor's own; the call adds 1    */
   const float *lr_device; /* learning rate on the device, or NULL: lr               */
   int64_t numel;
   int32_t dtype;          /* cpab_dtype of param and grad                           */

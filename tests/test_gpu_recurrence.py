@@ -335,6 +335,40 @@ def test_another_stream_and_a_captured_graph():
         assert off(a, b) <= tol(F32, 2)
 
 
+def test_long_series_in_pieces():
+    """Few channels, many samples: blocks that take pieces of one series, on
+    another stream, in a captured graph, and with a NaN that reaches the end."""
+    x, z, h0, dh, dl = inputs(1, 6000, 24, BF16, seed=9)
+    n = torch.tensor([5900], device=DEV, dtype=torch.int32)
+    xs = x.clone().requires_grad_(True)
+
+    def step():
+        h, last = gated_scan(xs, z, h0, n)
+        return (h, last, *torch.autograd.grad((h, last), xs, (dh, dl)))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        first = step()
+    torch.cuda.current_stream().wait_stream(s)
+    ref = reference(x, z, h0, n, dh, dl)
+    for got, want, t in zip(first, ref, (BF16, F32, BF16)):
+        assert off(got, want) <= tol(t, 2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        xs.copy_(x * 2)
+    for _ in range(3):
+        graph.replay()
+    for got, want, t in zip(out, reference(x * 2, z, h0, n, dh, dl), (BF16, F32, BF16)):
+        assert off(got, want) <= tol(t, 2)
+    x[0, 100, 3] = float("nan")
+    h, last = gated_scan(x, z, h0, n)
+    bad = torch.zeros(6000, 24, dtype=torch.bool, device=DEV)
+    bad[100:5900, 3] = True
+    assert torch.equal(torch.isnan(h[0]), bad) and torch.equal(torch.isnan(last[0]), bad[5899])
+
+
 def test_refusals():
     x = torch.zeros(2, 5, 4, device=DEV)
     with pytest.raises(ValueError):

@@ -167,3 +167,11 @@ def test_adamw_checks_its_options():
     opt = AdamW(p)
     opt.step()                                         # no gradients: nothing to do
     assert p[0] not in opt.state or not opt.state[p[0]]
+
+
+def test_a_norm_without_residual_has_its_inputs_type():
+    L = _native.lib()
+    a = [2, 0, 0, P, 8, None, 0, P, 4, 8, 1e-6, P, None, None, None]
+    assert L.cpab_b200_rms_norm(*a) == -1 and "without a residual" in err()
+    a = [2, 0, 0, P, 8, None, 0, P, 4, 8, 1e-6, P, P, None, None]
+    assert L.cpab_b200_rms_norm_quantized(*a) == -1 and "without a residual" in err()
