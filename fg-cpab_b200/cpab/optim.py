@@ -1,5 +1,5 @@
-"""AdamW over all tensors of a network in one kernel launch, its states in 32
-or 8 bits.
+"""AdamW over all tensors of a network, one kernel launch for those of one type
+and state kind (256 at most), its states in 32 or 8 bits.
 
     m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2
     p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
@@ -32,7 +32,7 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999
 
 
 def _step(groups, seed, workspace):
-    """One launch over groups of (params, grads, exp_avgs, exp_avg_sqs, scales
+    """One call over groups of (params, grads, exp_avgs, exp_avg_sqs, scales
     or None, steps, lr, betas, eps, weight_decay)."""
     p, g, m, v, sc, st, counts, hyper, lrs = [], [], [], [], [], [], [], [], []
     any_scales = any(q[4] is not None for q in groups)

@@ -1,4 +1,5 @@
-// One AdamW step over many tensors in one launch.
+// One AdamW step over many tensors in few launches: 256 tensors of one type and one
+// kind of states each.
 //
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
@@ -16,6 +17,12 @@
 // The tensors' addresses travel in the kernel's parameters, so nothing is
 // copied to the device first and a captured graph keeps them.  Blocks take runs
 // of chunks of 2048 elements; a chunk belongs to one tensor.
+//
+// With float32 states memory bounds it: 200 million float32 parameters (28 bytes
+// each) take 857 us (6.5 TB/s; a copy: 6.46).  With 8-bit states 16 bytes and
+// about 75 instructions, mostly the integer units' (hash, cut, the near test), are
+// left of a parameter: 627 us (5.1 TB/s), 0.73 of the time for 0.57 of the
+// bytes.  A kernel for all types, branching per tensor, spilled and took 1100 us.
 #include <cuda_fp8.h>
 
 #include <cmath>
@@ -31,8 +38,11 @@ constexpr int kChunkElems = 2048;  // 8 elements a thread, 8 scale blocks
 constexpr int kScaleBlock = 256;   // elements that share a scale: one warp's
 constexpr float kE4m3Max = 448.0f;
 constexpr float kTiny = 1.17549435e-38f;  // 2^-126, the smallest scale
-// Blocks of an SM that the registers leave room for; blocks of a launch per SM
-// at most, if each has kChunksEach chunks (a block's begin is 200 instructions).
+// Blocks of an SM that the registers leave room for (8-bit states: 2, 3 and 4
+// take 701, 622 and 719 us for 200 million); blocks of a launch per SM at most, if
+// each has kChunksEach chunks (a block's begin is 200 instructions: one chunk a
+// block takes 925 us with 8-bit states, 839 against 857 with float32 ones, and
+// 700 against 689 of bfloat16 parameters).
 constexpr int kResident32 = 4, kResident8 = 3, kPerSm32 = 32, kPerSm8 = 6, kChunksEach = 8;
 static_assert(kChunkElems == kThreads * 8 && kScaleBlock == 32 * 8, "a warp holds a scale block");
 
@@ -109,13 +119,15 @@ struct Rates {
 // formulas written as elementary operations, which the tests compare with bit
 // for bit.  The parameter's update goes through the hardware's approximate
 // reciprocal roots (about 2^-22 of an update that is 1e-3 of it); a second moment
-// below 2^-126, which they would flush to 0, counts as 2^-126 there.
+// below 2^-126, which they would flush to 0, counts as 2^-126 there.  One that
+// overflowed has an infinite root (not inf * 0): its parameter only decays.
 __device__ __forceinline__ float update(const Rates &r, float p, float g, float &m, float &v, float &root) {
   m = __fadd_rn(__fmul_rn(m, r.b1), __fmul_rn(g, r.ob1));
   v = __fadd_rn(__fmul_rn(v, r.b2), __fmul_rn(__fmul_rn(g, g), r.ob2));
   const float least = fmaxf(v, kTiny);
   float inverse;
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(least));
+  inverse = fmaxf(inverse, 0x1p-65f);  // (2^-64 is that of the largest number)
   const float den = fmaf(least * inverse, r.root, r.eps);
   root = v * inverse;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(den));

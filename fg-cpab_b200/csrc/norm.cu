@@ -14,6 +14,11 @@
 // shared memory.  The weight's gradient is summed per thread over the rows a
 // block visits, then over blocks in a second kernel in a fixed order (same
 // result every run; no atomics).
+//
+// All of it is bound by memory: 32768x4096 bf16 with a residual moves 1.07 GB
+// each way, the forward in 167 us (6.4 TB/s; a copy: 6.46), the gradient in 192
+// (5.6 TB/s: beside the row it holds its weights' sums, which leaves 768 threads
+// on an SM; in float32, with half as many elements a thread, 6.5).
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -256,7 +261,10 @@ struct Weights {
 };
 
 // T: x and y; S: the stream.  With EDGE blocks stride over rows so that a
-// thread's rows have one shift.
+// thread's rows have one shift.  65537x1536 bf16: 124 us (6.5 TB/s), in 8 bits
+// 134 (5.3 TB/s: half as many registers again for the products with the weights,
+// and the conversions); 65536x999, where rows begin inside a vector: 125 us (one
+// element at a time: 317).
 template <typename T, typename S, int VEC, int NV, bool QUANT, bool EDGE>
 __global__ void __launch_bounds__(kMost, EDGE || QUANT || NV * VEC > 24 ? 2 : 3) k_norm(const __grid_constant__ NormArgs p) {
   __shared__ float shared[2][2 * kMost / 32];
@@ -356,7 +364,8 @@ __global__ void __launch_bounds__(kMost, EDGE || QUANT || NV * VEC > 24 ? 2 : 3)
 }
 
 // x here is the stream s as kept (x itself without a residual), of type S.
-// With t = dy r: dw = sum t s, ds = gs + t w - s (r^2 mean(t w s)).
+// With t = dy r: dw = sum t s, ds = gs + t w - s (r^2 mean(t w s)).  65537x1536
+// bf16: 165 us (4.9 TB/s), 32768x2048 float32: 165 us (6.5 TB/s).
 template <typename T, typename S, int VEC, int NV, bool EDGE, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
     k_norm_backward(const __grid_constant__ NormArgs p) {
@@ -446,7 +455,8 @@ __global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
   }
 }
 
-// dw = the sum over the partial rows, 32 columns a block.
+// dw = the sum over the partial rows, 32 columns a block: 444 rows of 4096
+// columns (7 MB, most of it still in L2) take 5 us beside the gradient's 187.
 template <typename W>
 __global__ void __launch_bounds__(1024) k_norm_weight(const float *partial, int64_t n, int64_t D, W *dw) {
   __shared__ float part[32][33];
@@ -464,7 +474,10 @@ __global__ void __launch_bounds__(1024) k_norm_weight(const float *partial, int6
 }
 
 // A row's vectors and threads: enough threads (a power of two) that each holds
-// at most `held` vectors; one more vector where rows begin inside one.
+// at most `held` vectors; one more vector where rows begin inside one.  Of 1, 2, 3
+// and 4 vectors the forward of 32768x4096 bf16 takes 195, 167, 167 and 185 us,
+// of 65537x1536 158, 140, 124 and 124; the gradient with 1, 2 and 4 346, 192 and
+// 353 us, 220, 165 and 286.
 struct Shape {
   int threads_log2, block, groups;
   int per;            // vectors a thread holds

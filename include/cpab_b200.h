@@ -464,7 +464,7 @@ typedef struct {
   const void *grad;       /* [numel] of dtype                                       */
   void *exp_avg;          /* [numel] float32, or e4m3 codes of the first moment     */
   void *exp_avg_sq;       /* [numel] float32, or e4m3 codes of the second's root    */
-  float *scales;          /* state_bits 8: [ceil(numel / 256), 2] (first moment, root) */
+  float *scales;          /* state_bits 8: [ceil(numel / 256), 2] (first moment, root), 8-byte aligned */
   float *step;            /* steps taken so far, a tensor's own; the call adds 1    */
   const float *lr_device; /* learning rate on the device, or NULL: lr               */
   int64_t numel;
@@ -475,7 +475,7 @@ typedef struct {
 
 /*
  * One AdamW step (decoupled weight decay, bias correction) over `count`
- * tensors (an array in host memory), 256 of them a launch:
+ * tensors (an array in host memory), 256 of one type and state_bits a launch:
  *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
  *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
  * in float32.  8-bit states are e4m3 codes of m and sqrt(v) times one float32

@@ -335,6 +335,23 @@ def test_values_that_are_not_finite():
     assert torch.allclose(p, torch.full_like(p, 0.99))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_an_overflowed_second_moment_stops_its_parameter(dtype):
+    """g^2 beyond float32 with a finite first moment: the update is m / inf = 0,
+    and only the decay is left (bound: three roundings of the parameter)."""
+    p = torch.full((300,), 2.0, device=DEV, dtype=dtype)
+    g = torch.zeros_like(p)
+    g[7] = 1e25
+    m, v, step = torch.zeros(300, device=DEV), torch.zeros(300, device=DEV), torch.zeros((), device=DEV)
+    want = 2.0
+    for _ in range(3):
+        adamw_([p], [g], [m], [v], [step], lr=0.5, weight_decay=0.25)
+        want *= 1.0 - 0.5 * 0.25
+        assert torch.isinf(v[7]) and torch.isfinite(m[7])
+        assert abs(p[7].item() - want) <= want * (3 * 3 * 2.0 ** -24 + 3 * ROUND[dtype])
+        g[7] = 0.0
+
+
 def test_refusals():
     def lists():
         z = lambda dt=F32, n=10: [torch.zeros(n, device=DEV, dtype=dt)]  # noqa: E731
