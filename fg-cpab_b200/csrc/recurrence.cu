@@ -9,7 +9,8 @@
 // A step (a, b): h -> a h + b; two steps compose to (a2 a1, a2 b1 + b2), which
 // is associative.  A block owns a tile of channels of one piece of a series and
 // walks it stage by stage: cp.async brings the next stages into shared memory,
-// each thread reads a segment of kSteps samples of its channels from there and
+// each thread reads a segment of kFwdSteps or
+// kBwdSteps samples of its channels from there and
 // composes them, and the segments' compositions are scanned over the warp
 // (shuffles) and the block (shared memory) to give each segment the state it
 // starts from; a second pass over the registers writes the segment's states.
@@ -29,9 +30,9 @@
 // sample and channel, against 23 and 45 instructions (two of them the special
 // functions'): with tiles enough the blocks issue 72% and 75% of the time and
 // move 5.9 and 5.4 TB/s (64x512x2048 bf16: 69 and 123 us; a copy: 6.46 TB/s).
-// Tiles of 64-byte rows and blocks of 4 warps were the fastest of 32, 64 and 128
-// bytes (64x512x2048 forward 89, 75, 81 us when they were compared): two blocks
-// already fill an SM, so small ones share out evenly.  With few tiles the spread
+// Tiles of 64-byte rows and blocks of 4 warps are the fastest of 32, 64 and 128
+// bytes (64x512x2048: forward 85, 69, 81 us, gradient 141, 123 of 32 and 64).
+// With few tiles the spread
 // over the SMs costs most (16x2048x1024: 512 tiles on 148 SMs, 41 and 71 us,
 // 5.0 and 4.8 TB/s); clusters of blocks that exchange their compositions stage
 // by stage were slower than composing the spans first (1x65536x512: 76 and 143
@@ -398,7 +399,9 @@ __device__ __forceinline__ void wait_for_stage(int ring) {
 
 // The compositions of spans of kSpan samples: forward (A, H) with the state
 // after one A state + H, for the gradient (A, R) with c at its first sample
-// A c + R.  A block takes a span of 32 lanes' channels, a warp a part of it.
+// A c + R.  A block takes a span of 32 lanes' channels, a warp a part of it:
+// 1x65536x512 bf16 is read in about 25 us (134 MB, 5.4 TB/s; what the main kernel reads
+// again comes from L2 in part).
 constexpr int kTotalWarps = 8, kTotalSteps = kSpan / kTotalWarps;
 
 template <typename T>
@@ -520,6 +523,9 @@ __device__ __forceinline__ Lane<V> through_spans(const ScanArgs &p, const At &at
   return c;
 }
 
+// The forward.  Segments of 16 samples: their composition over the warp and the
+// block costs 6 shuffles and 4 reads of shared memory per segment, which 8
+// samples do not pay for.  Two stages in flight: a third costs a block of an SM.
 template <typename T, int LOG2, bool ALIGNED>
 __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_scan(const __grid_constant__ ScanArgs p) {
   constexpr int L = kFwdSteps, V = 4 / sizeof(T), kWarps = warps_of(LOG2);
@@ -637,6 +643,10 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
     store_state(p.last + at.b * p.D, at.d, p.D, carry);
 }
 
+// The gradient.  Both directions are composed in one pass over a stage: from the
+// kept state forward for h_{t-1}, and from the last sample back for c.  a, f, x
+// and dh of a segment stay in registers between, which 8 samples of leave room
+// for (128 registers a thread, no spills).
 template <typename T, int LOG2, bool ALIGNED>
 __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_scan_backward(const __grid_constant__ ScanArgs p) {
   constexpr int L = kBwdSteps, V = 4 / sizeof(T), kWarps = warps_of(LOG2);
@@ -809,7 +819,10 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
 // Series of a few samples (the forward: of up to kChunk where there are channels
 // enough): a thread walks a lane's channels of one series sample by
 // sample, with the loads of M samples in flight.  A tile's blocks would
-// have nothing to split, and spend their time beginning.
+// have nothing to split, and spend their time beginning.  256 series of 4096
+// channels bf16 in place of tiles: 4 samples 58 -> 21 us (gradient 56 -> 20; the
+// host's call alone is 20), 8: 56 -> 21 (60 -> 25), 16: 58 -> 30, 32: 52 -> 49,
+// 64: 98 -> 87 us (4.7 TB/s); the gradient of 16 samples 55 -> 66, so it stops at 8.
 constexpr int kShort = 16;
 
 template <typename T, bool WORDS>
@@ -919,7 +932,9 @@ cudaError_t scan_short(const ScanArgs &a, int64_t B, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
-// One sample of B streams whose states are rows of a table.
+// One sample of B streams whose states are rows of a table.  64x512 bf16 moves
+// 0.5 MB: a launch (2 us on the device) and the host's call (7 us) bound it, so a
+// thread does an element or two and the whole GPU is not needed.
 template <typename T, int VEC>
 __global__ void k_scan_step(const T *x, int64_t xs, const T *gate, int64_t gs, int64_t n, int64_t D,
                             const int32_t *slots, int64_t rows, float *state, T *h) {
@@ -965,6 +980,10 @@ Shape shape_of(int64_t B, int64_t T, int64_t D, int vec, bool back, bool aligned
   // each SM.  A block takes a unit of time per stage and some to begin, longer
   // on an SM that waits for it alone; composing the spans reads as much again
   // as two thirds (the gradient: two fifths) of what the main kernel moves.
+  // In one piece and cut, bf16: 1x65536x512 453 and 71 us (gradient 821 and 104),
+  // 2x32768x1024 232 and 131 (425 and 194), 1x4096x512 32 and 23 (54 and 22),
+  // 4x8192x1024 62 and 64 (118 and 103); but 8x4096x1024 48 and 72 (85 and 105),
+  // 4x8192x2048 91 and 132 (161 and 195), which stay in one.
   const int64_t stage = stage_at(warps), stages = (T + stage - 1) / stage, sms = device_info().sm_count;
   const int64_t tiles = B * s.tiles, spans = (T + kSpan - 1) / kSpan;
   const int64_t full = 16 / warps_of(s.lanes_log2) * sms;
@@ -1011,7 +1030,6 @@ cudaError_t scan_launch(const ScanArgs &a, const Shape &s, int64_t B, cudaStream
 template <typename T, bool BACK>
 cudaError_t scan_as(ScanArgs a, int64_t B, cudaStream_t stream) {
   constexpr int V = 4 / sizeof(T);
-  // (256x16x4096 bf16: forward 66 -> 32 us, gradient 54 -> 66 us; 256x3x4001: 72 -> 19, 75 -> 24 us)
   if (a.T <= 4) return scan_short<T, 4, BACK>(a, B, stream);
   if (a.T <= 8) return scan_short<T, 8, BACK>(a, B, stream);
   // 1024 lanes on each SM keep the forward's loads coming.
