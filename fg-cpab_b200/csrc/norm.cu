@@ -16,7 +16,7 @@
 // result every run; no atomics).
 //
 // All of it is bound by memory: 32768x4096 bf16 with a residual moves 1.07 GB
-// each way, the forward in 167 us (6.4 TB/s; a copy: 6.46), the gradient in 192
+// each way, the forward in 160 us (6.7 TB/s; a copy: 6.46), the gradient in 193
 // (5.6 TB/s: beside the row it holds its weights' sums, which leaves 768 threads
 // on an SM; in float32, with half as many elements a thread, 6.5).
 #include <cuda_fp8.h>
@@ -31,8 +31,8 @@ namespace {
 constexpr int kBlock = 256;        // threads of a block whose rows take fewer
 constexpr int kMost = 512;         // threads of a row at most
 // Threads of an SM that the gradient's registers leave room for, by the elements a
-// thread holds.  (32768x4096 bf16, 16 elements: 228 us at 512 threads, 192 at 768,
-// 225 at 1024; 65536x999 f32, 8 elements: 388, 296 and 260 us.)
+// thread holds.  (32768x4096 bf16, 16 elements: 228 us at 512 threads, 193 at 768,
+// 225 at 1024; 32768x2048 f32, 8 elements: 209, 176 and 165 us.)
 __host__ __device__ constexpr int resident_of(int elements) { return elements <= 8 ? 1024 : elements <= 16 ? 768 : 512; }
 constexpr int64_t kMaxWidth = 16384;
 constexpr float kE4m3Max = 448.0f;
@@ -181,18 +181,18 @@ struct Span {
 
 // Where rows do not begin on a vector, all tensors' rows begin as many elements
 // (`shift`) after one, and the vectors that hold a row are taken as they lie:
-// those at its ends hold elements of the rows beside it too, which are masked.
-// Only past the last row there may be nothing to read.
+// those at its ends hold elements of the rows beside it too, which mask_span makes
+// zeros (later: a thread's loads do not wait for one another).  Only past the last
+// row there may be nothing to read.
 template <typename T, int VEC, bool EDGE>
 __device__ __forceinline__ void load_span(Row<T, VEC> &r, const T *row, const Span &s, bool last) {
-  if (!EDGE || (s.lo == 0 && s.hi == VEC)) {
-    r.load(row + s.c);
-  } else if (!last || s.hi == VEC) {
-    r.load(row + s.c);
-    r.zero_outside(s.lo, s.hi);
-  } else {
-    r.load_some(row + s.c, s.lo, s.hi);
-  }
+  if (EDGE && last && s.hi < VEC) r.load_some(row + s.c, s.lo, s.hi);
+  else r.load(row + s.c);
+}
+
+template <typename T, int VEC, bool EDGE>
+__device__ __forceinline__ void mask_span(Row<T, VEC> &r, const Span &s) {
+  if (EDGE && (s.lo > 0 || s.hi < VEC)) r.zero_outside(s.lo, s.hi);
 }
 
 template <typename T, int VEC, bool EDGE>
@@ -242,60 +242,123 @@ __device__ __forceinline__ Span span_of(int v, int shift, int D) {
   return s;
 }
 
-// Weights of a thread's vectors, kept in registers where its rows all begin
-// alike and they fit, else read from the caches for every row.
-template <typename T, int VEC, int NV, bool EDGE, bool KEEP>
+// Weights of a thread's vectors: where rows begin inside a vector (and so do the
+// weights, as far into one for all of a thread's rows) kept as float32 in shared
+// memory, 16 bytes of each thread side by side; else read from the caches.
+template <typename T, int VEC, int NV, bool EDGE>
 struct Weights {
-  float kept[KEEP ? NV : 1][VEC];
-  __device__ __forceinline__ Weights(const NormArgs &p, int log2, int j, int shift) {
-    if constexpr (KEEP) {
+  static_assert(!EDGE || VEC % 4 == 0, "whole 16 bytes");
+  using Part = Pack<float, 4>;
+  Part *mine;
+  float now[VEC];
+  __device__ __forceinline__ Weights(const NormArgs &p, float *shared, int log2, int j, int shift) {
+    if constexpr (EDGE) {
+      mine = reinterpret_cast<Part *>(shared) + threadIdx.x;
+#pragma unroll(NV <= 4 ? NV : 1)
+      for (int k = 0; k < NV; ++k) {
+        load_weight<T, VEC, EDGE>(p, span_of<VEC, EDGE>((k << log2) + j, shift, (int)p.D), now);
 #pragma unroll
-      for (int k = 0; k < NV; ++k)
-        load_weight<T, VEC, EDGE>(p, span_of<VEC, EDGE>((k << log2) + j, shift, (int)p.D), kept[k]);
+        for (int q = 0; q < VEC; q += 4) mine[(k * VEC + q) / 4 * blockDim.x] = {{now[q], now[q + 1], now[q + 2], now[q + 3]}};
+      }
     }
   }
   __device__ __forceinline__ const float (&of(const NormArgs &p, int k, const Span &at))[VEC] {
-    if (!KEEP) load_weight<T, VEC, EDGE>(p, at, kept[0]);
-    return kept[KEEP ? k : 0];
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int q = 0; q < VEC; q += 4) {
+        const Part part = mine[(k * VEC + q) / 4 * blockDim.x];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) now[q + i] = part.v[i];
+      }
+    } else {
+      load_weight<T, VEC, EDGE>(p, at, now);
+    }
+    return now;
   }
 };
 
+// Bytes of shared memory that Weights takes.
+constexpr size_t weights_bytes(int block, int elements, bool edge) {
+  return edge ? (size_t)block * elements * sizeof(float) : 0;
+}
+
+// Blocks of 512 threads that k_norm's registers should leave room for, and whether
+// there are enough of them to hold what a thread loads of x and the residual
+// (`words` registers) at once.  Early against as they are used, bf16: 32768x4096
+// (16 words) 160 and 167 us, 4096x16384 (32 words, 2 blocks) 85 and 106, 65536x999
+// 105 and 125, in 8 bits 110 and 124; but 65537x1536 (24 words, 3 blocks) 132 and
+// 124, in 8 bits 149 and 134; f32 4096x8192 (32 words, 3 blocks) 112 and 87.
+template <typename T, typename S>
+__host__ __device__ constexpr int words_of(int elements) { return elements * (int)(sizeof(T) + sizeof(S)) / 4; }
+template <typename T, typename S>
+__host__ __device__ constexpr int blocks_of_norm(int vec, int nv, bool quant, bool edge) {
+  if (quant) return 2;
+  if (!edge) return nv * vec > 24 ? 2 : 3;
+  const int words = words_of<T, S>(nv * vec);
+  return words > 48 ? 1 : vec == 4 && words <= 16 ? 3 : 2;
+}
+template <typename T, typename S>
+__host__ __device__ constexpr bool loads_early(int vec, int nv, bool quant, bool edge) {
+  const int words = words_of<T, S>(nv * vec);
+  if (vec == 1) return false;
+  if (quant) return nv * vec <= 16 && words <= (edge ? 16 : 24);
+  const int blocks = blocks_of_norm<T, S>(vec, nv, quant, edge);
+  return blocks == 1 || words <= (blocks == 3 ? 16 : 32);
+}
+
 // T: x and y; S: the stream.  With EDGE blocks stride over rows so that a
-// thread's rows have one shift.  65537x1536 bf16: 124 us (6.5 TB/s), in 8 bits
-// 134 (5.3 TB/s: half as many registers again for the products with the weights,
-// and the conversions); 65536x999, where rows begin inside a vector: 125 us (one
+// thread's rows have one shift.  65537x1536 bf16: 125 us (6.5 TB/s), in 8 bits
+// 136 (5.2 TB/s: it needs half as many registers again for the products with the
+// weights); 65536x999, where rows begin inside a vector: 105 us (5.0 TB/s; one
 // element at a time: 317).
 template <typename T, typename S, int VEC, int NV, bool QUANT, bool EDGE>
-__global__ void __launch_bounds__(kMost, EDGE || QUANT || NV * VEC > 24 ? 2 : 3) k_norm(const __grid_constant__ NormArgs p) {
+__global__ void __launch_bounds__(kMost, blocks_of_norm<T, S>(VEC, NV, QUANT, EDGE)) k_norm(const __grid_constant__ NormArgs p) {
+  extern __shared__ float4 memory[];  // Weights
   __shared__ float shared[2][2 * kMost / 32];
+  // All of a row's loads before its first value is used, where registers allow it.
+  constexpr bool kEarly = loads_early<T, S>(VEC, NV, QUANT, EDGE);
   const int log2 = p.threads_log2, j = threadIdx.x & ((1 << log2) - 1), groups = blockDim.x >> log2;
   const int D = (int)p.D;
   int64_t row = (int64_t)blockIdx.x * groups + (threadIdx.x >> log2);
   const int shift = EDGE ? (int)(row * p.D % VEC) : 0;
-  Weights<T, VEC, NV, EDGE, EDGE && NV * VEC <= 24> weights(p, log2, j, shift);
+  Weights<T, VEC, NV, EDGE> weights(p, reinterpret_cast<float *>(memory), log2, j, shift);
   int half = 0;
   // (as many rounds for each of the block's rows: the sums wait for one another)
   for (int64_t first = (int64_t)blockIdx.x * groups; first < p.rows; first += (int64_t)gridDim.x * groups) {
     const bool on = row < p.rows, last = row == p.rows - 1;
     const T *x = static_cast<const T *>(p.x) + row * p.xs;
     const S *res = static_cast<const S *>(p.res) + row * p.rs;
-    Row<S, VEC> v[QUANT ? 1 : NV];  // the stream as it is kept
-    float t[QUANT ? NV : 1][VEC];   // or times the weights
+    constexpr int kHold = QUANT && !kEarly ? 1 : NV;
+    Row<S, VEC> v[kHold];          // the stream as it is kept
+    Row<T, VEC> in[kEarly ? NV : 1];
+    float t[QUANT ? NV : 1][VEC];  // or times the weights
     float sum = 0.0f, top = 0.0f;
+    auto load = [&](int k, const Span &at) {
+      load_span<T, VEC, EDGE>(in[kEarly ? k : 0], x, at, last);
+      if (p.res != nullptr) load_span<S, VEC, EDGE>(v[k % kHold], res, at, last);
+    };
+    if (kEarly) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
+        if (on && at.any()) load(k, at);
+      }
+    }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
       if (on && at.any()) {
-        Row<S, VEC> &s = v[QUANT ? 0 : k];
-        Row<T, VEC> in;
-        load_span<T, VEC, EDGE>(in, x, at, last);
+        Row<S, VEC> &s = v[k % kHold];
+        Row<T, VEC> &x_k = in[kEarly ? k : 0];
+        if (!kEarly) load(k, at);
+        mask_span<T, VEC, EDGE>(x_k, at);
         if (p.res != nullptr) {
-          load_span<S, VEC, EDGE>(s, res, at, last);
-          add_to(s, in);
+          mask_span<S, VEC, EDGE>(s, at);
+          add_to(s, x_k);
           store_span<S, VEC, EDGE>(static_cast<S *>(p.s) + row * p.D, at, s);
         } else if constexpr (sizeof(T) == sizeof(S)) {
 #pragma unroll
-          for (int i = 0; i < Row<S, VEC>::kWords; ++i) s.w[i] = in.w[i];
+          for (int i = 0; i < Row<S, VEC>::kWords; ++i) s.w[i] = x_k.w[i];
         }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) sum = fmaf(s[i], s[i], sum);
@@ -365,19 +428,21 @@ __global__ void __launch_bounds__(kMost, EDGE || QUANT || NV * VEC > 24 ? 2 : 3)
 
 // x here is the stream s as kept (x itself without a residual), of type S.
 // With t = dy r: dw = sum t s, ds = gs + t w - s (r^2 mean(t w s)).  65537x1536
-// bf16: 165 us (4.9 TB/s), 32768x2048 float32: 165 us (6.5 TB/s).
+// bf16: 165 us (4.9 TB/s), 32768x2048 float32: 165 us (6.5 TB/s), 65536x999 bf16,
+// where rows begin inside a vector: 121 us (4.3 TB/s).
 template <typename T, typename S, int VEC, int NV, bool EDGE, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
     k_norm_backward(const __grid_constant__ NormArgs p) {
   // Of wide rows a thread holds too much to fetch gs early.
   constexpr bool kLean = NV * VEC > 16;
-  extern __shared__ float sums[];  // [groups, D] where a block has several groups
+  extern __shared__ float4 memory[];  // Weights, then [groups, D] where a block has several groups
+  float *sums = reinterpret_cast<float *>(memory);
   __shared__ float shared[2][kMost / 32];
   const int log2 = p.threads_log2, j = threadIdx.x & ((1 << log2) - 1), groups = BLOCK >> log2;
   const int group = threadIdx.x >> log2, D = (int)p.D;
   int64_t row = (int64_t)blockIdx.x * groups + group;
   const int shift = EDGE ? (int)(row * p.D % VEC) : 0;
-  Weights<T, VEC, NV, EDGE, EDGE && NV * VEC <= 8> weights(p, log2, j, shift);
+  Weights<T, VEC, NV, EDGE> weights(p, sums, log2, j, shift);
   float dw[NV][VEC];
 #pragma unroll
   for (int k = 0; k < NV; ++k)
@@ -406,6 +471,8 @@ __global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
     for (int k = 0; k < NV; ++k) {
       const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
       if (on && at.any()) {
+        mask_span<S, VEC, EDGE>(v[k], at);
+        mask_span<T, VEC, EDGE>(g[k], at);
         const float (&w)[VEC] = weights.of(p, k, at);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
@@ -437,6 +504,7 @@ __global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
     row += (int64_t)gridDim.x * groups;
   }
   if (p.partial == nullptr) return;
+  if (EDGE && groups > 1) __syncthreads();  // (the last row's weights have been read)
   // The block's groups hold the same columns: added one after another.
   float *to = groups > 1 ? sums + group * D : p.partial + (int64_t)blockIdx.x * D;
 #pragma unroll
@@ -456,7 +524,7 @@ __global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
 }
 
 // dw = the sum over the partial rows, 32 columns a block: 444 rows of 4096
-// columns (7 MB, most of it still in L2) take 5 us beside the gradient's 187.
+// columns (7 MB) take 7 us beside the gradient's 188.
 template <typename W>
 __global__ void __launch_bounds__(1024) k_norm_weight(const float *partial, int64_t n, int64_t D, W *dw) {
   __shared__ float part[32][33];
@@ -512,20 +580,33 @@ int64_t blocks_of(int64_t rows, const Shape &s, int vec, bool edge, bool residen
   return n;
 }
 
+// Lets a kernel have that much dynamic shared memory (4 KB beside it are its own).
+cudaError_t more_shared(const void *kernel, size_t bytes) {
+  if (bytes <= 44 * 1024) return cudaSuccess;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
 template <typename T, typename S, int VEC, int NV, bool EDGE>
 cudaError_t norm_launch(const NormArgs &a, const Shape &s, bool quant, cudaStream_t stream) {
   const unsigned grid = (unsigned)blocks_of(a.rows, s, VEC, EDGE, false);
-  if (quant) k_norm<T, S, VEC, NV, true, EDGE><<<grid, s.block, 0, stream>>>(a);
-  else k_norm<T, S, VEC, NV, false, EDGE><<<grid, s.block, 0, stream>>>(a);
+  const size_t smem = weights_bytes(s.block, NV * VEC, EDGE);
+  const auto kernel = quant ? k_norm<T, S, VEC, NV, true, EDGE> : k_norm<T, S, VEC, NV, false, EDGE>;
+  const cudaError_t e = more_shared(reinterpret_cast<const void *>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<grid, s.block, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
 template <typename T, typename S, int VEC, int NV, bool EDGE>
 cudaError_t norm_backward_launch(const NormArgs &a, const Shape &s, cudaStream_t stream) {
   const unsigned grid = (unsigned)blocks_of(a.rows, s, VEC, EDGE, true);
-  const size_t smem = s.groups > 1 ? (size_t)s.groups * a.D * sizeof(float) : 0;
-  if (s.block == kBlock) k_norm_backward<T, S, VEC, NV, EDGE, kBlock><<<grid, kBlock, smem, stream>>>(a);
-  else k_norm_backward<T, S, VEC, NV, EDGE, kMost><<<grid, kMost, smem, stream>>>(a);
+  const size_t sums = s.groups > 1 ? (size_t)s.groups * a.D * sizeof(float) : 0;
+  const size_t weights = weights_bytes(s.block, NV * VEC, EDGE), smem = sums > weights ? sums : weights;
+  const auto kernel = s.block == kBlock ? k_norm_backward<T, S, VEC, NV, EDGE, kBlock>
+                                        : k_norm_backward<T, S, VEC, NV, EDGE, kMost>;
+  const cudaError_t e = more_shared(reinterpret_cast<const void *>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<grid, s.block, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
