@@ -9,11 +9,10 @@
 // A step (a, b): h -> a h + b; two steps compose to (a2 a1, a2 b1 + b2), which
 // is associative.  A block owns a tile of channels of one piece of a series and
 // walks it stage by stage: cp.async brings the next stages into shared memory,
-// each thread reads a segment of kFwdSteps or
-// kBwdSteps samples of its channels from there and
-// composes them, and the segments' compositions are scanned over the warp
-// (shuffles) and the block (shared memory) to give each segment the state it
-// starts from; a second pass over the registers writes the segment's states.
+// each thread reads a segment of kFwdSteps or kBwdSteps samples of its channels
+// from there and composes them, and the segments' compositions are scanned over
+// the warp (shuffles) and the block (shared memory) to give each segment the state
+// it starts from; a second pass over the registers writes the segment's states.
 //
 // A series is one piece where there are tiles enough to fill the GPU.  Else a
 // kernel before composes every kSpan samples, and a block begins at the state
@@ -27,16 +26,15 @@
 // cost more bytes and lose the difference h_{t-1} - x_t where it is small).
 //
 // What bounds it.  In 16 bits the forward moves 6 and the gradient 10 bytes per
-// sample and channel, against 23 and 45 instructions (two of them the special
+// sample and channel, against 24 and 47 instructions (two of them the special
 // functions'): with tiles enough the blocks issue 72% and 75% of the time and
 // move 5.9 and 5.4 TB/s (64x512x2048 bf16: 69 and 123 us; a copy: 6.46 TB/s).
 // Tiles of 64-byte rows and blocks of 4 warps are the fastest of 32, 64 and 128
 // bytes (64x512x2048: forward 85, 69, 81 us, gradient 141, 123 of 32 and 64).
-// With few tiles the spread
-// over the SMs costs most (16x2048x1024: 512 tiles on 148 SMs, 41 and 71 us,
-// 5.0 and 4.8 TB/s); clusters of blocks that exchange their compositions stage
-// by stage were slower than composing the spans first (1x65536x512: 76 and 143
-// us with the best cluster sizes, 71 and 104 with spans).
+// With few tiles the spread over the SMs costs most (16x2048x1024: 512 tiles on
+// 148 SMs, 41 and 71 us, 5.0 and 4.8 TB/s); clusters of blocks that exchange their
+// compositions stage by stage were slower than composing the spans first
+// (1x65536x512: 76 and 143 us with the best cluster sizes, 67 and 97 with spans).
 #include <type_traits>
 
 #include "sequence.cuh"
@@ -47,7 +45,10 @@ namespace {
 constexpr int kChunk = 64;     // samples between two kept states
 constexpr int kFwdSteps = 16;  // samples of a thread's segment (divide kChunk)
 constexpr int kBwdSteps = 8;
-constexpr int kSpan = 512;     // samples composed together where a series is cut into pieces
+// Samples composed together where a series is cut into pieces, of which these are
+// multiples (128, 256, 512 samples: 1x65536x512 bf16 70, 67, 70 us, gradient 102, 97,
+// 103; 3x9000x333 42, 48, 56; 1x65536x256 f32 72, 66, 64, gradient 112, 96, 91).
+constexpr int kSpan = 256;
 static_assert(kChunk % kFwdSteps == 0 && kChunk % kBwdSteps == 0, "states start segments");
 // Warps of a full block with 2^log2 lanes along the channels: a stage has 8
 // segments.
@@ -400,8 +401,9 @@ __device__ __forceinline__ void wait_for_stage(int ring) {
 // The compositions of spans of kSpan samples: forward (A, H) with the state
 // after one A state + H, for the gradient (A, R) with c at its first sample
 // A c + R.  A block takes a span of 32 lanes' channels, a warp a part of it:
-// 1x65536x512 bf16 is read in about 25 us (134 MB, 5.4 TB/s; what the main kernel reads
-// again comes from L2 in part).
+// 1x65536x512 bf16 in 30 us (134 MB, 4.5 TB/s, 65% of the issue slots), read once
+// more by the main kernel.  The spans that no piece needs (those of
+// the last piece, for the gradient of the first) are left out.
 constexpr int kTotalWarps = 8, kTotalSteps = kSpan / kTotalWarps;
 
 template <typename T>
@@ -409,6 +411,13 @@ __device__ __forceinline__ uint32_t load_word(const T *row, int n, bool words) {
   if (sizeof(T) == 4 || words) return *reinterpret_cast<const uint32_t *>(row);
   const unsigned short *q = reinterpret_cast<const unsigned short *>(row);
   return q[0] | (n > 1 ? (uint32_t)q[1] << 16 : 0u);
+}
+
+// How many of a series' spans are composed: those before its last piece, for the
+// gradient those after its first.
+template <bool BACK>
+__host__ __device__ __forceinline__ int64_t spans_needed(const ScanArgs &p) {
+  return BACK ? (p.T + kSpan - 1) / kSpan - p.piece / kSpan : (p.pieces - 1) * (p.piece / kSpan);
 }
 
 template <typename T, bool BACK>
@@ -420,7 +429,7 @@ __global__ void __launch_bounds__(kTotalWarps * 32) k_scan_totals(const __grid_c
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t tiles = (p.D + 32 * V - 1) / (32 * V), spans = (p.T + kSpan - 1) / kSpan;
   const int64_t c = blockIdx.x / tiles, d = (blockIdx.x % tiles) * (32 * V) + lane * V;
-  const int64_t b = c / spans, span = c % spans;
+  const int64_t needed = spans_needed<BACK>(p), b = c / needed, span = c % needed + (BACK ? spans - needed : 0);
   const int n = (int)min(p.D - d, (int64_t)V);
   int len = (int)p.T;
   if (p.lengths != nullptr) len = min(max(p.lengths[b], 0), len);
@@ -980,9 +989,9 @@ Shape shape_of(int64_t B, int64_t T, int64_t D, int vec, bool back, bool aligned
   // each SM.  A block takes a unit of time per stage and some to begin, longer
   // on an SM that waits for it alone; composing the spans reads as much again
   // as two thirds (the gradient: two fifths) of what the main kernel moves.
-  // In one piece and cut, bf16: 1x65536x512 453 and 71 us (gradient 821 and 104),
-  // 2x32768x1024 232 and 131 (425 and 194), 1x4096x512 32 and 23 (54 and 22),
-  // 4x8192x1024 62 and 64 (118 and 103); but 8x4096x1024 48 and 72 (85 and 105),
+  // In one piece and cut, bf16: 1x65536x512 453 and 67 us (gradient 821 and 97),
+  // 2x32768x1024 232 and 130 (425 and 187), 1x4096x512 32 and 23 (54 and 22),
+  // 4x8192x1024 62 and 65 (118 and 99); but 8x4096x1024 48 and 72 (85 and 105),
   // 4x8192x2048 91 and 132 (161 and 195), which stay in one.
   const int64_t stage = stage_at(warps), stages = (T + stage - 1) / stage, sms = device_info().sm_count;
   const int64_t tiles = B * s.tiles, spans = (T + kSpan - 1) / kSpan;
@@ -1014,8 +1023,8 @@ cudaError_t scan_launch(const ScanArgs &a, const Shape &s, int64_t B, cudaStream
   cudaLaunchConfig_t c{};
   cudaLaunchAttribute attr{};
   if (s.pieces > 1) {  // begins, and fetches its first stages, while the pieces are composed
-    const int64_t vec = 4 / sizeof(T), tiles = (a.D + 32 * vec - 1) / (32 * vec), spans = (a.T + kSpan - 1) / kSpan;
-    k_scan_totals<T, BACK><<<(unsigned)(B * spans * tiles), kTotalWarps * 32, 0, stream>>>(a);
+    const int64_t vec = 4 / sizeof(T), tiles = (a.D + 32 * vec - 1) / (32 * vec);
+    k_scan_totals<T, BACK><<<(unsigned)(B * spans_needed<BACK>(a) * tiles), kTotalWarps * 32, 0, stream>>>(a);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -369,9 +369,9 @@ typedef enum { CPAB_F32 = 0, CPAB_F16 = 1, CPAB_BF16 = 2 } cpab_dtype;
  * from the state h0 ([B, D] float32, NULL: zeros).  x and gate are [B, T, D]
  * with the given strides of series and samples (so both may be halves of one
  * projection); h is [B, T, D] contiguous, of the same type; the state is
- * float32 throughout.  T may be up to 2^31 - 4096, B * D up to 2^30.  lengths ([B] int32, NULL: all T; values outside [0, T]
- * are taken as 0 or T): samples from a series' length on are not read and
- * their h is 0.  h_last ([B, D] float32, may be NULL) receives the state after
+ * float32 throughout.  T may be up to 2^31 - 4096, B * D up to 2^30.  lengths
+ * ([B] int32, NULL: all T; values outside [0, T] are taken as 0 or T): samples
+ * from a series' length on are not read and their h is 0.  h_last ([B, D] float32, may be NULL) receives the state after
  * the last sample.  states ([B, ceil(T / c), D] float32 with c =
  * cpab_b200_gated_scan_chunk(), may be NULL) receives the states that
  * cpab_b200_gated_scan_backward needs.  workspace: 8-byte aligned,
