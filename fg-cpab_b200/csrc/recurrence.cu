@@ -51,8 +51,10 @@ constexpr int kBwdSteps = 8;
 constexpr int kSpan = 256;
 static_assert(kChunk % kFwdSteps == 0 && kChunk % kBwdSteps == 0, "states start segments");
 // Warps of a full block with 2^log2 lanes along the channels: a stage has 8
-// segments.
+// segments (16 in blocks of 8 warps, for tiles that are too few to keep 4 blocks on
+// an SM).  16 warps fit on an SM.
 __host__ __device__ constexpr int warps_of(int log2) { return log2 == 4 ? 4 : 2; }
+constexpr int kWide = 8, kResidentWarps = 16;
 static_assert((8 * kBwdSteps) % kChunk == 0, "a full block's stage starts on a kept state");
 
 struct ScanArgs {
@@ -244,10 +246,10 @@ __device__ __forceinline__ Rows<T> rows_of(const void *tensor, int64_t at, int64
 
 // copy_stage for the stages of a full block whose rows start on 16 bytes and
 // are all there, with what a thread's addresses have in common kept.
-template <typename T, int L, int LOG2>
+template <typename T, int L, int LOG2, int WARPS>
 struct Feed {
   using S = Stage<L, LOG2, true>;
-  static constexpr int kThreads = warps_of(LOG2) * 32, kRows = kThreads / S::kCopies;  // rows copied at a time
+  static constexpr int kThreads = WARPS * 32, kRows = kThreads / S::kCopies;  // rows copied at a time
   static_assert(kRows % L == 0, "a thread's rows lie equally far apart in shared memory");
   const char *src;          // the thread's first copy of the next stage
   int64_t row_step, stage_step;
@@ -535,9 +537,9 @@ __device__ __forceinline__ Lane<V> through_spans(const ScanArgs &p, const At &at
 // The forward.  Segments of 16 samples: their composition over the warp and the
 // block costs 6 shuffles and 4 reads of shared memory per segment, which 8
 // samples do not pay for.  Two stages in flight: a third costs a block of an SM.
-template <typename T, int LOG2, bool ALIGNED>
-__global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_scan(const __grid_constant__ ScanArgs p) {
-  constexpr int L = kFwdSteps, V = 4 / sizeof(T), kWarps = warps_of(LOG2);
+template <typename T, int LOG2, int WARPS, bool ALIGNED>
+__global__ void __launch_bounds__(WARPS * 32, kResidentWarps / WARPS) k_scan(const __grid_constant__ ScanArgs p) {
+  constexpr int L = kFwdSteps, V = 4 / sizeof(T), kWarps = WARPS;
   using At = Place<L, LOG2, V>;
   extern __shared__ uint4 ring_memory[];
   __shared__ float2 warp_total[kWarps][At::kLanes][V], span_total[kWarps * 32][V];
@@ -553,8 +555,8 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
   uint32_t *ring = reinterpret_cast<uint32_t *>(ring_memory);
 
   const bool whole = ALIGNED && blockDim.x == kWarps * 32 && at.channels == At::kLanes * V;
-  Feed<T, L, LOG2> x_feed(x, at.first, at.stage, 1), g_feed(g, at.first, at.stage, 1);
-  const uint32_t place = shared_address(ring) + Feed<T, L, LOG2>::place();
+  Feed<T, L, LOG2, WARPS> x_feed(x, at.first, at.stage, 1), g_feed(g, at.first, at.stage, 1);
+  const uint32_t place = shared_address(ring) + Feed<T, L, LOG2, WARPS>::place();
   auto fetch = [&](int k, int slot) {
     if (k < at.live) {
       const int s0 = at.first + k * at.stage;
@@ -656,9 +658,9 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
 // kept state forward for h_{t-1}, and from the last sample back for c.  a, f, x
 // and dh of a segment stay in registers between, which 8 samples of leave room
 // for (128 registers a thread, no spills).
-template <typename T, int LOG2, bool ALIGNED>
-__global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_scan_backward(const __grid_constant__ ScanArgs p) {
-  constexpr int L = kBwdSteps, V = 4 / sizeof(T), kWarps = warps_of(LOG2);
+template <typename T, int LOG2, int WARPS, bool ALIGNED>
+__global__ void __launch_bounds__(WARPS * 32, kResidentWarps / WARPS) k_scan_backward(const __grid_constant__ ScanArgs p) {
+  constexpr int L = kBwdSteps, V = 4 / sizeof(T), kWarps = WARPS;
   using At = Place<L, LOG2, V>;
   extern __shared__ uint4 ring_memory[];
   __shared__ float2 up_total[kWarps][At::kLanes][V], down_total[kWarps][At::kLanes][V];
@@ -679,8 +681,8 @@ __global__ void __launch_bounds__(warps_of(LOG2) * 32, 16 / warps_of(LOG2)) k_sc
   // Stage k counts from the last one with samples back.
   const int s_last = at.first + (at.live - 1) * at.stage;
   const bool whole = ALIGNED && blockDim.x == kWarps * 32 && at.channels == At::kLanes * V && p.grad_h != nullptr;
-  Feed<T, L, LOG2> x_feed(x, s_last, at.stage, -1), g_feed(g, s_last, at.stage, -1), d_feed(dh, s_last, at.stage, -1);
-  const uint32_t place = shared_address(ring) + Feed<T, L, LOG2>::place();
+  Feed<T, L, LOG2, WARPS> x_feed(x, s_last, at.stage, -1), g_feed(g, s_last, at.stage, -1), d_feed(dh, s_last, at.stage, -1);
+  const uint32_t place = shared_address(ring) + Feed<T, L, LOG2, WARPS>::place();
   auto fetch = [&](int k, int slot) {
     if (k < at.live) {
       const int s0 = s_last - k * at.stage;
@@ -971,7 +973,7 @@ __global__ void k_scan_step(const T *x, int64_t xs, const T *gate, int64_t gs, i
 
 // How a launch covers the series.
 struct Shape {
-  int lanes_log2, threads, ring, smem;
+  int lanes_log2, full_warps, threads, ring, smem;
   int64_t tiles, piece, pieces;
 };
 
@@ -982,29 +984,39 @@ Shape shape_of(int64_t B, int64_t T, int64_t D, int vec, bool back, bool aligned
   s.lanes_log2 = D <= 8 * vec ? 3 : 4;
   s.tiles = (D + ((int64_t)vec << s.lanes_log2) - 1) / ((int64_t)vec << s.lanes_log2);
   auto stage_at = [&](int warps) { return (int64_t)warps * (32 >> s.lanes_log2) * steps; };
+  s.full_warps = warps_of(s.lanes_log2);
   int warps = 1;
-  while (warps < warps_of(s.lanes_log2) && stage_at(warps) < T) warps *= 2;
-  s.threads = warps * 32;
+  while (warps < s.full_warps && stage_at(warps) < T) warps *= 2;
   // One piece, or as many as give four blocks (what its registers hold) to
   // each SM.  A block takes a unit of time per stage and some to begin, longer
   // on an SM that waits for it alone; composing the spans reads as much again
   // as two thirds (the gradient: two fifths) of what the main kernel moves.
   // In one piece and cut, bf16: 1x65536x512 453 and 67 us (gradient 821 and 97),
   // 2x32768x1024 232 and 130 (425 and 187), 1x4096x512 32 and 23 (54 and 22),
-  // 4x8192x1024 62 and 65 (118 and 99); but 8x4096x1024 48 and 72 (85 and 105),
+  // 6x8192x1024 84 and 92 (150 and 129); but 8x4096x1024 48 and 72 (85 and 105),
   // 4x8192x2048 91 and 132 (161 and 195), which stay in one.
-  const int64_t stage = stage_at(warps), stages = (T + stage - 1) / stage, sms = device_info().sm_count;
+  // Blocks of 4 and of 8 warps where an SM has two tiles at most, in one piece:
+  // 8x16384x1024 177 and 157 us (gradient 316 and 304), 4x8192x2048 92 and 85 (162 and
+  // 153), 8x8192x999 215 and 165 (352 and 286); but 16x2048x1024 41 and 46 (71 and 81).
+  const int64_t stages = (T + stage_at(warps) - 1) / stage_at(warps), sms = device_info().sm_count;
   const int64_t tiles = B * s.tiles, spans = (T + kSpan - 1) / kSpan;
-  const int64_t full = 16 / warps_of(s.lanes_log2) * sms;
+  const int64_t full = kResidentWarps / s.full_warps * sms;
   int64_t each = (spans * tiles + full - 1) / full;  // spans of a piece
   const double share = (double)(tiles * stages) / (double)sms;
   const int64_t fullest = (tiles + sms - 1) / sms;
-  const double whole = (double)fullest * (double)(stages + 1) * (fullest == 1 ? 1.4 : 1.0);
-  s.piece = stages * stage, s.pieces = 1;
+  const bool wide = s.lanes_log2 == 4 && fullest <= 2 && T >= 2 * stage_at(kWide);
+  const double whole = (double)fullest * (double)(stages + 1) * (fullest == 1 ? 1.4 : 1.0) *
+                       (wide && !back ? 0.88 : 1.0);
+  s.pieces = 1;
   if (spans > 1 && tiles < full && share * (back ? 1.4 : 1.67) + 8.0 < whole && each < spans) {
     s.piece = each * kSpan;
     s.pieces = (T + s.piece - 1) / s.piece;
+  } else if (wide) {
+    s.full_warps = warps = kWide;
   }
+  s.threads = warps * 32;
+  const int64_t stage = stage_at(warps);
+  if (s.pieces == 1) s.piece = (T + stage - 1) / stage * stage;
   const int64_t rounds = s.piece / stage;
   const int ring = back ? 3 : 2;
   s.ring = (int)(rounds < ring ? rounds : ring);
@@ -1012,11 +1024,11 @@ Shape shape_of(int64_t B, int64_t T, int64_t D, int vec, bool back, bool aligned
   return s;
 }
 
-template <typename T, int LOG2, bool BACK, bool ALIGNED>
+template <typename T, int LOG2, int WARPS, bool BACK, bool ALIGNED>
 cudaError_t scan_launch(const ScanArgs &a, const Shape &s, int64_t B, cudaStream_t stream) {
-  const auto kernel = BACK ? k_scan_backward<T, LOG2, ALIGNED> : k_scan<T, LOG2, ALIGNED>;
+  const auto kernel = BACK ? k_scan_backward<T, LOG2, WARPS, ALIGNED> : k_scan<T, LOG2, WARPS, ALIGNED>;
   cudaError_t e = cudaSuccess;
-  if (s.smem > 44 * 1024) {  // (4 KB beside it are the kernel's own)
+  if (s.smem > 40 * 1024) {  // (8 KB beside it are the kernel's own)
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem);
     if (e != cudaSuccess) return e;
   }
@@ -1036,6 +1048,13 @@ cudaError_t scan_launch(const ScanArgs &a, const Shape &s, int64_t B, cudaStream
   return cudaLaunchKernelEx(&c, kernel, a);
 }
 
+template <typename T, bool BACK, bool ALIGNED>
+cudaError_t scan_shape(const ScanArgs &a, const Shape &s, int64_t B, cudaStream_t stream) {
+  if (s.lanes_log2 == 3) return scan_launch<T, 3, warps_of(3), BACK, ALIGNED>(a, s, B, stream);
+  if (s.full_warps == kWide) return scan_launch<T, 4, kWide, BACK, ALIGNED>(a, s, B, stream);
+  return scan_launch<T, 4, warps_of(4), BACK, ALIGNED>(a, s, B, stream);
+}
+
 template <typename T, bool BACK>
 cudaError_t scan_as(ScanArgs a, int64_t B, cudaStream_t stream) {
   constexpr int V = 4 / sizeof(T);
@@ -1046,11 +1065,7 @@ cudaError_t scan_as(ScanArgs a, int64_t B, cudaStream_t stream) {
     return scan_short<T, kShort, false>(a, B, stream);
   const Shape s = shape_of(B, a.T, a.D, V, BACK, a.aligned);
   a.tiles = s.tiles, a.piece = s.piece, a.pieces = (int)s.pieces, a.ring = s.ring;
-  if (a.aligned)
-    return s.lanes_log2 == 4 ? scan_launch<T, 4, BACK, true>(a, s, B, stream)
-                             : scan_launch<T, 3, BACK, true>(a, s, B, stream);
-  return s.lanes_log2 == 4 ? scan_launch<T, 4, BACK, false>(a, s, B, stream)
-                           : scan_launch<T, 3, BACK, false>(a, s, B, stream);
+  return a.aligned ? scan_shape<T, BACK, true>(a, s, B, stream) : scan_shape<T, BACK, false>(a, s, B, stream);
 }
 
 // Fills in what the kernels need to know of the inputs' and outputs' places.

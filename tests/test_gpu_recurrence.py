@@ -369,6 +369,26 @@ def test_long_series_in_pieces():
     assert torch.equal(torch.isnan(h[0]), bad) and torch.equal(torch.isnan(last[0]), bad[5899])
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("channels", [512, 509])
+@pytest.mark.parametrize("length", [640, 1111])
+def test_one_or_two_tiles_on_an_sm(dtype, channels, length):
+    """Tiles enough for a GPU's SMs but not for several on each: wide blocks,
+    whole and ragged, rows on and off 16 bytes."""
+    B = 10 if dtype == F32 else 12                        # 150 to 320 tiles
+    D = channels if dtype != F32 else channels // 2
+    x, z, h0, dh, dl = inputs(B, length, D, dtype, seed=11)
+    n = torch.randint(0, length + 1, (B,), generator=torch.Generator().manual_seed(2)).int().to(DEV)
+    n[:4] = torch.tensor([0, 1, length, length - 1], dtype=torch.int32)
+    leaves = [t.requires_grad_(True) for t in (x, z, h0)]
+    h, last = gated_scan(x, z, h0, n)
+    grads = torch.autograd.grad((h, last), leaves, (dh, dl))
+    ref = reference(x.detach(), z.detach(), h0.detach(), n, dh, dl)
+    assert off(h, ref[0]) <= tol(dtype) and off(last, ref[1]) <= tol(F32)
+    for g, r, t in zip(grads, ref[2:], (dtype, dtype, F32)):
+        assert off(g, r) <= tol(t, 2)
+
+
 def test_refusals():
     x = torch.zeros(2, 5, 4, device=DEV)
     with pytest.raises(ValueError):
