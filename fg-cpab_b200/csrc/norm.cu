@@ -433,8 +433,11 @@ __global__ void __launch_bounds__(kMost, blocks_of_norm<T, S>(VEC, NV, QUANT, ED
 template <typename T, typename S, int VEC, int NV, bool EDGE, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
     k_norm_backward(const __grid_constant__ NormArgs p) {
-  // Of wide rows a thread holds too much to fetch gs early.
-  constexpr bool kLean = NV * VEC > 16;
+  // Of wide rows a thread holds too much to fetch gs early, and of them and of a
+  // float32 stream beside 16 bits also to keep the products dy r w (4096x9001 f32:
+  // 344 us, again from the weights 224; 32768x4096 bf16 and f32 360 and 335; but
+  // bf16 alone 195 and 211).
+  constexpr bool kLean = NV * VEC > 16, kAgain = kLean || sizeof(T) != sizeof(S);
   extern __shared__ float4 memory[];  // Weights, then [groups, D] where a block has several groups
   float *sums = reinterpret_cast<float *>(memory);
   __shared__ float shared[2][kMost / 32];
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
         if (!kLean && p.gs != nullptr) load_span<S, VEC, EDGE>(a[k], gs, at, last);
       }
     }
-    float tw[NV][VEC];
+    float tw[kAgain ? 1 : NV][VEC];
     float sum = 0.0f, none = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -478,8 +481,8 @@ __global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
         for (int i = 0; i < VEC; ++i) {
           const float t = g[k][i] * r, s = v[k][i];
           dw[k][i] = fmaf(t, s, dw[k][i]);
-          tw[k][i] = t * w[i];
-          sum = fmaf(tw[k][i], s, sum);
+          tw[kAgain ? 0 : k][i] = t * w[i];
+          sum = fmaf(tw[kAgain ? 0 : k][i], s, sum);
         }
       }
     }
@@ -491,14 +494,20 @@ __global__ void __launch_bounds__(BLOCK, resident_of(NV * VEC) / BLOCK)
       const Span at = span_of<VEC, EDGE>((k << log2) + j, shift, D);
       if (on && at.any()) {
         if (kLean && p.gs != nullptr) load_span<S, VEC, EDGE>(a[0], gs, at, last);
+        float (&d)[VEC] = tw[kAgain ? 0 : k];
+        if constexpr (kAgain) {
+          const float (&w)[VEC] = weights.of(p, k, at);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) tw[k][i] = fmaf(v[k][i], m, tw[k][i]);
+          for (int i = 0; i < VEC; ++i) d[i] = g[k][i] * r * w[i];
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) d[i] = fmaf(v[k][i], m, d[i]);
         if (p.gs != nullptr) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) tw[k][i] += a[kLean ? 0 : k][i];
+          for (int i = 0; i < VEC; ++i) d[i] += a[kLean ? 0 : k][i];
         }
-        store_span<T, VEC, EDGE>(static_cast<T *>(p.dx) + row * p.D, at, tw[k]);
-        if (p.dres != nullptr) store_span<S, VEC, EDGE>(static_cast<S *>(p.dres) + row * p.D, at, tw[k]);
+        store_span<T, VEC, EDGE>(static_cast<T *>(p.dx) + row * p.D, at, d);
+        if (p.dres != nullptr) store_span<S, VEC, EDGE>(static_cast<S *>(p.dres) + row * p.D, at, d);
       }
     }
     row += (int64_t)gridDim.x * groups;
