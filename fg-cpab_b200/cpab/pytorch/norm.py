@@ -37,8 +37,9 @@ class _RmsNorm(torch.autograd.Function):
         return (y,) if s is None else (y, s)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy, gs=None):
+        if torch.is_grad_enabled():
+            raise RuntimeError("rms_norm can be differentiated once only (create_graph=True)")
         s, weight, rstd = ctx.saved_tensors
         if gy is None:
             return (gs.to(ctx.x_type) if gs is not None else None), None, gs, None

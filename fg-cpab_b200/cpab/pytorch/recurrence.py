@@ -56,8 +56,9 @@ class _GatedScan(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dlast):
+        if torch.is_grad_enabled():
+            raise RuntimeError("gated_scan can be differentiated once only (create_graph=True)")
         if dh is None and dlast is None:
             return None, None, None, None
         x, gate, states, lengths = ctx.saved_tensors

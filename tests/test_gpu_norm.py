@@ -240,6 +240,15 @@ def test_refusals():
         torch.autograd.grad(g.sum(), x)
 
 
+def test_the_python_node_refuses_a_second_gradient_too():
+    x, w = torch.ones(3, 8, device=DEV, requires_grad=True), torch.ones(8, device=DEV)
+    with _ext.python_path():
+        y = rms_norm(x, w)
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad((y * x).sum(), x, create_graph=True)
+        torch.autograd.grad((y * x).sum(), x)
+
+
 def test_offsets_past_32_bits():
     n, D = (1 << 17) + 5, 16384
     x = torch.empty(n, D, device=DEV, dtype=BF16).normal_()

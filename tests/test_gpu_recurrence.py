@@ -389,6 +389,16 @@ def test_one_or_two_tiles_on_an_sm(dtype, channels, length):
         assert off(g, r) <= tol(t, 2)
 
 
+def test_the_python_node_refuses_a_second_gradient_too():
+    x, z, h0, _, _ = inputs(2, 9, 8, F32)
+    x.requires_grad_(True)
+    with _ext.python_path():
+        h, _ = gated_scan(x, z, h0)
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad((h * x).sum(), x, create_graph=True)
+        torch.autograd.grad((h * x).sum(), x)
+
+
 def test_refusals():
     x = torch.zeros(2, 5, 4, device=DEV)
     with pytest.raises(ValueError):
