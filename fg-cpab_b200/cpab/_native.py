@@ -695,6 +695,10 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, scales, steps, counts, hyper, lr
     if not (len(params) == len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(steps)) or \
             len(scales) not in (0, len(params)):
         raise ValueError("adamw: lists of different lengths")
+    if any(lr is not None and (lr.device != device or lr.dtype != torch.float32 or lr.numel() != 1)
+           for lr in lrs):
+        raise RuntimeError("adamw: a learning rate on the device must be one float32 on the "
+                           "parameters' device, %s" % device)
     table, alive, k = (_AdamWTensor * len(params))(), [], 0
     for group, n in enumerate(counts):
         for _ in range(n):

@@ -23,8 +23,8 @@ def adamw_(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999
     steps taken so far, counted up by the call.  A parameter's states are both
     float32, or both float8_e4m3fn codes (exp_avg_sqs then holds those of the
     second moment's square root) with scales[i] float32 [ceil(numel / 256), 2]
-    (columns: first moment, root).  lr: a number, or one float32 on the device
-    (a schedule inside a captured graph).  seed chooses the random bits of the
+    (columns: first moment, root).  lr: a number, or one float32 on the params'
+    device (a schedule inside a captured graph).  seed chooses the random bits of the
     8-bit rounding.  workspace: one int32, 0 (a program that steps often
     keeps one; calls that overlap on the GPU need one each)."""
     _step([(params, grads, exp_avgs, exp_avg_sqs, scales, steps, lr, betas, eps, weight_decay)],
@@ -52,6 +52,8 @@ def _step(groups, seed, workspace):
         on_device = torch.is_tensor(lr)
         if on_device and (not lr.is_cuda or lr.dtype != torch.float32 or lr.numel() != 1):
             raise ValueError("lr must be a number or one float32 element on the device")
+        if on_device and n and lr.device != params[0].device:
+            raise ValueError("lr is on %s, the parameters on %s" % (lr.device, params[0].device))
         lrs.append(lr if on_device else None)
         hyper += [0.0 if on_device else float(lr), float(betas[0]), float(betas[1]), float(eps), float(wd)]
     if not p:
@@ -136,9 +138,11 @@ class AdamW(torch.optim.Optimizer):
                 to[5].append(s["step"])
             for device, to in lists.items():
                 scales = to[4] if any(t is not None for t in to[4]) else None
+                lr = group["lr"]
+                if torch.is_tensor(lr) and lr.is_cuda and lr.device != device:
+                    lr = lr.to(device, non_blocking=True)
                 by_device.setdefault(device, []).append(
-                    (*to[:4], scales, to[5], group["lr"], group["betas"], group["eps"],
-                     group["weight_decay"]))
+                    (*to[:4], scales, to[5], lr, group["betas"], group["eps"], group["weight_decay"]))
         for device, groups in by_device.items():
             workspace = self._workspace.get(device)
             if workspace is None:

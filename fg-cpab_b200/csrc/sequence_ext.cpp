@@ -351,6 +351,9 @@ void adamw(const pybind11::list &params, const pybind11::list &grads, const pybi
   if (n == 0) return;
   const at::Device device = item(params, 0, "parameter")->device();
   TORCH_CHECK(device.is_cuda(), "params must be CUDA tensors (no CPU path)");
+  for (const MaybeTensor &lr : lr_tensors)
+    TORCH_CHECK(!lr.has_value() || (lr->device() == device && lr->scalar_type() == at::kFloat && lr->numel() == 1),
+                "adamw: a learning rate on the device must be one float32 on the parameters' device, ", device);
   const c10::cuda::CUDAGuard guard(device);
   std::vector<cpab_adamw_tensor> list(n);
   std::vector<Tensor> copies;  // gradients laid out as their parameters

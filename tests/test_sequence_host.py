@@ -175,3 +175,36 @@ def test_a_norm_without_residual_has_its_inputs_type():
     assert L.cpab_b200_rms_norm(*a) == -1 and "without a residual" in err()
     a = [2, 0, 0, P, 8, None, 0, P, 4, 8, 1e-6, P, P, None, None]
     assert L.cpab_b200_rms_norm_quantized(*a) == -1 and "without a residual" in err()
+
+
+def test_a_learning_rate_on_another_device_is_refused(path):
+    """By the call and by both of its native forms, before anything is launched
+    (tensors without memory, so no GPU is needed)."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        p, step, rate = (torch.empty(n, device=d) for n, d in ((4, "cuda:0"), (1, "cuda:0"), (1, "cuda:1")))
+        with pytest.raises(ValueError, match="lr"):
+            adamw_([p], [p], [p], [p], [step], lr=rate)
+        ticket = torch.empty(1, device="cuda:0", dtype=torch.int32)
+        fn = _native.adamw if _ext.module() is None else _ext.module().adamw
+        with pytest.raises(RuntimeError, match="learning rate"):
+            fn([p], [p], [p], [p], [], [step], [1], [0.0, 0.9, 0.999, 1e-8, 0.0], [rate], 0, ticket)
+
+
+def test_a_group_on_two_devices_has_its_learning_rate_on_both(monkeypatch):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from cpab import optim
+    calls = []
+    monkeypatch.setattr(optim, "_step", lambda groups, seed, workspace: calls.append((groups, workspace)))
+    with FakeTensorMode():
+        ps = [torch.nn.Parameter(torch.empty(5, device=d)) for d in ("cuda:0", "cuda:1", "cuda:0")]
+        for p in ps:
+            p.grad = torch.empty_like(p)
+        rate = torch.empty((), device="cuda:0")
+        AdamW(ps, lr=rate).step()
+    assert len(calls) == 2
+    for (group,), workspace in calls:
+        params, lr = group[0], group[6]
+        assert {t.device for t in (*params, lr, workspace)} == {params[0].device}
+        assert (lr is rate) == (params[0].device == rate.device)
