@@ -499,6 +499,12 @@ def _adjacent(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _written(*tensors):
+    """Counts a write through a raw pointer as torch's own operations count
+    theirs, so that a backward through the old value raises."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def check_scan(x, gate, h0, lengths):
     _cuda(x)
     if x.dim() != 3:
@@ -592,6 +598,7 @@ def gated_scan_step(x, gate, state, slots):
     slots = _contiguous(slots)
     h = torch.empty((B, D), device=x.device, dtype=x.dtype)
     gp = _ptr(ga) if ga is not None else _ptr(xa) + D * x.element_size()
+    _written(state)
     with _on(x.device):
         _check(lib().cpab_b200_gated_scan_step(
             _dtype(x, "x"), _ptr(xa), xa.stride(0), gp, (ga if ga is not None else xa).stride(0), B,
@@ -731,6 +738,8 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, scales, steps, counts, hyper, lr
                         not sc.is_contiguous() or sc.numel() != 2 * blocks:
                     raise ValueError("adamw: tensor %d: 8-bit states need float32 scales [%d, 2]"
                                      % (k, blocks))
+                _written(sc)
+            _written(p, m, v, step)
             t = table[k]
             t.param, t.grad, t.exp_avg, t.exp_avg_sq = _ptr(p), _ptr(g), _ptr(m), _ptr(v)
             t.scales, t.step, t.lr_device = _ptr(sc), _ptr(step), _ptr(lrs[group])

@@ -52,6 +52,12 @@ void require(const Tensor &t, const Tensor &like, at::ScalarType dtype, at::IntA
   TORCH_CHECK_VALUE(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
 }
 
+// Counts a write through a raw pointer as torch's own operations count theirs, so
+// that a backward through the old value raises (an inference tensor has no count).
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // No gradient of these gradients: refuse instead of treating them as constants.
 void once(const char *name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " can be differentiated once only (create_graph=True)");
@@ -205,6 +211,7 @@ Tensor gated_scan_step(const Tensor &x, const MaybeTensor &gate_, const Tensor &
   const Tensor xc = channels_adjacent(x), gc = gate.defined() ? channels_adjacent(gate) : gate;
   const Tensor sl = slots.defined() ? slots.contiguous() : slots;
   const Tensor h = at::empty({B, D}, x.options());
+  written(state);
   const void *gp = gate.defined() ? ptr(gc) : static_cast<const char *>(ptr(xc)) + D * x.element_size();
   check(cpab_b200_gated_scan_step(dtype, ptr(xc), xc.stride(0), gp, gate.defined() ? gc.stride(0) : xc.stride(0),
                                   B, D, static_cast<const int32_t *>(ptr(sl)), state.size(0), fptr_mut(state),
@@ -393,7 +400,9 @@ void adamw(const pybind11::list &params, const pybind11::list &grads, const pybi
                               t->is_contiguous() && t->numel() == 2 * blocks,
                           "adamw: tensor ", k, ": 8-bit states need float32 scales [", blocks, ", 2]");
         sc = fptr_mut(*t);
+        written(*t);
       }
+      for (const Tensor *t : {&p, &m, &v, &step}) written(*t);
       cpab_adamw_tensor &t = list[k];
       t.param = ptr_mut(p), t.grad = ptr(copied ? copies.back() : *grad), t.exp_avg = ptr_mut(m);
       t.exp_avg_sq = ptr_mut(v), t.scales = sc, t.step = fptr_mut(step), t.numel = p.numel();

@@ -14,6 +14,7 @@ import torch
 
 from cpab import _ext, _native
 from cpab.optim import AdamW, adamw_
+from cpab.pytorch.norm import rms_norm
 
 pytestmark = [pytest.mark.gpu,
               pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA GPU")]
@@ -394,3 +395,28 @@ def test_offsets_past_32_bits():
     assert torch.allclose(p[-300:].float(), torch.full((300,), -1e-2, device=DEV), rtol=2 ** -8)
     assert not p[:-300].any() and math.isclose(float(sc[-1, 0]), 0.1 / 448, rel_tol=1e-6)
     assert (m[-300:].float() > 0).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("python", [False, True])
+def test_autograd_sees_the_step(bits, python):
+    """As of torch's own in-place operations: a backward through a value that the
+    step has replaced raises instead of using the new one."""
+    p = torch.nn.Parameter(torch.randn(300, device=DEV))
+    opt = AdamW([p], state_bits=bits, min_8bit_size=1)
+    p.grad = torch.ones_like(p)
+    with _ext.python_path() if python else contextlib.nullcontext():
+        opt.step()
+        old, normed = (p * p).sum(), rms_norm(torch.randn(3, 300, device=DEV), p).sum()
+        written = [p, *opt.state[p].values()]
+        before = [t._version for t in written]
+        opt.step()
+        assert all(t._version > n for t, n in zip(written, before))
+        for loss in (old, normed):
+            with pytest.raises(RuntimeError, match="modified by an inplace"):
+                loss.backward()
+        with torch.inference_mode():                       # such tensors count no versions
+            q, g, m, v = (torch.ones(10, device=DEV) for _ in range(4))
+            step = torch.zeros((), device=DEV)
+        adamw_([q], [g], [m], [v], [step], lr=1e-2)
+        assert float(step) == 1

@@ -7,6 +7,8 @@ the state's size) and fades with the state's own memory 1 / (1 - a), 23 samples
 on average for the gates drawn here, so it grows like the root of half of that:
 about 6e-7; 8 times that is allowed.  An output in 16 bits is off by at most
 its unit roundoff on top.  Gradients carry two such chains: twice as much."""
+import contextlib
+
 import pytest
 import torch
 
@@ -449,3 +451,20 @@ def test_offsets_past_32_bits():
     assert off(h[:, -100:], r[0][:, -100:]) <= tol(BF16) and off(last, r[1]) <= tol(F32)
     assert off(gx[:, -150:], r[2][:, -150:]) <= tol(BF16, 2)
     assert off(gz[:, -150:], r[3][:, -150:]) <= tol(BF16, 2)
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_autograd_sees_the_step_of_a_state(python):
+    """A backward through the old state raises instead of using the new one."""
+    x, z, _, _, _ = inputs(4, 1, 10, F32)
+    w = torch.ones(4, 10, device=DEV, requires_grad=True)
+    state = torch.randn(2, 4, 10, device=DEV)
+    with _ext.python_path() if python else contextlib.nullcontext():
+        loss = (w * state[1]).sum()
+        gated_scan_step(x[:, 0], z[:, 0], state[1])
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            loss.backward()
+        with torch.inference_mode():                       # such tensors count no versions
+            state = torch.zeros(4, 10, device=DEV)
+        h = gated_scan_step(x[:, 0], z[:, 0], state)
+        assert torch.equal(h, state)
