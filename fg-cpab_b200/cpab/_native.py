@@ -499,6 +499,18 @@ def _adjacent(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def needs_grad(*tensors):
+    """Whether the call has to go through its node, which refuses forward mode."""
+    return has_tangent(*tensors) or (
+        torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+
+
+def has_tangent(*tensors):
+    """Whether a forward-mode derivative flows into one of them."""
+    return any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+               for t in tensors)
+
+
 def _written(*tensors):
     """Counts a write through a raw pointer as torch's own operations count
     theirs, so that a backward through the old value raises."""
@@ -578,6 +590,8 @@ def gated_scan_backward(x, gate, lengths, states, dh, dlast, want_h0):
 
 def gated_scan_step(x, gate, state, slots):
     _cuda(x)
+    if has_tangent(x, gate, state):
+        raise RuntimeError("gated_scan_step has no gradient, of forward mode neither")
     if x.dim() != 2:
         raise ValueError("x must be [B, D], got %s" % (tuple(x.shape),))
     if gate is not None:
@@ -645,6 +659,8 @@ def rms_norm(x, weight, residual, eps, keep):
 
 def rms_norm_quantized(x, weight, residual, eps):
     """(q, scale) or (q, scale, sum)."""
+    if has_tangent(x, weight, residual):
+        raise RuntimeError("rms_norm_quantized has no gradient, of forward mode neither")
     alive, args = _norm_args(x, weight, residual, eps)
     q = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
     scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)

@@ -14,11 +14,11 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     """x [..., D] float32, float16 or bfloat16 (D at most 16384); weight [D]
     and residual [..., D] of x's type or float32.  Returns y (x's type), or
     (y, s) with a residual (s of the residual's type).  Differentiable (once)
-    in x, weight and residual."""
+    in x, weight and residual, backward only."""
     ext = _ext.module()
     if ext is None:
         _native.check_norm(x, weight, residual)
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+        if _native.needs_grad(x, weight, residual):
             out = _RmsNorm.apply(x, weight, residual, float(eps))
         else:
             out = _native.rms_norm(x, weight, residual, float(eps), False)[:2]

@@ -35,13 +35,13 @@ def gated_scan(x, gate=None, h0=None, lengths=None):
     infinity or a NaN.
 
     Returns (h [B, T, D] of x's type, last [B, D] float32, the state after
-    each series' last sample).  Differentiable (once) in x, gate and h0; any
-    strides, without a copy where the channels are adjacent."""
+    each series' last sample).  Differentiable (once, backward only) in x,
+    gate and h0; any strides, without a copy where the channels are adjacent."""
     lengths = _int32(lengths, "lengths", x.shape[1] if x.dim() > 1 else 0)
     ext = _ext.module()
     if ext is None:
         _native.check_scan(x, gate, h0, lengths)
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, h0)):
+        if _native.needs_grad(x, gate, h0):
             return _GatedScan.apply(x, gate, h0, lengths)
         return _native.gated_scan(x, gate, h0, lengths, False)[:2]
     return _ext.call(ext.gated_scan, x, gate, h0, lengths)

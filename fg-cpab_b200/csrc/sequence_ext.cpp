@@ -63,7 +63,16 @@ void once(const char *name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " can be differentiated once only (create_graph=True)");
 }
 
+// Whether a forward-mode derivative flows into one of ts.
+bool has_tangent(std::initializer_list<const Tensor *> ts) {
+  for (const Tensor *t : ts)
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined()) return true;
+  return false;
+}
+
+// Whether the call has to go through its node, which refuses forward mode.
 bool needs_grad(std::initializer_list<const Tensor *> ts) {
+  if (has_tangent(ts)) return true;
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor *t : ts)
     if (t->defined() && t->requires_grad()) return true;
@@ -197,6 +206,7 @@ Tensor gated_scan_step(const Tensor &x, const MaybeTensor &gate_, const Tensor &
                        const MaybeTensor &slots_) {
   const Tensor gate = given(gate_), slots = given(slots_);
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (no CPU path)");
+  TORCH_CHECK(!has_tangent({&x, &gate, &state}), "gated_scan_step has no gradient, of forward mode neither");
   const int dtype = dtype_of(x, "x");
   TORCH_CHECK_VALUE(x.dim() == 2, "x must be [B, D], got ", x.sizes());
   if (gate.defined()) require(gate, x, x.scalar_type(), x.sizes(), "gate");
@@ -317,6 +327,8 @@ std::vector<Tensor> rms_norm_quantized(const Tensor &x, const Tensor &weight, co
                                        double eps) {
   const Tensor residual = given(residual_);
   check_norm(x, weight, residual);
+  TORCH_CHECK(!has_tangent({&x, &weight, &residual}),
+              "rms_norm_quantized has no gradient, of forward mode neither");
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor xr = rows_of(x), rr = residual.defined() ? rows_of(residual) : Tensor();
   const Tensor w = weight.contiguous();

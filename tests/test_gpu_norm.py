@@ -261,3 +261,21 @@ def test_offsets_past_32_bits():
     ry, _, rg, _ = reference(x[-3:].detach(), w, None, EPS, dy[-3:])
     assert off(y[-3:], ry) <= 1e-6 + ROUND[BF16] and off(g[-3:], rg) <= 1e-6 + ROUND[BF16]
     assert not g[:-3].any()
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(python, grad):
+    """Instead of coming out as none."""
+    from torch.autograd import forward_ad
+    x, res, w, _, _ = inputs(5, 8, F32, F32, F32)
+    with (_ext.python_path() if python else contextlib.nullcontext()), torch.set_grad_enabled(grad), \
+            forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args in ((dual(x), w, res), (x, dual(w), res), (x, w, dual(res)), (dual(x), w)):
+            with pytest.raises(RuntimeError, match="jvp|forward"):
+                rms_norm(*args)
+            with pytest.raises(RuntimeError, match="no gradient"):
+                rms_norm_quantized(*args)
+        rms_norm(x, w, res)
+        rms_norm_quantized(x, w, res)

@@ -468,3 +468,21 @@ def test_autograd_sees_the_step_of_a_state(python):
             state = torch.zeros(4, 10, device=DEV)
         h = gated_scan_step(x[:, 0], z[:, 0], state)
         assert torch.equal(h, state)
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(python, grad):
+    """Instead of coming out as none."""
+    from torch.autograd import forward_ad
+    x, z, h0, _, _ = inputs(2, 9, 8, F32)
+    with (_ext.python_path() if python else contextlib.nullcontext()), torch.set_grad_enabled(grad), \
+            forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args in ((dual(x), z, h0), (x, dual(z), h0), (x, z, dual(h0))):
+            with pytest.raises(RuntimeError, match="jvp|forward"):
+                gated_scan(*args)
+        for args in ((dual(x[:, 0]), z[:, 0], h0), (x[:, 0], dual(z[:, 0]), h0), (x[:, 0], z[:, 0], dual(h0))):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                gated_scan_step(*args)
+        gated_scan(x, z, h0)
