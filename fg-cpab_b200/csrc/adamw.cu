@@ -38,6 +38,9 @@ constexpr int kChunkElems = 2048;  // 8 elements a thread, 8 scale blocks
 constexpr int kScaleBlock = 256;   // elements that share a scale: one warp's
 constexpr float kE4m3Max = 448.0f;
 constexpr float kTiny = 1.17549435e-38f;  // 2^-126, the smallest scale
+// The scale of roots where a second moment overflowed: 2^64 / 448, whose largest
+// code stands for 2^64, the square of which is infinite again.
+constexpr float kOverflowed = 0x1p64f / kE4m3Max;
 // Blocks of an SM that the registers leave room for (8-bit states: 2, 3 and 4
 // take 701, 622 and 719 us for 200 million); blocks of a launch per SM at most, if
 // each has kChunksEach chunks (a block's begin is 200 instructions: one chunk a
@@ -120,7 +123,9 @@ struct Rates {
 // for bit.  The parameter's update goes through the hardware's approximate
 // reciprocal roots (about 2^-22 of an update that is 1e-3 of it); a second moment
 // below 2^-126, which they would flush to 0, counts as 2^-126 there.  One that
-// overflowed has an infinite root (not inf * 0): its parameter only decays.
+// overflowed has an infinite root (not inf * 0): its parameter only decays.  (8-bit
+// states keep it so by kOverflowed; its block's small elements, whose roots are then
+// far below the block's least code, all but stand still meanwhile.)
 __device__ __forceinline__ float update(const Rates &r, float p, float g, float &m, float &v, float &root) {
   m = __fadd_rn(__fmul_rn(m, r.b1), __fmul_rn(g, r.ob1));
   v = __fadd_rn(__fmul_rn(v, r.b2), __fmul_rn(__fmul_rn(g, g), r.ob2));
@@ -266,7 +271,8 @@ __device__ __forceinline__ void step_block(const Here &t, int64_t first) {
       }
     float ms = __fmul_rn(warp_max(__float_as_uint(mt)), 1.0f / kE4m3Max);
     float rs = __fmul_rn(__fsqrt_rn(warp_max(vt)), 1.0f / kE4m3Max);
-    if (!(rs <= 3.0e38f)) ms = rs;
+    if (rs != rs) ms = rs;
+    rs = rs > kOverflowed ? kOverflowed : rs;  // (a NaN stays)
     if (ms < kTiny) ms = kTiny;
     if (rs < kTiny) rs = kTiny;
     if (lane == 0) *reinterpret_cast<float2 *>(t.scales + first / kScaleBlock * 2) = make_float2(ms, rs);

@@ -420,3 +420,38 @@ def test_autograd_sees_the_step(bits, python):
             step = torch.zeros((), device=DEV)
         adamw_([q], [g], [m], [v], [step], lr=1e-2)
         assert float(step) == 1
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_an_overflowed_second_moment_in_8_bits(dtype):
+    """One gradient whose square overflows: its element only decays, the others of
+    its block stay finite and the other blocks do not notice."""
+    n, hyper = 700, dict(lr=0.5, weight_decay=0.25)
+    g = torch.Generator().manual_seed(3)
+    grads = torch.randn(6, n, generator=g).to(DEV, dtype)
+    grads[1:, 300] = 0
+    runs = []
+    for size in (0.0, 1e25):
+        p = torch.full((n,), 2.0, device=DEV, dtype=dtype)
+        m, v = (torch.zeros(n, device=DEV, dtype=F8) for _ in range(2))
+        sc, step, seen = torch.zeros(3, 2, device=DEV), torch.zeros((), device=DEV), []
+        for k in range(6):
+            grad = grads[k].clone()
+            if k == 0:
+                grad[300] = size
+            adamw_([p], [grad], [m], [v], [step], scales=[sc], seed=4, **hyper)
+            seen.append(p.clone())
+        assert torch.isfinite(m.float()).all() and torch.isfinite(v.float()).all() and torch.isfinite(sc).all()
+        runs.append(torch.stack(seen))
+    plain, big = runs
+    assert torch.isfinite(big).all()
+    other = torch.ones(n, dtype=torch.bool, device=DEV)
+    other[256:512] = False
+    assert torch.equal(big[:, other], plain[:, other])
+    mates = ~other
+    mates[300] = False
+    assert torch.equal(big[0, mates], plain[0, mates])
+    want = 2.0
+    for k in range(6):                                     # (as of the 32-bit states)
+        want *= 1.0 - 0.5 * 0.25
+        assert abs(big[k, 300].item() - want) <= want * (6 * 3 * 2.0 ** -24 + 6 * ROUND[dtype])
