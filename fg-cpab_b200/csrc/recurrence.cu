@@ -138,7 +138,13 @@ __device__ __forceinline__ uint32_t closed_gate(__half) { return 0x7C007C00u; }
 // approximate exponential and reciprocal (2 and 1 units in the last place).
 // f = e / (1 + e) keeps its relative precision as a -> 1; where e > 1, 1 - a
 // loses none and is right for e = inf too.
-template <int V>
+// The exponential's argument t = -z log2(e) is rounded, which is off by up to
+// 2^-24 |t| ln 2 of e: 3e-7 at |z| = 7, 2e-6 at 40.  In float32 (PRECISE) what is
+// left of -z beside t ln 2 is put back, where e is neither 0 nor infinite: e is
+// then as good as the instruction.  16-bit values are rounded to 2^-12 of their
+// size at best, so there the three instructions (of 24 a sample and channel that
+// bound the kernel) are saved.
+template <bool PRECISE, int V>
 __device__ __forceinline__ void gate_of(Lane<V> z, Lane<V> &a, Lane<V> &f) {
   const Lane<V> t = z * all<V>(-1.4426950408889634f);
   Lane<V> e;
@@ -146,6 +152,7 @@ __device__ __forceinline__ void gate_of(Lane<V> z, Lane<V> &a, Lane<V> &f) {
   for (int i = 0; i < V; ++i) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t[i]));
+    if (PRECISE && fabsf(t[i]) < 126.0f) r = fmaf(r, fmaf(t[i], -0.6931471805599453f, -z[i]), r);
     e.set(i, r);
   }
   const Lane<V> d = e + all<V>(1.0f);
@@ -477,7 +484,7 @@ __global__ void __launch_bounds__(kTotalWarps * 32) k_scan_totals(const __grid_c
     for (int k = 0; k < L; ++k) {
       const int i = BACK ? L - 1 - k : k;
       Lane<V> a, f;
-      gate_of(unpack(gw[i], T{}), a, f);
+      gate_of<sizeof(T) == 4>(unpack(gw[i], T{}), a, f);
       H = BACK ? a * (H + unpack(uw[i], T{})) : fma(a, H, f * unpack(uw[i], T{}));
       A = A * a;
     }
@@ -593,7 +600,7 @@ __global__ void __launch_bounds__(WARPS * 32, kResidentWarps / WARPS) k_scan(con
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       Lane<V> f;
-      gate_of(unpack(gs[i], T{}), a[i], f);
+      gate_of<sizeof(T) == 4>(unpack(gs[i], T{}), a[i], f);
       in[i] = f * unpack(xs[i], T{});
       H = fma(a[i], H, in[i]);
       A = A * a[i];
@@ -729,7 +736,7 @@ __global__ void __launch_bounds__(WARPS * 32, kResidentWarps / WARPS) k_scan_bac
     Lane<V> A = all<V>(1.0f), H = all<V>(0.0f), R = all<V>(0.0f);
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      gate_of(unpack(gs[i], T{}), a[i], f[i]);
+      gate_of<sizeof(T) == 4>(unpack(gs[i], T{}), a[i], f[i]);
       xv[i] = unpack(xs[i], T{});
       gr[i] = unpack(ds[i], T{});
       H = fma(a[i], H, f[i] * xv[i]);
@@ -873,7 +880,7 @@ __global__ void __launch_bounds__(256) k_scan_short(const __grid_constant__ Scan
 #pragma unroll
     for (int k = 0; k < M; ++k) {
       Lane<V> a, f;
-      gate_of(unpack(gw[k], T{}), a, f);
+      gate_of<sizeof(T) == 4>(unpack(gw[k], T{}), a, f);
       state = fma(a, state, f * unpack(xw[k], T{}));
       if (t0 + k < samples)
         store_lane<WORDS>(h + (t0 + k) * p.D, t0 + k < len ? state : all<V>(0.0f), n);
@@ -912,7 +919,7 @@ __global__ void __launch_bounds__(256) k_scan_short_backward(const __grid_consta
 #pragma unroll
   for (int k = 0; k < M; ++k) {
     Lane<V> a, f;
-    gate_of(unpack(gw[k], T{}), a, f);
+    gate_of<sizeof(T) == 4>(unpack(gw[k], T{}), a, f);
     const Lane<V> before = state;
     state = fma(a, before, f * u[k]);
     u[k] = fma(u[k], all<V>(-1.0f), before);
@@ -921,7 +928,7 @@ __global__ void __launch_bounds__(256) k_scan_short_backward(const __grid_consta
   for (int k = M - 1; k >= 0; --k) {
     if (k < samples) {
       Lane<V> a, f;
-      gate_of(unpack(gw[k], T{}), a, f);
+      gate_of<sizeof(T) == 4>(unpack(gw[k], T{}), a, f);
       const Lane<V> delta = unpack(dw[k], T{}) + c;
       c = a * delta;
       const bool live = k < len;
@@ -962,7 +969,7 @@ __global__ void k_scan_step(const T *x, int64_t xs, const T *gate, int64_t gs, i
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
       Lane<1> a, f;
-      gate_of(all<1>(to_f32(gv.v[v])), a, f);
+      gate_of<sizeof(T) == 4>(all<1>(to_f32(gv.v[v])), a, f);
       const float s = fmaf(a[0], st[v], f[0] * to_f32(xv.v[v]));
       st[v] = s;
       out.v[v] = from_f32<T>(s);

@@ -486,3 +486,32 @@ def test_forward_mode_derivatives_are_refused(python, grad):
             with pytest.raises(RuntimeError, match="no gradient"):
                 gated_scan_step(*args)
         gated_scan(x, z, h0)
+
+
+def test_float32_gates_keep_their_relative_precision():
+    """a and 1 - a of gates up to 40 against float64.  Bound: the exponential
+    instruction's 2^-22, 2e-9 x 58 left of its argument, 2^-23 of the reciprocal and
+    four roundings (the correction, 1 + e, e a and, of dz, one product): 7e-7; dz,
+    a product of both, twice that."""
+    z = torch.linspace(-40, 40, 1 << 14, device=DEV)
+    one, none = torch.ones_like(z), torch.zeros_like(z)
+    a, f = torch.sigmoid(z.double()), torch.sigmoid(-z.double())
+
+    def close(got, want, k=1):
+        return float((got.detach().double() / want - 1).abs().max()) <= k * 7e-7
+    # one sample (a thread per channel), and the first of 40 whose others change nothing (tiles)
+    for T in (1, 40):
+        def series(first, rest):
+            return torch.cat([first[None, None], torch.full((1, T - 1, z.numel()), rest, device=DEV)], 1)
+        for x, h0, want in ((one, none, f), (none, one, a)):
+            xs, zs = series(x, 0.0).requires_grad_(True), series(z, float("inf")).requires_grad_(True)
+            hs = h0[None].clone().requires_grad_(True)
+            h, last = gated_scan(xs, zs, hs)
+            assert close(h[0, 0], want) and close(last[0], want), T
+            gx, gz, gh = torch.autograd.grad(last, (xs, zs, hs), one[None])
+            assert close(gx[0, 0], f) and close(gh[0], a), T
+            assert close(gz[0, 0], a * f * (1.0 if h0 is one else -1.0), 2), T
+    state = one[None].clone()
+    assert close(gated_scan_step(none[None], z[None], state)[0], a)
+    state.zero_()
+    assert close(gated_scan_step(one[None], z[None], state)[0], f)
