@@ -183,7 +183,7 @@ struct Span {
 // (`shift`) after one, and the vectors that hold a row are taken as they lie:
 // those at its ends hold elements of the rows beside it too, which mask_span makes
 // zeros (later: a thread's loads do not wait for one another).  Only past the last
-// row there may be nothing to read.
+// row there may be nothing to read (rows do not overlap: lie_of).
 template <typename T, int VEC, bool EDGE>
 __device__ __forceinline__ void load_span(Row<T, VEC> &r, const T *row, const Span &s, bool last) {
   if (EDGE && last && s.hi < VEC) r.load_some(row + s.c, s.lo, s.hi);
@@ -676,6 +676,9 @@ Lie lie_of(const NormArgs &a, int e, int f, int x_size) {
   const bool strides = (a.xs - a.D) % vec == 0 && (a.res == nullptr || (a.rs - a.D) % vec == 0);
   if (!strides) return kAnyhow;
   if (a.D % vec == 0) return aligned_to(a.w, 0, 4, 16) ? kOnVectors : kAnyhow;
+  // Rows that overlap (windows of one signal): the vector at a row's end could reach
+  // past the last row's.
+  if (a.xs < a.D || (a.res != nullptr && a.rs < a.D)) return kAnyhow;
   // One at a time what is narrower than 32 columns, where a vector's masks cost
   // more (15 columns bf16: 241 against 488 us, 31: 234 and 302, the gradient 304
   // and 322; 31 columns f32: 126 and 142, 166 and 226; but 95 columns bf16: 210

@@ -279,3 +279,21 @@ def test_forward_mode_derivatives_are_refused(python, grad):
                 rms_norm_quantized(*args)
         rms_norm(x, w, res)
         rms_norm_quantized(x, w, res)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_that_overlap(dtype):
+    """Windows of one signal, a row a step of 1 or 8 further on: nothing lies
+    between or after them."""
+    for step, D in ((1, 33), (8, 40), (8, 48), (1, 41)):
+        signal = torch.randn(400, generator=torch.Generator().manual_seed(2)).to(DEV, dtype)
+        x = signal.unfold(0, D, step).detach().requires_grad_(True)
+        _, res, w, dy, ds = inputs(x.shape[0], D, dtype, dtype, F32)
+        y, s = rms_norm(x, w, residual=res, eps=EPS)
+        (g,) = torch.autograd.grad((y, s), x, (dy, ds))
+        want = reference(x.detach(), w, res, EPS, dy, ds)
+        assert off(y, want[0]) <= 1e-6 + ROUND[dtype] and off(g, want[2]) <= 1e-6 + ROUND[dtype]
+        y = rms_norm(x, w, eps=EPS)
+        (g,) = torch.autograd.grad(y, x, dy)
+        want = reference(x.detach(), w, None, EPS, dy)
+        assert off(y, want[0]) <= 1e-6 + ROUND[dtype] and off(g, want[2]) <= 1e-6 + ROUND[dtype]
