@@ -50,9 +50,15 @@ class SeriesLocalizer(nn.Module):
     def forward(self, series, lengths=None):
         """series [B, channels, L], lengths [B] or None (all L) -> theta
         [B, theta_dim] from each series' first lengths[b] samples (0 for a
-        series without one: the identity)."""
+        series without one: the identity).  What series holds after them does
+        not matter, nor to the gradients."""
         if series.dim() != 3 or series.shape[1] != self.channels or series.shape[2] < 1:
             raise ValueError("series must be [B, %d, L], got %s" % (self.channels, tuple(series.shape)))
+        if lengths is not None:
+            # (gated_scan passes over them by itself, but the weights' gradients of
+            # the norms and projections would be sums with 0 x NaN)
+            seen = torch.arange(series.shape[2], device=series.device) < lengths[:, None, None]
+            series = series.masked_fill(~seen, 0.0)
         s = self.embed(series.transpose(1, 2))
         update = None
         for block in self.blocks:

@@ -135,3 +135,23 @@ def test_example_learns(bits):
     path = ex.follow(net, x[0])
     assert path.shape == (192, warp.theta_dim)
     assert (path[-1] - whole).abs().max() <= 1e-3 * whole.abs().max().clamp_min(1.0)
+
+
+def test_samples_past_a_series_end_do_not_matter():
+    """Whatever they hold: theta and the gradients are those of zeros there."""
+    net = network()
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(4, 3, 70, generator=g).to(DEV)
+    up = torch.randn(4, 11, generator=g).to(DEV)
+    n = torch.tensor([70, 1, 0, 33], device=DEV)
+    past = torch.arange(70, device=DEV)[None, None] >= n[:, None, None]
+    seen = []
+    for fill in (0.0, float("nan"), float("inf"), 3e38):
+        net.zero_grad()
+        series = torch.where(past, torch.full_like(x, fill), x).requires_grad_(True)
+        theta = net(series, n)
+        theta.backward(up)
+        assert not theta[2].any() and not series.grad[past.expand_as(x)].any()
+        seen.append([theta.detach(), series.grad, *(p.grad.clone() for p in net.parameters())])
+    for other in seen[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(seen[0], other))
