@@ -76,7 +76,9 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits=8 keeps the states of parameters of at least min_8bit_size
     elements as e4m3 codes (state names exp_avg, root_avg_sq, scales): 2.03
-    instead of 8 bytes per parameter.  seed: of their stochastic rounding."""
+    instead of 8 bytes per parameter.  seed: of their stochastic rounding (an
+    option of the groups, so that state_dict keeps it and a resumed run rounds as
+    it would have)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *,
                  state_bits=32, min_8bit_size=4096, seed=0):
@@ -89,9 +91,19 @@ class AdamW(torch.optim.Optimizer):
         if state_bits not in (8, 32):
             raise ValueError("state_bits must be 8 or 32, got %r" % (state_bits,))
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
-                                      state_bits=state_bits, min_8bit_size=min_8bit_size))
-        self.seed = int(seed)
+                                      state_bits=state_bits, min_8bit_size=min_8bit_size,
+                                      seed=int(seed)))
         self._workspace = {}
+
+    @property
+    def seed(self):
+        """The first group's; setting it sets every group's."""
+        return self.param_groups[0]["seed"]
+
+    @seed.setter
+    def seed(self, value):
+        for group in self.param_groups:
+            group["seed"] = int(value)
 
     def _state(self, p, group):
         state = self.state[p]
@@ -114,7 +126,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        by_device = {}
+        calls = {}  # by device and seed
         for group in self.param_groups:
             lists = {}
             for p in group["params"]:
@@ -141,19 +153,24 @@ class AdamW(torch.optim.Optimizer):
                 lr = group["lr"]
                 if torch.is_tensor(lr) and lr.is_cuda and lr.device != device:
                     lr = lr.to(device, non_blocking=True)
-                by_device.setdefault(device, []).append(
+                calls.setdefault((device, group["seed"]), []).append(
                     (*to[:4], scales, to[5], lr, group["betas"], group["eps"], group["weight_decay"]))
-        for device, groups in by_device.items():
+        for (device, seed), groups in calls.items():
             workspace = self._workspace.get(device)
             if workspace is None:
                 workspace = self._workspace[device] = torch.zeros(1, device=device, dtype=torch.int32)
-            _step(groups, self.seed, workspace)
+            _step(groups, seed, workspace)
         return loss
 
     def load_state_dict(self, state_dict):
         """As torch's, which casts states to their parameter's type: the
-        states' own types are put back."""
-        super().load_state_dict(state_dict)
+        states' own types are put back.  A saved group without a seed leaves
+        the group's own."""
+        groups = state_dict["param_groups"]
+        if len(groups) == len(self.param_groups):
+            groups = [{"seed": own["seed"], **saved}
+                      for own, saved in zip(self.param_groups, groups)]
+        super().load_state_dict({**state_dict, "param_groups": groups})
         params = [p for g in self.param_groups for p in g["params"]]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, params):

@@ -455,3 +455,36 @@ def test_an_overflowed_second_moment_in_8_bits(dtype):
     for k in range(6):                                     # (as of the 32-bit states)
         want *= 1.0 - 0.5 * 0.25
         assert abs(big[k, 300].item() - want) <= want * (6 * 3 * 2.0 ** -24 + 6 * ROUND[dtype])
+
+
+def test_an_8_bit_run_resumes_with_its_random_bits():
+    torch.manual_seed(0)
+    p = torch.nn.Parameter(torch.randn(3000, device=DEV))
+    opt = AdamW([p], state_bits=8, min_8bit_size=1, seed=5)
+    p.grad = torch.randn_like(p)
+    opt.step()
+    q = torch.nn.Parameter(p.detach().clone())
+    two = AdamW([q], state_bits=8, min_8bit_size=1)
+    two.load_state_dict(copy.deepcopy(opt.state_dict()))
+    q.grad = p.grad.clone()
+    opt.step()
+    two.step()
+    assert torch.equal(p, q)
+    for k, t in opt.state[p].items():
+        assert torch.equal(t.float(), two.state[q][k].float())
+
+
+def test_groups_with_seeds_of_their_own():
+    """A group's codes are those of an optimizer with its seed."""
+    ps = [torch.nn.Parameter(torch.zeros(500, device=DEV)) for _ in range(3)]
+    g = torch.randn(500, generator=torch.Generator().manual_seed(1)).to(DEV)
+    for p in ps:
+        p.grad = g.clone()
+    kinds = dict(state_bits=8, min_8bit_size=1)
+    both = AdamW([{"params": [ps[0]], "seed": 1}, {"params": [ps[1]], "seed": 2}], **kinds)
+    one = AdamW([ps[2]], seed=2, **kinds)
+    both.step()
+    one.step()
+    codes = lambda o, p: o.state[p]["exp_avg"].float()  # noqa: E731
+    assert torch.equal(codes(both, ps[1]), codes(one, ps[2]))
+    assert not torch.equal(codes(both, ps[0]), codes(both, ps[1]))

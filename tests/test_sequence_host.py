@@ -208,3 +208,19 @@ def test_a_group_on_two_devices_has_its_learning_rate_on_both(monkeypatch):
         params, lr = group[0], group[6]
         assert {t.device for t in (*params, lr, workspace)} == {params[0].device}
         assert (lr is rate) == (params[0].device == rate.device)
+
+
+def test_the_seed_is_part_of_the_state_dict():
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = AdamW([p], state_bits=8, seed=7)
+    two = AdamW([p], state_bits=8)
+    assert two.seed == 0
+    two.load_state_dict(opt.state_dict())
+    assert two.seed == 7
+    old = opt.state_dict()                                 # one without a seed leaves it alone
+    del old["param_groups"][0]["seed"]
+    three = AdamW([p], seed=9)
+    three.load_state_dict(old)
+    assert three.seed == 9
+    three.seed = 2
+    assert three.state_dict()["param_groups"][0]["seed"] == 2
