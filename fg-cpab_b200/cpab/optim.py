@@ -95,6 +95,13 @@ class AdamW(torch.optim.Optimizer):
                                       seed=int(seed)))
         self._workspace = {}
 
+    def __setstate__(self, state):
+        # (of copies and pickles, which hold the options, groups and states only)
+        super().__setstate__(state)
+        self.__dict__.setdefault("_workspace", {})
+        for options in (self.defaults, *self.param_groups):
+            options.setdefault("seed", 0)
+
     @property
     def seed(self):
         """The first group's; setting it sets every group's."""

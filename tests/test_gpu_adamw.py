@@ -488,3 +488,27 @@ def test_groups_with_seeds_of_their_own():
     codes = lambda o, p: o.state[p]["exp_avg"].float()  # noqa: E731
     assert torch.equal(codes(both, ps[1]), codes(one, ps[2]))
     assert not torch.equal(codes(both, ps[0]), codes(both, ps[1]))
+
+
+def test_copies_and_pickles_take_the_same_step():
+    import io
+    torch.manual_seed(0)
+    p = torch.nn.Parameter(torch.randn(700, device=DEV))
+    opt = AdamW([p], state_bits=8, min_8bit_size=1, seed=5)
+    for k in range(3):
+        p.grad = torch.randn_like(p)
+        opt.step()
+    file = io.BytesIO()                                    # (torch pickles 8-bit tensors by its own save only)
+    torch.save(opt, file)
+    file.seek(0)
+    two, three = copy.deepcopy(opt), torch.load(file, weights_only=False)
+    grad = torch.randn_like(p)
+    for o in (opt, two, three):
+        (q,) = o.param_groups[0]["params"]
+        q.grad = grad.clone()
+        o.step()
+    for o in (two, three):
+        (q,) = o.param_groups[0]["params"]
+        assert q is not p and torch.equal(p, q)
+        for k, t in opt.state[p].items():
+            assert torch.equal(t.float(), o.state[q][k].float())

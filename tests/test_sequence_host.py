@@ -224,3 +224,17 @@ def test_the_seed_is_part_of_the_state_dict():
     assert three.seed == 9
     three.seed = 2
     assert three.state_dict()["param_groups"][0]["seed"] == 2
+
+
+def test_copies_and_pickles_of_adamw_step():
+    """They come as far as the original: to the refusal of CPU tensors."""
+    import copy
+    import pickle
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = AdamW([p], lr=0.25, state_bits=8, seed=7)
+    for twin in (opt, copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        (q,) = twin.param_groups[0]["params"]
+        q.grad = torch.ones(3)
+        assert twin.seed == 7 and twin.param_groups[0]["lr"] == 0.25
+        with pytest.raises(RuntimeError, match="CUDA"):
+            twin.step()
