@@ -70,9 +70,11 @@ def _step(groups, seed, workspace):
 
 
 class AdamW(torch.optim.Optimizer):
-    """torch.optim.AdamW's constructor and state names (step, exp_avg,
-    exp_avg_sq) with the step of adamw_; step() can be captured in a CUDA graph
-    (counts and, if given as a tensor, lr live on the device).
+    """lr, betas, eps and weight_decay of torch.optim.AdamW's constructor (not
+    amsgrad, maximize nor the choices of its implementations), its state names
+    (step, exp_avg, exp_avg_sq) and state dicts, with the step of adamw_; step()
+    can be captured in a CUDA graph (counts and, if given as a tensor, lr live on
+    the device).
 
     state_bits=8 keeps the states of parameters of at least min_8bit_size
     elements as e4m3 codes (state names exp_avg, root_avg_sq, scales): 2.03
@@ -171,11 +173,15 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, which casts states to their parameter's type: the
-        states' own types are put back.  A saved group without a seed leaves
-        the group's own."""
+        states' own types are put back (float32 for 16-bit moments of torch's
+        AdamW).  Options that a saved group lacks stay as they are; amsgrad and
+        maximize, which this step does not have, are refused."""
         groups = state_dict["param_groups"]
+        for option in ("amsgrad", "maximize"):
+            if any(saved.get(option) for saved in groups):
+                raise ValueError("AdamW has no %s, which the state dict asks for" % option)
         if len(groups) == len(self.param_groups):
-            groups = [{"seed": own["seed"], **saved}
+            groups = [{**{k: own[k] for k in self.defaults if k in own}, **saved}
                       for own, saved in zip(self.param_groups, groups)]
         super().load_state_dict({**state_dict, "param_groups": groups})
         params = [p for g in self.param_groups for p in g["params"]]
@@ -185,4 +191,5 @@ class AdamW(torch.optim.Optimizer):
             if saved:
                 for k, v in saved.items():
                     if torch.is_tensor(v):
-                        self.state[p][k] = v.detach().clone().to(p.device)
+                        kind = v.dtype if v.dtype == torch.float8_e4m3fn else torch.float32
+                        self.state[p][k] = v.detach().to(p.device, kind, copy=True)

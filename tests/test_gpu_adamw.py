@@ -512,3 +512,28 @@ def test_copies_and_pickles_take_the_same_step():
         assert q is not p and torch.equal(p, q)
         for k, t in opt.state[p].items():
             assert torch.equal(t.float(), o.state[q][k].float())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_run_of_torchs_adamw_goes_on(dtype):
+    """From its state dict.  float32: torch's parameters to the steps' roundings.
+    bfloat16: torch rounds the moments too; a step is lr long at most, and each
+    side rounds the parameter once a step."""
+    torch.manual_seed(0)
+    p = torch.nn.Parameter((0.1 * torch.randn(40, 30, device=DEV)).to(dtype))
+    theirs = torch.optim.AdamW([p], lr=1e-3)
+    for _ in range(3):
+        p.grad = torch.randn_like(p)
+        theirs.step()
+    q = torch.nn.Parameter(p.detach().clone())
+    ours = AdamW([q])
+    ours.load_state_dict(theirs.state_dict())
+    assert ours.state[q]["exp_avg"].dtype == F32
+    for _ in range(5):
+        p.grad = torch.randn_like(p)
+        q.grad = p.grad.clone()
+        theirs.step()
+        ours.step()
+    assert float(ours.state[q]["step"]) == 8
+    room = 1e-5 if dtype == F32 else 5 * (1e-3 + 2 * ROUND[dtype] * float(p.detach().abs().max()))
+    assert float((p - q).detach().abs().max()) <= room

@@ -238,3 +238,26 @@ def test_copies_and_pickles_of_adamw_step():
         assert twin.seed == 7 and twin.param_groups[0]["lr"] == 0.25
         with pytest.raises(RuntimeError, match="CUDA"):
             twin.step()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_state_dict_of_torchs_adamw(dtype):
+    """Is taken: options that it lacks are the new optimizer's own, 16-bit moments
+    become float32.  Options that this step does not have are refused."""
+    p, q = (torch.nn.Parameter(torch.ones(6, 4, dtype=dtype)) for _ in range(2))
+    theirs = torch.optim.AdamW([p, q], lr=3e-3, weight_decay=0.2)
+    p.grad = torch.full_like(p, 0.5)                       # q has no gradient yet, so no state
+    theirs.step()
+    opt = AdamW([p, q], min_8bit_size=5, state_bits=8)
+    opt.load_state_dict(theirs.state_dict())
+    group = opt.param_groups[0]
+    assert group["lr"] == 3e-3 and group["weight_decay"] == 0.2 and group["state_bits"] == 8
+    state, want = opt.state[p], theirs.state[p]
+    assert float(state["step"]) == 1
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert state[k].dtype == torch.float32 and torch.equal(state[k], want[k].float())
+    assert "scales" in opt._state(q, group)
+    for option in ("amsgrad", "maximize"):
+        with pytest.raises(ValueError, match=option):
+            opt.load_state_dict(torch.optim.AdamW([p, q], **{option: True}).state_dict())
+    assert opt.param_groups[0]["lr"] == 3e-3               # a refused one changes nothing
