@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from cpab import _ext, _native
-from cpab.optim import AdamW, adamw_
+from cpab.optim import AdamW, _step, adamw_
 from cpab.pytorch.norm import rms_norm
 
 pytestmark = [pytest.mark.gpu,
@@ -537,3 +537,22 @@ def test_a_run_of_torchs_adamw_goes_on(dtype):
     assert float(ours.state[q]["step"]) == 8
     room = 1e-5 if dtype == F32 else 5 * (1e-3 + 2 * ROUND[dtype] * float(p.detach().abs().max()))
     assert float((p - q).detach().abs().max()) <= room
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_block_goes_from_tensor_to_tensor(dtype, bits):
+    """130 tensors of odd sizes and 2300 chunks in one launch, so that a block's run
+    holds chunks of several; a step count of each, two groups' hyperparameters."""
+    sizes = [1 + (7919 * i) % 9000 for i in range(100)] + [1 + (104729 * i) % 300000 for i in range(30)]
+    L = make(sizes, dtype, bits)
+    old, cut = copies(L), 60
+    other = dict(lr=5e-4, betas=(0.8, 0.99), eps=1e-6, weight_decay=0.0)
+    groups = []
+    for part, h in ((slice(0, cut), HYPER), (slice(cut, None), other)):
+        groups.append((*(L[k][part] for k in ("p", "g", "m", "v")), L["scales"][part] if bits == 8 else None,
+                       L["step"][part], h["lr"], h["betas"], h["eps"], h["weight_decay"]))
+    _step(groups, 9, torch.zeros(1, device=DEV, dtype=torch.int32))
+    for part, h in ((range(cut), HYPER), (range(cut, len(sizes)), other)):
+        check({k: [v[i] for i in part] for k, v in L.items()}, {k: [v[i] for i in part] for k, v in old.items()},
+              dtype, 9, hyper=h, index=list(part))

@@ -297,3 +297,28 @@ def test_rows_that_overlap(dtype):
         (g,) = torch.autograd.grad(y, x, dy)
         want = reference(x.detach(), w, None, EPS, dy)
         assert off(y, want[0]) <= 1e-6 + ROUND[dtype] and off(g, want[2]) <= 1e-6 + ROUND[dtype]
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shape", [(7013, 999), (5003, 1537), (5003, 1024), (60013, 33), (1201, 9001)])
+def test_many_rows_for_each_thread(shape, types):
+    """More rows than the gradient's blocks hold at once, on vectors and inside
+    them: the weight's gradient summed over rows (of random sign, so its error
+    grows as it does)."""
+    x, res, w, dy, ds = inputs(*shape, *types)
+    leaves = [t.requires_grad_(True) for t in (x, w, res)]
+    y, s = rms_norm(x, w, residual=res, eps=EPS)
+    gx, gw, gr = torch.autograd.grad((y, s), leaves, (dy, ds))
+    ry, rs, rg, rw = reference(x.detach(), w, res.detach(), EPS, dy, ds)
+    assert torch.equal(s.double(), rs) and off(y, ry) <= 1e-6 + ROUND[types[0]]
+    assert off(gx, rg) <= 1e-6 + ROUND[types[0]] and off(gr, rg) <= 1e-6 + ROUND[types[1]]
+    assert off(gw, rw) <= 2e-6 + ROUND[types[2]]
+    last = off(gx[-50:], rg[-50:])                         # (a row by itself hardly shows in the whole)
+    assert last <= 1e-6 + ROUND[types[0]]
+    with torch.no_grad():
+        q, scale, _ = rms_norm_quantized(x, w, residual=res, eps=EPS)
+    top = ry.abs().amax(1)
+    assert ((scale.double() - top / 448).abs() <= 1e-6 * top / 448).all()
+    v = q.double() * scale.double()[:, None]
+    room = torch.maximum(ry.abs() / 16, scale.double()[:, None] / 1024) + 1e-5 * top[:, None]
+    assert ((v - ry).abs() <= room).all()
