@@ -399,11 +399,11 @@ struct Place {
   }
 };
 
+// `ring` is 1, 2 or 3 (shape_of).
 __device__ __forceinline__ void wait_for_stage(int ring) {
   if (ring == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
   else if (ring == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else if (ring == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else asm volatile("cp.async.wait_group 2;" ::: "memory");
   __syncthreads();
 }
 
