@@ -4,10 +4,12 @@
 //
 // per channel, for gate logits z and inputs x [B, T, D] in f32, f16 or bf16
 // and a float32 state.  Both a and 1 - a come from one exponential in float32
-// (1 - a = sigmoid(-z) keeps its relative precision as a -> 1).
+// (1 - a = sigmoid(-z) keeps its relative precision as a -> 1: gate_of).
 //
 // A step (a, b): h -> a h + b; two steps compose to (a2 a1, a2 b1 + b2), which
-// is associative.  A block owns a tile of channels of one piece of a series and
+// is associative.  (Where the a's are so near 1 that a product's second-order term
+// falls below half its last place, that term is lost each time: 8192 samples of
+// logits N(12, 1.5), a memory of 50,000, are 8e-6 off, sample by sample 3e-6.)  A block owns a tile of channels of one piece of a series and
 // walks it stage by stage: cp.async brings the next stages into shared memory,
 // each thread reads a segment of kFwdSteps or kBwdSteps samples of its channels
 // from there and composes them, and the segments' compositions are scanned over
@@ -134,39 +136,64 @@ __device__ __forceinline__ uint32_t closed_gate(float) { return 0x7F800000u; }
 __device__ __forceinline__ uint32_t closed_gate(__nv_bfloat16) { return 0x7F807F80u; }
 __device__ __forceinline__ uint32_t closed_gate(__half) { return 0x7C007C00u; }
 
-// a = sigmoid(z) and f = 1 - a = sigmoid(-z) from e = exp(-z), by the hardware's
-// approximate exponential and reciprocal (2 and 1 units in the last place).
-// f = e / (1 + e) keeps its relative precision as a -> 1; where e > 1, 1 - a
-// loses none and is right for e = inf too.
-// The exponential's argument t = -z log2(e) is rounded, which is off by up to
-// 2^-24 |t| ln 2 of e: 3e-7 at |z| = 7, 2e-6 at 40.  In float32 (PRECISE) what is
-// left of -z beside t ln 2 is put back, where e is neither 0 nor infinite: e is
-// then as good as the instruction.  16-bit values are rounded to 2^-12 of their
-// size at best, so there the three instructions (of 24 a sample and channel that
-// bound the kernel) are saved.
+// The hardware's approximate exponential (2^t) and reciprocal: 2 and 1 units in the
+// last place.
+__device__ __forceinline__ float exp2_near(float t) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_near(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
+
+// a = sigmoid(z) and f = 1 - a = sigmoid(-z) from one exponential; f = e / (1 + e)
+// with e = exp(-z) keeps its size's precision as a -> 1.
+//
+// In float32 (PRECISE) both are as good as the two instructions.  The exponential's
+// argument t is rounded, which is off by up to 2^-24 |t| ln 2 of e (3e-7 at |z| = 7,
+// 2e-6 at 40): what is left of z beside t ln 2 is put back.  And the larger of a
+// and f is 1 less the smaller, rounded once: the reciprocal itself is off by 1.3e-8
+// on average near a logit of 7, which a memory of 1 / (1 - a) samples adds up
+// (states of 8192 samples of logits N(7, 1.5): 3.0e-6 off against 3.6e-7, the same
+// recursion sample by sample 7.5e-7).
+//
+// 16-bit inputs are rounded to 2^-12 of their size at best, and so are the outputs.
+// There that precision is not worth its five instructions a sample and channel, of
+// 24 that bound the kernel (the last two cost 8x16384x1024 bf16 160 -> 167 us and its
+// gradient 293 -> 309; float32, bound by memory, hardly shows them: 8x8192x512 78 and
+// 119 us with and without, 8x8192x499 190 -> 192, 256x4x4096 18 -> 20 and 23 -> 27).
 template <bool PRECISE, int V>
 __device__ __forceinline__ void gate_of(Lane<V> z, Lane<V> &a, Lane<V> &f) {
-  const Lane<V> t = z * all<V>(-1.4426950408889634f);
-  Lane<V> e;
+  constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  if constexpr (PRECISE) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t[i]));
-    if (PRECISE && fabsf(t[i]) < 126.0f) r = fmaf(r, fmaf(t[i], -0.6931471805599453f, -z[i]), r);
-    e.set(i, r);
+    for (int i = 0; i < V; ++i) {
+      const float t = fabsf(z[i]) * -kLog2E;
+      float e = exp2_near(t);  // of -|z|
+      if (t > -126.0f) e = fmaf(e, fmaf(t, -kLn2, -fabsf(z[i])), e);
+      const float r = reciprocal_near(e + 1.0f), less = e * r, more = fmaf(-e, r, 1.0f);
+      a.set(i, z[i] > 0.0f ? more : less);
+      f.set(i, z[i] > 0.0f ? less : more);
+    }
+  } else {
+    // (step by step over the lane's channels: together they cost the gradient 4%)
+    const Lane<V> t = z * all<V>(-kLog2E);
+    Lane<V> e;
+#pragma unroll
+    for (int i = 0; i < V; ++i) e.set(i, exp2_near(t[i]));
+    const Lane<V> d = e + all<V>(1.0f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) a.set(i, reciprocal_near(d[i]));
+    f = e * a;
+    // (where e > 1, 1 - a loses nothing and is right for e = inf too)
+    const Lane<V> g = fma(a, all<V>(-1.0f), all<V>(1.0f));
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (e[i] > 1.0f) f.set(i, g[i]);
   }
-  const Lane<V> d = e + all<V>(1.0f);
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d[i]));
-    a.set(i, r);
-  }
-  f = e * a;
-  const Lane<V> g = fma(a, all<V>(-1.0f), all<V>(1.0f));
-#pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (e[i] > 1.0f) f.set(i, g[i]);
 }
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) {

@@ -515,3 +515,27 @@ def test_float32_gates_keep_their_relative_precision():
     assert close(gated_scan_step(none[None], z[None], state)[0], a)
     state.zero_()
     assert close(gated_scan_step(one[None], z[None], state)[0], f)
+
+
+@pytest.mark.parametrize("shift", [7.0, 12.0])
+@pytest.mark.parametrize("length", [8192, 63])
+def test_long_memories(shift, length):
+    """Gates of memories of a thousand samples: in float32 the states are as near to
+    float64 as the recursion in elementary float32 operations is; twice that is
+    allowed.  Of memories longer than the series that holds sample by sample only:
+    composed steps multiply factors (1 - j u)(1 - k u), whose j k u^2 is always
+    rounded away, so the head's bound for a memory of `length` samples is taken."""
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(2, length, 64, generator=g).to(DEV)
+    z = (torch.randn(2, length, 64, generator=g) * 1.5 + shift).to(DEV)
+    want, _ = reference(x, z, None, None)
+    a, f, h, plain = torch.sigmoid(z), torch.sigmoid(-z), torch.zeros(2, 64, device=DEV), []
+    for t in range(length):
+        h = a[:, t] * h + f[:, t] * x[:, t]
+        plain.append(h)
+    room = 2 * off(torch.stack(plain, 1), want) if shift == 7 else 8 * 3 * 2.0 ** -24 * (length / 2) ** 0.5
+    assert off(gated_scan(x, z)[0], want) <= room
+    state = torch.zeros(2, 64, device=DEV)
+    for t in range(length):
+        h = gated_scan_step(x[:, t], z[:, t], state)
+    assert off(h, want[:, -1]) <= 2 * off(plain[-1], want[:, -1])
