@@ -74,7 +74,7 @@ class AdamW(torch.optim.Optimizer):
     amsgrad, maximize nor the choices of its implementations), its state names
     (step, exp_avg, exp_avg_sq) and state dicts, with the step of adamw_; step()
     can be captured in a CUDA graph (counts and, if given as a tensor, lr live on
-    the device).
+    the device) once the parameters have states, that is after one step.
 
     state_bits=8 keeps the states of parameters of at least min_8bit_size
     elements as e4m3 codes (state names exp_avg, root_avg_sq, scales): 2.03
@@ -117,6 +117,9 @@ class AdamW(torch.optim.Optimizer):
     def _state(self, p, group):
         state = self.state[p]
         if not state:
+            if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: a parameter without a state in a captured step: every replay "
+                                   "would begin anew; take one step, or load states, before the capture")
             state["step"] = torch.zeros((), device=p.device, dtype=torch.float32)
             eight = group["state_bits"] == 8 and p.numel() >= group["min_8bit_size"]
             kind = torch.float8_e4m3fn if eight else torch.float32

@@ -556,3 +556,21 @@ def test_a_block_goes_from_tensor_to_tensor(dtype, bits):
     for part, h in ((range(cut), HYPER), (range(cut, len(sizes)), other)):
         check({k: [v[i] for i in part] for k, v in L.items()}, {k: [v[i] for i in part] for k, v in old.items()},
               dtype, 9, hyper=h, index=list(part))
+
+
+def test_a_first_step_is_not_captured():
+    """Its states' zeros would be part of the graph, and every replay a first step."""
+    p = torch.nn.Parameter(torch.randn(300, device=DEV))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p])
+    before = p.detach().clone()
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+    assert float(opt.state[p]["step"]) == 4 and not torch.equal(p, before)
