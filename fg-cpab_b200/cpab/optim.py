@@ -69,6 +69,10 @@ def _step(groups, seed, workspace):
         _ext.call(ext.adamw, p, g, m, v, sc, st, counts, hyper, lrs, int(seed) & 0xFFFFFFFF, workspace)
 
 
+def _capturing():
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 class AdamW(torch.optim.Optimizer):
     """lr, betas, eps and weight_decay of torch.optim.AdamW's constructor (not
     amsgrad, maximize nor the choices of its implementations), its state names
@@ -117,7 +121,7 @@ class AdamW(torch.optim.Optimizer):
     def _state(self, p, group):
         state = self.state[p]
         if not state:
-            if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            if _capturing():
                 raise RuntimeError("AdamW: a parameter without a state in a captured step: every replay "
                                    "would begin anew; take one step, or load states, before the capture")
             state["step"] = torch.zeros((), device=p.device, dtype=torch.float32)
@@ -170,7 +174,9 @@ class AdamW(torch.optim.Optimizer):
         for (device, seed), groups in calls.items():
             workspace = self._workspace.get(device)
             if workspace is None:
-                workspace = self._workspace[device] = torch.zeros(1, device=device, dtype=torch.int32)
+                workspace = torch.zeros(1, device=device, dtype=torch.int32)
+                if not _capturing():  # (there it is 0 in replays only)
+                    self._workspace[device] = workspace
             _step(groups, seed, workspace)
         return loss
 

@@ -574,3 +574,26 @@ def test_a_first_step_is_not_captured():
     for _ in range(3):
         graph.replay()
     assert float(opt.state[p]["step"]) == 4 and not torch.equal(p, before)
+
+
+def test_loaded_states_step_first_in_a_capture():
+    """What the capture allocates is not kept for the steps outside of it."""
+    p = torch.nn.Parameter(torch.randn(300, device=DEV))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p])
+    opt.step()
+    q = torch.nn.Parameter(p.detach().clone())
+    q.grad = p.grad.clone()
+    two = AdamW([q])
+    two.load_state_dict(opt.state_dict())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        two.step()
+    assert not two._workspace
+    two.step()
+    graph.replay()
+    graph.replay()
+    two.step()
+    for _ in range(4):
+        opt.step()
+    assert float(two.state[q]["step"]) == 5 and torch.equal(p, q)
