@@ -322,3 +322,16 @@ def test_many_rows_for_each_thread(shape, types):
     v = q.double() * scale.double()[:, None]
     room = torch.maximum(ry.abs() / 16, scale.double()[:, None] / 1024) + 1e-5 * top[:, None]
     assert ((v - ry).abs() <= room).all()
+
+
+def test_an_8_bit_scale_is_rounded_once():
+    """Rows of ones and minus ones: r is 1, y the weights, the scale the float32
+    nearest to their largest magnitude / 448."""
+    g = torch.Generator().manual_seed(6)
+    x = torch.where(torch.rand(64, 256, generator=g) < 0.5, -1.0, 1.0).to(DEV)
+    for _ in range(40):
+        w = torch.randn(256, generator=g)
+        assert torch.equal(rms_norm(x, w.to(DEV), eps=0.0), x * w.to(DEV))
+        _, scale = rms_norm_quantized(x, w.to(DEV), eps=0.0)
+        want = (w.abs().max().double() / 448).float()
+        assert torch.equal(scale.cpu(), want.expand(64))
