@@ -101,7 +101,8 @@ class SeriesLocalizer(nn.Module):
         new_states, updated in place, slots [B] the streams' rows of it (None:
         row b; -1: no sample now, whose theta means nothing).  Returns theta
         [B, theta_dim] of the streams so far.  quantized: norms and input
-        projections in 8 bits (see quantize)."""
+        projections in 8 bits (see quantize), whose products torch gives in
+        16 bits only."""
         s = self.embed(samples)
         update = None
         for k, block in enumerate(self.blocks):

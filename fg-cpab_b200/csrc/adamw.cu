@@ -19,10 +19,10 @@
 // of chunks of 2048 elements; a chunk belongs to one tensor.
 //
 // With float32 states memory bounds it: 200 million float32 parameters (28 bytes
-// each) take 857 us (6.5 TB/s; a copy: 6.46).  With 8-bit states 16 bytes and
+// each) take 854 us (6.6 TB/s; a copy: 6.46).  With 8-bit states 16 bytes and
 // about 75 instructions, mostly the integer units' (hash, cut, the near test), are
-// left of a parameter: 627 us (5.1 TB/s), 0.73 of the time for 0.57 of the
-// bytes.  A kernel for all types, branching per tensor, spilled and took 1100 us.
+// left of a parameter: 622 us (5.2 TB/s), 0.73 of the time for 0.57 of the
+// bytes; of bfloat16 parameters 10 bytes, 588 us (3.4 TB/s, 70% of the issue slots).  A kernel for all types, branching per tensor, spilled and took 1100 us.
 #include <cuda_fp8.h>
 
 #include <cmath>
@@ -121,7 +121,9 @@ struct Rates {
 // The moments' separate roundings (no fused multiply-adds) are those of the
 // formulas written as elementary operations, which the tests compare with bit
 // for bit.  The parameter's update goes through the hardware's approximate
-// reciprocal roots (about 2^-22 of an update that is 1e-3 of it); a second moment
+// reciprocal roots: 6.7e-8 of an update that is 1e-3 of the parameter off (rms; 3.1e-7
+// at most), against 5.2e-8 (2.1e-7) of correctly rounded ones, which take 200 million
+// parameters 703 against 622 us with 8-bit states (float32: 863 and 854).  A second moment
 // below 2^-126, which they would flush to 0, counts as 2^-126 there.  One that
 // overflowed has an infinite root (not inf * 0): its parameter only decays.  (8-bit
 // states keep it so by kOverflowed; its block's small elements, whose roots are then

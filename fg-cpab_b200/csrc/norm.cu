@@ -15,10 +15,14 @@
 // block visits, then over blocks in a second kernel in a fixed order (same
 // result every run; no atomics).
 //
-// All of it is bound by memory: 32768x4096 bf16 with a residual moves 1.07 GB
-// each way, the forward in 160 us (6.7 TB/s; a copy: 6.46), the gradient in 193
-// (5.6 TB/s: beside the row it holds its weights' sums, which leaves 768 threads
-// on an SM; in float32, with half as many elements a thread, 6.5).
+// Rows on vectors, of up to 8192 columns, are bound by memory: 32768x4096 bf16 with a
+// residual moves 1.07 GB each way, the forward in 160 us (6.7 TB/s; a copy: 6.46), the
+// gradient in 193 (5.6 TB/s: beside the row it holds its weights' sums, which leaves
+// 768 threads on an SM; in float32, with half as many elements a thread, 6.5).  Other
+// rows take longer for their bytes: inside vectors the masks (65536x999: 66% of the
+// issue slots), of over 8192 columns 512 threads on an SM and, of float32 inside
+// vectors, spills (4096x13209: 42% and 30% of the issue slots, 3.9 and 2.9 TB/s).
+// Means are sums times the rounded 1 / D (at most 2^-25 of r).
 #include <cuda_fp8.h>
 
 #include <type_traits>

@@ -9,12 +9,14 @@
 // A step (a, b): h -> a h + b; two steps compose to (a2 a1, a2 b1 + b2), which
 // is associative.  (Where the a's are so near 1 that a product's second-order term
 // falls below half its last place, that term is lost each time: 8192 samples of
-// logits N(12, 1.5), a memory of 50,000, are 8e-6 off, sample by sample 3e-6.)  A block owns a tile of channels of one piece of a series and
-// walks it stage by stage: cp.async brings the next stages into shared memory,
-// each thread reads a segment of kFwdSteps or kBwdSteps samples of its channels
-// from there and composes them, and the segments' compositions are scanned over
-// the warp (shuffles) and the block (shared memory) to give each segment the state
-// it starts from; a second pass over the registers writes the segment's states.
+// logits N(12, 1.5), a memory of 50,000, are 8e-6 off, sample by sample 3e-6.)
+//
+// A block owns a tile of channels of one piece of a series and walks it stage by
+// stage: cp.async brings the next stages into shared memory, each thread reads a
+// segment of kFwdSteps or kBwdSteps samples of its channels from there and composes
+// them, and the segments' compositions are scanned over the warp (shuffles) and the
+// block (shared memory) to give each segment the state it starts from; a second
+// pass over the registers writes the segment's states.
 //
 // A series is one piece where there are tiles enough to fill the GPU.  Else a
 // kernel before composes every kSpan samples, and a block begins at the state
@@ -160,11 +162,13 @@ __device__ __forceinline__ float reciprocal_near(float d) {
 // (states of 8192 samples of logits N(7, 1.5): 3.0e-6 off against 3.6e-7, the same
 // recursion sample by sample 7.5e-7).
 //
-// 16-bit inputs are rounded to 2^-12 of their size at best, and so are the outputs.
+// 16-bit inputs are rounded to 2^-12 of their size at best, and so are the outputs (the
+// last state, in float32, holds no more than they gave).
 // There that precision is not worth its five instructions a sample and channel, of
 // 24 that bound the kernel (the last two cost 8x16384x1024 bf16 160 -> 167 us and its
-// gradient 293 -> 309; float32, bound by memory, hardly shows them: 8x8192x512 78 and
-// 119 us with and without, 8x8192x499 190 -> 192, 256x4x4096 18 -> 20 and 23 -> 27).
+// gradient 293 -> 309; float32, with twice the bytes and 52% of the issue slots taken,
+// hardly shows them: 8x8192x512 78 and 119 us with and without, 8x8192x499 190 -> 192,
+// 256x4x4096 18 -> 20 and 23 -> 27).
 template <bool PRECISE, int V>
 __device__ __forceinline__ void gate_of(Lane<V> z, Lane<V> &a, Lane<V> &f) {
   constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
