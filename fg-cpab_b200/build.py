@@ -25,9 +25,10 @@ LIB_PATH = os.path.join(OUT_DIR, LIB_NAME)
 OBJ_DIR = os.path.join(HERE, "_build")
 
 SOURCES = ["integrate.cu", "warp.cu", "basis.cu", "resample.cu", "capi.cu", "noalloc.cu",
-           "recurrence.cu", "norm.cu", "adamw.cu"]
+           "recurrence.cu", "norm.cu", "adamw.cu", "product.cu",
+           "muon.cu"]
 HEADERS = ["cpab_device.cuh", "integrate_body.cuh", "launch.h", "resample_device.cuh",
-           "sequence.cuh"]
+           "sequence.cuh", "tensor_core.cuh", "product_core.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

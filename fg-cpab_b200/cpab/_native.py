@@ -62,6 +62,14 @@ _SIGNATURES = {
     "cpab_b200_rms_norm_backward": [_c_int, _c_int, _c_int, _p, _c_i64, _p, _p, _c_i64, _c_i64,
                                     _p, _p, _p, _p, _p, _p, _p],
     "cpab_b200_adamw": [_p, _c_int, ctypes.c_uint32, _p, _p],
+    "cpab_b200_quantize_blocks": [_c_int, _p, _c_i64, _c_i64, _c_i64, _p, _c_i64, _p, _c_i64, _p,
+                                  _c_i64, _p, _c_i64, _c_int, _p, _p, _p],
+    "cpab_b200_matmul_quantized": [_c_int, _p, _p, _c_i64, _c_i64, _c_i64, _c_int, _p, _p, _c_i64,
+                                   _p],
+    "cpab_b200_orthogonalize": [_c_int, _p, _c_i64, _c_i64, _c_i64, _c_int, _p, ctypes.c_double, _p,
+                                _p, _p],
+    "cpab_b200_muon": [_p, _c_int, ctypes.c_double, _p, ctypes.c_double, _c_int, ctypes.c_double,
+                       _c_int, _p, ctypes.c_double, _c_int, _p, _p],
 }
 
 # Entry points that return something else than a status.
@@ -72,6 +80,9 @@ _OTHERS = {
     "cpab_b200_gated_scan_chunk": (ctypes.c_int, []),
     "cpab_b200_gated_scan_workspace": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
     "cpab_b200_rms_norm_workspace": (_c_i64, [_c_int, _c_i64, _c_i64]),
+    "cpab_b200_quantize_blocks_workspace": (_c_i64, [_c_i64, _c_i64]),
+    "cpab_b200_orthogonalize_workspace": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
+    "cpab_b200_muon_workspace": (_c_i64, [_p, _c_int]),
 }
 
 EXPORTS = tuple(_SIGNATURES) + tuple(_OTHERS)
@@ -765,3 +776,202 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, scales, steps, counts, hyper, lr
     with _on(device):
         _check(lib().cpab_b200_adamw(ctypes.byref(table), len(params), seed & 0xFFFFFFFF,
                                      _ptr(workspace), _stream(device)))
+
+
+# Projections in 8 bits.
+
+class _Quantized(ctypes.Structure):
+    """cpab_quantized."""
+    _fields_ = [("codes", _p), ("row", _c_i64), ("scale", _p), ("scale_row", _c_i64)]
+
+
+def check_quantize(x):
+    _cuda(x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must be [..., K] with K > 0, got %s" % (tuple(x.shape),))
+
+
+def check_linear(x, weight, bias):
+    check_quantize(x)
+    if weight.dim() != 2:
+        raise ValueError("weight must be [N, K], got %s" % (tuple(weight.shape),))
+    for t, name, shape in ((weight, "weight", (weight.shape[0], x.shape[-1])),
+                           (bias, "bias", (weight.shape[0],))):
+        if t is not None:
+            if t.dtype not in (torch.float32, x.dtype):
+                raise TypeError("%s must be float32 or of x's type, got %s" % (name, t.dtype))
+            _like(t, x, name, t.dtype, shape)
+
+
+def _codes(lead, K, device):
+    """Codes [*lead, K] whose rows begin on multiples of 16 bytes, and scales
+    [*lead, ceil(K / 128)] whose rows begin on multiples of 4."""
+    blocks = (K + 127) // 128
+    q = torch.empty((*lead, (K + 15) // 16 * 16), device=device, dtype=torch.float8_e4m3fn)[..., :K]
+    s = torch.empty((*lead, (blocks + 3) // 4 * 4), device=device, dtype=torch.uint8)[..., :blocks]
+    return q, s.view(torch.float8_e8m0fnu)
+
+
+def _pitch(t):
+    """The distance of rows of codes or scales as _codes lays them out."""
+    unit = 16 if t.dtype == torch.float8_e4m3fn else 4
+    return (t.shape[-1] + unit - 1) // unit * unit
+
+
+def quantize_blocks(x, rows=True, transposed=False, sum_dtype=None):
+    """(q, scale, qt, scale_t, sums), None where not asked for."""
+    xr = _rows(x)
+    R, K = xr.shape
+    q = s = qt = st = sums = work = None
+    if rows:
+        q, s = _codes(x.shape[:-1], K, x.device)
+    if transposed:
+        qt, st = _codes((K,), R, x.device) if R else (
+            torch.empty((K, 0), device=x.device, dtype=torch.float8_e4m3fn),
+            torch.empty((K, 0), device=x.device, dtype=torch.float8_e8m0fnu))
+    if sum_dtype is not None:
+        sums = torch.empty(K, device=x.device, dtype=sum_dtype)
+        work = torch.empty(lib().cpab_b200_quantize_blocks_workspace(R, K), device=x.device,
+                           dtype=torch.float32)
+    with _on(x.device):
+        _check(lib().cpab_b200_quantize_blocks(
+            _dtype(x, "x"), _ptr(xr), xr.stride(0), R, K, _ptr(q), _pitch(q) if rows else 0, _ptr(s),
+            _pitch(s) if rows else 0, _ptr(qt), _pitch(qt) if transposed else 0, _ptr(st),
+            _pitch(st) if transposed else 0, _DTYPES[sum_dtype] if sums is not None else 0,
+            _ptr(sums), _ptr(work), _stream(x.device)))
+    return q, s, qt, st, sums
+
+
+def _quantized(q, scale, name):
+    """(tensors to keep alive, rows, K, cpab_quantized) of codes [..., K]."""
+    if q.dtype != torch.float8_e4m3fn:
+        raise TypeError("%s must be float8_e4m3fn, got %s" % (name, q.dtype))
+    if q.dim() < 1 or q.shape[-1] < 1:
+        raise ValueError("%s must be [..., K] with K > 0, got %s" % (name, tuple(q.shape)))
+    K, lead = q.shape[-1], tuple(q.shape[:-1])
+    blocks = (K + 127) // 128
+    if scale.device != q.device:
+        raise RuntimeError("%s's scale is on %s, the codes on %s" % (name, scale.device, q.device))
+    if scale.dtype not in (torch.float8_e8m0fnu, torch.float32):
+        raise TypeError("%s's scale must be float8_e8m0fnu (for each 128 codes) or float32 (for each row), "
+                        "got %s" % (name, scale.dtype))
+    per_row = scale.dtype == torch.float32
+    want = lead if per_row else (*lead, blocks)
+    if tuple(scale.shape) != want:
+        raise ValueError("%s's scale must have shape %s, got %s" % (name, want, tuple(scale.shape)))
+    qr = q if q.dim() == 2 else q.reshape(-1, K)
+    rows = qr.shape[0]
+    if (K > 1 and qr.stride(1) != 1) or (rows > 1 and (qr.stride(0) % 16 or qr.stride(0) < K)) or \
+            qr.data_ptr() % 16:
+        qr = _codes((rows,), K, q.device)[0].copy_(qr)
+    if per_row:
+        sr = scale.reshape(-1).contiguous()
+        scale_row = 0
+    else:
+        sr = scale if scale.dim() == 2 else scale.reshape(-1, blocks)
+        if (blocks > 1 and sr.stride(1) != 1) or (rows > 1 and sr.stride(0) < blocks):
+            sr = sr.contiguous()
+        scale_row = sr.stride(0) if rows > 1 else (blocks + 3) // 4 * 4
+        if rows == 1 and (sr.data_ptr() % 4 or sr.untyped_storage().nbytes() - sr.storage_offset() < scale_row):
+            scale_row = blocks | 1  # (read byte by byte)
+    row = qr.stride(0) if rows > 1 else (K + 15) // 16 * 16
+    return (qr, sr), rows, K, _Quantized(_ptr(qr), row, _ptr(sr), scale_row)
+
+
+def matmul_quantized(q, scale, weight, weight_scale, bias, dtype):
+    if not q.is_cuda:
+        raise RuntimeError("q must be a CUDA tensor (no CPU path)")
+    if dtype not in _DTYPES:
+        raise TypeError("dtype must be float32, float16 or bfloat16, got %s" % dtype)
+    if weight.dim() != 2:
+        raise ValueError("weight must be [N, K], got %s" % (tuple(weight.shape),))
+    if weight.device != q.device:
+        raise RuntimeError("weight is on %s, q on %s" % (weight.device, q.device))
+    alive, M, K, x = _quantized(q, scale, "q")
+    alive_w, N, Kw, w = _quantized(weight, weight_scale, "weight")
+    if Kw != K:
+        raise ValueError("weight must be [N, %d], got %s" % (K, tuple(weight.shape)))
+    if bias is not None:
+        if bias.dtype not in (torch.float32, dtype):
+            raise TypeError("bias must be float32 or of the result's type, got %s" % bias.dtype)
+        _like(bias, q, "bias", bias.dtype, (N,))
+        bias = bias.contiguous()
+    y = torch.empty((*q.shape[:-1], N), device=q.device, dtype=dtype)
+    with _on(q.device):
+        _check(lib().cpab_b200_matmul_quantized(
+            _DTYPES[dtype], ctypes.byref(x), ctypes.byref(w), M, N, K,
+            _DTYPES[bias.dtype] if bias is not None else _DTYPES[dtype], _ptr(bias), _ptr(y), N,
+            _stream(q.device)))
+    return y
+
+
+# Orthogonalised directions.
+
+class _MuonTensor(ctypes.Structure):
+    """cpab_muon_tensor."""
+    _fields_ = [("param", _p), ("grad", _p), ("momentum", _p), ("rows", _c_i64), ("columns", _c_i64),
+                ("dtype", ctypes.c_int32)]
+
+
+def _doubles(values):
+    return (ctypes.c_double * 3)(*values)
+
+
+def orthogonalize(x, steps, coefficients, eps):
+    _cuda(x)
+    if has_tangent(x):
+        raise RuntimeError("orthogonalize has no gradient, of forward mode neither")
+    if x.dim() < 2:
+        raise ValueError("x must be [..., m, n], got %s" % (tuple(x.shape),))
+    xc = x.contiguous()
+    m, n = x.shape[-2:]
+    batch = x.numel() // (m * n) if x.numel() else 0
+    out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    dt = _dtype(x, "x")
+    work = torch.empty(lib().cpab_b200_orthogonalize_workspace(dt, batch, m, n), device=x.device,
+                       dtype=torch.uint8)
+    with _on(x.device):
+        _check(lib().cpab_b200_orthogonalize(dt, _ptr(xc), batch, m, n, steps, _doubles(coefficients), eps,
+                                             _ptr(out), _ptr(work), _stream(x.device)))
+    return out
+
+
+def muon(params, grads, momenta, lr, lr_device, momentum, nesterov, weight_decay, steps, coefficients,
+         eps, adjust):
+    """lr_device: the learning rate as one float32 on the device, or None."""
+    if not (len(params) == len(grads) == len(momenta)):
+        raise ValueError("muon: lists of different lengths")
+    if not params:
+        return
+    device = params[0].device
+    if not params[0].is_cuda:
+        raise RuntimeError("params must be CUDA tensors (no CPU path)")
+    if lr_device is not None and (lr_device.device != device or lr_device.dtype != torch.float32
+                                  or lr_device.numel() != 1):
+        raise RuntimeError("muon: a learning rate on the device must be one float32 on the parameters' "
+                           "device, %s" % device)
+    table, alive = (_MuonTensor * len(params))(), []
+    for k, (p, g, m) in enumerate(zip(params, grads, momenta)):
+        if any(t.device != device for t in (p, g, m)):
+            raise RuntimeError("muon: tensor %d: all tensors must be on one device" % k)
+        if g.dtype != p.dtype:
+            raise TypeError("muon: tensor %d: gradient of type %s for a parameter of type %s"
+                            % (k, g.dtype, p.dtype))
+        if m.dtype != torch.float32:
+            raise TypeError("muon: tensor %d: momentum must be float32, got %s" % (k, m.dtype))
+        if p.dim() != 2 or not (g.shape == p.shape == m.shape):
+            raise ValueError("muon: tensor %d: parameter, gradient and momentum must be matrices of one "
+                             "shape, got %s" % (k, tuple(p.shape)))
+        if not p.is_contiguous() or not m.is_contiguous():
+            raise ValueError("muon: tensor %d: parameter and momentum must be contiguous" % k)
+        if not g.is_contiguous():
+            g = g.contiguous()
+            alive.append(g)
+        table[k] = _MuonTensor(_ptr(p), _ptr(g), _ptr(m), p.shape[0], p.shape[1], _dtype(p, "a parameter"))
+        _written(p, m)
+    work = torch.empty(lib().cpab_b200_muon_workspace(ctypes.byref(table), len(params)), device=device,
+                       dtype=torch.uint8)
+    with _on(device):
+        _check(lib().cpab_b200_muon(ctypes.byref(table), len(params), lr, _ptr(lr_device), momentum,
+                                    int(nesterov), weight_decay, steps, _doubles(coefficients), eps, adjust,
+                                    _ptr(work), _stream(device)))

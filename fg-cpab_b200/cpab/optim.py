@@ -202,3 +202,44 @@ class AdamW(torch.optim.Optimizer):
                     if torch.is_tensor(v):
                         kind = v.dtype if v.dtype == torch.float8_e4m3fn else torch.float32
                         self.state[p][k] = v.detach().to(p.device, kind, copy=True)
+
+
+# Newton-Schulz coefficients of the quintic a x + b x^3 + c x^5 whose iterates
+# rise fastest from 0 and stay within 0.7 to 1.2 near 1.
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    """x [..., m, n] float32, float16 or bfloat16 -> as many matrices of x's type
+    with x's singular vectors and singular values near 1 (0.7 to 1.2 with the
+    default coefficients; values under about 1e-3 of the norm stay below):
+    X = x / (|x|_F + eps), then `steps` times X = a X + (b A + c A A) X with
+    A = X X^T.  16-bit matrices are multiplied as halves, float32 ones as pairs
+    of halves (22 bits).  No gradient."""
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("orthogonalize has no gradient; call it under torch.no_grad()")
+    return _native.orthogonalize(x, int(steps), coefficients, float(eps))
+
+
+_ADJUST = {"original": 0, "match_rms_adamw": 1}
+
+
+@torch.no_grad()
+def muon_(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weight_decay=0.1, steps=5,
+          coefficients=COEFFICIENTS, eps=1e-7, adjust_lr="original"):
+    """One step over lists of CUDA matrices, in place:
+
+        m = momentum m + (1 - momentum) g
+        u = (1 - momentum) g + momentum m        (nesterov; else u = m)
+        p = p (1 - lr weight_decay) - lr r orthogonalize(u)
+
+    with r = sqrt(max(1, rows / columns)) (adjust_lr "original") or
+    0.2 sqrt(max(rows, columns)) ("match_rms_adamw": steps as large as AdamW's).
+    params and grads float32, float16 or bfloat16, momenta float32.  lr: a
+    number, or one float32 on the params' device."""
+    if adjust_lr not in _ADJUST:
+        raise ValueError("adjust_lr must be 'original' or 'match_rms_adamw', got %r" % (adjust_lr,))
+    on_device = torch.is_tensor(lr)
+    _native.muon(params, grads, momenta, 0.0 if on_device else float(lr), lr if on_device else None,
+                 float(momentum), bool(nesterov), float(weight_decay), int(steps), coefficients, float(eps),
+                 _ADJUST[adjust_lr])

@@ -1,0 +1,294 @@
+// The product kernel's skeleton: a persistent block (or pair of blocks that share
+// one tile of 256 rows) walks tiles of C = A B^T; one warp fetches operand tiles
+// into a ring of stages, one issues the matrix instructions, two bring scale words,
+// eight move the accumulators from tensor memory to registers (each a quarter of the
+// block's rows and half of the columns), hand the accumulator back at once, and give
+// the values to the policy.
+//
+// The policy P says what is multiplied:
+//   kCtas, kBN        blocks to a tile (128 rows each), its columns
+//   kScaled           e4m3 codes with e8m0 scales (128 codes a step), else halves (64)
+//   kParts            2: operands are sums of two halves; a stage holds both, and
+//                     takes part x part of all but the remainders' product
+//   kBMn              B's rows run along the other axis than the summed one
+//   kAcc              accumulators in turn
+//   kSegment          stages to an accumulator, whose sums are then added in
+//                     registers (0: a tile's all).  The tensor cores cut, not round,
+//                     what a float32 sum cannot hold, so an error of up to 2^-24 of
+//                     the sum a step piles up where a tile has hundreds of steps
+//   Shared            what its epilogue keeps in shared memory
+//   int tiles()                     tiles of this launch
+//   Tile tile(int i)                {m0, n0, steps, ...}
+//   load(tile, step, a, b, bar, rank)    issues the copies of one stage; the second
+//                     parts lie kAHalf and kBHalf bytes behind the first
+//   scale_words_a / _b(tile, rank, row, group) -> the row's scales of four steps
+//   begin(tile, shared, thread)     before a tile's accumulators are waited for
+//   store(tile, shared, rank, row, column, values)  16 values of one row
+#pragma once
+
+#include "tensor_core.cuh"
+
+namespace cpab {
+namespace tc {
+
+constexpr int kCoreThreads = 384;
+constexpr int kEpilogueThreads = 256;
+constexpr int kAHalf = 128 * 128;  // bytes of one part of A a block holds per stage
+
+// The epilogue's warps alone.
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory"); }
+
+template <class P>
+struct CoreShape {
+  static constexpr int kBHalf = P::kBN / P::kCtas * 128;  // bytes of one part of B a block holds
+  static constexpr int kStageBytes = P::kParts * (kAHalf + kBHalf);
+  static constexpr int kScaleChunks = P::kScaled ? 1 + (P::kBN + 127) / 128 : 0;  // 512 bytes each
+  static constexpr int kScaleSlots = P::kScaled ? 3 : 0;
+  static constexpr int kScaleBytes = kScaleSlots * kScaleChunks * 512;
+  static constexpr int kFixed = 1024 /* alignment */ + 512 /* barriers */ + kScaleBytes + (int)sizeof(typename P::Shared);
+  static constexpr int kRoom = 227 * 1024 - kFixed;
+  static constexpr int kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
+  static constexpr int kBytes = kFixed + kStages * kStageBytes;
+  static constexpr int kScaleColumn = P::kAcc * P::kBN;  // first tensor-memory column of the scales
+  static constexpr int kColumnsUsed = kScaleColumn + 4 * kScaleChunks;
+  static constexpr int kColumns = kColumnsUsed <= 128 ? 128 : kColumnsUsed <= 256 ? 256 : 512;
+  static_assert(sizeof(typename P::Shared) % 16 == 0, "barriers lie behind it");
+  static_assert(kStages >= 3 && kColumnsUsed <= 512, "a tile too large");
+  static_assert(kStageBytes % 1024 == 0, "swizzle atoms");
+};
+
+struct CoreBarriers {
+  uint64_t full[8], empty[8], scale_full[3], scale_empty[3], acc_full[2], acc_empty[2];
+  uint32_t tmem;
+  int gave_up;
+};
+
+// Counts kernels in which a wait ran out; their unfinished tiles are stored as NaN.
+static __device__ unsigned g_gave_up;
+
+// N columns from tensor memory, NaN where the tile was given up.
+template <int N>
+__device__ __forceinline__ void read_accumulators(bool ok, uint32_t addr, float (&v)[N]) {
+  if (ok) {
+#pragma unroll
+    for (int c = 0; c < N; c += 32) tmem_load(addr + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
+    tmem_load_wait();
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = __uint_as_float(0x7FFFFFFFu);
+  }
+}
+
+template <class P>
+__device__ __forceinline__ void core(const P &p) {
+  using S = CoreShape<P>;
+  constexpr int C = P::kCtas;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *scales = smem + S::kStages * S::kStageBytes;
+  auto *shared = reinterpret_cast<typename P::Shared *>(scales + S::kScaleBytes);
+  auto *bars = reinterpret_cast<CoreBarriers *>(reinterpret_cast<uint8_t *>(shared) + sizeof(typename P::Shared));
+  const uint32_t stage0 = smem_u32(smem), scale0 = smem_u32(scales);
+  const uint32_t full = smem_u32(bars->full), empty = smem_u32(bars->empty);
+  const uint32_t sfull = smem_u32(bars->scale_full), sempty = smem_u32(bars->scale_empty);
+  const uint32_t afull = smem_u32(bars->acc_full), aempty = smem_u32(bars->acc_empty);
+  constexpr int kLength = P::kSegment > 0 ? P::kSegment : 1 << 30;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = C == 2 ? cluster_rank() : 0;
+
+  dep_launch();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
+    for (int i = 0; i < 3; ++i) bar_init(sfull + 8 * i, 2 * C), bar_init(sempty + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) bar_init(afull + 8 * i, 1), bar_init(aempty + 8 * i, 8 * C);
+    bars->gave_up = 0;
+    bar_init_fence();
+  }
+  if (warp == 2) tmem_alloc<C>(smem_u32(&bars->tmem), S::kColumns);
+  fence_before();
+  if constexpr (C == 2) cluster_sync();
+  else __syncthreads();
+  fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&bars->tmem);
+  volatile int *gave_up = &bars->gave_up;
+  dep_wait();
+
+  const int tiles = p.tiles(), first = blockIdx.x / C, stride = gridDim.x / C;
+  // The pair's shared barriers are the first block's.
+  const uint32_t full0 = C == 2 ? mapa(full, 0) : full;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0, phase = 0;
+      for (int i = first; i < tiles && !*gave_up; i += stride) {
+        const auto t = p.tile(i);
+        for (int k = 0; k < t.steps; ++k) {
+          if (!bar_wait(empty + 8 * s, phase ^ 1)) { *gave_up = 1; break; }
+          if (rank == 0) bar_expect(full + 8 * s, C * S::kStageBytes);
+          const uint32_t a = stage0 + s * S::kStageBytes;
+          p.load(t, k, a, a + P::kParts * kAHalf, full0 + 8 * s, rank);
+          if (++s == S::kStages) s = 0, phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int s = 0, phase = 0, sc = 0, sphase = 0, acc = 0, aphase = 0;
+      for (int i = first; i < tiles && !*gave_up; i += stride) {
+        const auto t = p.tile(i);
+        for (int k = 0; k < t.steps; ++k) {
+          const bool fresh = k % kLength == 0;
+          if (fresh) {
+            if (!bar_wait(aempty + 8 * acc, aphase ^ 1)) { *gave_up = 1; break; }
+            fence_after();
+          }
+          const uint32_t d = tmem + acc * P::kBN;
+          if constexpr (P::kScaled) {
+            if ((k & 3) == 0) {
+              if (!bar_wait(sfull + 8 * sc, sphase)) { *gave_up = 1; break; }
+              fence_after();
+              const uint32_t from = scale0 + sc * S::kScaleChunks * 512;
+              for (int c = 0; c < S::kScaleChunks; ++c)
+                scales_to_tmem<C>(tmem + S::kScaleColumn + 4 * c, plain_desc(from + 512 * c));
+              mma_commit<C>(sempty + 8 * sc);
+              if (++sc == 3) sc = 0, sphase ^= 1;
+            }
+          }
+          if (!bar_wait(full + 8 * s, phase)) { *gave_up = 1; break; }
+          fence_after();
+          const uint32_t a = stage0 + s * S::kStageBytes, b = a + P::kParts * kAHalf;
+          const uint64_t da = swizzled_desc(a), db = swizzled_desc(b, P::kBMn ? 8192 : 16);
+          // (the small products first, while the sum is small)
+#pragma unroll
+          for (int part = P::kParts == 2 ? 2 : 0; part >= 0; --part) {
+            const uint64_t pa = da + (part == 2 ? kAHalf >> 4 : 0), pb = db + (part == 1 ? S::kBHalf >> 4 : 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool add = !fresh || j > 0 || part != (P::kParts == 2 ? 2 : 0);
+              if constexpr (P::kScaled) {
+                // (the descriptor's scale bytes are those of this step of the four)
+                mma_mx<C>(d, pa + 2 * j, pb + 2 * j, idesc_mx(128 * C, P::kBN, 0) | ((k & 3) << 4) | ((k & 3) << 29),
+                          tmem + S::kScaleColumn, tmem + S::kScaleColumn + 4, add);
+              } else {
+                mma_f16<C>(d, pa + 2 * j, pb + (P::kBMn ? 128 : 2) * j, idesc_f16(128 * C, P::kBN, P::kBMn), add);
+              }
+            }
+          }
+          mma_commit<C>(empty + 8 * s);
+          if (++s == S::kStages) s = 0, phase ^= 1;
+          if (k + 1 == t.steps || (k + 1) % kLength == 0) {
+            mma_commit<C>(afull + 8 * acc);
+            if (++acc == P::kAcc) acc = 0, aphase ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp < 4) {
+    if constexpr (P::kScaled) {
+      // Scale words of four steps: chunk 0 is A's 128 rows, the others B's.
+      int sc = 0, sphase = 0;
+      bool ok = true;
+      for (int i = first; i < tiles && ok; i += stride) {
+        const auto t = p.tile(i);
+        for (int g = 0; 4 * g < t.steps && ok; ++g) {
+          uint32_t w[4 * (S::kScaleChunks - 1)];
+          constexpr int kB = S::kScaleChunks - 1;
+          if (warp == 2) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = p.scale_words_a(t, rank, lane + 32 * j, g);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4 * kB; ++j) w[j] = p.scale_words_b(t, lane + 32 * j, g);
+          }
+          ok = bar_wait(sempty + 8 * sc, sphase ^ 1);
+          uint8_t *to = scales + sc * S::kScaleChunks * 512 + 16 * lane;
+          if (warp == 2) {
+            *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < kB; ++c)
+              *reinterpret_cast<uint4 *>(to + 512 * (1 + c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+          }
+          proxy_fence();
+          __syncwarp();
+          if (lane == 0 && ok) {
+            if constexpr (C == 2) bar_arrive_cluster(mapa(sfull + 8 * sc, 0));
+            else bar_arrive(sfull + 8 * sc);
+          }
+          if (++sc == 3) sc = 0, sphase ^= 1;
+        }
+      }
+      if (!ok) *gave_up = 1;
+    }
+  } else {
+    constexpr int kHalf = P::kBN / 2;
+    // Where another accumulator is free the values are taken 32 at a time, else all
+    // at once, so that the accumulator is free early.
+    constexpr int kHold = P::kSegment > 0 || P::kAcc == 1 ? kHalf : 32;
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    int acc = 0, aphase = 0;
+    bool ok = true;
+    for (int i = first; i < tiles; i += stride) {
+      const auto t = p.tile(i);
+      p.begin(t, *shared, threadIdx.x - 128);
+      const int row = t.m0 + (int)rank * 128 + quarter * 32 + lane;
+      const int segments = P::kSegment > 0 ? (t.steps + kLength - 1) / kLength : 1;
+      float v[kHold];
+      for (int g = 0; g < segments; ++g) {
+        ok = ok && bar_wait(afull + 8 * acc, aphase);
+        ok = __all_sync(~0u, ok);
+        fence_after();
+        const uint32_t d = tmem + acc * P::kBN + half * kHalf + ((uint32_t)(quarter * 32) << 16);
+        if constexpr (kHold < kHalf) {
+#pragma unroll 1
+          for (int c = 0; c < kHalf; c += kHold) {
+            read_accumulators(ok, d + c, v);
+#pragma unroll
+            for (int j = 0; j < kHold; j += 16) p.store(t, *shared, row, half * kHalf + c + j, v + j);
+          }
+        } else if (P::kSegment == 0 || g == 0) {
+          read_accumulators(ok, d, v);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kHalf; c += 32) {
+            float w[32];
+            read_accumulators(ok, d + c, w);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[c + j] += w[j];
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0 && ok) {
+          if constexpr (C == 2) bar_arrive_cluster(mapa(aempty + 8 * acc, 0));
+          else bar_arrive(aempty + 8 * acc);
+        }
+        if (++acc == P::kAcc) acc = 0, aphase ^= 1;
+      }
+      if constexpr (kHold == kHalf) {
+#pragma unroll
+        for (int c = 0; c < kHalf; c += 16) p.store(t, *shared, row, half * kHalf + c, v + c);
+      }
+    }
+    if (!ok) *gave_up = 1;
+  }
+
+  __syncwarp();
+  __syncthreads();
+  if (*gave_up) {
+    // Copies in flight land before the block ends.
+    if (threadIdx.x == 0) {
+      atomicAdd(&g_gave_up, 1u);
+      for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    }
+    __syncthreads();
+  }
+  fence_before();
+  if constexpr (C == 2) cluster_sync();
+  else __syncthreads();
+  fence_after();
+  if (warp == 2) tmem_free<C>(tmem, S::kColumns);
+}
+
+}  // namespace tc
+}  // namespace cpab

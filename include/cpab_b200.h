@@ -486,6 +486,89 @@ typedef struct {
 int cpab_b200_adamw(const cpab_adamw_tensor *tensors, int count, uint32_t seed, int32_t *workspace,
                     cpab_stream_t stream);
 
+/*
+ * Matrices in 8 bits: e4m3 codes with a scale for each 128 of them along the
+ * summed axis, or one for a whole row.  Row r's codes begin `row` bytes after
+ * row r - 1's; codes and rows begin on multiples of 16 bytes.
+ */
+typedef struct {
+  const uint8_t *codes;   /* e4m3                                                    */
+  int64_t row;            /* bytes from one row to the next, a multiple of 16        */
+  const void *scale;      /* scale_row > 0: e8m0 (the power of two 2^(byte - 127); 255: NaN),
+                             one for each 128 codes of a row, scale_row bytes from a row's to
+                             the next one's; scale_row 0: float32, one for each row   */
+  int64_t scale_row;
+} cpab_quantized;
+
+/* Floats of the workspace of cpab_b200_quantize_blocks. */
+int64_t cpab_b200_quantize_blocks_workspace(int64_t rows, int64_t columns);
+
+/*
+ * Codes of x ([rows, columns] of dtype, rows x_row elements apart): for each 128
+ * elements of a row (the last block may be short) the scale is the least power of two s >= 2^-126 with
+ * max|x| <= 448 s, the codes are e4m3(x / s), rounded to nearest even.  A block
+ * that holds an infinity or a NaN has the scale NaN and NaN codes.  q and scale
+ * receive those of the rows, qt and scale_t ([columns, rows]) those of the
+ * transposed matrix (each pair may be NULL); rows of codes are multiples of 16 bytes
+ * apart and begin on 16, and what follows a row's codes up to the next multiple of 8
+ * is overwritten.  column_sum ([columns] of sum_dtype, may be NULL; needs the
+ * workspace) receives the sums of x's columns, in a fixed order.
+ */
+int cpab_b200_quantize_blocks(int dtype, const void *x, int64_t x_row, int64_t rows, int64_t columns,
+                              uint8_t *q, int64_t q_row, uint8_t *scale, int64_t scale_row,
+                              uint8_t *qt, int64_t qt_row, uint8_t *scale_t, int64_t scale_t_row,
+                              int sum_dtype, void *column_sum, float *workspace,
+                              cpab_stream_t stream);
+
+/*
+ * y[m, n] = sum_k x[m, k] weight[n, k] + bias[n] of quantized x [M, K] and weight
+ * [N, K], summed in float32 and rounded once to dtype; bias [N] of dtype or
+ * float32, or NULL; y's rows are y_row elements apart.
+ */
+int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, const cpab_quantized *weight,
+                               int64_t M, int64_t N, int64_t K, int bias_dtype, const void *bias,
+                               void *y, int64_t y_row, cpab_stream_t stream);
+
+/*
+ * Moves matrices towards their orthogonal factor (all singular values towards 1)
+ * by Newton-Schulz products: X = x / (|x|_F + eps), then `steps` times
+ *   A = X X^T,  X = a X + (b A + c A A) X      (a, b, c: coefficients[0..2], host)
+ * for each of `batch` contiguous matrices [rows, columns] of dtype; out is shaped
+ * as x and may be x.  Matrices of 16 bits are multiplied as halves, float32 ones as
+ * pairs of halves (22 bits).  coefficients must keep the singular values and the
+ * products' within 60.  workspace: cpab_b200_orthogonalize_workspace bytes, 256-byte
+ * aligned.
+ */
+int64_t cpab_b200_orthogonalize_workspace(int dtype, int64_t batch, int64_t rows, int64_t columns);
+int cpab_b200_orthogonalize(int dtype, const void *x, int64_t batch, int64_t rows, int64_t columns,
+                            int steps, const double *coefficients, double eps, void *out,
+                            void *workspace, cpab_stream_t stream);
+
+/* One matrix of cpab_b200_muon (device pointers, contiguous). */
+typedef struct {
+  void *param;      /* [rows, columns] of dtype, updated        */
+  const void *grad; /* [rows, columns] of dtype                 */
+  float *momentum;  /* [rows, columns], updated                 */
+  int64_t rows, columns;
+  int32_t dtype;    /* cpab_dtype of param and grad             */
+} cpab_muon_tensor;
+
+/*
+ * One step of an optimizer that moves matrices along orthogonalised momenta, over
+ * `count` of them (an array in host memory):
+ *   m = momentum m + (1 - momentum) g,   u = nesterov ? (1 - momentum) g + momentum m : m,
+ *   p = p (1 - lr weight_decay) - lr r O(u)
+ * with O that of cpab_b200_orthogonalize, r = sqrt(max(1, rows / columns)) (adjust 0)
+ * or 0.2 sqrt(max(rows, columns)) (adjust 1).  lr_device: the learning rate as one
+ * float32 on the device, or NULL: lr.  workspace: cpab_b200_muon_workspace bytes,
+ * 256-byte aligned.
+ */
+int64_t cpab_b200_muon_workspace(const cpab_muon_tensor *tensors, int count);
+int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double lr, const float *lr_device,
+                   double momentum, int nesterov, double weight_decay, int steps,
+                   const double *coefficients, double eps, int adjust, void *workspace,
+                   cpab_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
