@@ -88,12 +88,12 @@ def build(force=False, verbose=False, extra_flags=(), out=None):
 
 EXT_NAME = "_cpab_ext"
 EXT_PATH = os.path.join(OUT_DIR, EXT_NAME + ".so")
-EXT_SOURCES = ["torch_ext.cpp", "sequence_ext.cpp"]
+EXT_SOURCES = ["torch_ext.cpp", "sequence_ext.cpp", "projection_ext.cpp"]
 
 
 def build_ext(force=False, verbose=False):
-    """Compile the C++ autograd nodes (csrc/torch_ext.cpp and
-    csrc/sequence_ext.cpp, host code only) into cpab/_cpab_ext.so against this
+    """Compile the C++ autograd nodes (csrc/torch_ext.cpp,
+    csrc/sequence_ext.cpp and csrc/projection_ext.cpp, host code only) into cpab/_cpab_ext.so against this
     Python's torch, linked to libcpab_b200.so (found next to it at run time).
     Returns its path."""
     import sysconfig
@@ -103,7 +103,8 @@ def build_ext(force=False, verbose=False):
 
     lib = build(verbose=verbose)
     srcs = [os.path.join(CSRC, f) for f in EXT_SOURCES]
-    dep_time = max(_mtime(__file__), _mtime(os.path.join(INCLUDE, "cpab_b200.h")))
+    dep_time = max(_mtime(__file__), _mtime(os.path.join(INCLUDE, "cpab_b200.h")),
+                   _mtime(os.path.join(CSRC, "ext_common.h")))
     cuda_home = cpp_extension.CUDA_HOME or "/usr/local/cuda"
     incs = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], INCLUDE,
                                             os.path.join(cuda_home, "include")]

@@ -826,9 +826,7 @@ def quantize_blocks(x, rows=True, transposed=False, sum_dtype=None):
     if rows:
         q, s = _codes(x.shape[:-1], K, x.device)
     if transposed:
-        qt, st = _codes((K,), R, x.device) if R else (
-            torch.empty((K, 0), device=x.device, dtype=torch.float8_e4m3fn),
-            torch.empty((K, 0), device=x.device, dtype=torch.float8_e8m0fnu))
+        qt, st = _codes((K,), R, x.device)
     if sum_dtype is not None:
         sums = torch.empty(K, device=x.device, dtype=sum_dtype)
         work = torch.empty(lib().cpab_b200_quantize_blocks_workspace(R, K), device=x.device,
@@ -872,8 +870,6 @@ def _quantized(q, scale, name):
         if (blocks > 1 and sr.stride(1) != 1) or (rows > 1 and sr.stride(0) < blocks):
             sr = sr.contiguous()
         scale_row = sr.stride(0) if rows > 1 else (blocks + 3) // 4 * 4
-        if rows == 1 and (sr.data_ptr() % 4 or sr.untyped_storage().nbytes() - sr.storage_offset() < scale_row):
-            scale_row = blocks | 1  # (read byte by byte)
     row = qr.stride(0) if rows > 1 else (K + 15) // 16 * 16
     return (qr, sr), rows, K, _Quantized(_ptr(qr), row, _ptr(sr), scale_row)
 
@@ -887,6 +883,8 @@ def matmul_quantized(q, scale, weight, weight_scale, bias, dtype):
         raise ValueError("weight must be [N, K], got %s" % (tuple(weight.shape),))
     if weight.device != q.device:
         raise RuntimeError("weight is on %s, q on %s" % (weight.device, q.device))
+    if has_tangent(bias):
+        raise RuntimeError("matmul_quantized has no gradient, of forward mode neither")
     alive, M, K, x = _quantized(q, scale, "q")
     alive_w, N, Kw, w = _quantized(weight, weight_scale, "weight")
     if Kw != K:

@@ -9,6 +9,8 @@ and of sqrt(v) with one float32 scale per 256 elements, rounded
 stochastically (their averages move by less than a code's spacing per step,
 so rounding to nearest would stop them).  No counterpart in the reference.
 """
+import functools
+
 import torch
 
 from . import _ext, _native
@@ -209,6 +211,11 @@ class AdamW(torch.optim.Optimizer):
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
+def _triple(coefficients):
+    a, b, c = (float(v) for v in coefficients)
+    return a, b, c
+
+
 def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     """x [..., m, n] float32, float16 or bfloat16 -> as many matrices of x's type
     with x's singular vectors and singular values near 1 (0.7 to 1.2 with the
@@ -218,7 +225,9 @@ def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     of halves (22 bits).  No gradient."""
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError("orthogonalize has no gradient; call it under torch.no_grad()")
-    return _native.orthogonalize(x, int(steps), coefficients, float(eps))
+    ext = _ext.module()
+    fn = _native.orthogonalize if ext is None else functools.partial(_ext.call, ext.orthogonalize)
+    return fn(x, int(steps), _triple(coefficients), float(eps))
 
 
 _ADJUST = {"original": 0, "match_rms_adamw": 1}
@@ -240,6 +249,8 @@ def muon_(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weight_de
     if adjust_lr not in _ADJUST:
         raise ValueError("adjust_lr must be 'original' or 'match_rms_adamw', got %r" % (adjust_lr,))
     on_device = torch.is_tensor(lr)
-    _native.muon(params, grads, momenta, 0.0 if on_device else float(lr), lr if on_device else None,
-                 float(momentum), bool(nesterov), float(weight_decay), int(steps), coefficients, float(eps),
-                 _ADJUST[adjust_lr])
+    ext = _ext.module()
+    fn = _native.muon if ext is None else functools.partial(_ext.call, ext.muon)
+    fn(list(params), list(grads), list(momenta), 0.0 if on_device else float(lr), lr if on_device else None,
+       float(momentum), bool(nesterov), float(weight_decay), int(steps), _triple(coefficients), float(eps),
+       _ADJUST[adjust_lr])

@@ -22,6 +22,9 @@ def quantize_blocks(x, transposed=False):
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError("quantize_blocks has no gradient; call it under torch.no_grad(), or use "
                            "linear_quantized")
+    ext = _ext.module()
+    if ext is not None:
+        return tuple(_ext.call(ext.quantize_blocks, x, bool(transposed)))
     _native.check_quantize(x)
     if _native.has_tangent(x):
         raise RuntimeError("quantize_blocks has no gradient, of forward mode neither")
@@ -40,7 +43,10 @@ def matmul_quantized(q, scale, weight, weight_scale, bias=None, dtype=torch.bflo
     if torch.is_grad_enabled() and bias is not None and bias.requires_grad:
         raise RuntimeError("matmul_quantized has no gradient; call it under torch.no_grad(), or use "
                            "linear_quantized")
-    return _native.matmul_quantized(q, scale, weight, weight_scale, bias, dtype)
+    ext = _ext.module()
+    if ext is None:
+        return _native.matmul_quantized(q, scale, weight, weight_scale, bias, dtype)
+    return _ext.call(ext.matmul_quantized, q, scale, weight, weight_scale, bias, dtype)
 
 
 def linear_quantized(x, weight, bias=None):
@@ -50,6 +56,9 @@ def linear_quantized(x, weight, bias=None):
     that its product sums.  x float32, float16 or bfloat16; weight and bias of
     x's type or float32.  Differentiable (once, backward only) in x, weight and
     bias, as if the codes were the values."""
+    ext = _ext.module()
+    if ext is not None:
+        return _ext.call(ext.linear_quantized, x, weight, bias)
     _native.check_linear(x, weight, bias)
     if _native.needs_grad(x, weight, bias):
         return _LinearQuantized.apply(x, weight, bias)

@@ -76,6 +76,8 @@ __device__ __forceinline__ float direction(const Prepared &p, const PrepareArgs 
 // leave float32's range where its element does not).
 __global__ void __launch_bounds__(256) k_direction(const __grid_constant__ PrepareArgs a) {
   const Prepared &p = a.m[blockIdx.y];
+  tc::dep_launch();
+  tc::dep_wait();
   const int64_t n = (int64_t)p.rows * p.cols;
   double sum = 0;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
@@ -111,6 +113,8 @@ __device__ __forceinline__ void store_halves(__half *hi, __half *lo, int64_t i, 
 __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ PrepareArgs a, int partials) {
   const Prepared &p = a.m[blockIdx.y];
   const int tiles_x = (p.cols + 63) / 64, tiles = tiles_x * ((p.rows + 63) / 64);
+  tc::dep_launch();
+  tc::dep_wait();
   if ((int)blockIdx.x >= tiles) return;
   __shared__ double part[8];
   __shared__ float tile[64][65];
@@ -161,6 +165,7 @@ struct FinalGroup {
   int64_t stride;
   int first;                       // -1: out and stride
   int dtype, turned, update;       // turned: stored transposed; update: a parameter's step
+  int wide;                        // all rows begin on 32 bytes
   float decay, rate;               // p (1 - lr decay) - lr rate O
   const float *lr_device;
   float lr;
@@ -182,7 +187,7 @@ struct PhaseArgs<true> {
 
 template <int PHASE, int PARTS, int CTAS, int BN>
 struct Schulz {
-  static constexpr int kCtas = CTAS, kBN = BN, kAcc = 2, kParts = PARTS;
+  static constexpr int kCtas = CTAS, kBN = BN, kAcc = 2, kParts = PARTS, kChunk = 16;
   // (16-bit results: up to 1.5e-5 of the sum at 4096 summed, against 2^-12 of its operands)
   static constexpr int kSegment = PARTS == 2 ? 4 : 0;
   static constexpr bool kScaled = false, kBMn = PHASE >= kUpdate, kSymmetric = PHASE <= kSquare;
@@ -235,8 +240,6 @@ struct Schulz {
       }
     }
   }
-  __device__ uint32_t scale_words_a(const Tile &, uint32_t, int, int) const { return 0; }
-  __device__ uint32_t scale_words_b(const Tile &, int, int) const { return 0; }
   __device__ void begin(const Tile &, Shared &, int) const {}
 
   __device__ void store(const Tile &t, const Shared &, int row, int c, const float *acc) const {
@@ -310,14 +313,46 @@ struct Schulz {
       const int e = f.dtype == CPAB_F32 ? 4 : 2;
       void *out = f.first >= 0 ? p.table[f.first + t.z] : static_cast<char *>(f.out) + t.z * f.stride * e;
       const float lr = f.lr_device != nullptr ? *f.lr_device : f.lr;
-      const float keep = 1.f - lr * f.decay, move = lr * f.rate;
+      const float keep = f.update ? 1.f - lr * f.decay : 0.f, move = (f.update ? -lr * f.rate : 1.f) * (1.f / kUnit);
+      if (f.wide && col + 16 <= q.n) {
+        const int64_t i = (int64_t)row * q.n + col;
+        if (f.dtype == CPAB_F32) whole<float>(static_cast<float *>(out) + i, f.update, keep, move, v);
+        else if (f.dtype == CPAB_F16) whole<__half>(static_cast<__half *>(out) + i, f.update, keep, move, v);
+        else whole<__nv_bfloat16>(static_cast<__nv_bfloat16 *>(out) + i, f.update, keep, move, v);
+        return;
+      }
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         if (col + j >= q.n) break;
         const int64_t i = f.turned ? (int64_t)(col + j) * q.m + row : (int64_t)row * q.n + col + j;
-        float o = v[j] * (1.f / kUnit);
-        if (f.update) o = read_as(out, f.dtype, i) * keep - move * o;
-        write_as(out, f.dtype, i, o);
+        const float o = move * v[j];
+        write_as(out, f.dtype, i, f.update ? fmaf(keep, read_as(out, f.dtype, i), o) : o);
+      }
+    }
+  }
+  // 16 values of a row that begins on 32 bytes.
+  template <typename T>
+  static __device__ void whole(T *out, int update, float keep, float move, const float (&v)[16]) {
+    uint32_t w[8];
+    if constexpr (sizeof(T) == 2) {
+      if (update) tc::load_sector(out, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 x = update ? unpack_pair<T>(w[j]) : make_float2(0.f, 0.f);
+        const float a = move * v[2 * j], b = move * v[2 * j + 1];
+        w[j] = update ? pack_pair<T>(fmaf(keep, x.x, a), fmaf(keep, x.y, b)) : pack_pair<T>(a, b);
+      }
+      tc::store_sector(out, w);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 16; h += 8) {
+        if (update) tc::load_sector(out + h, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float o = move * v[h + j];
+          w[j] = __float_as_uint(update ? fmaf(keep, __uint_as_float(w[j]), o) : o);
+        }
+        tc::store_sector(out + h, w);
       }
     }
   }
@@ -344,19 +379,8 @@ cudaError_t launch_phase_as(PhaseArgs<PHASE == kFinal> &a, const int *batch, cud
     if (tiles >= int64_t(1) << 30) return cudaErrorInvalidValue;
     q.end = (int)tiles;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(CTAS * std::min<int64_t>(tiles, device_info().sm_count / CTAS)));
-  cfg.blockDim = dim3(tc::kCoreThreads);
-  cfg.dynamicSmemBytes = S::kBytes;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {CTAS, 1, 1};
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  return tc::launch(kernel, (unsigned)(CTAS * std::min<int64_t>(tiles, device_info().sm_count / CTAS)), tc::kCoreThreads,
+                    S::kBytes, CTAS, s, a);
 }
 
 // ---- a sequence of launches ---------------------------------------------------------
@@ -506,9 +530,9 @@ cudaError_t prepare(const std::vector<Prepared> &list, float momentum, int neste
     }
     a.momentum = momentum, a.nesterov = nesterov, a.eps = eps;
     const int partials = (int)std::min<int64_t>(kPartials, (most + 2047) / 2048);
-    k_direction<<<dim3(partials, n), 256, 0, s>>>(a);
-    k_normalise<<<dim3((unsigned)std::min<int64_t>(tiles, 65535), n), 256, 0, s>>>(a, partials);
-    const cudaError_t e = cudaGetLastError();
+    cudaError_t e = tc::launch(k_direction, dim3(partials, n), 256, 0, 1, s, a);
+    if (e == cudaSuccess)
+      e = tc::launch(k_normalise, dim3((unsigned)std::min<int64_t>(tiles, 65535), n), 256, 0, 1, s, a, partials);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -573,6 +597,7 @@ extern "C" int cpab_b200_orthogonalize(int dtype, const void *x, int64_t batch, 
   cudaError_t e = prepare(list, 0.f, 0, eps, s);
   FinalGroup f = {};
   f.out = out, f.stride = rows * columns, f.first = -1, f.dtype = dtype, f.turned = t.turned();
+  f.wide = !t.turned() && aligned_to(out, columns, dtype_size(dtype), 32);
   const float c[3] = {(float)coefficients[0], (float)coefficients[1], (float)coefficients[2]};
   if (e == cudaSuccess) e = schulz(sets, places, &f, nullptr, 0, steps, c, s);
   return launch_status(e, "orthogonalize");
@@ -676,6 +701,8 @@ extern "C" int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double
         const cpab_muon_tensor &m = tensors[q.tensors[k]];
         const int64_t at = z * t.m() * t.x_pitch();
         table[k] = m.param;
+        if (z == 0) f.wide = !t.turned();
+        f.wide = f.wide && aligned_to(m.param, t.cols, dtype_size(t.dtype), 32);
         in.push_back({m.grad, m.momentum, places[g].x[0][0] + at, places[g].x[0][1] + at, partials + k * kPartials,
                       t.x_pitch(), t.rows, t.cols, t.dtype, t.turned()});
       }

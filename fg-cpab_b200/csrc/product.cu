@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "product_core.cuh"
 #include "sequence.cuh"
@@ -76,13 +77,54 @@ struct QuantizeArgs {
   float *sums;             // [ceil(rows / 128), columns]: columns' sums over each tile, or null
 };
 
+// The eight elements of a row that a thread holds, as read: magnitudes, their maximum
+// and float32 values.  Magnitudes of 16-bit types are compared two at a time, as
+// whole numbers.
+template <typename T>
+struct Eight {
+  uint32_t w[4];
+  __device__ float2 pair(int k) const { return unpack_pair<T>(w[k]); }
+  // Bits of the larger magnitude of two words each, element by element.
+  static __device__ uint32_t larger(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+  __device__ uint32_t magnitude(int k) const { return w[k] & 0x7FFF7FFFu; }
+  __device__ uint32_t most() const {
+    const uint32_t m = larger(larger(magnitude(0), magnitude(1)), larger(magnitude(2), magnitude(3)));
+    return max(m & 0xFFFFu, m >> 16);
+  }
+  static constexpr int kWords = 4;
+  // float32 bits of the element's magnitude
+  static __device__ uint32_t bits(uint32_t m) {
+    if constexpr (sizeof(T) == 4) return m;
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return m << 16;
+    else return __float_as_uint(__half2float(__ushort_as_half((uint16_t)m)));
+  }
+};
+template <>
+struct Eight<float> {
+  uint32_t w[8];
+  __device__ float2 pair(int k) const { return make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1])); }
+  static __device__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+  __device__ uint32_t magnitude(int k) const { return w[k] & 0x7FFFFFFFu; }
+  __device__ uint32_t most() const {
+    uint32_t m = magnitude(0);
+#pragma unroll
+    for (int k = 1; k < 8; ++k) m = max(m, magnitude(k));
+    return m;
+  }
+  static constexpr int kWords = 8;
+  static __device__ uint32_t bits(uint32_t m) { return m; }
+};
+
 // A block takes a tile of 128 x 128; a thread 8 rows x 8 columns of it, so that a
 // row's block is 16 threads' (half a warp's) and a column's 8 codes are one word
-// pair of the transposed codes.
+// pair of the transposed codes, which cross through shared memory.
 template <typename T, bool VEC, bool ROWS, bool COLUMNS, bool SUMS>
-__global__ void __launch_bounds__(256) k_quantize(const QuantizeArgs a) {
-  __shared__ uint32_t most_of[COLUMNS ? 16 : 1][COLUMNS ? 128 : 1];
-  __shared__ float sum_of[SUMS ? 16 : 1][SUMS ? 128 : 1];
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize(const QuantizeArgs a) {
+  using E = Eight<T>;
+  constexpr int W = E::kWords;
+  __shared__ uint32_t most_of[COLUMNS ? 8 : 1][COLUMNS ? 16 * W : 1];
+  __shared__ float inverse[COLUMNS ? 128 : 1];
+  __shared__ float sum_of[SUMS ? 8 : 1][SUMS ? 128 : 1];
   __shared__ uint2 turned[COLUMNS ? 128 * 16 : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane & 15, band = 2 * warp + (lane >> 4);  // this thread's columns 8 l.., rows 8 band..
@@ -90,62 +132,60 @@ __global__ void __launch_bounds__(256) k_quantize(const QuantizeArgs a) {
   const int64_t ty = blockIdx.x / tiles_x, tx = blockIdx.x % tiles_x;
   const int64_t c0 = tx * 128 + 8 * l, r0 = ty * 128 + 8 * band;
   const T *x = static_cast<const T *>(a.x) + r0 * a.x_row + c0;
+  tc::dep_launch();
+  tc::dep_wait();
 
-  float v[8][8];
+  E v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const bool in = r0 + i < a.rows;
-    if (VEC) {
-      constexpr int N = 16 / sizeof(T);
+    if (VEC && in && c0 + 8 <= a.columns) {
 #pragma unroll
-      for (int j = 0; j < 8; j += N) {
-        Pack<T, N> p;
-        if (in && c0 + j + N <= a.columns) {
-          p = *reinterpret_cast<const Pack<T, N> *>(x + i * a.x_row + j);
+      for (int k = 0; k < W; k += 4)
+        *reinterpret_cast<uint4 *>(v[i].w + k) =
+            *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(x + i * a.x_row) + k);
+    } else {  // (nothing is read past a row's end)
 #pragma unroll
-          for (int k = 0; k < N; ++k) v[i][j + k] = to_f32(p.v[k]);
-        } else {  // (nothing is read past a row's end)
-#pragma unroll
-          for (int k = 0; k < N; ++k)
-            v[i][j + k] = in && c0 + j + k < a.columns ? to_f32(x[i * a.x_row + j + k]) : 0.f;
-        }
+      for (int k = 0; k < 4; ++k) {
+        const float e0 = in && c0 + 2 * k < a.columns ? to_f32(x[i * a.x_row + 2 * k]) : 0.f;
+        const float e1 = in && c0 + 2 * k + 1 < a.columns ? to_f32(x[i * a.x_row + 2 * k + 1]) : 0.f;
+        if constexpr (sizeof(T) == 2) v[i].w[k] = pack_pair<T>(e0, e1);
+        else v[i].w[2 * k] = __float_as_uint(e0), v[i].w[2 * k + 1] = __float_as_uint(e1);
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = in && c0 + j < a.columns ? to_f32(x[i * a.x_row + j]) : 0.f;
     }
   }
 
   if (COLUMNS) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t most = 0;
+    for (int k = 0; k < W; ++k) {
+      uint32_t most = v[0].magnitude(k);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
-      most_of[band][8 * l + j] = most;
+      for (int i = 1; i < 8; ++i) most = E::larger(most, v[i].magnitude(k));
+      most = E::larger(most, __shfl_xor_sync(~0u, most, 16));
+      if (lane < 16) most_of[warp][l * W + k] = most;
     }
   }
   if (SUMS) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float s = 0.f;
+    for (int k = 0; k < 4; ++k) {
+      float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[i][j];
-      sum_of[band][8 * l + j] = s;
+      for (int i = 0; i < 8; ++i) s.x += v[i].pair(k).x, s.y += v[i].pair(k).y;
+      s.x += __shfl_xor_sync(~0u, s.x, 16);
+      s.y += __shfl_xor_sync(~0u, s.y, 16);
+      if (lane < 16) *reinterpret_cast<float2 *>(&sum_of[warp][8 * l + 2 * k]) = s;
     }
   }
   if (ROWS) {
     const uint32_t half = 0xFFFFu << (lane & 16);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      uint32_t most = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
-      const uint32_t e = scale_exponent(__reduce_max_sync(half, most));
+      const uint32_t e = scale_exponent(E::bits(__reduce_max_sync(half, v[i].most())));
       const float r = inverse_scale(e);
+      const float2 p0 = v[i].pair(0), p1 = v[i].pair(1), p2 = v[i].pair(2), p3 = v[i].pair(3);
       uint2 w;
-      w.x = codes_of(v[i][0] * r, v[i][1] * r, v[i][2] * r, v[i][3] * r);
-      w.y = codes_of(v[i][4] * r, v[i][5] * r, v[i][6] * r, v[i][7] * r);
+      w.x = codes_of(p0.x * r, p0.y * r, p1.x * r, p1.y * r);
+      w.y = codes_of(p2.x * r, p2.y * r, p3.x * r, p3.y * r);
       if (r0 + i < a.rows) {
         // (rows are padded to multiples of 16 codes)
         if (c0 < a.columns) *reinterpret_cast<uint2 *>(a.q + (r0 + i) * a.q_row + c0) = w;
@@ -155,29 +195,43 @@ __global__ void __launch_bounds__(256) k_quantize(const QuantizeArgs a) {
   }
   if (!COLUMNS && !SUMS) return;
   __syncthreads();
-  if (COLUMNS) {
-    // (all bands' threads of a column find its maximum, of which they keep the scale)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
+  if (threadIdx.x < 128) {
+    const int c = threadIdx.x;
+    const int64_t column = tx * 128 + c;
+    if (COLUMNS) {
       uint32_t most = 0;
 #pragma unroll
-      for (int b = 0; b < 16; ++b) most = max(most, most_of[b][8 * l + j]);
-      const uint32_t e = scale_exponent(most);
-      const float r = inverse_scale(e);
-      uint2 w;
-      w.x = codes_of(v[0][j] * r, v[1][j] * r, v[2][j] * r, v[3][j] * r);
-      w.y = codes_of(v[4][j] * r, v[5][j] * r, v[6][j] * r, v[7][j] * r);
-      turned[(8 * l + j) * 16 + (band ^ l)] = w;  // (so that half a warp's words lie in different banks)
-      if (band == 0 && c0 + j < a.columns) a.scale_t[(c0 + j) * a.scale_t_row + ty] = (uint8_t)e;
+      for (int b = 0; b < 8; ++b) {
+        const uint32_t m = sizeof(T) == 2 ? most_of[b][c >> 1] >> (16 * (c & 1)) & 0xFFFFu : most_of[b][c];
+        most = max(most, m);
+      }
+      const uint32_t e = scale_exponent(E::bits(most));
+      inverse[c] = inverse_scale(e);
+      if (column < a.columns) a.scale_t[column * a.scale_t_row + ty] = (uint8_t)e;
+    }
+    if (SUMS && column < a.columns) {
+      float s = 0.f;
+#pragma unroll
+      for (int b = 0; b < 8; ++b) s += sum_of[b][c];
+      a.sums[ty * a.columns + column] = s;
     }
   }
-  if (SUMS && threadIdx.x < 128 && tx * 128 + threadIdx.x < a.columns) {
-    float s = 0.f;
-#pragma unroll
-    for (int b = 0; b < 16; ++b) s += sum_of[b][threadIdx.x];
-    a.sums[ty * a.columns + tx * 128 + threadIdx.x] = s;
-  }
   if (!COLUMNS) return;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 r = *reinterpret_cast<const float2 *>(&inverse[8 * l + 2 * k]);
+    float2 p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = v[i].pair(k);
+    uint2 w;
+    w.x = codes_of(p[0].x * r.x, p[1].x * r.x, p[2].x * r.x, p[3].x * r.x);
+    w.y = codes_of(p[4].x * r.x, p[5].x * r.x, p[6].x * r.x, p[7].x * r.x);
+    turned[(8 * l + 2 * k) * 16 + (band ^ l)] = w;  // (so that half a warp's words lie in different banks)
+    w.x = codes_of(p[0].y * r.y, p[1].y * r.y, p[2].y * r.y, p[3].y * r.y);
+    w.y = codes_of(p[4].y * r.y, p[5].y * r.y, p[6].y * r.y, p[7].y * r.y);
+    turned[(8 * l + 2 * k + 1) * 16 + (band ^ l)] = w;
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -188,33 +242,49 @@ __global__ void __launch_bounds__(256) k_quantize(const QuantizeArgs a) {
   }
 }
 
-// Columns' sums over the tiles, in order.
+// Columns' sums over the tiles, in a fixed order: 32 columns a block, each by 8
+// threads.
 template <typename T>
 __global__ void __launch_bounds__(256) k_sum_tiles(const float *sums, int64_t tiles, int64_t columns, T *out) {
-  const int64_t c = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= columns) return;
+  __shared__ float part[8][32];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + x;
+  tc::dep_launch();
+  tc::dep_wait();
   float s = 0.f;
-  for (int64_t t = 0; t < tiles; ++t) s += sums[t * columns + c];
-  out[c] = from_f32<T>(s);
+  if (c < columns) {
+#pragma unroll 8
+    for (int64_t t = y; t < tiles; t += 8) s += sums[t * columns + c];
+  }
+  part[y][x] = s;
+  __syncthreads();
+  if (y == 0 && c < columns) {
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += part[k][x];
+    out[c] = from_f32<T>(s);
+  }
 }
 
 template <typename T, bool VEC>
-void launch_quantize_as(const QuantizeArgs &a, unsigned grid, cudaStream_t s) {
+cudaError_t launch_quantize_as(const QuantizeArgs &a, unsigned grid, cudaStream_t s) {
   const bool rows = a.q != nullptr, columns = a.qt != nullptr;
+  auto go = [&](void (*kernel)(QuantizeArgs)) { return tc::launch(kernel, grid, 256, 0, 1, s, a); };
   if (a.sums != nullptr) {
-    if (rows && columns) k_quantize<T, VEC, true, true, true><<<grid, 256, 0, s>>>(a);
-    else if (rows) k_quantize<T, VEC, true, false, true><<<grid, 256, 0, s>>>(a);
-    else if (columns) k_quantize<T, VEC, false, true, true><<<grid, 256, 0, s>>>(a);
-    else k_quantize<T, VEC, false, false, true><<<grid, 256, 0, s>>>(a);
-  } else if (rows && columns) k_quantize<T, VEC, true, true, false><<<grid, 256, 0, s>>>(a);
-  else if (rows) k_quantize<T, VEC, true, false, false><<<grid, 256, 0, s>>>(a);
-  else k_quantize<T, VEC, false, true, false><<<grid, 256, 0, s>>>(a);
+    if (rows && columns) return go(k_quantize<T, VEC, true, true, true>);
+    if (rows) return go(k_quantize<T, VEC, true, false, true>);
+    if (columns) return go(k_quantize<T, VEC, false, true, true>);
+    return go(k_quantize<T, VEC, false, false, true>);
+  }
+  if (rows && columns) return go(k_quantize<T, VEC, true, true, false>);
+  if (rows) return go(k_quantize<T, VEC, true, false, false>);
+  return go(k_quantize<T, VEC, false, true, false>);
 }
 
 template <typename T>
-void launch_quantize(const QuantizeArgs &a, unsigned grid, cudaStream_t s) {
-  if (aligned_to(a.x, a.x_row, sizeof(T), 16)) launch_quantize_as<T, true>(a, grid, s);
-  else launch_quantize_as<T, false>(a, grid, s);
+cudaError_t launch_quantize(const QuantizeArgs &a, unsigned grid, cudaStream_t s) {
+  return aligned_to(a.x, a.x_row, sizeof(T), 16) ? launch_quantize_as<T, true>(a, grid, s)
+                                                 : launch_quantize_as<T, false>(a, grid, s);
 }
 
 // ---- products ------------------------------------------------------------------
@@ -222,7 +292,7 @@ void launch_quantize(const QuantizeArgs &a, unsigned grid, cudaStream_t s) {
 struct Scales {
   const uint8_t *bytes;  // e8m0 [rows, row], or null: all 1
   int64_t row;
-  int words;             // rows begin on multiples of 4 bytes and hold whole words
+  int words;             // rows begin on multiples of 4 bytes
 };
 
 struct ProductArgs {
@@ -234,29 +304,45 @@ struct ProductArgs {
   int64_t y_row;
   int M, N, steps;
   int tiles_m, tiles_n;
-  int wide;              // y's rows begin on 32 bytes
+  int wide;              // y's rows begin on 16 bytes
 };
 
-__device__ __forceinline__ uint32_t scale_word(const Scales &s, int row, int rows, int group, int blocks) {
-  if (s.bytes == nullptr || row >= rows) return 0x7F7F7F7Fu;
-  const uint8_t *p = s.bytes + (int64_t)row * s.row + 4 * group;
-  if (s.words) return __ldg(reinterpret_cast<const uint32_t *>(p));
-  uint32_t w = 0;
+// A row's scales of 8 steps.  Rows outside hold no codes: any scale but NaN.
+__device__ __forceinline__ void scale_words(const Scales &s, int row, int rows, int group, int blocks, uint32_t (&w)[2]) {
+  if (s.bytes == nullptr || row >= rows) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (4 * group + i < blocks) w |= (uint32_t)__ldg(p + i) << (8 * i);
-  return w;
+    for (int q = 0; q < 2; ++q) w[q] = 0x7F7F7F7Fu;
+    return;
+  }
+  const int first = 8 * group;
+  const uint8_t *p = s.bytes + (int64_t)row * s.row + first;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    w[q] = 0;
+    if (s.words && first + 4 * q + 4 <= blocks) {
+      w[q] = __ldg(reinterpret_cast<const uint32_t *>(p) + q);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (first + 4 * q + i < blocks) w[q] |= (uint32_t)__ldg(p + 4 * q + i) << (8 * i);
+    }
+  }
 }
 
 // y = A B^T in tiles of 128 CTAS x BN.
 template <typename T, typename TB, int CTAS, int BN>
 struct Product {
   static constexpr int kCtas = CTAS, kBN = BN, kAcc = BN * 2 + 16 <= 512 ? 2 : 1, kParts = 1, kSegment = 0;
+  static constexpr int kChunk = 64 / sizeof(T);  // 64 bytes of a row at a time
   static constexpr bool kScaled = true, kBMn = false;
   // A tile's columns' scales and bias; the next tile's are written while slow warps
   // still read this one's.
   struct alignas(16) Shared {
     float scale[2][BN], bias[2][BN];
+    // Each warp's 32 rows of 64 bytes (and 16 of padding, for the banks) on their way
+    // out, so that four threads store a row's 64 bytes and not each thread its own
+    // row's 32.
+    uint4 rows[8][32][5];
   };
   struct Tile {
     int m0, n0, steps, slot;
@@ -275,11 +361,11 @@ struct Product {
     tc::tile_load<CTAS>(sa, &a.a, bar, k * 128, t.m0 + rank * 128, 0);
     tc::tile_load<CTAS>(sb, &a.b, bar, k * 128, t.n0 + rank * (BN / CTAS), 0);
   }
-  __device__ uint32_t scale_words_a(const Tile &t, uint32_t rank, int row, int g) const {
-    return scale_word(a.sa, t.m0 + rank * 128 + row, a.M, g, a.steps);
+  __device__ void scales_a(const Tile &t, uint32_t rank, int row, int g, uint32_t (&w)[2]) const {
+    scale_words(a.sa, t.m0 + rank * 128 + row, a.M, g, a.steps, w);
   }
-  __device__ uint32_t scale_words_b(const Tile &t, int row, int g) const {
-    return scale_word(a.sb, t.n0 + row, a.N, g, a.steps);
+  __device__ void scales_b(const Tile &t, int row, int g, uint32_t (&w)[2]) const {
+    scale_words(a.sb, t.n0 + row, a.N, g, a.steps, w);
   }
   __device__ void begin(const Tile &t, Shared &sh, int thread) const {
     if (a.rb == nullptr && a.bias == nullptr) return;
@@ -291,36 +377,46 @@ struct Product {
     }
     tc::epilogue_sync();
   }
-  __device__ void store(const Tile &t, const Shared &sh, int row, int c, const float *acc) const {
-    const int col = t.n0 + c;
-    if (row >= a.M || col >= a.N) return;
-    float v[16];
-    const float ra = a.ra != nullptr ? a.ra[row] : 1.f;
+  __device__ void store(const Tile &t, Shared &sh, int row, int c, const float *acc) const {
+    const int col = t.n0 + c, lane = threadIdx.x & 31;
+    if (col >= a.N) return;
+    uint4(&rows)[32][5] = sh.rows[(threadIdx.x >> 5) - 4];
+    const float ra = a.ra != nullptr && row < a.M ? a.ra[row] : 1.f;
+    const bool columns = a.rb != nullptr || a.bias != nullptr;
+    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = acc[j] * ra;
-    if (a.rb != nullptr || a.bias != nullptr) {
+    for (int h = 0; h < 4; ++h) {  // 16 bytes
+      constexpr int E = 16 / sizeof(T);
+      float v[E];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = fmaf(v[j], sh.scale[t.slot][c + j], sh.bias[t.slot][c + j]);
-    }
-    T *y = static_cast<T *>(a.y) + (int64_t)row * a.y_row + col;
-    if (a.wide && col + 16 <= a.N) {
-      uint32_t w[8];
-      if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = pack_pair<T>(v[2 * j], v[2 * j + 1]);
-        tc::store_sector(y, w);
-      } else {
-#pragma unroll
-        for (int h = 0; h < 16; h += 8) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[h + j]);
-          tc::store_sector(y + h, w);
-        }
+      for (int j = 0; j < E; ++j) {
+        v[j] = acc[h * E + j] * ra;
+        if (columns) v[j] = fmaf(v[j], sh.scale[t.slot][c + h * E + j], sh.bias[t.slot][c + h * E + j]);
       }
-    } else {
+      uint4 w;
+      if constexpr (sizeof(T) == 2)
+        w = make_uint4(pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]), pack_pair<T>(v[4], v[5]), pack_pair<T>(v[6], v[7]));
+      else
+        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      rows[lane][h] = w;
+    }
+    __syncwarp();
+    const int first = row - lane;  // of the warp's rows
+    if (a.wide && col + kChunk <= a.N) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (col + j < a.N) y[j] = from_f32<T>(v[j]);
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2);
+        if (first + r < a.M)
+          *reinterpret_cast<uint4 *>(static_cast<T *>(a.y) + (int64_t)(first + r) * a.y_row + col + (lane & 3) * (16 / sizeof(T))) =
+              rows[r][lane & 3];
+      }
+    } else {  // rows that begin anywhere, or end here: element by element
+      constexpr int R = 32 / kChunk;  // rows at a time
+      const int x = lane % kChunk;
+      T *y = static_cast<T *>(a.y) + col + x;
+#pragma unroll 4
+      for (int r = lane / kChunk; r < 32; r += R)
+        if (first + r < a.M && col + x < a.N) y[(int64_t)(first + r) * a.y_row] = reinterpret_cast<const T *>(rows[r])[x];
     }
   }
 };
@@ -339,22 +435,35 @@ cudaError_t launch_product_as(ProductArgs &a, cudaStream_t s) {
   a.tiles_m = (a.M + 128 * CTAS - 1) / (128 * CTAS);
   a.tiles_n = (a.N + BN - 1) / BN;
   const int tiles = a.tiles_m * a.tiles_n, groups = device_info().sm_count / CTAS;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(CTAS * std::min(tiles, groups)));
-  cfg.blockDim = dim3(tc::kCoreThreads);
-  cfg.dynamicSmemBytes = S::kBytes;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {CTAS, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  return tc::launch(kernel, (unsigned)(CTAS * std::min(tiles, groups)), tc::kCoreThreads, S::kBytes, CTAS, s, a);
+}
+
+// The tile of the least time: 128 x 64, 128 x 128, or 256 x 256 by a pair of blocks.
+// Measured (us, bf16): a wave of tiles costs 0.3 + 0.26 s, 0.4 + 0.29 s and 1.5 + 0.40 s
+// for s steps of 128, a launch 3, 3 and 4.8 more.  1024^3: 5.3, 6.1, 9.4 us; 2048^3:
+// 20.7, 13.4, 12.8; 16384 x 4096 x 2048: 249, 144, 111.
+int tile_of(int64_t M, int64_t N, int64_t steps) {
+  const int64_t sms = device_info().sm_count;
+  const float launch[3] = {3.f, 3.f, 4.8f}, wave[3] = {0.3f, 0.4f, 1.5f}, step[3] = {0.26f, 0.29f, 0.40f};
+  const int64_t rows[3] = {128, 128, 256}, columns[3] = {64, 128, 256};
+  int best = 0;
+  float least = 0.f;
+  for (int k = 0; k < 3; ++k) {
+    const int64_t tiles = (M + rows[k] - 1) / rows[k] * ((N + columns[k] - 1) / columns[k]);
+    const int64_t slots = std::max<int64_t>(1, k == 2 ? sms / 2 : sms), waves = (tiles + slots - 1) / slots;
+    const float t = launch[k] + (float)waves * (wave[k] + step[k] * (float)steps);
+    if (k == 0 || t < least) best = k, least = t;
+  }
+  return best;
 }
 
 template <typename T, typename TB>
 cudaError_t launch_product(ProductArgs &a, cudaStream_t s) {
-  return a.M > 128 && a.N > 128 ? launch_product_as<T, TB, 2, 256>(a, s) : launch_product_as<T, TB, 1, 128>(a, s);
+  switch (tile_of(a.M, a.N, a.steps)) {
+    case 2: return launch_product_as<T, TB, 2, 256>(a, s);
+    case 1: return launch_product_as<T, TB, 1, 128>(a, s);
+    default: return launch_product_as<T, TB, 1, 64>(a, s);
+  }
 }
 
 // What an operand lacks, or null; fills the map and scales.
@@ -396,9 +505,9 @@ extern "C" int cpab_b200_quantize_blocks(int dtype, const void *x, int64_t x_row
   const int64_t tiles_y = (rows + 127) / 128, tiles_x = (columns + 127) / 128;
   if (rows >= int64_t(1) << 31 || columns >= int64_t(1) << 31 || tiles_x * tiles_y >= int64_t(1) << 31)
     return report_error(CPAB_ERR_SIZE, "%s", "quantize_blocks: too many elements");
-  if (q == nullptr && qt == nullptr && column_sum == nullptr)
-    return report_error(CPAB_ERR_ARG, "%s", "quantize_blocks: nothing to write");
   if (rows > 0 && columns > 0) {
+    if (q == nullptr && qt == nullptr && column_sum == nullptr)
+      return report_error(CPAB_ERR_ARG, "%s", "quantize_blocks: nothing to write");
     if (x == nullptr) return report_error(CPAB_ERR_ARG, "%s", "quantize_blocks: null x");
     if (q != nullptr && (scale == nullptr || reinterpret_cast<uintptr_t>(q) % 16 || q_row % 16 || q_row < columns ||
                          scale_row < tiles_x))
@@ -412,22 +521,23 @@ extern "C" int cpab_b200_quantize_blocks(int dtype, const void *x, int64_t x_row
       return report_error(CPAB_ERR_ARG, "%s", "quantize_blocks: column sums need a workspace");
   }
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
   if (rows > 0 && columns > 0) {
     const QuantizeArgs a = {x, x_row, rows, columns, q, scale, q_row, scale_row, qt, scale_t, qt_row, scale_t_row,
                             column_sum != nullptr ? workspace : nullptr};
     const unsigned grid = (unsigned)(tiles_x * tiles_y);
-    if (dtype == CPAB_F32) launch_quantize<float>(a, grid, s);
-    else if (dtype == CPAB_F16) launch_quantize<__half>(a, grid, s);
-    else launch_quantize<__nv_bfloat16>(a, grid, s);
+    e = dtype == CPAB_F32   ? launch_quantize<float>(a, grid, s)
+        : dtype == CPAB_F16 ? launch_quantize<__half>(a, grid, s)
+                            : launch_quantize<__nv_bfloat16>(a, grid, s);
   }
-  if (column_sum != nullptr && columns > 0) {
-    const unsigned grid = (unsigned)((columns + 255) / 256);
+  if (e == cudaSuccess && column_sum != nullptr && columns > 0) {
+    const unsigned grid = (unsigned)((columns + 31) / 32);
     const int64_t n = rows > 0 ? tiles_y : 0;
-    if (sum_dtype == CPAB_F32) k_sum_tiles<<<grid, 256, 0, s>>>(workspace, n, columns, static_cast<float *>(column_sum));
-    else if (sum_dtype == CPAB_F16) k_sum_tiles<<<grid, 256, 0, s>>>(workspace, n, columns, static_cast<__half *>(column_sum));
-    else k_sum_tiles<<<grid, 256, 0, s>>>(workspace, n, columns, static_cast<__nv_bfloat16 *>(column_sum));
+    if (sum_dtype == CPAB_F32) e = tc::launch(k_sum_tiles<float>, grid, 256, 0, 1, s, static_cast<const float *>(workspace), n, columns, static_cast<float *>(column_sum));
+    else if (sum_dtype == CPAB_F16) e = tc::launch(k_sum_tiles<__half>, grid, 256, 0, 1, s, static_cast<const float *>(workspace), n, columns, static_cast<__half *>(column_sum));
+    else e = tc::launch(k_sum_tiles<__nv_bfloat16>, grid, 256, 0, 1, s, static_cast<const float *>(workspace), n, columns, static_cast<__nv_bfloat16 *>(column_sum));
   }
-  return launch_status(cudaGetLastError(), "quantize_blocks");
+  return launch_status(e, "quantize_blocks");
 }
 
 extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, const cpab_quantized *weight, int64_t M,
@@ -438,16 +548,16 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   if (x == nullptr || weight == nullptr) return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: null operand");
   if (M < 0 || N < 0 || K < 1 || y_row < N) return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: sizes out of range");
   constexpr int64_t kMost = (int64_t(1) << 31) - 512;
-  if (M > kMost || N > kMost || K > kMost || (M + 127) / 128 * ((N + 127) / 128) >= kMost)
+  if (M > kMost || N > kMost || K > kMost || (M + 127) / 128 * ((N + 63) / 64) >= kMost)
     return report_error(CPAB_ERR_SIZE, "%s", "matmul_quantized: sizes too large");
   if (M == 0 || N == 0) return report_error(CPAB_OK, "%s", "");
   if (y == nullptr) return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: null y");
   ProductArgs a = {};
   const char *why = operand(*x, M, K, 128, &a.a, &a.sa, &a.ra);
-  if (why == nullptr) why = operand(*weight, N, K, 128, &a.b, &a.sb, &a.rb);
+  if (why == nullptr) why = operand(*weight, N, K, tile_of(M, N, (K + kBlock - 1) / kBlock) == 0 ? 64 : 128, &a.b, &a.sb, &a.rb);
   if (why != nullptr) return report_error(CPAB_ERR_ARG, "matmul_quantized: %s", why);
   a.bias = bias, a.y = y, a.y_row = y_row, a.M = (int)M, a.N = (int)N, a.steps = (int)((K + kBlock - 1) / kBlock);
-  a.wide = aligned_to(y, y_row, dtype_size(dtype), 32);
+  a.wide = aligned_to(y, y_row, dtype_size(dtype), 16);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == CPAB_F32) e = launch_product<float, float>(a, s);

@@ -12,6 +12,7 @@
 //                     takes part x part of all but the remainders' product
 //   kBMn              B's rows run along the other axis than the summed one
 //   kAcc              accumulators in turn
+//   kChunk            columns that store takes at a time: 16 or 32
 //   kSegment          stages to an accumulator, whose sums are then added in
 //                     registers (0: a tile's all).  The tensor cores cut, not round,
 //                     what a float32 sum cannot hold, so an error of up to 2^-24 of
@@ -21,9 +22,10 @@
 //   Tile tile(int i)                {m0, n0, steps, ...}
 //   load(tile, step, a, b, bar, rank)    issues the copies of one stage; the second
 //                     parts lie kAHalf and kBHalf bytes behind the first
-//   scale_words_a / _b(tile, rank, row, group) -> the row's scales of four steps
+//   scales_a / _b(tile, rank, row, group, words)  a row's scales of 8 steps, four to a word
 //   begin(tile, shared, thread)     before a tile's accumulators are waited for
-//   store(tile, shared, rank, row, column, values)  16 values of one row
+//   store(tile, shared, row, column, values)  kChunk values of this thread's row; the
+//                     warp's rows are 32 in order
 #pragma once
 
 #include "tensor_core.cuh"
@@ -42,15 +44,19 @@ template <class P>
 struct CoreShape {
   static constexpr int kBHalf = P::kBN / P::kCtas * 128;  // bytes of one part of B a block holds
   static constexpr int kStageBytes = P::kParts * (kAHalf + kBHalf);
-  static constexpr int kScaleChunks = P::kScaled ? 1 + (P::kBN + 127) / 128 : 0;  // 512 bytes each
-  static constexpr int kScaleSlots = P::kScaled ? 3 : 0;
-  static constexpr int kScaleBytes = kScaleSlots * kScaleChunks * 512;
+  // Scale words: a chunk is those of 128 rows and four steps (512 bytes, four columns
+  // of tensor memory); a slot holds 8 steps', in shared memory and in tensor memory
+  // alike.
+  static constexpr int kScaleChunks = P::kScaled ? 1 + (P::kBN + 127) / 128 : 0;
+  static constexpr int kScaleSlots = 2;
+  static constexpr int kSlotBytes = 2 * kScaleChunks * 512, kSlotColumns = 2 * kScaleChunks * 4;
+  static constexpr int kScaleBytes = kScaleSlots * kSlotBytes;
   static constexpr int kFixed = 1024 /* alignment */ + 512 /* barriers */ + kScaleBytes + (int)sizeof(typename P::Shared);
   static constexpr int kRoom = 227 * 1024 - kFixed;
   static constexpr int kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
   static constexpr int kBytes = kFixed + kStages * kStageBytes;
   static constexpr int kScaleColumn = P::kAcc * P::kBN;  // first tensor-memory column of the scales
-  static constexpr int kColumnsUsed = kScaleColumn + 4 * kScaleChunks;
+  static constexpr int kColumnsUsed = kScaleColumn + kScaleSlots * kSlotColumns;
   static constexpr int kColumns = kColumnsUsed <= 128 ? 128 : kColumnsUsed <= 256 ? 256 : 512;
   static_assert(sizeof(typename P::Shared) % 16 == 0, "barriers lie behind it");
   static_assert(kStages >= 3 && kColumnsUsed <= 512, "a tile too large");
@@ -58,7 +64,7 @@ struct CoreShape {
 };
 
 struct CoreBarriers {
-  uint64_t full[8], empty[8], scale_full[3], scale_empty[3], acc_full[2], acc_empty[2];
+  uint64_t full[8], empty[8], scale_full[2], scale_empty[2], acc_full[2], acc_empty[2];
   uint32_t tmem;
   int gave_up;
 };
@@ -93,13 +99,13 @@ __device__ __forceinline__ void core(const P &p) {
   const uint32_t sfull = smem_u32(bars->scale_full), sempty = smem_u32(bars->scale_empty);
   const uint32_t afull = smem_u32(bars->acc_full), aempty = smem_u32(bars->acc_empty);
   constexpr int kLength = P::kSegment > 0 ? P::kSegment : 1 << 30;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = C == 2 ? cluster_rank() : 0;
 
   dep_launch();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) bar_init(full + 8 * i, 1), bar_init(empty + 8 * i, 1);
-    for (int i = 0; i < 3; ++i) bar_init(sfull + 8 * i, 2 * C), bar_init(sempty + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) bar_init(sfull + 8 * i, 2 * C), bar_init(sempty + 8 * i, 1);
     for (int i = 0; i < 2; ++i) bar_init(afull + 8 * i, 1), bar_init(aempty + 8 * i, 8 * C);
     bars->gave_up = 0;
     bar_init_fence();
@@ -109,7 +115,7 @@ __device__ __forceinline__ void core(const P &p) {
   if constexpr (C == 2) cluster_sync();
   else __syncthreads();
   fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&bars->tmem);
+  const uint32_t tmem = __shfl_sync(~0u, *reinterpret_cast<volatile uint32_t *>(&bars->tmem), 0);
   volatile int *gave_up = &bars->gave_up;
   dep_wait();
 
@@ -118,96 +124,106 @@ __device__ __forceinline__ void core(const P &p) {
   const uint32_t full0 = C == 2 ? mapa(full, 0) : full;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0, phase = 0;
-      for (int i = first; i < tiles && !*gave_up; i += stride) {
-        const auto t = p.tile(i);
-        for (int k = 0; k < t.steps; ++k) {
-          if (!bar_wait(empty + 8 * s, phase ^ 1)) { *gave_up = 1; break; }
+    int s = 0, phase = 0;
+    bool ok = true;
+    for (int i = first; i < tiles && ok; i += stride) {
+      const auto t = p.tile(i);
+      for (int k = 0; k < t.steps; ++k) {
+        ok = bar_wait_warp(empty + 8 * s, phase ^ 1);
+        if (!ok) break;
+        if (elect()) {
           if (rank == 0) bar_expect(full + 8 * s, C * S::kStageBytes);
           const uint32_t a = stage0 + s * S::kStageBytes;
           p.load(t, k, a, a + P::kParts * kAHalf, full0 + 8 * s, rank);
-          if (++s == S::kStages) s = 0, phase ^= 1;
         }
+        __syncwarp();
+        if (++s == S::kStages) s = 0, phase ^= 1;
       }
     }
+    if (!ok) *gave_up = 1;
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       int s = 0, phase = 0, sc = 0, sphase = 0, acc = 0, aphase = 0;
-      for (int i = first; i < tiles && !*gave_up; i += stride) {
+      bool ok = true;
+      for (int i = first; i < tiles && ok; i += stride) {
         const auto t = p.tile(i);
         for (int k = 0; k < t.steps; ++k) {
           const bool fresh = k % kLength == 0;
-          if (fresh) {
-            if (!bar_wait(aempty + 8 * acc, aphase ^ 1)) { *gave_up = 1; break; }
-            fence_after();
-          }
-          const uint32_t d = tmem + acc * P::kBN;
+          if (fresh && !(ok = bar_wait_warp(aempty + 8 * acc, aphase ^ 1))) break;
           if constexpr (P::kScaled) {
-            if ((k & 3) == 0) {
-              if (!bar_wait(sfull + 8 * sc, sphase)) { *gave_up = 1; break; }
+            if ((k & 7) == 0) {
+              if ((k > 0 || i != first) && ++sc == S::kScaleSlots) sc = 0, sphase ^= 1;
+              if (!(ok = bar_wait_warp(sfull + 8 * sc, sphase))) break;
               fence_after();
-              const uint32_t from = scale0 + sc * S::kScaleChunks * 512;
-              for (int c = 0; c < S::kScaleChunks; ++c)
-                scales_to_tmem<C>(tmem + S::kScaleColumn + 4 * c, plain_desc(from + 512 * c));
-              mma_commit<C>(sempty + 8 * sc);
-              if (++sc == 3) sc = 0, sphase ^= 1;
+              const uint32_t from = scale0 + sc * S::kSlotBytes, to = tmem + S::kScaleColumn + sc * S::kSlotColumns;
+              const int chunks = min(2, (t.steps - k + 3) >> 2) * S::kScaleChunks;
+              if (elect()) {
+                for (int c = 0; c < chunks; ++c) scales_to_tmem<C>(to + 4 * c, plain_desc(from + 512 * c));
+                mma_commit<C>(sempty + 8 * sc);
+              }
+              __syncwarp();
             }
           }
-          if (!bar_wait(full + 8 * s, phase)) { *gave_up = 1; break; }
+          if (!(ok = bar_wait_warp(full + 8 * s, phase))) break;
           fence_after();
+          const bool last = k + 1 == t.steps || (k + 1) % kLength == 0;
+          const uint32_t d = tmem + acc * P::kBN;
           const uint32_t a = stage0 + s * S::kStageBytes, b = a + P::kParts * kAHalf;
           const uint64_t da = swizzled_desc(a), db = swizzled_desc(b, P::kBMn ? 8192 : 16);
-          // (the small products first, while the sum is small)
+          const uint32_t words = tmem + S::kScaleColumn + sc * S::kSlotColumns + ((k & 7) >> 2) * S::kScaleChunks * 4;
+          if (elect()) {
+            // (the small products first, while the sum is small)
 #pragma unroll
-          for (int part = P::kParts == 2 ? 2 : 0; part >= 0; --part) {
-            const uint64_t pa = da + (part == 2 ? kAHalf >> 4 : 0), pb = db + (part == 1 ? S::kBHalf >> 4 : 0);
+            for (int part = P::kParts == 2 ? 2 : 0; part >= 0; --part) {
+              const uint64_t pa = da + (part == 2 ? kAHalf >> 4 : 0), pb = db + (part == 1 ? S::kBHalf >> 4 : 0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const bool add = !fresh || j > 0 || part != (P::kParts == 2 ? 2 : 0);
-              if constexpr (P::kScaled) {
-                // (the descriptor's scale bytes are those of this step of the four)
-                mma_mx<C>(d, pa + 2 * j, pb + 2 * j, idesc_mx(128 * C, P::kBN, 0) | ((k & 3) << 4) | ((k & 3) << 29),
-                          tmem + S::kScaleColumn, tmem + S::kScaleColumn + 4, add);
-              } else {
-                mma_f16<C>(d, pa + 2 * j, pb + (P::kBMn ? 128 : 2) * j, idesc_f16(128 * C, P::kBN, P::kBMn), add);
+              for (int j = 0; j < 4; ++j) {
+                const bool add = !fresh || j > 0 || part != (P::kParts == 2 ? 2 : 0);
+                if constexpr (P::kScaled) {
+                  // (the descriptor's scale bytes are those of this step of the four)
+                  mma_mx<C>(d, pa + 2 * j, pb + 2 * j, idesc_mx(128 * C, P::kBN, 0) | ((k & 3) << 4) | ((k & 3) << 29),
+                            words, words + 4, add);
+                } else {
+                  mma_f16<C>(d, pa + 2 * j, pb + (P::kBMn ? 128 : 2) * j, idesc_f16(128 * C, P::kBN, P::kBMn), add);
+                }
               }
             }
+            mma_commit<C>(empty + 8 * s);
+            if (last) mma_commit<C>(afull + 8 * acc);
           }
-          mma_commit<C>(empty + 8 * s);
+          __syncwarp();
           if (++s == S::kStages) s = 0, phase ^= 1;
-          if (k + 1 == t.steps || (k + 1) % kLength == 0) {
-            mma_commit<C>(afull + 8 * acc);
-            if (++acc == P::kAcc) acc = 0, aphase ^= 1;
-          }
+          if (last && ++acc == P::kAcc) acc = 0, aphase ^= 1;
         }
       }
+      if (!ok) *gave_up = 1;
     }
   } else if (warp < 4) {
     if constexpr (P::kScaled) {
-      // Scale words of four steps: chunk 0 is A's 128 rows, the others B's.
+      // Warp 2 brings A's words (the first chunk of each four steps), warp 3 B's.
+      constexpr int kB = S::kScaleChunks - 1;
       int sc = 0, sphase = 0;
       bool ok = true;
       for (int i = first; i < tiles && ok; i += stride) {
         const auto t = p.tile(i);
-        for (int g = 0; 4 * g < t.steps && ok; ++g) {
-          uint32_t w[4 * (S::kScaleChunks - 1)];
-          constexpr int kB = S::kScaleChunks - 1;
-          if (warp == 2) {
+        for (int g = 0; 8 * g < t.steps && ok; ++g) {
+          uint32_t w[kB][4][2];  // [chunk][row lane + 32 j][word]
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = p.scale_words_a(t, rank, lane + 32 * j, g);
-          } else {
+          for (int c = 0; c < kB; ++c)
 #pragma unroll
-            for (int j = 0; j < 4 * kB; ++j) w[j] = p.scale_words_b(t, lane + 32 * j, g);
-          }
+            for (int j = 0; j < 4; ++j) {
+              if (warp == 3) p.scales_b(t, 128 * c + lane + 32 * j, g, w[c][j]);
+              else if (c == 0) p.scales_a(t, rank, lane + 32 * j, g, w[c][j]);
+            }
           ok = bar_wait(sempty + 8 * sc, sphase ^ 1);
-          uint8_t *to = scales + sc * S::kScaleChunks * 512 + 16 * lane;
-          if (warp == 2) {
-            *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-          } else {
+          uint8_t *to = scales + sc * S::kSlotBytes + 16 * lane + (warp == 3 ? 512 : 0);
 #pragma unroll
-            for (int c = 0; c < kB; ++c)
-              *reinterpret_cast<uint4 *>(to + 512 * (1 + c)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+          for (int c = 0; c < kB; ++c) {
+            if (warp == 2 && c > 0) break;
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              *reinterpret_cast<uint4 *>(to + 512 * (q * S::kScaleChunks + c)) =
+                  make_uint4(w[c][0][q], w[c][1][q], w[c][2][q], w[c][3][q]);
           }
           proxy_fence();
           __syncwarp();
@@ -215,7 +231,7 @@ __device__ __forceinline__ void core(const P &p) {
             if constexpr (C == 2) bar_arrive_cluster(mapa(sfull + 8 * sc, 0));
             else bar_arrive(sfull + 8 * sc);
           }
-          if (++sc == 3) sc = 0, sphase ^= 1;
+          if (++sc == S::kScaleSlots) sc = 0, sphase ^= 1;
         }
       }
       if (!ok) *gave_up = 1;
@@ -244,7 +260,7 @@ __device__ __forceinline__ void core(const P &p) {
           for (int c = 0; c < kHalf; c += kHold) {
             read_accumulators(ok, d + c, v);
 #pragma unroll
-            for (int j = 0; j < kHold; j += 16) p.store(t, *shared, row, half * kHalf + c + j, v + j);
+            for (int j = 0; j < kHold; j += P::kChunk) p.store(t, *shared, row, half * kHalf + c + j, v + j);
           }
         } else if (P::kSegment == 0 || g == 0) {
           read_accumulators(ok, d, v);
@@ -267,7 +283,7 @@ __device__ __forceinline__ void core(const P &p) {
       }
       if constexpr (kHold == kHalf) {
 #pragma unroll
-        for (int c = 0; c < kHalf; c += 16) p.store(t, *shared, row, half * kHalf + c, v + c);
+        for (int c = 0; c < kHalf; c += P::kChunk) p.store(t, *shared, row, half * kHalf + c, v + c);
       }
     }
     if (!ok) *gave_up = 1;

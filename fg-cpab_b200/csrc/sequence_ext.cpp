@@ -4,80 +4,9 @@
 // reason torch_ext.cpp gives: a step's host time.  The Python twins
 // (cpab/pytorch/recurrence.py, cpab/pytorch/norm.py, cpab/_native.py) issue the
 // same C ABI calls with the same arguments.
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/extension.h>
-
-#include <optional>
-#include <tuple>
-#include <vector>
-
-#include "cpab_b200.h"
+#include "ext_common.h"
 
 namespace {
-
-using torch::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-// An argument that may be None; the code below it takes an undefined tensor.
-using MaybeTensor = std::optional<Tensor>;
-Tensor given(const MaybeTensor &t) { return t.has_value() ? *t : Tensor(); }
-
-void check(int status) {
-  TORCH_CHECK(status == 0, "libcpab_b200: ", cpab_b200_last_error());
-}
-
-cpab_stream_t stream_of(const Tensor &t) {
-  return reinterpret_cast<cpab_stream_t>(at::cuda::getCurrentCUDAStream(t.device().index()).stream());
-}
-
-const void *ptr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-void *ptr_mut(const Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
-const float *fptr(const Tensor &t) { return static_cast<const float *>(ptr(t)); }
-float *fptr_mut(const Tensor &t) { return static_cast<float *>(ptr_mut(t)); }
-
-int dtype_of(const Tensor &t, const char *name) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return CPAB_F32;
-    case at::kHalf: return CPAB_F16;
-    case at::kBFloat16: return CPAB_BF16;
-    default: TORCH_CHECK_TYPE(false, name, " must be float32, float16 or bfloat16, got ", t.scalar_type());
-  }
-}
-
-void require(const Tensor &t, const Tensor &like, at::ScalarType dtype, at::IntArrayRef shape, const char *name) {
-  TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device(), ", x on ", like.device());
-  TORCH_CHECK_TYPE(t.scalar_type() == dtype, name, " must be ", dtype, ", got ", t.scalar_type());
-  TORCH_CHECK_VALUE(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
-}
-
-// Counts a write through a raw pointer as torch's own operations count theirs, so
-// that a backward through the old value raises (an inference tensor has no count).
-void written(const Tensor &t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
-// No gradient of these gradients: refuse instead of treating them as constants.
-void once(const char *name) {
-  TORCH_CHECK(!at::GradMode::is_enabled(), name, " can be differentiated once only (create_graph=True)");
-}
-
-// Whether a forward-mode derivative flows into one of ts.
-bool has_tangent(std::initializer_list<const Tensor *> ts) {
-  for (const Tensor *t : ts)
-    if (t->defined() && t->_fw_grad(/*level=*/0).defined()) return true;
-  return false;
-}
-
-// Whether the call has to go through its node, which refuses forward mode.
-bool needs_grad(std::initializer_list<const Tensor *> ts) {
-  if (has_tangent(ts)) return true;
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor *t : ts)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
-}
 
 // ---- gated_scan --------------------------------------------------------------
 
@@ -90,8 +19,6 @@ struct ScanInput {
   const void *xp, *gp;
   int64_t xb, xt, gb, gt;
 };
-
-Tensor channels_adjacent(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 
 ScanInput scan_input(const Tensor &x, const Tensor &gate) {
   ScanInput s;
@@ -231,12 +158,6 @@ Tensor gated_scan_step(const Tensor &x, const MaybeTensor &gate_, const Tensor &
 
 // ---- rms_norm ------------------------------------------------------------------
 
-// t [..., D] as rows of adjacent columns.
-Tensor rows_of(const Tensor &t) {
-  const Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / t.size(-1), t.size(-1)});
-  return channels_adjacent(r);
-}
-
 void check_norm(const Tensor &x, const Tensor &weight, const Tensor &residual) {
   TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor (no CPU path)");
   dtype_of(x, "x");
@@ -346,15 +267,6 @@ std::vector<Tensor> rms_norm_quantized(const Tensor &x, const Tensor &weight, co
 
 // ---- adamw ---------------------------------------------------------------------
 
-// Element i of a Python list of tensors (null where it is None and `maybe`),
-// read in place: a step's lists hold every tensor of a network.
-const Tensor *item(const pybind11::list &list, size_t i, const char *name, bool maybe = false) {
-  PyObject *o = PyList_GET_ITEM(list.ptr(), (Py_ssize_t)i);
-  if (maybe && o == Py_None) return nullptr;
-  TORCH_CHECK_TYPE(THPVariable_Check(o), "adamw: ", name, " ", i, " is no tensor");
-  return &THPVariable_Unpack(o);
-}
-
 // counts[g] tensors of group g one after another in the lists; hyper holds a
 // group's (lr, beta1, beta2, eps, weight_decay); lr_tensors a group's learning
 // rate on the device (None: hyper's).  scales is empty where every state has
@@ -368,7 +280,7 @@ void adamw(const pybind11::list &params, const pybind11::list &grads, const pybi
                         (scales.empty() || scales.size() == n),
                     "adamw: lists of different lengths");
   if (n == 0) return;
-  const at::Device device = item(params, 0, "parameter")->device();
+  const at::Device device = item(params, 0, "adamw: parameter")->device();
   TORCH_CHECK(device.is_cuda(), "params must be CUDA tensors (no CPU path)");
   for (const MaybeTensor &lr : lr_tensors)
     TORCH_CHECK(!lr.has_value() || (lr->device() == device && lr->scalar_type() == at::kFloat && lr->numel() == 1),
@@ -379,9 +291,9 @@ void adamw(const pybind11::list &params, const pybind11::list &grads, const pybi
   size_t k = 0;
   for (size_t g = 0; g < counts.size(); ++g) {
     for (int64_t i = 0; i < counts[g]; ++i, ++k) {
-      const Tensor &p = *item(params, k, "parameter"), &m = *item(exp_avgs, k, "first moment");
-      const Tensor &v = *item(exp_avg_sqs, k, "second moment"), &step = *item(steps, k, "step");
-      const Tensor *grad = item(grads, k, "gradient");
+      const Tensor &p = *item(params, k, "adamw: parameter"), &m = *item(exp_avgs, k, "adamw: first moment");
+      const Tensor &v = *item(exp_avg_sqs, k, "adamw: second moment"), &step = *item(steps, k, "adamw: step");
+      const Tensor *grad = item(grads, k, "adamw: gradient");
       const bool eight = m.scalar_type() == at::kFloat8_e4m3fn;
       TORCH_CHECK(p.device() == device && grad->device() == device && m.device() == device &&
                       v.device() == device && step.device() == device,
@@ -407,7 +319,7 @@ void adamw(const pybind11::list &params, const pybind11::list &grads, const pybi
       float *sc = nullptr;
       if (eight) {
         const int64_t blocks = (p.numel() + 255) / 256;
-        const Tensor *t = scales.empty() ? nullptr : item(scales, k, "scales", true);
+        const Tensor *t = scales.empty() ? nullptr : item(scales, k, "adamw: scales", true);
         TORCH_CHECK_VALUE(t != nullptr && t->device() == device && t->scalar_type() == at::kFloat &&
                               t->is_contiguous() && t->numel() == 2 * blocks,
                           "adamw: tensor ", k, ": 8-bit states need float32 scales [", blocks, ", 2]");
@@ -425,7 +337,7 @@ void adamw(const pybind11::list &params, const pybind11::list &grads, const pybi
     }
   }
   check(cpab_b200_adamw(list.data(), (int)n, (uint32_t)seed, static_cast<int32_t *>(ptr_mut(workspace)),
-                        stream_of(*item(params, 0, "parameter"))));
+                        stream_of(*item(params, 0, "adamw: parameter"))));
 }
 
 }  // namespace

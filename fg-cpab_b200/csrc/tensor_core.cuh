@@ -62,6 +62,18 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   return false;
 }
 
+// The same for a whole warp, with one answer.
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(~0u, bar_wait(bar, parity)); }
+
+// One lane of a whole warp.  (Copies and matrix instructions take their operands from
+// the warp's uniform registers: warps that issue them run their loops whole and elect
+// a lane for the issue alone.  With loops of lane 0 a matrix instruction took twice
+// its time: 8192 x 8192 x 8192 codes 482 us.)
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -214,6 +226,22 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
                  ::"r"(bar), "h"((uint16_t)3) : "memory");
   else
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// A launch in clusters of `cluster` blocks that may begin while the stream's last
+// kernel ends (a kernel so launched calls dep_wait before it touches memory).
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), dim3 grid, unsigned block, size_t shared, unsigned cluster, cudaStream_t s,
+                   const A &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid, cfg.blockDim = dim3(block), cfg.dynamicSmemBytes = shared, cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 }  // namespace tc

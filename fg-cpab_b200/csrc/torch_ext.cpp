@@ -305,10 +305,12 @@ Tensor transform(Tensor points, Tensor theta, std::vector<Tensor> basis, int64_t
 
 // The sequence-network operators (sequence_ext.cpp).
 void bind_sequence(pybind11::module &m);
+void bind_projection(pybind11::module &m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "autograd nodes over libcpab_b200 (C++)";
   bind_sequence(m);
+  bind_projection(m);
   m.def("transform", &transform,
         "points, theta, basis (6 CSR tensors of B and B^T), d, dense, nc, nstepsolver, "
         "adaptive, order or None, compute_points_grad, batched -> transformed points");
