@@ -3,10 +3,13 @@ of its own length and predicts the theta of the CPAB warp that aligns it with
 the template; then follow one signal sample by sample.
 
     python examples/align_series.py [--steps 300] [--length 512] [--state-bits 8]
+                                    [--projection-bits 8] [--muon]
 
 Every sequence operator of the package works here as in use: rms_norm and
-gated_scan (with ragged lengths) in the network and its gradient, AdamW with
-32- or 8-bit states, gated_scan_step and rms_norm_quantized in the stream.
+gated_scan (with ragged lengths) in the network and its gradient, with its
+projections' products in 8 bits if asked for; AdamW with 32- or 8-bit states,
+or Muon for the blocks' matrices beside it; gated_scan_step,
+rms_norm_quantized and matmul_quantized in the stream.
 """
 import argparse
 import os
@@ -17,7 +20,7 @@ sys.path.insert(0, os.path.join(ROOT, "fg-cpab_b200"))
 
 import torch  # noqa: E402
 
-from cpab.optim import AdamW  # noqa: E402
+from cpab.optim import AdamW, Muon  # noqa: E402
 from cpab.pytorch.localizer import SeriesLocalizer  # noqa: E402
 from cpab.pytorch.warp import CpabWarp  # noqa: E402
 
@@ -42,13 +45,17 @@ def with_time(x):
 
 
 def train(steps=300, length=512, size=32, state_bits=32, width=128, depth=2, lr=8e-3, seed=0,
-          device="cuda", report=50, tess=8):
+          device="cuda", report=50, tess=8, projection_bits=16, muon=False):
     """Returns (network, warp, losses)."""
     torch.manual_seed(seed)
     g = torch.Generator(device=device).manual_seed(seed)
     warp = CpabWarp([tess], padding_mode="border").to(device)
-    net = SeriesLocalizer(2, warp.theta_dim, width, depth).to(device)
-    opt = AdamW(net.parameters(), lr=lr, betas=(0.9, 0.98), weight_decay=0.01, state_bits=state_bits)
+    net = SeriesLocalizer(2, warp.theta_dim, width, depth, projection_bits=projection_bits).to(device)
+    matrices = [p for p in net.blocks.parameters() if p.dim() == 2] if muon else []
+    opts = [AdamW([p for p in net.parameters() if not any(p is q for q in matrices)], lr=lr,
+                  betas=(0.9, 0.98), weight_decay=0.01, state_bits=state_bits)]
+    if muon:
+        opts.append(Muon(matrices, lr=lr, weight_decay=0.01, adjust_lr_fn="match_rms_adamw"))
     base = template(length, device)
     losses = []
     for step in range(steps):
@@ -60,9 +67,10 @@ def train(steps=300, length=512, size=32, state_bits=32, width=128, depth=2, lr=
         aligned = warp(x, theta)
         seen = torch.arange(length, device=device)[None, None] < lengths[:, None, None]
         loss = ((aligned - base).square() * seen).sum() / seen.sum()
-        opt.zero_grad()
+        net.zero_grad()
         loss.backward()
-        opt.step()
+        for opt in opts:
+            opt.step()
         losses.append(loss.detach())
         if report and (step + 1) % report == 0:
             print("step %d: loss %.5f" % (step + 1, torch.stack(losses[-report:]).mean().item()))
@@ -81,8 +89,11 @@ def main():
     ap.add_argument("--steps", type=int, default=300)
     ap.add_argument("--length", type=int, default=512)
     ap.add_argument("--state-bits", type=int, default=32, choices=(8, 32))
+    ap.add_argument("--projection-bits", type=int, default=16, choices=(8, 16))
+    ap.add_argument("--muon", action="store_true")
     a = ap.parse_args()
-    net, warp, losses = train(a.steps, a.length, state_bits=a.state_bits)
+    net, warp, losses = train(a.steps, a.length, state_bits=a.state_bits,
+                              projection_bits=a.projection_bits, muon=a.muon)
     print("loss: %.5f (first 20 steps), %.5f (last 20)" % (sum(losses[:20]) / 20, sum(losses[-20:]) / 20))
     x, theta = batch(warp, template(a.length, "cuda"), 1, 0.02, torch.Generator("cuda").manual_seed(7))
     x = with_time(x)

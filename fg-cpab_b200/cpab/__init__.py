@@ -8,8 +8,9 @@ the compute path is libcpab_b200.so (hand-written CUDA for B200).
 
 Networks that predict theta from long signals: ``cpab.pytorch.recurrence``
 (gated_scan, gated_scan_step), ``cpab.pytorch.norm`` (rms_norm,
-rms_norm_quantized), ``cpab.optim`` (AdamW, adamw_), and, made of them,
-``cpab.pytorch.localizer.SeriesLocalizer``.
+rms_norm_quantized), ``cpab.pytorch.projection`` (linear_quantized,
+quantize_blocks, matmul_quantized), ``cpab.optim`` (AdamW, adamw_, Muon, muon_,
+orthogonalize), and, made of them, ``cpab.pytorch.localizer.SeriesLocalizer``.
 """
 from .cpab import Cpab
 

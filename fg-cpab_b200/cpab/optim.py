@@ -1,13 +1,22 @@
 """AdamW over all tensors of a network, one kernel launch for those of one type
-and state kind (256 at most), its states in 32 or 8 bits.
+and state kind (256 at most), its states in 32 or 8 bits; and Muon, whose steps
+move matrices along orthogonalised momenta.
 
+AdamW:
     m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2
     p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 
 in float32 whatever the parameters' type.  8-bit states are e4m3 codes of m
 and of sqrt(v) with one float32 scale per 256 elements, rounded
 stochastically (their averages move by less than a code's spacing per step,
-so rounding to nearest would stop them).  No counterpart in the reference.
+so rounding to nearest would stop them).
+
+Muon (matrices only):
+    m = momentum m + (1 - momentum) g,   u = (1 - momentum) g + momentum m  (nesterov)
+    p = p (1 - lr wd) - lr r O(u)
+
+where O moves all singular values of u towards 1 (orthogonalize).  No
+counterpart in the reference.
 """
 import functools
 
@@ -249,8 +258,89 @@ def muon_(params, grads, momenta, *, lr, momentum=0.95, nesterov=True, weight_de
     if adjust_lr not in _ADJUST:
         raise ValueError("adjust_lr must be 'original' or 'match_rms_adamw', got %r" % (adjust_lr,))
     on_device = torch.is_tensor(lr)
+    if on_device and (not lr.is_cuda or lr.dtype != torch.float32 or lr.numel() != 1):
+        raise ValueError("lr must be a number or one float32 element on the device")
     ext = _ext.module()
     fn = _native.muon if ext is None else functools.partial(_ext.call, ext.muon)
     fn(list(params), list(grads), list(momenta), 0.0 if on_device else float(lr), lr if on_device else None,
        float(momentum), bool(nesterov), float(weight_decay), int(steps), _triple(coefficients), float(eps),
        _ADJUST[adjust_lr])
+
+
+class Muon(torch.optim.Optimizer):
+    """Options, state name (momentum_buffer) and state dicts of torch.optim.Muon,
+    with the step of muon_: matrices only (take AdamW for vectors), momenta
+    float32 whatever the parameters' type.  adjust_lr_fn: None or "original",
+    or "match_rms_adamw", with which lr and weight_decay of AdamW can be kept.
+    step() can be captured in a CUDA graph once the parameters have states, that
+    is after one step; lr may then be a float32 tensor on the device."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
+                 ns_coefficients=COEFFICIENTS, eps=1e-7, ns_steps=5, adjust_lr_fn=None):
+        if not torch.is_tensor(lr) and not lr >= 0:
+            raise ValueError("lr must not be negative, got %r" % (lr,))
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("momentum must be in [0, 1), got %r" % (momentum,))
+        if not weight_decay >= 0 or not eps >= 0:
+            raise ValueError("eps and weight_decay must not be negative")
+        if not 1 <= int(ns_steps) <= 64:
+            raise ValueError("ns_steps must be 1 to 64, got %r" % (ns_steps,))
+        if adjust_lr_fn not in (None, *_ADJUST):
+            raise ValueError("adjust_lr_fn must be 'original' or 'match_rms_adamw', got %r" % (adjust_lr_fn,))
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                                      ns_coefficients=_triple(ns_coefficients), eps=eps, ns_steps=int(ns_steps),
+                                      adjust_lr_fn=adjust_lr_fn))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                self.param_groups.pop()
+                raise ValueError("Muon takes matrices only, got a parameter of shape %s" % (tuple(p.shape),))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step over every parameter that has a gradient."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            lists = {}
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if g.is_sparse:
+                    raise RuntimeError("Muon does not take sparse gradients")
+                state = self.state[p]
+                if not state:
+                    if _capturing():
+                        raise RuntimeError("Muon: a parameter without a state in a captured step: every replay "
+                                           "would begin anew; take one step, or load states, before the capture")
+                    state["momentum_buffer"] = torch.zeros(p.shape, device=p.device, dtype=torch.float32)
+                to = lists.setdefault(p.device, ([], [], []))
+                to[0].append(p)
+                to[1].append(g)
+                to[2].append(state["momentum_buffer"])
+            for device, to in lists.items():
+                lr = group["lr"]
+                if torch.is_tensor(lr) and lr.is_cuda and lr.device != device:
+                    lr = lr.to(device, non_blocking=True)
+                muon_(*to, lr=lr, momentum=group["momentum"], nesterov=group["nesterov"],
+                      weight_decay=group["weight_decay"], steps=group["ns_steps"],
+                      coefficients=group["ns_coefficients"], eps=group["eps"],
+                      adjust_lr=group["adjust_lr_fn"] or "original")
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch's, which casts states to their parameter's type: momenta
+        are put back to float32."""
+        super().load_state_dict(state_dict)
+        params = [p for g in self.param_groups for p in g["params"]]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, params):
+            saved = state_dict["state"].get(i)
+            if saved:
+                self.state[p]["momentum_buffer"] = saved["momentum_buffer"].detach().to(
+                    p.device, torch.float32, copy=True).contiguous()

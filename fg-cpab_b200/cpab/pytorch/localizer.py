@@ -16,6 +16,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .norm import rms_norm, rms_norm_quantized
+from .projection import linear_quantized, matmul_quantized
 from .recurrence import gated_scan, gated_scan_step
 
 
@@ -33,12 +34,16 @@ class RecurrentBlock(nn.Module):
 
 class SeriesLocalizer(nn.Module):
     """SeriesLocalizer(channels, theta_dim, width, depth)(series, lengths) ->
-    theta; theta starts at 0 (the identity warp)."""
+    theta; theta starts at 0 (the identity warp).  projection_bits=8: the blocks'
+    projections and their gradients are 8-bit products (linear_quantized)."""
 
-    def __init__(self, channels, theta_dim, width=128, depth=2, eps=1e-6):
+    def __init__(self, channels, theta_dim, width=128, depth=2, eps=1e-6, projection_bits=16):
         super().__init__()
         if depth < 1 or width < 1:
             raise ValueError("width and depth must be at least 1")
+        if projection_bits not in (8, 16):
+            raise ValueError("projection_bits must be 8 or 16, got %r" % (projection_bits,))
+        self.projection_bits = projection_bits
         self.channels, self.theta_dim, self.width, self.eps = channels, theta_dim, width, eps
         self.embed = nn.Linear(channels, width)
         self.blocks = nn.ModuleList(RecurrentBlock(width) for _ in range(depth))
@@ -66,13 +71,18 @@ class SeriesLocalizer(nn.Module):
                 y = rms_norm(s, block.norm, eps=self.eps)
             else:
                 y, s = rms_norm(update, block.norm, residual=s, eps=self.eps)
-            h, _ = gated_scan(block.in_proj(y), lengths=lengths)
-            update = block.out_proj(h)
+            h, _ = gated_scan(self._project(block.in_proj, y), lengths=lengths)
+            update = self._project(block.out_proj, h)
         if lengths is None:
             return self._theta(update[:, -1], s[:, -1])
         at = (lengths.long().clamp(1, series.shape[2]) - 1)[:, None, None].expand(-1, 1, self.width)
         theta = self._theta(update.gather(1, at)[:, 0], s.gather(1, at)[:, 0])
         return theta * (lengths > 0)[:, None]
+
+    def _project(self, proj, x):
+        if self.projection_bits == 8:
+            return linear_quantized(x, proj.weight, proj.bias)
+        return proj(x)
 
     def _theta(self, update, s):
         y, _ = rms_norm(update.contiguous(), self.norm, residual=s.contiguous(), eps=self.eps)
@@ -101,8 +111,8 @@ class SeriesLocalizer(nn.Module):
         new_states, updated in place, slots [B] the streams' rows of it (None:
         row b; -1: no sample now, whose theta means nothing).  Returns theta
         [B, theta_dim] of the streams so far.  quantized: norms and input
-        projections in 8 bits (see quantize), whose products torch gives in
-        16 bits only."""
+        projections in 8 bits (see quantize), whose products are rounded to
+        16 bits."""
         s = self.embed(samples)
         update = None
         for k, block in enumerate(self.blocks):
@@ -111,8 +121,7 @@ class SeriesLocalizer(nn.Module):
                                          residual=None if update is None else s, eps=self.eps)
                 if update is not None:
                     s = out[2]
-                z = torch._scaled_mm(out[0], block.in_proj_q.t(), scale_a=out[1][:, None],
-                                     scale_b=block.in_proj_scale[None], out_dtype=torch.bfloat16)
+                z = matmul_quantized(out[0], out[1], block.in_proj_q, block.in_proj_scale)
                 z = z.to(s.dtype) + block.in_proj.bias
             else:
                 if update is None:

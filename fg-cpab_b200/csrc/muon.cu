@@ -10,16 +10,20 @@
 // stored twice.  A matrix is kept as 2^10 times its values in two halves, a value
 // rounded to a half and its remainder (22 bits together):
 //
-//   - parameters and matrices of 16 bits are multiplied by their first halves (11
-//     bits, 2^-12 off); the remainder enters the terms a X and b A, which would
+//   - parameters and matrices of 16 bits, of more than 256 rows, are multiplied by
+//     their first halves (11 bits, 2^-12 off); the remainder enters the terms a X and b A, which would
 //     otherwise drown small singular values beside large ones.  The result is
-//     1.5e-3 to 2.7e-3 off (relative 2-norm, normal matrices of 64 to 1500 rows),
+//     1.5e-3 to 2.7e-3 off (relative 2-norm, normal matrices of up to 1500 rows),
 //     about a rounding to bfloat16 (1.7e-3).
-//   - float32 ones take three products, first x first + first x remainder +
+//   - float32 ones and small ones take three products, first x first + first x remainder +
 //     remainder x first (4e-7 to 3e-6 off): a float32 parameter keeps that many
 //     bits of its update.
 //
-// 2^10 keeps values from 6e-8 in a half's normal range and leaves room to 64.
+// 2^10 keeps values from 6e-8 in a half's normal range and leaves room to 64.  Where
+// eps is not small beside |G|_F, X is: it is kept as theta Y with theta a power of two
+// and |Y|_F in (1/2, 1], and the steps are taken in Y with
+//   Y <- r (a + theta^2 b Y Y^T + theta^4 c (Y Y^T)^2) Y,   r = theta / theta',
+// theta' = min(1, 2^ceil(log2 a) theta), until theta is 1.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -34,6 +38,10 @@ constexpr float kUnit = 1024.f;       // stored = value * kUnit
 constexpr int kPartials = 256;        // partial sums of squares of a matrix
 constexpr int kGroups = 8;            // shapes in a launch
 constexpr int kPrepared = 64;         // matrices in a launch that reads them
+// Matrices of so few rows take pairs of halves whatever their type: their launches are
+// bound by latency, and a few singular values do not average the errors of halves (a
+// single one was 5e-3 off).
+constexpr int kFewRows = 256;
 constexpr int kMatrices = 128;        // parameters in a sequence of launches
 
 __device__ __forceinline__ float read_as(const void *p, int dtype, int64_t i) {
@@ -54,6 +62,7 @@ struct Prepared {
   float *momentum;    // float32, updated; null: the matrix itself is taken
   __half *hi, *lo;    // [m, pitch]
   double *partials;   // [kPartials]
+  float *terms;       // [kTerms]
   int64_t pitch;
   int rows, cols;
   int dtype;
@@ -62,9 +71,28 @@ struct Prepared {
 struct PrepareArgs {
   Prepared m[kPrepared];
   float momentum;
-  int nesterov;
-  double eps;
+  int nesterov, steps;
+  double eps, a, b, c;
 };
+
+// Each step's coefficients for Y, three floats, and the last theta behind them.
+constexpr int kMostSteps = 64;
+constexpr int kTerms = 3 * kMostSteps + 1;
+
+__device__ __forceinline__ double first_theta(double norm, double eps) {
+  const double x = norm / (norm + eps);
+  if (!(x > 0.0) || x >= 0.5) return 1.0;  // (of zeros, and of NaN, 1)
+  return exp2(ceil(log2(x)));
+}
+__device__ __forceinline__ void write_terms(float *to, double theta, double a, double b, double c, int steps) {
+  const double growth = exp2(ceil(log2(fmax(1.0, fabs(a)))));
+  for (int k = 0; k < steps; ++k) {
+    const double next = fmin(1.0, growth * theta), r = theta / next, q = theta * theta;
+    to[3 * k] = (float)(a * r), to[3 * k + 1] = (float)(b * q * r), to[3 * k + 2] = (float)(c * q * q * r);
+    theta = next;
+  }
+  to[3 * kMostSteps] = (float)theta;
+}
 
 // The direction: m = momentum m + (1 - momentum) g, and with nesterov
 // (1 - momentum) g + momentum m of the new m.
@@ -126,7 +154,8 @@ __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ Prepa
   __syncthreads();
   sum = 0;
   for (int i = 0; i < 8; ++i) sum += part[i];
-  const double scale = (double)kUnit / (sqrt(sum) + a.eps);
+  const double norm = sqrt(sum), theta = first_theta(norm, a.eps), scale = (double)kUnit / ((norm + a.eps) * theta);
+  if (blockIdx.x == 0 && threadIdx.x == 0) write_terms(p.terms, theta, a.a, a.b, a.c, a.steps);
   for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
     const int r0 = t / tiles_x * 64, c0 = t % tiles_x * 64, x = threadIdx.x & 63;
     for (int y = threadIdx.x >> 6; y < 64; y += 4) {
@@ -159,6 +188,7 @@ struct PhaseGroup {
   int steps;                       // stages of 64 summed
   int tiles_m, tiles_n, end;       // tiles of one matrix; end of the group's in the launch
   int write_lo;
+  const float *terms;              // of the set's first matrix, kTerms apart
 };
 struct FinalGroup {
   void *out;                       // of matrix z: out + z * stride elements, or table[first + z]
@@ -173,16 +203,14 @@ struct FinalGroup {
 template <bool FINAL>
 struct PhaseArgs {
   PhaseGroup g[kGroups];
-  int groups;
-  float a, b, c;
+  int groups, step;
 };
 template <>
 struct PhaseArgs<true> {
   PhaseGroup g[kGroups];
   FinalGroup f[kGroups];
   void *table[kMatrices];
-  int groups;
-  float a, b, c;
+  int groups, step;
 };
 
 template <int PHASE, int PARTS, int CTAS, int BN>
@@ -251,7 +279,8 @@ struct Schulz {
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = acc[j] * (1.f / kUnit);
     if constexpr (PHASE != kGram) {
-      const float mine = PHASE == kSquare ? p.b : p.a, product = PHASE == kSquare ? p.c : 1.f;
+      const float *terms = q.terms + t.z * kTerms + 3 * p.step;
+      const float mine = terms[PHASE == kSquare ? 1 : 0], product = PHASE == kSquare ? terms[2] : 1.f;
       const int64_t at = t.z * q.read_plane + row * q.read_pitch + col;
       const __half *hi = q.read[0] + at, *lo = q.read[1] + at;
       if (whole) {
@@ -313,7 +342,8 @@ struct Schulz {
       const int e = f.dtype == CPAB_F32 ? 4 : 2;
       void *out = f.first >= 0 ? p.table[f.first + t.z] : static_cast<char *>(f.out) + t.z * f.stride * e;
       const float lr = f.lr_device != nullptr ? *f.lr_device : f.lr;
-      const float keep = f.update ? 1.f - lr * f.decay : 0.f, move = (f.update ? -lr * f.rate : 1.f) * (1.f / kUnit);
+      const float last = q.terms[t.z * kTerms + 3 * kMostSteps] * (1.f / kUnit);
+      const float keep = f.update ? 1.f - lr * f.decay : 0.f, move = (f.update ? -lr * f.rate : 1.f) * last;
       if (f.wide && col + 16 <= q.n) {
         const int64_t i = (int64_t)row * q.n + col;
         if (f.dtype == CPAB_F32) whole<float>(static_cast<float *>(out) + i, f.update, keep, move, v);
@@ -391,7 +421,7 @@ struct Set {
   int m() const { return std::min(rows, cols); }
   int n() const { return std::max(rows, cols); }
   bool turned() const { return rows > cols; }
-  int parts() const { return dtype == CPAB_F32 ? 2 : 1; }
+  int parts() const { return dtype == CPAB_F32 || m() <= kFewRows ? 2 : 1; }
   // (rows begin on 32 bytes: whole sectors are moved)
   int64_t x_pitch() const { return (n() + 15) / 16 * 16; }
   int64_t a_pitch() const { return (m() + 15) / 16 * 16; }
@@ -402,6 +432,7 @@ int64_t round_up(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Places {
   __half *x[2][2], *a[2], *b[2];  // [buffer][half]
+  float *terms;
 };
 // Bytes of the sets' workspace; with `base`, the places too.
 int64_t place(const std::vector<Set> &sets, int64_t matrices, char *base, std::vector<Places> *places, double **partials) {
@@ -416,6 +447,8 @@ int64_t place(const std::vector<Set> &sets, int64_t matrices, char *base, std::v
   if (partials != nullptr) *partials = reinterpret_cast<double *>(d);
   for (size_t i = 0; i < sets.size(); ++i) {
     const Set &s = sets[i];
+    float *terms = reinterpret_cast<float *>(take((int64_t)s.batch * kTerms * (int64_t)sizeof(float)));
+    if (places != nullptr) (*places)[i].terms = terms;
     for (int k = 0; k < 8; ++k) {
       __half *p = reinterpret_cast<__half *>(take(2 * (k < 4 ? s.x_halves() : s.a_halves())));
       if (places == nullptr) continue;
@@ -446,17 +479,17 @@ cudaError_t launch_phase(PhaseArgs<PHASE == kFinal> &a, const int *batch, cudaSt
 // The products of at most kGroups sets, all of one kind.
 template <int PARTS>
 cudaError_t schulz_as(const std::vector<Set> &sets, const std::vector<Places> &places, const FinalGroup *finals,
-                   void *const *table, int table_size, int steps, const float *coefficients, cudaStream_t s) {
+                      void *const *table, int table_size, int steps, cudaStream_t s) {
   int batch[kGroups];
   PhaseArgs<false> a;
   PhaseArgs<true> last;
   const int groups = (int)sets.size();
   a.groups = last.groups = groups;
-  a.a = last.a = coefficients[0], a.b = last.b = coefficients[1], a.c = last.c = coefficients[2];
   for (int i = 0; i < table_size; ++i) last.table[i] = table[i];
   for (int g = 0; g < groups; ++g) last.f[g] = finals[g], batch[g] = sets[g].batch;
   for (int step = 0; step < steps; ++step) {
     const int now = step & 1;
+    a.step = last.step = step;
     bool ok = true;
     cudaError_t e;
     for (int g = 0; g < groups; ++g) {
@@ -468,6 +501,7 @@ cudaError_t schulz_as(const std::vector<Set> &sets, const std::vector<Places> &p
         q.b[h] = q.a[h];
         q.read[h] = nullptr, q.write[h] = w.a[h];
       }
+      q.terms = w.terms;
       q.write_pitch = t.a_pitch(), q.write_plane = t.m() * t.a_pitch();
       q.m = q.n = t.m(), q.steps = (t.n() + 63) / 64, q.write_lo = 1;
     }
@@ -512,13 +546,14 @@ cudaError_t schulz_as(const std::vector<Set> &sets, const std::vector<Places> &p
 }
 
 cudaError_t schulz(const std::vector<Set> &sets, const std::vector<Places> &places, const FinalGroup *finals,
-                   void *const *table, int table_size, int steps, const float *coefficients, cudaStream_t s) {
-  return sets[0].parts() == 2 ? schulz_as<2>(sets, places, finals, table, table_size, steps, coefficients, s)
-                              : schulz_as<1>(sets, places, finals, table, table_size, steps, coefficients, s);
+                   void *const *table, int table_size, int steps, cudaStream_t s) {
+  return sets[0].parts() == 2 ? schulz_as<2>(sets, places, finals, table, table_size, steps, s)
+                              : schulz_as<1>(sets, places, finals, table, table_size, steps, s);
 }
 
 // Launches what reads the matrices in.
-cudaError_t prepare(const std::vector<Prepared> &list, float momentum, int nesterov, double eps, cudaStream_t s) {
+cudaError_t prepare(const std::vector<Prepared> &list, float momentum, int nesterov, int steps, const double *c,
+                    double eps, cudaStream_t s) {
   for (size_t first = 0; first < list.size(); first += kPrepared) {
     const int n = (int)std::min<size_t>(kPrepared, list.size() - first);
     PrepareArgs a;
@@ -528,7 +563,7 @@ cudaError_t prepare(const std::vector<Prepared> &list, float momentum, int neste
       most = std::max(most, (int64_t)a.m[i].rows * a.m[i].cols);
       tiles = std::max(tiles, (int64_t)((a.m[i].rows + 63) / 64) * ((a.m[i].cols + 63) / 64));
     }
-    a.momentum = momentum, a.nesterov = nesterov, a.eps = eps;
+    a.momentum = momentum, a.nesterov = nesterov, a.steps = steps, a.eps = eps, a.a = c[0], a.b = c[1], a.c = c[2];
     const int partials = (int)std::min<int64_t>(kPartials, (most + 2047) / 2048);
     cudaError_t e = tc::launch(k_direction, dim3(partials, n), 256, 0, 1, s, a);
     if (e == cudaSuccess)
@@ -541,7 +576,7 @@ cudaError_t prepare(const std::vector<Prepared> &list, float momentum, int neste
 constexpr int64_t kMostRows = 1 << 20;
 
 const char *check_steps(int steps, const double *c, double eps) {
-  if (steps < 1 || steps > 64) return "steps must be 1 to 64";
+  if (steps < 1 || steps > kMostSteps) return "steps must be 1 to 64";
   if (!(eps >= 0)) return "eps must not be negative";
   // Where the singular values of X can be after each step, and the magnitudes of what is stored.
   double most = 1;
@@ -549,12 +584,13 @@ const char *check_steps(int steps, const double *c, double eps) {
     double next = 0;
     for (int i = 0; i <= 1000; ++i) {
       const double x = most * i / 1000, q = x * x, b = c[1] * q + c[2] * q * q;
-      if (!(std::fabs(b) < 60) || !(q < 60)) return "coefficients let values outgrow their range of 60";
-      next = std::max(next, std::fabs(c[0] * x + b * x));
+      const double value = std::fabs(c[0] * x + b * x);
+      if (!(std::fabs(c[0]) < 60) || !(std::fabs(b) < 60) || !(q < 60) || !(value < 60))
+        return "coefficients let values outgrow their range of 60";
+      next = std::max(next, value);
     }
     most = next;
   }
-  if (!(most < 60)) return "coefficients let values outgrow their range of 60";
   return nullptr;
 }
 
@@ -592,14 +628,13 @@ extern "C" int cpab_b200_orthogonalize(int dtype, const void *x, int64_t batch, 
   for (int64_t z = 0; z < batch; ++z) {
     const int64_t at = z * t.m() * t.x_pitch();
     list[z] = {static_cast<const char *>(x) + z * rows * columns * dtype_size(dtype), nullptr, places[0].x[0][0] + at,
-               places[0].x[0][1] + at, partials + z * kPartials, t.x_pitch(), (int)rows, (int)columns, dtype, t.turned()};
+               places[0].x[0][1] + at, partials + z * kPartials, places[0].terms + z * kTerms, t.x_pitch(), (int)rows, (int)columns, dtype, t.turned()};
   }
-  cudaError_t e = prepare(list, 0.f, 0, eps, s);
+  cudaError_t e = prepare(list, 0.f, 0, steps, coefficients, eps, s);
   FinalGroup f = {};
   f.out = out, f.stride = rows * columns, f.first = -1, f.dtype = dtype, f.turned = t.turned();
   f.wide = !t.turned() && aligned_to(out, columns, dtype_size(dtype), 32);
-  const float c[3] = {(float)coefficients[0], (float)coefficients[1], (float)coefficients[2]};
-  if (e == cudaSuccess) e = schulz(sets, places, &f, nullptr, 0, steps, c, s);
+  if (e == cudaSuccess) e = schulz(sets, places, &f, nullptr, 0, steps, s);
   return launch_status(e, "orthogonalize");
 }
 
@@ -680,7 +715,6 @@ extern "C" int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double
   if (!list.empty() && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256))
     return report_error(CPAB_ERR_ARG, "%s", "muon: null workspace, or one off 256 bytes");
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const float c[3] = {(float)coefficients[0], (float)coefficients[1], (float)coefficients[2]};
   cudaError_t e = cudaSuccess;
   for (const Sequence &q : list) {
     std::vector<Places> places;
@@ -704,11 +738,11 @@ extern "C" int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double
         if (z == 0) f.wide = !t.turned();
         f.wide = f.wide && aligned_to(m.param, t.cols, dtype_size(t.dtype), 32);
         in.push_back({m.grad, m.momentum, places[g].x[0][0] + at, places[g].x[0][1] + at, partials + k * kPartials,
-                      t.x_pitch(), t.rows, t.cols, t.dtype, t.turned()});
+                      places[g].terms + z * kTerms, t.x_pitch(), t.rows, t.cols, t.dtype, t.turned()});
       }
     }
-    if ((e = prepare(in, (float)momentum, nesterov, eps, s)) != cudaSuccess) break;
-    if ((e = schulz(q.sets, places, finals.data(), table, (int)in.size(), steps, c, s)) != cudaSuccess) break;
+    if ((e = prepare(in, (float)momentum, nesterov, steps, coefficients, eps, s)) != cudaSuccess) break;
+    if ((e = schulz(q.sets, places, finals.data(), table, (int)in.size(), steps, s)) != cudaSuccess) break;
   }
   return launch_status(e, "muon");
 }

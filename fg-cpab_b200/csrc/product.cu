@@ -466,9 +466,8 @@ cudaError_t launch_product(ProductArgs &a, cudaStream_t s) {
   }
 }
 
-// What an operand lacks, or null; fills the map and scales.
-const char *operand(const cpab_quantized &o, int64_t rows, int64_t K, int box_rows, CUtensorMap *map, Scales *blocks,
-                    const float **per_row) {
+// What an operand lacks, or null; fills its scales.
+const char *operand(const cpab_quantized &o, int64_t K, Scales *blocks, const float **per_row) {
   if (o.codes == nullptr || o.scale == nullptr) return "null codes or scales";
   if (reinterpret_cast<uintptr_t>(o.codes) % 16 || o.row % 16 || o.row < K)
     return "codes must begin on 16 bytes, each row on a multiple of 16 that holds it";
@@ -482,7 +481,6 @@ const char *operand(const cpab_quantized &o, int64_t rows, int64_t K, int box_ro
     const bool words = reinterpret_cast<uintptr_t>(o.scale) % 4 == 0 && o.scale_row % 4 == 0;
     *blocks = {static_cast<const uint8_t *>(o.scale), o.scale_row, words};
   }
-  if (!make_tile_map(map, false, o.codes, K, rows, 1, o.row, o.row * rows, box_rows)) return "no tensor map for the codes";
   return nullptr;
 }
 
@@ -553,8 +551,14 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   if (M == 0 || N == 0) return report_error(CPAB_OK, "%s", "");
   if (y == nullptr) return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: null y");
   ProductArgs a = {};
-  const char *why = operand(*x, M, K, 128, &a.a, &a.sa, &a.ra);
-  if (why == nullptr) why = operand(*weight, N, K, tile_of(M, N, (K + kBlock - 1) / kBlock) == 0 ? 64 : 128, &a.b, &a.sb, &a.rb);
+  const char *why = operand(*x, K, &a.sa, &a.ra);
+  if (why == nullptr) why = operand(*weight, K, &a.sb, &a.rb);
+  if (why == nullptr) {
+    const int columns = tile_of(M, N, (K + kBlock - 1) / kBlock) == 0 ? 64 : 128;  // of B a block loads
+    if (!make_tile_map(&a.a, false, x->codes, K, M, 1, x->row, x->row * M, 128) ||
+        !make_tile_map(&a.b, false, weight->codes, K, N, 1, weight->row, weight->row * N, columns))
+      why = "no tensor map for the codes";
+  }
   if (why != nullptr) return report_error(CPAB_ERR_ARG, "matmul_quantized: %s", why);
   a.bias = bias, a.y = y, a.y_row = y_row, a.M = (int)M, a.N = (int)N, a.steps = (int)((K + kBlock - 1) / kBlock);
   a.wide = aligned_to(y, y_row, dtype_size(dtype), 16);

@@ -91,7 +91,6 @@ struct Operand {
 Operand operand(const Tensor &q, const Tensor &scale, const char *name) {
   TORCH_CHECK_TYPE(q.scalar_type() == kCodes, name, " must be float8_e4m3fn, got ", q.scalar_type());
   TORCH_CHECK_VALUE(q.dim() >= 1 && q.size(-1) > 0, name, " must be [..., K] with K > 0, got ", q.sizes());
-  TORCH_CHECK(scale.device() == q.device(), name, "'s scale is on ", scale.device(), ", the codes on ", q.device());
   const bool per_row = scale.scalar_type() == at::kFloat;
   TORCH_CHECK_TYPE(per_row || scale.scalar_type() == kScales, name,
                    "'s scale must be float8_e8m0fnu (for each 128 codes) or float32 (for each row), got ",
@@ -150,6 +149,8 @@ Tensor matmul_quantized(const Tensor &q, const Tensor &scale, const Tensor &weig
                    "dtype must be float32, float16 or bfloat16, got ", type);
   TORCH_CHECK_VALUE(weight.dim() == 2, "weight must be [N, K], got ", weight.sizes());
   TORCH_CHECK(weight.device() == q.device(), "weight is on ", weight.device(), ", q on ", q.device());
+  for (const Tensor *t : {&scale, &weight_scale})
+    TORCH_CHECK(t->device() == q.device(), "a scale is on ", t->device(), ", the codes on ", q.device());
   TORCH_CHECK(!has_tangent({&bias}), "matmul_quantized has no gradient, of forward mode neither");
   const c10::cuda::CUDAGuard guard(q.device());
   const Operand x = operand(q, scale, "q"), w = operand(weight, weight_scale, "weight");
