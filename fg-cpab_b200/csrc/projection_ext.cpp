@@ -281,7 +281,6 @@ void muon(const pybind11::list &params, const pybind11::list &grads, const pybin
   TORCH_CHECK(!lr_device.defined() || (lr_device.device() == device && lr_device.scalar_type() == at::kFloat &&
                                        lr_device.numel() == 1),
               "muon: a learning rate on the device must be one float32 on the parameters' device, ", device);
-  const c10::cuda::CUDAGuard guard(device);
   std::vector<cpab_muon_tensor> list(n);
   std::vector<Tensor> copies;  // contiguous gradients
   for (size_t k = 0; k < n; ++k) {
@@ -303,6 +302,7 @@ void muon(const pybind11::list &params, const pybind11::list &grads, const pybin
     }
     list[k] = {ptr_mut(p), ptr(*grad), fptr_mut(m), p.size(0), p.size(1), dtype_of(p, "a parameter")};
   }
+  const c10::cuda::CUDAGuard guard(device);
   for (size_t k = 0; k < n; ++k)
     for (const Tensor *t : {item(params, k, "muon: parameter"), item(momenta, k, "muon: momentum")}) written(*t);
   const Tensor work = at::empty({cpab_b200_muon_workspace(list.data(), (int)n)}, first.options().dtype(at::kByte));
