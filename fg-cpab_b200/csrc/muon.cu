@@ -67,6 +67,7 @@ struct Prepared {
   int rows, cols;
   int dtype;
   int turned;         // hi and lo are [cols, rows]
+  int vectors;        // grad and momentum begin on 16 bytes
 };
 struct PrepareArgs {
   Prepared m[kPrepared];
@@ -94,10 +95,25 @@ __device__ __forceinline__ void write_terms(float *to, double theta, double a, d
   to[3 * kMostSteps] = (float)theta;
 }
 
-// The direction: m = momentum m + (1 - momentum) g, and with nesterov
-// (1 - momentum) g + momentum m of the new m.
-__device__ __forceinline__ float direction(const Prepared &p, const PrepareArgs &a, int64_t i, float m) {
-  return a.nesterov ? (1.f - a.momentum) * read_as(p.grad, p.dtype, i) + a.momentum * m : m;
+// Eight elements from i on as float32 (wide: whole vectors).
+__device__ __forceinline__ void read_eight(const void *p, int dtype, int64_t i, float (&v)[8]) {
+  if (dtype == CPAB_F32) {
+    const float4 x = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+    const float4 y = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + 4);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    return;
+  }
+  const uint4 w = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
+  const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 x = dtype == CPAB_F16 ? unpack_pair<__half>(q[k]) : unpack_pair<__nv_bfloat16>(q[k]);
+    v[2 * k] = x.x, v[2 * k + 1] = x.y;
+  }
+}
+__device__ __forceinline__ void write_eight(float *p, const float (&v)[8]) {
+  *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
 }
 
 // Momenta, and partial sums of the directions' squares (in float64: a square may
@@ -107,17 +123,33 @@ __global__ void __launch_bounds__(256) k_direction(const __grid_constant__ Prepa
   tc::dep_launch();
   tc::dep_wait();
   const int64_t n = (int64_t)p.rows * p.cols;
+  const bool moving = p.momentum != nullptr;
+  const float k = a.momentum;
   double sum = 0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    float u;
-    if (p.momentum != nullptr) {
-      const float m = a.momentum * p.momentum[i] + (1.f - a.momentum) * read_as(p.grad, p.dtype, i);
-      p.momentum[i] = m;
-      u = direction(p, a, i, m);
-    } else {
-      u = read_as(p.grad, p.dtype, i);
+  auto one = [&](float g, float m, float *next) {
+    float u = g;
+    if (moving) {
+      m = k * m + (1.f - k) * g;
+      u = a.nesterov ? (1.f - k) * g + k * m : m;
     }
+    *next = m;
     sum += (double)u * (double)u;
+  };
+  // (eights of whole vectors, then what is left)
+  const int64_t eights = p.vectors ? n / 8 : 0;
+#pragma unroll 2
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < eights; e += (int64_t)gridDim.x * 256) {
+    float g[8], m[8] = {};
+    read_eight(p.grad, p.dtype, 8 * e, g);
+    if (moving) read_eight(p.momentum, CPAB_F32, 8 * e, m);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) one(g[j], m[j], &m[j]);
+    if (moving) write_eight(p.momentum + 8 * e, m);
+  }
+  for (int64_t i = 8 * eights + (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float m = moving ? p.momentum[i] : 0.f;
+    one(read_as(p.grad, p.dtype, i), m, &m);
+    if (moving) p.momentum[i] = m;
   }
   __shared__ double part[8];
 #pragma unroll
@@ -131,13 +163,21 @@ __global__ void __launch_bounds__(256) k_direction(const __grid_constant__ Prepa
   }
 }
 
-__device__ __forceinline__ void store_halves(__half *hi, __half *lo, int64_t i, float v) {
-  const __half h = __float2half_rn(v);
-  hi[i] = h;
-  lo[i] = __float2half_rn(v - __half2float(h));
+// Eight neighbours as halves and their remainders (rows are padded to 16).
+__device__ __forceinline__ void store_eight(__half *hi, __half *lo, int64_t i, const float (&v)[8]) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    h[k] = pack_pair<__half>(v[2 * k], v[2 * k + 1]);
+    const float2 x = unpack_pair<__half>(h[k]);
+    l[k] = pack_pair<__half>(v[2 * k] - x.x, v[2 * k + 1] - x.y);
+  }
+  *reinterpret_cast<uint4 *>(hi + i) = make_uint4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<uint4 *>(lo + i) = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// Directions over their norms, as halves; tiles of 64 x 64.
+// Directions over their norms, as halves; tiles of 64 x 64, a thread eight columns
+// of two rows (turned ones: eight rows of two columns on the way out).
 __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ PrepareArgs a, int partials) {
   const Prepared &p = a.m[blockIdx.y];
   const int tiles_x = (p.cols + 63) / 64, tiles = tiles_x * ((p.rows + 63) / 64);
@@ -156,32 +196,143 @@ __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ Prepa
   for (int i = 0; i < 8; ++i) sum += part[i];
   const double norm = sqrt(sum), theta = first_theta(norm, a.eps), scale = (double)kUnit / ((norm + a.eps) * theta);
   if (blockIdx.x == 0 && threadIdx.x == 0) write_terms(p.terms, theta, a.a, a.b, a.c, a.steps);
+  const bool moving = p.momentum != nullptr, whole = p.vectors && p.cols % 8 == 0;
+  const int x = (threadIdx.x & 7) * 8, y0 = threadIdx.x >> 3;
   for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int r0 = t / tiles_x * 64, c0 = t % tiles_x * 64, x = threadIdx.x & 63;
-    for (int y = threadIdx.x >> 6; y < 64; y += 4) {
-      if (r0 + y >= p.rows || c0 + x >= p.cols) continue;
+    const int r0 = t / tiles_x * 64, c0 = t % tiles_x * 64;
+#pragma unroll
+    for (int y = y0; y < 64; y += 32) {
       const int64_t i = (int64_t)(r0 + y) * p.cols + c0 + x;
-      const float u = p.momentum != nullptr ? direction(p, a, i, p.momentum[i]) : read_as(p.grad, p.dtype, i);
-      const float v = (float)((double)u * scale);
-      if (p.turned) tile[y][x] = v;
-      else store_halves(p.hi, p.lo, (int64_t)(r0 + y) * p.pitch + c0 + x, v);
+      if (r0 + y >= p.rows || c0 + x >= p.cols) continue;
+      float g[8], m[8] = {};
+      if (whole) {
+        read_eight(p.grad, p.dtype, i, g);
+        if (moving) read_eight(p.momentum, CPAB_F32, i, m);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = c0 + x + j < p.cols;
+          g[j] = in ? read_as(p.grad, p.dtype, i + j) : 0.f;
+          if (moving) m[j] = in ? p.momentum[i + j] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float u = !moving ? g[j] : a.nesterov ? (1.f - a.momentum) * g[j] + a.momentum * m[j] : m[j];
+        g[j] = (float)((double)u * scale);
+        if (p.turned) tile[y][x + j] = g[j];
+      }
+      if (!p.turned) store_eight(p.hi, p.lo, (int64_t)(r0 + y) * p.pitch + c0 + x, g);
     }
     if (!p.turned) continue;
     __syncthreads();
-    for (int y = threadIdx.x >> 6; y < 64; y += 4)
-      if (c0 + y < p.cols && r0 + x < p.rows)
-        store_halves(p.hi, p.lo, (int64_t)(c0 + y) * p.pitch + r0 + x, tile[x][y]);
+#pragma unroll
+    for (int y = y0; y < 64; y += 32) {
+      if (c0 + y < p.cols && r0 + x < p.rows) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = r0 + x + j < p.rows ? tile[x + j][y] : 0.f;
+        store_eight(p.hi, p.lo, (int64_t)(c0 + y) * p.pitch + r0 + x, v);
+      }
+    }
     __syncthreads();
+  }
+}
+
+// ---- what comes out ------------------------------------------------------------
+
+struct Finished {
+  const __half *hi, *lo;  // [m, pitch]
+  const float *terms;
+  void *out;              // [rows, cols] of dtype, contiguous
+  int64_t pitch;
+  float rate;             // update: p (1 - lr decay) - lr rate O
+  int rows, cols, dtype, turned, update;
+  int vectors;            // out's rows begin on 16 bytes
+};
+struct FinishArgs {
+  Finished m[kPrepared];
+  float lr, decay;
+  const float *lr_device;
+};
+
+// Results, or parameters' steps; tiles as those of k_normalise.  (In the last
+// product's epilogue, where a thread has a row's columns, transposed parameters cost
+// 430 us more for 42 million of them than this pass's 80.)
+__global__ void __launch_bounds__(256) k_finish(const __grid_constant__ FinishArgs a) {
+  const Finished &p = a.m[blockIdx.y];
+  const int tiles_x = (p.cols + 63) / 64, tiles = tiles_x * ((p.rows + 63) / 64);
+  tc::dep_launch();
+  tc::dep_wait();
+  if ((int)blockIdx.x >= tiles) return;
+  __shared__ float tile[64][65];
+  const float lr = a.lr_device != nullptr ? *a.lr_device : a.lr, theta = p.terms[3 * kMostSteps] * (1.f / kUnit);
+  const float keep = 1.f - lr * a.decay, move = p.update ? -lr * p.rate * theta : theta;
+  const int x = (threadIdx.x & 7) * 8, y0 = threadIdx.x >> 3;
+  auto read = [&](int64_t i, float(&v)[8]) {
+    float l[8];
+    read_eight(p.hi, CPAB_F16, i, v);
+    read_eight(p.lo, CPAB_F16, i, l);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += l[j];
+  };
+  for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int r0 = t / tiles_x * 64, c0 = t % tiles_x * 64;
+    if (p.turned) {
+#pragma unroll
+      for (int y = y0; y < 64; y += 32) {
+        float v[8] = {};
+        if (c0 + y < p.cols && r0 + x < p.rows) read((int64_t)(c0 + y) * p.pitch + r0 + x, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tile[x + j][y] = v[j];
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int y = y0; y < 64; y += 32) {
+      if (r0 + y >= p.rows || c0 + x >= p.cols) continue;
+      const int64_t i = (int64_t)(r0 + y) * p.cols + c0 + x;
+      float v[8];
+      if (p.turned) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = tile[y][x + j];
+      } else {
+        read((int64_t)(r0 + y) * p.pitch + c0 + x, v);
+      }
+      if (p.vectors && c0 + x + 8 <= p.cols) {
+        float old[8] = {};
+        if (p.update) read_eight(p.out, p.dtype, i, old);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = p.update ? fmaf(keep, old[j], move * v[j]) : move * v[j];
+        if (p.dtype == CPAB_F32) {
+          write_eight(static_cast<float *>(p.out) + i, v);
+        } else {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            w[j] = p.dtype == CPAB_F16 ? pack_pair<__half>(v[2 * j], v[2 * j + 1])
+                                       : pack_pair<__nv_bfloat16>(v[2 * j], v[2 * j + 1]);
+          *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c0 + x + j < p.cols)
+            write_as(p.out, p.dtype, i + j,
+                     p.update ? fmaf(keep, read_as(p.out, p.dtype, i + j), move * v[j]) : move * v[j]);
+      }
+    }
+    if (p.turned) __syncthreads();
   }
 }
 
 // ---- the products ------------------------------------------------------------------
 
-enum Phase { kGram, kSquare, kUpdate, kFinal };
+enum Phase { kGram, kSquare, kUpdate };
 
 struct PhaseGroup {
   CUtensorMap a[2], b[2];          // first halves and remainders of the operands
-  const __half *read[2];           // A (kSquare) or X (kUpdate, kFinal)
+  const __half *read[2];           // A (kSquare) or X (kUpdate)
   __half *write[2];                // A, B or the next X
   int64_t read_pitch, read_plane, write_pitch, write_plane;
   int m, n;                        // of the result
@@ -190,32 +341,15 @@ struct PhaseGroup {
   int write_lo;
   const float *terms;              // of the set's first matrix, kTerms apart
 };
-struct FinalGroup {
-  void *out;                       // of matrix z: out + z * stride elements, or table[first + z]
-  int64_t stride;
-  int first;                       // -1: out and stride
-  int dtype, turned, update;       // turned: stored transposed; update: a parameter's step
-  int wide;                        // all rows begin on 32 bytes
-  float decay, rate;               // p (1 - lr decay) - lr rate O
-  const float *lr_device;
-  float lr;
-};
-template <bool FINAL>
 struct PhaseArgs {
   PhaseGroup g[kGroups];
-  int groups, step;
-};
-template <>
-struct PhaseArgs<true> {
-  PhaseGroup g[kGroups];
-  FinalGroup f[kGroups];
-  void *table[kMatrices];
   int groups, step;
 };
 
 template <int PHASE, int PARTS, int CTAS, int BN>
 struct Schulz {
-  static constexpr int kCtas = CTAS, kBN = BN, kAcc = 2, kParts = PARTS, kChunk = 16;
+  static constexpr int kCtas = CTAS, kBN = BN, kAcc = 2, kParts = PARTS;
+  static constexpr int kChunk = PARTS == 2 && BN == 256 ? 16 : 32;
   // (16-bit results: up to 1.5e-5 of the sum at 4096 summed, against 2^-12 of its operands)
   static constexpr int kSegment = PARTS == 2 ? 4 : 0;
   static constexpr bool kScaled = false, kBMn = PHASE >= kUpdate, kSymmetric = PHASE <= kSquare;
@@ -228,7 +362,7 @@ struct Schulz {
     int m0, n0, steps, z, g;
     bool mirror;
   };
-  const PhaseArgs<PHASE == kFinal> &p;
+  const PhaseArgs &p;
 
   __device__ int tiles() const { return p.g[p.groups - 1].end; }
   __device__ Tile tile(int i) const {
@@ -270,119 +404,76 @@ struct Schulz {
   }
   __device__ void begin(const Tile &, Shared &, int) const {}
 
-  __device__ void store(const Tile &t, const Shared &, int row, int c, const float *acc) const {
-    const PhaseGroup &q = p.g[t.g];
-    const int col = t.n0 + c;
-    if (row >= q.m || col >= q.n) return;
-    const bool whole = col + 16 <= q.n;
-    float v[16];
+  // A's or X's halves in the place of what is stored.  (Read when a chunk is stored and
+  // not one ahead, their latency alone was half of an update's time.)
+  struct Ahead {
+    uint32_t hi[PHASE == kGram ? 1 : kChunk / 2], lo[PHASE == kGram ? 1 : kChunk / 2];
+  };
+  __device__ Ahead ahead(const Tile &t, int row, int c) const {
+    Ahead w;
+    if constexpr (PHASE != kGram) {
+      const PhaseGroup &q = p.g[t.g];
+      const int col = t.n0 + c;
+      const int64_t at = t.z * q.read_plane + row * q.read_pitch + col;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = acc[j] * (1.f / kUnit);
+      for (int k = 0; k < kChunk; k += 16) {
+        uint32_t h[8] = {}, l[8] = {};
+        if (row < q.m && col + k < q.n) {  // (rows are padded to 16)
+          tc::load_sector(q.read[0] + at + k, h);
+          tc::load_sector(q.read[1] + at + k, l);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w.hi[k / 2 + j] = h[j], w.lo[k / 2 + j] = l[j];
+      }
+    }
+    return w;
+  }
+  __device__ void store(const Tile &t, const Shared &, int row, int c, const float *acc, const Ahead &w) const {
+    const PhaseGroup &q = p.g[t.g];
+    float mine = 0.f, product = 1.f / kUnit;
     if constexpr (PHASE != kGram) {
       const float *terms = q.terms + t.z * kTerms + 3 * p.step;
-      const float mine = terms[PHASE == kSquare ? 1 : 0], product = PHASE == kSquare ? terms[2] : 1.f;
-      const int64_t at = t.z * q.read_plane + row * q.read_pitch + col;
-      const __half *hi = q.read[0] + at, *lo = q.read[1] + at;
-      if (whole) {
-        uint32_t h[8], l[8];
-        tc::load_sector(hi, h);
-        tc::load_sector(lo, l);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float2 x = unpack_pair<__half>(h[j]), y = unpack_pair<__half>(l[j]);
-          v[2 * j] = mine * (x.x + y.x) + product * v[2 * j];
-          v[2 * j + 1] = mine * (x.y + y.y) + product * v[2 * j + 1];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (col + j < q.n) v[j] = mine * (__half2float(hi[j]) + __half2float(lo[j])) + product * v[j];
-      }
-    }
-    if constexpr (PHASE == kFinal) {
-      finish(t, q, row, col, v);
-      return;
+      mine = terms[PHASE == kSquare ? 1 : 0];
+      if (PHASE == kSquare) product *= terms[2];
     }
     __half *hi = q.write[0] + t.z * q.write_plane, *lo = q.write[1] + t.z * q.write_plane;
-    const int64_t at = row * q.write_pitch + col;
-    uint32_t h[8], l[8];
+    const int odd = threadIdx.x & 1;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      h[j] = pack_pair<__half>(v[2 * j], v[2 * j + 1]);
-      const float2 x = unpack_pair<__half>(h[j]);
-      l[j] = pack_pair<__half>(v[2 * j] - x.x, v[2 * j + 1] - x.y);
-    }
-    if (whole) {
-      tc::store_sector(hi + at, h);
-      if (q.write_lo) tc::store_sector(lo + at, l);
-    }
-    if (!whole || t.mirror) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (col + j < q.n) {
-          const uint16_t x = (uint16_t)(h[j >> 1] >> (16 * (j & 1))), y = (uint16_t)(l[j >> 1] >> (16 * (j & 1)));
-          const __half xh = __ushort_as_half(x), yh = __ushort_as_half(y);
-          if (!whole) {
-            hi[at + j] = xh;
-            if (q.write_lo) lo[at + j] = yh;
-          }
-          if (t.mirror) {
-            const int64_t to = (int64_t)(col + j) * q.write_pitch + row;
-            hi[to] = xh;
-            if (q.write_lo) lo[to] = yh;
-          }
-        }
-    }
-  }
-
-  // The last step's values: the result, or a parameter's step.
-  __device__ void finish(const Tile &t, const PhaseGroup &q, int row, int col, float (&v)[16]) const {
-    if constexpr (PHASE == kFinal) {
-      const FinalGroup &f = p.f[t.g];
-      const int e = f.dtype == CPAB_F32 ? 4 : 2;
-      void *out = f.first >= 0 ? p.table[f.first + t.z] : static_cast<char *>(f.out) + t.z * f.stride * e;
-      const float lr = f.lr_device != nullptr ? *f.lr_device : f.lr;
-      const float last = q.terms[t.z * kTerms + 3 * kMostSteps] * (1.f / kUnit);
-      const float keep = f.update ? 1.f - lr * f.decay : 0.f, move = (f.update ? -lr * f.rate : 1.f) * last;
-      if (f.wide && col + 16 <= q.n) {
-        const int64_t i = (int64_t)row * q.n + col;
-        if (f.dtype == CPAB_F32) whole<float>(static_cast<float *>(out) + i, f.update, keep, move, v);
-        else if (f.dtype == CPAB_F16) whole<__half>(static_cast<__half *>(out) + i, f.update, keep, move, v);
-        else whole<__nv_bfloat16>(static_cast<__nv_bfloat16 *>(out) + i, f.update, keep, move, v);
-        return;
-      }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (col + j >= q.n) break;
-        const int64_t i = f.turned ? (int64_t)(col + j) * q.m + row : (int64_t)row * q.n + col + j;
-        const float o = move * v[j];
-        write_as(out, f.dtype, i, f.update ? fmaf(keep, read_as(out, f.dtype, i), o) : o);
-      }
-    }
-  }
-  // 16 values of a row that begins on 32 bytes.
-  template <typename T>
-  static __device__ void whole(T *out, int update, float keep, float move, const float (&v)[16]) {
-    uint32_t w[8];
-    if constexpr (sizeof(T) == 2) {
-      if (update) tc::load_sector(out, w);
+    for (int k = 0; k < kChunk; k += 16) {
+      const int col = t.n0 + c + k;
+      if (col >= q.n) return;
+      uint32_t h[8], l[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float2 x = update ? unpack_pair<T>(w[j]) : make_float2(0.f, 0.f);
-        const float a = move * v[2 * j], b = move * v[2 * j + 1];
-        w[j] = update ? pack_pair<T>(fmaf(keep, x.x, a), fmaf(keep, x.y, b)) : pack_pair<T>(a, b);
+        float a = acc[k + 2 * j] * product, b = acc[k + 2 * j + 1] * product;
+        if constexpr (PHASE != kGram) {
+          const float2 x = unpack_pair<__half>(w.hi[k / 2 + j]), y = unpack_pair<__half>(w.lo[k / 2 + j]);
+          a = fmaf(mine, x.x + y.x, a), b = fmaf(mine, x.y + y.y, b);
+        }
+        h[j] = pack_pair<__half>(a, b);
+        const float2 x = unpack_pair<__half>(h[j]);
+        l[j] = pack_pair<__half>(a - x.x, b - x.y);
       }
-      tc::store_sector(out, w);
-    } else {
-#pragma unroll
-      for (int h = 0; h < 16; h += 8) {
-        if (update) tc::load_sector(out + h, w);
+      // (what lies past a row's end, up to the next multiple of 16, is never read as a value)
+      if (row < q.m) {
+        const int64_t at = row * q.write_pitch + col;
+        tc::store_sector(hi + at, h);
+        if (q.write_lo) tc::store_sector(lo + at, l);
+      }
+      if (t.mirror) {
+        // Neighbouring rows' threads swap, so that each stores two rows of one column.
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float o = move * v[h + j];
-          w[j] = __float_as_uint(update ? fmaf(keep, __uint_as_float(w[j]), o) : o);
+          const uint32_t oh = __shfl_xor_sync(~0u, h[j], 1), ol = __shfl_xor_sync(~0u, l[j], 1);
+          const uint32_t th = odd ? __byte_perm(oh, h[j], 0x7632) : __byte_perm(h[j], oh, 0x5410);
+          const uint32_t tl = odd ? __byte_perm(ol, l[j], 0x7632) : __byte_perm(l[j], ol, 0x5410);
+          const int column = col + 2 * j + odd;
+          if (column < q.n && row < q.m) {
+            const int64_t to = (int64_t)column * q.write_pitch + (row & ~1);
+            *reinterpret_cast<uint32_t *>(hi + to) = th;
+            if (q.write_lo) *reinterpret_cast<uint32_t *>(lo + to) = tl;
+          }
         }
-        tc::store_sector(out + h, w);
       }
     }
   }
@@ -390,12 +481,12 @@ struct Schulz {
 
 template <int PHASE, int PARTS, int CTAS, int BN>
 __global__ void __launch_bounds__(tc::kCoreThreads, 1)
-    k_schulz(const __grid_constant__ PhaseArgs<PHASE == kFinal> a) {
+    k_schulz(const __grid_constant__ PhaseArgs a) {
   tc::core(Schulz<PHASE, PARTS, CTAS, BN>{a});
 }
 
 template <int PHASE, int PARTS, int CTAS, int BN>
-cudaError_t launch_phase_as(PhaseArgs<PHASE == kFinal> &a, const int *batch, cudaStream_t s) {
+cudaError_t launch_phase_as(PhaseArgs &a, const int *batch, cudaStream_t s) {
   using S = tc::CoreShape<Schulz<PHASE, PARTS, CTAS, BN>>;
   auto *kernel = k_schulz<PHASE, PARTS, CTAS, BN>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
@@ -466,7 +557,7 @@ bool map_of(CUtensorMap *map, const __half *p, int columns, int rows, int batch,
 }
 
 template <int PHASE, int PARTS>
-cudaError_t launch_phase(PhaseArgs<PHASE == kFinal> &a, const int *batch, cudaStream_t s) {
+cudaError_t launch_phase(PhaseArgs &a, const int *batch, cudaStream_t s) {
   int64_t tiles = 0;
   for (int g = 0; g < a.groups; ++g) {
     const int64_t tm = (a.g[g].m + 255) / 256, tn = (a.g[g].n + 255) / 256;
@@ -478,18 +569,15 @@ cudaError_t launch_phase(PhaseArgs<PHASE == kFinal> &a, const int *batch, cudaSt
 
 // The products of at most kGroups sets, all of one kind.
 template <int PARTS>
-cudaError_t schulz_as(const std::vector<Set> &sets, const std::vector<Places> &places, const FinalGroup *finals,
-                      void *const *table, int table_size, int steps, cudaStream_t s) {
+cudaError_t schulz_as(const std::vector<Set> &sets, const std::vector<Places> &places, int steps, cudaStream_t s) {
   int batch[kGroups];
-  PhaseArgs<false> a;
-  PhaseArgs<true> last;
+  PhaseArgs a;
   const int groups = (int)sets.size();
-  a.groups = last.groups = groups;
-  for (int i = 0; i < table_size; ++i) last.table[i] = table[i];
-  for (int g = 0; g < groups; ++g) last.f[g] = finals[g], batch[g] = sets[g].batch;
+  a.groups = groups;
+  for (int g = 0; g < groups; ++g) batch[g] = sets[g].batch;
   for (int step = 0; step < steps; ++step) {
     const int now = step & 1;
-    a.step = last.step = step;
+    a.step = step;
     bool ok = true;
     cudaError_t e;
     for (int g = 0; g < groups; ++g) {
@@ -534,21 +622,14 @@ cudaError_t schulz_as(const std::vector<Set> &sets, const std::vector<Places> &p
       q.n = t.n(), q.write_lo = 1;
     }
     if (!ok) return cudaErrorInvalidValue;
-    if (step + 1 < steps) {
-      e = launch_phase<kUpdate, PARTS>(a, batch, s);
-    } else {
-      for (int g = 0; g < groups; ++g) last.g[g] = a.g[g];
-      e = launch_phase<kFinal, PARTS>(last, batch, s);
-    }
+    e = launch_phase<kUpdate, PARTS>(a, batch, s);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
 
-cudaError_t schulz(const std::vector<Set> &sets, const std::vector<Places> &places, const FinalGroup *finals,
-                   void *const *table, int table_size, int steps, cudaStream_t s) {
-  return sets[0].parts() == 2 ? schulz_as<2>(sets, places, finals, table, table_size, steps, s)
-                              : schulz_as<1>(sets, places, finals, table, table_size, steps, s);
+cudaError_t schulz(const std::vector<Set> &sets, const std::vector<Places> &places, int steps, cudaStream_t s) {
+  return sets[0].parts() == 2 ? schulz_as<2>(sets, places, steps, s) : schulz_as<1>(sets, places, steps, s);
 }
 
 // Launches what reads the matrices in.
@@ -560,6 +641,8 @@ cudaError_t prepare(const std::vector<Prepared> &list, float momentum, int neste
     int64_t most = 0, tiles = 0;
     for (int i = 0; i < n; ++i) {
       a.m[i] = list[first + i];
+      a.m[i].vectors = reinterpret_cast<uintptr_t>(a.m[i].grad) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(a.m[i].momentum) % 16 == 0;
       most = std::max(most, (int64_t)a.m[i].rows * a.m[i].cols);
       tiles = std::max(tiles, (int64_t)((a.m[i].rows + 63) / 64) * ((a.m[i].cols + 63) / 64));
     }
@@ -571,6 +654,441 @@ cudaError_t prepare(const std::vector<Prepared> &list, float momentum, int neste
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
+}
+
+// Launches what writes the results.
+cudaError_t finish(const std::vector<Finished> &list, double lr, const float *lr_device, double decay, cudaStream_t s) {
+  for (size_t first = 0; first < list.size(); first += kPrepared) {
+    const int n = (int)std::min<size_t>(kPrepared, list.size() - first);
+    FinishArgs a;
+    int64_t tiles = 0;
+    for (int i = 0; i < n; ++i) {
+      Finished &m = a.m[i] = list[first + i];
+      m.vectors = aligned_to(m.out, m.cols, dtype_size(m.dtype), 16);
+      tiles = std::max(tiles, (int64_t)((m.rows + 63) / 64) * ((m.cols + 63) / 64));
+    }
+    a.lr = (float)lr, a.decay = (float)decay, a.lr_device = lr_device;
+    const cudaError_t e =
+        tc::launch(k_finish, dim3((unsigned)std::min<int64_t>(tiles, 65535), n), 256, 0, 1, s, a);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+// ---- small matrices ------------------------------------------------------------------
+//
+// A matrix of few rows stays in shared memory through all steps, its columns spread
+// over the blocks of a cluster: one launch in place of 18.  Each block forms its columns' part of X X^T; the blocks add the parts
+// of one share each, in order, and hand the sums to all; each squares a share of the
+// rows of A and hands B to all; each updates its own columns.  All as pairs of halves.
+
+constexpr int kSmallThreads = 512, kSmallWarps = kSmallThreads / 32;
+constexpr int kSmallRows = 128;
+constexpr int kSmallUnits = 3;    // 16 x 32 results a warp holds
+constexpr int kSmallSums = 9;     // times four sums a thread holds
+constexpr int kSmallBytes = 220 * 1024;
+
+struct Small {
+  const void *grad;
+  float *momentum;
+  void *out;
+  int rows, cols, dtype, update;
+  float rate;
+};
+struct SmallArgs {
+  Small m[kMatrices];
+  int64_t stride;        // > 0: matrix z is m[0]'s, z * stride elements on
+  float momentum, lr, decay;
+  const float *lr_device;
+  int nesterov, steps;
+  double eps, a, b, c;
+};
+
+// Sizes of a matrix's parts in a cluster of `blocks`.
+struct SmallShape {
+  int m, n, rows, columns;  // rows padded to 16, columns of a block padded to 16
+  __host__ __device__ SmallShape(int rows_, int cols, int blocks) {
+    m = rows_ < cols ? rows_ : cols, n = rows_ < cols ? cols : rows_;
+    rows = (m + 15) / 16 * 16;
+    columns = ((n + blocks - 1) / blocks + 15) / 16 * 16;
+  }
+  // (8 halves more than a row's: the eight rows of a matrix load lie in different banks)
+  __host__ __device__ int a_pitch() const { return rows + 8; }
+  __host__ __device__ int x_pitch() const { return columns + 8; }
+  __host__ __device__ int bytes() const { return rows * (a_pitch() + x_pitch()) * 4; }
+  bool fits(int blocks) const {
+    const int r = rows / 16, wide = (rows + 31) / 32;
+    return m <= kSmallRows && bytes() <= kSmallBytes && r * ((columns + 31) / 32) <= kSmallUnits * kSmallWarps &&
+           (r + blocks - 1) / blocks * wide <= kSmallUnits * kSmallWarps &&
+           (r + blocks - 1) / blocks * 4 * a_pitch() <= kSmallSums * kSmallThreads;
+  }
+};
+
+__device__ __forceinline__ void load_matrices(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void load_matrices_turned(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Pairs of halves in shared memory: `lo` lies `skip` bytes behind.
+struct Halves {
+  uint32_t hi, skip;
+  int pitch;
+  __device__ uint32_t at(int row, int column) const { return hi + (uint32_t)(row * pitch + column) * 2; }
+};
+
+// acc = A[row0.., :K] B: 16 rows and 32 columns (the second 16 where `both`); B's rows
+// are its columns' (B^T as it lies), or with TURNED the summed ones.
+template <bool TURNED>
+__device__ __forceinline__ void unit(const Halves &A, const Halves &B, int row0, int col0, int K, bool both, int lane,
+                                     float (&acc)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+  const uint32_t from = A.at(row0 + (lane & 15), (lane >> 4) * 8);
+  const uint32_t with = TURNED ? B.at(lane & 15, col0 + (lane >> 4) * 8)
+                               : B.at(col0 + (lane & 7) + ((lane >> 4) << 3), ((lane >> 3) & 1) * 8);
+  const uint32_t along = (TURNED ? 16 * B.pitch : 16) * 2, second = both ? (TURNED ? 16 : 16 * B.pitch) * 2 : 0;
+#pragma unroll 1
+  for (int k = 0; k < K / 16; ++k) {
+    uint32_t ah[4], al[4], bh[2][4], bl[2][4];
+    load_matrices(from + 32 * k, ah);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // (where there is no second half, the first again)
+      const uint32_t b = with + along * k + second * h;
+      if (TURNED) {
+        load_matrices_turned(b + B.skip, bl[h]);
+        load_matrices_turned(b, bh[h]);
+      } else {
+        load_matrices(b + B.skip, bl[h]);
+        load_matrices(b, bh[h]);
+      }
+    }
+    load_matrices(from + 32 * k + A.skip, al);
+    // (one sum's three products four instructions apart)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mma_16816(acc[i], ah, bl[i >> 1][2 * (i & 1)], bl[i >> 1][2 * (i & 1) + 1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mma_16816(acc[i], ah, bh[i >> 1][2 * (i & 1)], bh[i >> 1][2 * (i & 1) + 1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mma_16816(acc[i], al, bh[i >> 1][2 * (i & 1)], bh[i >> 1][2 * (i & 1) + 1]);
+  }
+}
+
+__device__ __forceinline__ float4 load_peer(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ double load_peer_double(uint32_t addr) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_peer(uint32_t addr, uint4 v) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ void store_peer(uint32_t addr, uint2 v) {
+  asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
+}
+__device__ __forceinline__ uint32_t load_word(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_word(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+// Two neighbours' value, and their halves.
+__device__ __forceinline__ float2 value_of(const Halves &h, int row, int column) {
+  const float2 x = unpack_pair<__half>(load_word(h.at(row, column)));
+  const float2 y = unpack_pair<__half>(load_word(h.at(row, column) + h.skip));
+  return make_float2(x.x + y.x, x.y + y.y);
+}
+__device__ __forceinline__ void halves_of(float a, float b, uint32_t *hi, uint32_t *lo) {
+  *hi = pack_pair<__half>(a, b);
+  const float2 x = unpack_pair<__half>(*hi);
+  *lo = pack_pair<__half>(a - x.x, b - x.y);
+}
+
+__global__ void __launch_bounds__(kSmallThreads, 1) k_schulz_small(const __grid_constant__ SmallArgs a) {
+  extern __shared__ __align__(16) uint8_t small_smem[];
+  __shared__ double part[kSmallWarps], mine;
+  __shared__ float terms[kTerms];
+  const int blocks = tc::cluster_blocks(), rank = (int)tc::cluster_rank();
+  const int z = blockIdx.x / blocks, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Small p = a.m[a.stride > 0 ? 0 : z];
+  if (a.stride > 0) {
+    const int64_t skip = z * a.stride * (p.dtype == CPAB_F32 ? 4 : 2);
+    p.grad = static_cast<const char *>(p.grad) + skip, p.out = static_cast<char *>(p.out) + skip;
+  }
+  const SmallShape t(p.rows, p.cols, blocks);
+  const bool turned = p.rows > p.cols;
+  const int n0 = rank * t.columns, own = max(0, min(t.columns, t.n - n0));  // this block's columns
+  const uint32_t base = tc::smem_u32(small_smem);
+  const Halves R = {base, (uint32_t)(t.rows * t.a_pitch() * 2), t.a_pitch()};
+  const Halves X = {base + 2 * R.skip, (uint32_t)(t.rows * t.x_pitch() * 2), t.x_pitch()};
+  tc::dep_launch();
+  tc::dep_wait();
+
+  // What goes in: element e of this block's part, in memory's order.
+  const int inner = turned ? t.m : own, count = t.m * own;
+  auto place = [&](int e, int *row, int *column) {
+    const int x = e % inner, y = e / inner;
+    *row = turned ? x : y, *column = turned ? y : x;
+    return turned ? (int64_t)(n0 + y) * p.cols + x : (int64_t)y * p.cols + n0 + x;
+  };
+  auto direction_of = [&](int64_t i, float m) {
+    const float g = read_as(p.grad, p.dtype, i);
+    return p.momentum == nullptr ? g : a.nesterov ? (1.f - a.momentum) * g + a.momentum * m : m;
+  };
+  double sum = 0;
+  for (int e = threadIdx.x; e < count; e += kSmallThreads) {
+    int row, column;
+    const int64_t i = place(e, &row, &column);
+    float m = 0.f;
+    if (p.momentum != nullptr) {
+      m = a.momentum * p.momentum[i] + (1.f - a.momentum) * read_as(p.grad, p.dtype, i);
+      p.momentum[i] = m;
+    }
+    const double u = direction_of(i, m);
+    sum += u * u;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  if (lane == 0) part[warp] = sum;
+  for (uint32_t w = threadIdx.x; w < X.skip / 2; w += kSmallThreads) store_word(X.hi + 4 * w, 0);  // (padding is 0)
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0;
+    for (int w = 0; w < kSmallWarps; ++w) sum += part[w];
+    mine = sum;
+  }
+  tc::cluster_sync();
+  sum = 0;
+  for (int c = 0; c < blocks; ++c) sum += load_peer_double(tc::mapa(tc::smem_u32(&mine), c));
+  const double norm = sqrt(sum), theta = first_theta(norm, a.eps), scale = (double)kUnit / ((norm + a.eps) * theta);
+  if (threadIdx.x == 0) write_terms(terms, theta, a.a, a.b, a.c, a.steps);
+  for (int e = threadIdx.x; e < count; e += kSmallThreads) {
+    int row, column;
+    const int64_t i = place(e, &row, &column);
+    const float v = (float)((double)direction_of(i, p.momentum != nullptr ? p.momentum[i] : 0.f) * scale);
+    const __half h = __float2half_rn(v);
+    __half *to = reinterpret_cast<__half *>(small_smem + 2 * R.skip) + row * X.pitch + column;
+    *to = h;
+    to[X.skip / 2] = __float2half_rn(v - __half2float(h));
+  }
+  __syncthreads();
+
+  const int row_blocks = t.rows / 16, wide = (t.rows + 31) / 32;
+  // This block's share of A's and B's rows, and the fours of their elements.
+  const int share0 = rank * row_blocks / blocks, shares = (rank + 1) * row_blocks / blocks - share0;
+  const int fours = shares * 4 * R.pitch;
+  const int fr = lane >> 2, fc = 2 * (lane & 3);                           // a fragment's row and column
+  for (int step = 0; step < a.steps; ++step) {
+    // The columns' part of X X^T, in float32 where A will lie.
+    for (int u = warp; u < row_blocks * wide; u += kSmallWarps) {
+      const int row = u / wide * 16, col = u % wide * 32;
+      const bool both = col + 16 < t.rows;
+      float acc[4][4];
+      unit<false>(X, X, row, col, t.columns, both, lane, acc);
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        if (f >= 2 && !both) break;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<float2 *>(small_smem + ((row + fr + 8 * h) * R.pitch + col + 8 * f + fc) * 4) =
+              make_float2(acc[f][2 * h] * (1.f / kUnit), acc[f][2 * h + 1] * (1.f / kUnit));
+      }
+    }
+    tc::cluster_sync();
+    float4 v[kSmallSums];
+#pragma unroll
+    for (int k = 0; k < kSmallSums; ++k) {
+      const int q = threadIdx.x + k * kSmallThreads;
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (q < fours) {
+        const uint32_t from = base + (uint32_t)(share0 * 16 * R.pitch + 4 * q) * 4;
+        // (all blocks' parts asked for before the first is added)
+        float4 x[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (c < blocks) x[c] = load_peer(tc::mapa(from, c));
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (c < blocks) v[k].x += x[c].x, v[k].y += x[c].y, v[k].z += x[c].z, v[k].w += x[c].w;
+      }
+    }
+    tc::cluster_sync();
+#pragma unroll
+    for (int k = 0; k < kSmallSums; ++k) {
+      const int q = threadIdx.x + k * kSmallThreads;
+      if (q < fours) {
+        uint2 hi, lo;
+        halves_of(v[k].x, v[k].y, &hi.x, &lo.x);
+        halves_of(v[k].z, v[k].w, &hi.y, &lo.y);
+        const uint32_t to = R.hi + (uint32_t)(share0 * 16 * R.pitch + 4 * q) * 2;
+        for (int c = 0; c < blocks; ++c) {
+          const uint32_t peer = tc::mapa(to, c);
+          store_peer(peer, hi);
+          store_peer(peer + R.skip, lo);
+        }
+      }
+    }
+    tc::cluster_sync();
+    // This block's rows of B = b A + c A A.
+    float acc[kSmallUnits][4][4];
+    const float ta = terms[3 * step], tb = terms[3 * step + 1], product = terms[3 * step + 2] * (1.f / kUnit);
+#pragma unroll
+    for (int k = 0; k < kSmallUnits; ++k) {
+      const int u = warp + k * kSmallWarps;
+      if (u < shares * wide) {
+        const int row = (share0 + u / wide) * 16, col = u % wide * 32;
+        unit<false>(R, R, row, col, t.rows, col + 16 < t.rows, lane, acc[k]);
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (f >= 2 && col + 16 >= t.rows) break;
+            const float2 w = value_of(R, row + fr + 8 * h, col + 8 * f + fc);
+            acc[k][f][2 * h] = tb * w.x + product * acc[k][f][2 * h];
+            acc[k][f][2 * h + 1] = tb * w.y + product * acc[k][f][2 * h + 1];
+          }
+      }
+    }
+    tc::cluster_sync();
+#pragma unroll
+    for (int k = 0; k < kSmallUnits; ++k) {
+      const int u = warp + k * kSmallWarps;
+      if (u < shares * wide) {
+        const int row = (share0 + u / wide) * 16, col = u % wide * 32;
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (f >= 2 && col + 16 >= t.rows) break;
+            uint32_t hi, lo;
+            halves_of(acc[k][f][2 * h], acc[k][f][2 * h + 1], &hi, &lo);
+            const uint32_t to = R.at(row + fr + 8 * h, col + 8 * f + fc);
+            store_word(to, hi);
+            store_word(to + R.skip, lo);
+          }
+      }
+    }
+    __syncthreads();
+    for (int q = threadIdx.x; q < fours; q += kSmallThreads) {  // (16 bytes: eight halves or remainders)
+      const int half = fours / 2;
+      const uint32_t at = (uint32_t)(share0 * 16 * R.pitch * 2 + 16 * (q < half ? q : q - half)) + (q < half ? 0 : R.skip);
+      const uint4 w = *reinterpret_cast<const uint4 *>(small_smem + at);
+      for (int c = 0; c < blocks; ++c)
+        if (c != rank) store_peer(tc::mapa(base + at, c), w);
+    }
+    tc::cluster_sync();
+    // X <- a X + B X, own columns.
+    const int across = (t.columns + 31) / 32;
+#pragma unroll
+    for (int k = 0; k < kSmallUnits; ++k) {
+      const int u = warp + k * kSmallWarps;
+      if (u < row_blocks * across) {
+        const int row = u / across * 16, col = u % across * 32;
+        unit<true>(R, X, row, col, t.rows, col + 16 < t.columns, lane, acc[k]);
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (f >= 2 && col + 16 >= t.columns) break;
+            const float2 w = value_of(X, row + fr + 8 * h, col + 8 * f + fc);
+            acc[k][f][2 * h] = ta * w.x + acc[k][f][2 * h] * (1.f / kUnit);
+            acc[k][f][2 * h + 1] = ta * w.y + acc[k][f][2 * h + 1] * (1.f / kUnit);
+          }
+      }
+    }
+    __syncthreads();
+    const bool end = step + 1 == a.steps;
+    const float lr = a.lr_device != nullptr ? *a.lr_device : a.lr;
+    const float final_theta = terms[3 * kMostSteps] * (1.f / kUnit);
+    const float keep = 1.f - lr * a.decay, move = p.update ? -lr * p.rate * final_theta : final_theta;
+#pragma unroll
+    for (int k = 0; k < kSmallUnits; ++k) {
+      const int u = warp + k * kSmallWarps;
+      if (u < row_blocks * across) {
+        const int row = u / across * 16, col = u % across * 32;
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (f >= 2 && col + 16 >= t.columns) break;
+            const int r = row + fr + 8 * h, c = col + 8 * f + fc;
+            if (!end) {
+              uint32_t hi, lo;
+              halves_of(acc[k][f][2 * h], acc[k][f][2 * h + 1], &hi, &lo);
+              store_word(X.at(r, c), hi);
+              store_word(X.at(r, c) + X.skip, lo);
+              continue;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (r >= t.m || c + j >= own) continue;
+              const int64_t i = turned ? (int64_t)(n0 + c + j) * p.cols + r : (int64_t)r * p.cols + n0 + c + j;
+              const float o = move * acc[k][f][2 * h + j];
+              write_as(p.out, p.dtype, i, p.update ? fmaf(keep, read_as(p.out, p.dtype, i), o) : o);
+            }
+          }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// The cluster for matrices of these shapes: the smallest that holds each, and twice
+// that while blocks are few and columns many; 0: some matrix is too large.
+int small_cluster(const Small *m, int shapes, int64_t count) {
+  for (int blocks = 1; blocks <= 8; blocks *= 2) {
+    int columns = 0;
+    bool ok = true;
+    for (int i = 0; i < shapes; ++i) {
+      const SmallShape t(m[i].rows, m[i].cols, blocks);
+      ok = ok && t.fits(blocks);
+      columns = std::max(columns, t.columns);
+    }
+    if (ok && (blocks == 8 || columns <= 32 || 2 * blocks * count > device_info().sm_count)) return blocks;
+    if (ok && blocks < 8) {
+      bool next = true;
+      for (int i = 0; i < shapes; ++i) next = next && SmallShape(m[i].rows, m[i].cols, 2 * blocks).fits(2 * blocks);
+      if (!next) return blocks;
+    }
+  }
+  return 0;
+}
+
+// Five steps by one launch and by a launch for each product (us, float32): 64 x 64 49,
+// 49 x 2048 90, 128 x 128 80, 128 x 300 104, 128 x 1000 143; 130 x 260 119, 192 x 192 130.
+// What the blocks hand each other (8 bytes a clock) grows with the rows' square.
+bool is_small(int64_t rows, int64_t columns) {
+  const int64_t m = std::min(rows, columns), n = std::max(rows, columns);
+  return m <= kSmallRows && n <= 1 << 16 && (m <= 64 || m * n <= 1 << 16) &&
+         SmallShape((int)rows, (int)columns, 8).fits(8);
+}
+
+cudaError_t launch_small(const SmallArgs &a, int shapes, int64_t count, cudaStream_t s) {
+  const int blocks = small_cluster(a.m, shapes, count);
+  int bytes = 0;
+  for (int i = 0; i < shapes; ++i) bytes = std::max(bytes, SmallShape(a.m[i].rows, a.m[i].cols, blocks).bytes());
+  const cudaError_t e = cudaFuncSetAttribute(k_schulz_small, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallBytes);
+  if (e != cudaSuccess) return e;
+  return tc::launch(k_schulz_small, (unsigned)(blocks * count), kSmallThreads, bytes, blocks, s, a);
 }
 
 constexpr int64_t kMostRows = 1 << 20;
@@ -602,6 +1120,7 @@ using namespace cpab;
 extern "C" int64_t cpab_b200_orthogonalize_workspace(int dtype, int64_t batch, int64_t rows, int64_t columns) {
   if (!dtype_ok(dtype) || batch < 1 || rows < 1 || columns < 1 || batch > 65536 || rows > kMostRows || columns > kMostRows)
     return 0;
+  if (is_small(rows, columns)) return 0;
   return place({{(int)rows, (int)columns, dtype, (int)batch}}, batch, nullptr, nullptr, nullptr);
 }
 
@@ -616,9 +1135,17 @@ extern "C" int cpab_b200_orthogonalize(int dtype, const void *x, int64_t batch, 
   if (batch == 0 || rows == 0 || columns == 0) return report_error(CPAB_OK, "%s", "");
   if (batch > 65536 || rows > kMostRows || columns > kMostRows)
     return report_error(CPAB_ERR_SIZE, "%s", "orthogonalize: at most 65536 matrices of 2^20 rows and columns");
-  if (x == nullptr || out == nullptr || workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256)
-    return report_error(CPAB_ERR_ARG, "%s", "orthogonalize: null pointer, or a workspace off 256 bytes");
+  if (x == nullptr || out == nullptr) return report_error(CPAB_ERR_ARG, "%s", "orthogonalize: null pointer");
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (is_small(rows, columns)) {
+    SmallArgs a = {};
+    a.m[0] = {x, nullptr, out, (int)rows, (int)columns, dtype, 0, 0.f};
+    a.stride = rows * columns, a.steps = steps, a.eps = eps;
+    a.a = coefficients[0], a.b = coefficients[1], a.c = coefficients[2];
+    return launch_status(launch_small(a, 1, batch, s), "orthogonalize");
+  }
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256)
+    return report_error(CPAB_ERR_ARG, "%s", "orthogonalize: a null workspace, or one off 256 bytes");
   const std::vector<Set> sets = {{(int)rows, (int)columns, dtype, (int)batch}};
   std::vector<Places> places;
   double *partials;
@@ -631,10 +1158,15 @@ extern "C" int cpab_b200_orthogonalize(int dtype, const void *x, int64_t batch, 
                places[0].x[0][1] + at, partials + z * kPartials, places[0].terms + z * kTerms, t.x_pitch(), (int)rows, (int)columns, dtype, t.turned()};
   }
   cudaError_t e = prepare(list, 0.f, 0, steps, coefficients, eps, s);
-  FinalGroup f = {};
-  f.out = out, f.stride = rows * columns, f.first = -1, f.dtype = dtype, f.turned = t.turned();
-  f.wide = !t.turned() && aligned_to(out, columns, dtype_size(dtype), 32);
-  if (e == cudaSuccess) e = schulz(sets, places, &f, nullptr, 0, steps, s);
+  if (e == cudaSuccess) e = schulz(sets, places, steps, s);
+  std::vector<Finished> results((size_t)batch);
+  for (int64_t z = 0; z < batch; ++z) {
+    const int64_t at = z * t.m() * t.x_pitch();
+    results[z] = {places[0].x[steps & 1][0] + at, places[0].x[steps & 1][1] + at, places[0].terms + z * kTerms,
+                  static_cast<char *>(out) + z * rows * columns * dtype_size(dtype), t.x_pitch(), 1.f, (int)rows,
+                  (int)columns, dtype, t.turned(), 0};
+  }
+  if (e == cudaSuccess) e = finish(results, 0.0, nullptr, 0.0, s);
   return launch_status(e, "orthogonalize");
 }
 
@@ -653,7 +1185,7 @@ std::vector<Sequence> sequences(const cpab_muon_tensor *tensors, int count) {
   std::vector<std::vector<int>> members;
   for (int i = 0; i < count; ++i) {
     const cpab_muon_tensor &t = tensors[i];
-    if (t.rows == 0 || t.columns == 0) continue;
+    if (t.rows == 0 || t.columns == 0 || is_small(t.rows, t.columns)) continue;
     size_t k = 0;
     while (k < shapes.size() && !(shapes[k].rows == t.rows && shapes[k].cols == t.columns && shapes[k].dtype == t.dtype &&
                                   shapes[k].batch < kMatrices))
@@ -716,33 +1248,46 @@ extern "C" int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double
     return report_error(CPAB_ERR_ARG, "%s", "muon: null workspace, or one off 256 bytes");
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
+  auto rate = [&](int64_t rows, int64_t columns) {
+    return (float)(adjust ? 0.2 * std::sqrt((double)std::max(rows, columns))
+                          : std::sqrt(std::max(1.0, (double)rows / (double)columns)));
+  };
+  SmallArgs small = {};
+  small.momentum = (float)momentum, small.lr = (float)lr, small.decay = (float)weight_decay, small.lr_device = lr_device;
+  small.nesterov = nesterov, small.steps = steps, small.eps = eps;
+  small.a = coefficients[0], small.b = coefficients[1], small.c = coefficients[2];
+  for (int i = 0, n = 0; i <= count; ++i) {
+    if (n > 0 && (n == kMatrices || i == count)) {
+      if ((e = launch_small(small, n, n, s)) != cudaSuccess) return launch_status(e, "muon");
+      n = 0;
+    }
+    if (i == count) break;
+    const cpab_muon_tensor &t = tensors[i];
+    if (t.rows > 0 && t.columns > 0 && is_small(t.rows, t.columns))
+      small.m[n++] = {t.grad, t.momentum, t.param, (int)t.rows, (int)t.columns, t.dtype, 1, rate(t.rows, t.columns)};
+  }
   for (const Sequence &q : list) {
     std::vector<Places> places;
     double *partials;
     place(q.sets, (int64_t)q.tensors.size(), static_cast<char *>(workspace), &places, &partials);
     std::vector<Prepared> in;
-    std::vector<FinalGroup> finals(q.sets.size());
-    void *table[kMatrices];
+    std::vector<Finished> out;
     for (size_t g = 0; g < q.sets.size(); ++g) {
       const Set &t = q.sets[g];
-      FinalGroup &f = finals[g];
-      f = {};
-      f.first = (int)in.size(), f.dtype = t.dtype, f.turned = t.turned(), f.update = 1;
-      f.decay = (float)weight_decay, f.lr = (float)lr, f.lr_device = lr_device;
-      f.rate = (float)(adjust ? 0.2 * std::sqrt((double)t.n()) : std::sqrt(std::max(1.0, (double)t.rows / t.cols)));
       for (int z = 0; z < t.batch; ++z) {
         const int k = (int)in.size();
         const cpab_muon_tensor &m = tensors[q.tensors[k]];
+        const Places &w = places[g];
         const int64_t at = z * t.m() * t.x_pitch();
-        table[k] = m.param;
-        if (z == 0) f.wide = !t.turned();
-        f.wide = f.wide && aligned_to(m.param, t.cols, dtype_size(t.dtype), 32);
-        in.push_back({m.grad, m.momentum, places[g].x[0][0] + at, places[g].x[0][1] + at, partials + k * kPartials,
-                      places[g].terms + z * kTerms, t.x_pitch(), t.rows, t.cols, t.dtype, t.turned()});
+        in.push_back({m.grad, m.momentum, w.x[0][0] + at, w.x[0][1] + at, partials + k * kPartials, w.terms + z * kTerms,
+                      t.x_pitch(), t.rows, t.cols, t.dtype, t.turned()});
+        out.push_back({w.x[steps & 1][0] + at, w.x[steps & 1][1] + at, w.terms + z * kTerms, m.param, t.x_pitch(),
+                       rate(t.rows, t.cols), t.rows, t.cols, t.dtype, t.turned(), 1});
       }
     }
     if ((e = prepare(in, (float)momentum, nesterov, steps, coefficients, eps, s)) != cudaSuccess) break;
-    if ((e = schulz(q.sets, places, finals.data(), table, (int)in.size(), steps, s)) != cudaSuccess) break;
+    if ((e = schulz(q.sets, places, steps, s)) != cudaSuccess) break;
+    if ((e = finish(out, lr, lr_device, weight_decay, s)) != cudaSuccess) break;
   }
   return launch_status(e, "muon");
 }

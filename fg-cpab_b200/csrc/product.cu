@@ -377,7 +377,9 @@ struct Product {
     }
     tc::epilogue_sync();
   }
-  __device__ void store(const Tile &t, Shared &sh, int row, int c, const float *acc) const {
+  struct Ahead {};
+  __device__ Ahead ahead(const Tile &, int, int) const { return {}; }
+  __device__ void store(const Tile &t, Shared &sh, int row, int c, const float *acc, const Ahead &) const {
     const int col = t.n0 + c, lane = threadIdx.x & 31;
     if (col >= a.N) return;
     uint4(&rows)[32][5] = sh.rows[(threadIdx.x >> 5) - 4];

@@ -24,8 +24,9 @@
 //                     parts lie kAHalf and kBHalf bytes behind the first
 //   scales_a / _b(tile, rank, row, group, words)  a row's scales of 8 steps, four to a word
 //   begin(tile, shared, thread)     before a tile's accumulators are waited for
-//   store(tile, shared, row, column, values)  kChunk values of this thread's row; the
-//                     warp's rows are 32 in order
+//   Ahead, ahead(tile, row, column)  what store reads besides, asked for a chunk early
+//   store(tile, shared, row, column, values, ahead)  kChunk values of this thread's row;
+//                     the warp's rows are 32 in order
 #pragma once
 
 #include "tensor_core.cuh"
@@ -250,6 +251,7 @@ __device__ __forceinline__ void core(const P &p) {
       const int row = t.m0 + (int)rank * 128 + quarter * 32 + lane;
       const int segments = P::kSegment > 0 ? (t.steps + kLength - 1) / kLength : 1;
       float v[kHold];
+      typename P::Ahead now = p.ahead(t, row, half * kHalf);
       for (int g = 0; g < segments; ++g) {
         ok = ok && bar_wait(afull + 8 * acc, aphase);
         ok = __all_sync(~0u, ok);
@@ -260,7 +262,12 @@ __device__ __forceinline__ void core(const P &p) {
           for (int c = 0; c < kHalf; c += kHold) {
             read_accumulators(ok, d + c, v);
 #pragma unroll
-            for (int j = 0; j < kHold; j += P::kChunk) p.store(t, *shared, row, half * kHalf + c + j, v + j);
+            for (int j = 0; j < kHold; j += P::kChunk) {
+              const int column = half * kHalf + c + j;
+              const typename P::Ahead next = p.ahead(t, row, c + j + P::kChunk < kHalf ? column + P::kChunk : column);
+              p.store(t, *shared, row, column, v + j, now);
+              now = next;
+            }
           }
         } else if (P::kSegment == 0 || g == 0) {
           read_accumulators(ok, d, v);
@@ -283,7 +290,11 @@ __device__ __forceinline__ void core(const P &p) {
       }
       if constexpr (kHold == kHalf) {
 #pragma unroll
-        for (int c = 0; c < kHalf; c += P::kChunk) p.store(t, *shared, row, half * kHalf + c, v + c);
+        for (int c = 0; c < kHalf; c += P::kChunk) {
+          const typename P::Ahead next = p.ahead(t, row, half * kHalf + (c + P::kChunk < kHalf ? c + P::kChunk : c));
+          p.store(t, *shared, row, half * kHalf + c, v + c, now);
+          now = next;
+        }
       }
     }
     if (!ok) *gave_up = 1;

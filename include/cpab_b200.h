@@ -536,8 +536,8 @@ int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, const cpab_qu
  * for each of `batch` contiguous matrices [rows, columns] of dtype; out is shaped
  * as x and may be x.  Matrices of 16 bits are multiplied as halves, float32 ones as
  * pairs of halves (22 bits).  coefficients must keep the singular values and the
- * products' within 60.  workspace: cpab_b200_orthogonalize_workspace bytes, 256-byte
- * aligned.
+ * products' within 60.  workspace: cpab_b200_orthogonalize_workspace bytes (0 for
+ * small matrices), 256-byte aligned.
  */
 int64_t cpab_b200_orthogonalize_workspace(int dtype, int64_t batch, int64_t rows, int64_t columns);
 int cpab_b200_orthogonalize(int dtype, const void *x, int64_t batch, int64_t rows, int64_t columns,

@@ -77,7 +77,7 @@ COEFFICIENTS = (ctypes.c_double * 3)(3.4445, -4.775, 2.0315)
 def test_orthogonalize_entry_point_validates():
     L = _native.lib()
     # dtype, x, batch, rows, columns, steps, coefficients, eps, out, workspace, stream
-    ok = [2, P, 1, 8, 8, 5, COEFFICIENTS, 1e-7, P, P, None]
+    ok = [2, P, 1, 300, 400, 5, COEFFICIENTS, 1e-7, P, P, None]
     f = L.cpab_b200_orthogonalize
     assert call(f, ok, a0=-1) == -1 and "type" in err()
     assert call(f, ok, a2=-1) == -1 and call(f, ok, a6=None) == -1
@@ -89,7 +89,7 @@ def test_orthogonalize_entry_point_validates():
     assert call(f, ok, a1=None) == -1 and call(f, ok, a8=None) == -1 and call(f, ok, a9=OFF) == -1
     assert call(f, ok, a2=0) == 0 and call(f, ok, a4=0) == 0 and err() == ""
     w = L.cpab_b200_orthogonalize_workspace
-    assert w(2, 1, 8, 8) > 0 and w(7, 1, 8, 8) == 0 and w(2, 0, 8, 8) == 0 and w(2, 1, 8, (1 << 20) + 1) == 0
+    assert w(2, 1, 300, 400) > 0 and w(2, 1, 130, 260) > 0 and w(2, 1, 64, 260) == 0 and w(7, 1, 8, 8) == 0 and w(2, 0, 8, 8) == 0 and w(2, 1, 8, (1 << 20) + 1) == 0
 
 
 def test_muon_entry_point_validates():
@@ -97,7 +97,7 @@ def test_muon_entry_point_validates():
     t = (_native._MuonTensor * 1)()
 
     def one(count=1, coefficients=COEFFICIENTS, steps=5, eps=1e-7, adjust=0, work=P, **kw):
-        base = dict(param=4096, grad=4096, momentum=4096, rows=4, columns=6, dtype=0)
+        base = dict(param=4096, grad=4096, momentum=4096, rows=300, columns=400, dtype=0)
         for k, v in {**base, **kw}.items():
             setattr(t[0], k, v)
         return L.cpab_b200_muon(ctypes.byref(t), count, 0.1, None, 0.9, 1, 0.1, steps, coefficients, eps, adjust, work,
