@@ -387,6 +387,12 @@ struct Schulz {
     }
     return t;
   }
+  __device__ void warm(const Tile &t) const {
+    const PhaseGroup &q = p.g[t.g];
+    if (threadIdx.x < PARTS) tc::prefetch_map(&q.a[threadIdx.x]), tc::prefetch_map(&q.b[threadIdx.x]);
+    tc::touch(q.read[0]), tc::touch(q.read[1]), tc::touch(q.write[0]), tc::touch(q.write[1]), tc::touch(q.terms);
+    tc::touch(q.read_plane), tc::touch(q.write_plane), tc::touch(q.write_lo), tc::touch(p.step);
+  }
   __device__ void load(const Tile &t, int k, uint32_t sa, uint32_t sb, uint32_t bar, uint32_t rank) const {
     const PhaseGroup &q = p.g[t.g];
     const int at = k * 64, n = t.n0 + rank * (BN / CTAS);
@@ -408,11 +414,16 @@ struct Schulz {
   // not one ahead, their latency alone was half of an update's time.)
   struct Ahead {
     uint32_t hi[PHASE == kGram ? 1 : kChunk / 2], lo[PHASE == kGram ? 1 : kChunk / 2];
+    float mine, product;  // coefficients of it and of the product
   };
   __device__ Ahead ahead(const Tile &t, int row, int c) const {
-    Ahead w;
+    Ahead w = {};
+    w.product = 1.f / kUnit;
     if constexpr (PHASE != kGram) {
       const PhaseGroup &q = p.g[t.g];
+      const float *terms = q.terms + t.z * kTerms + 3 * p.step;
+      w.mine = terms[PHASE == kSquare ? 1 : 0];
+      if (PHASE == kSquare) w.product *= terms[2];
       const int col = t.n0 + c;
       const int64_t at = t.z * q.read_plane + row * q.read_pitch + col;
 #pragma unroll
@@ -430,12 +441,6 @@ struct Schulz {
   }
   __device__ void store(const Tile &t, const Shared &, int row, int c, const float *acc, const Ahead &w) const {
     const PhaseGroup &q = p.g[t.g];
-    float mine = 0.f, product = 1.f / kUnit;
-    if constexpr (PHASE != kGram) {
-      const float *terms = q.terms + t.z * kTerms + 3 * p.step;
-      mine = terms[PHASE == kSquare ? 1 : 0];
-      if (PHASE == kSquare) product *= terms[2];
-    }
     __half *hi = q.write[0] + t.z * q.write_plane, *lo = q.write[1] + t.z * q.write_plane;
     const int odd = threadIdx.x & 1;
 #pragma unroll
@@ -445,10 +450,10 @@ struct Schulz {
       uint32_t h[8], l[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        float a = acc[k + 2 * j] * product, b = acc[k + 2 * j + 1] * product;
+        float a = acc[k + 2 * j] * w.product, b = acc[k + 2 * j + 1] * w.product;
         if constexpr (PHASE != kGram) {
           const float2 x = unpack_pair<__half>(w.hi[k / 2 + j]), y = unpack_pair<__half>(w.lo[k / 2 + j]);
-          a = fmaf(mine, x.x + y.x, a), b = fmaf(mine, x.y + y.y, b);
+          a = fmaf(w.mine, x.x + y.x, a), b = fmaf(w.mine, x.y + y.y, b);
         }
         h[j] = pack_pair<__half>(a, b);
         const float2 x = unpack_pair<__half>(h[j]);
@@ -1180,12 +1185,27 @@ struct Sequence {
   std::vector<int> tensors;
 };
 
+// Whether a tensor's step is taken by the kernel for small matrices: not where others
+// go through the products as pairs of halves anyway, whose launches it joins.
+struct Split {
+  bool joined = false;
+  Split(const cpab_muon_tensor *tensors, int count) {
+    for (int i = 0; i < count && !joined; ++i) {
+      const cpab_muon_tensor &t = tensors[i];
+      joined = t.rows > 0 && t.columns > 0 && !is_small(t.rows, t.columns) &&
+               Set{(int)t.rows, (int)t.columns, t.dtype, 1}.parts() == 2;
+    }
+  }
+  bool small(const cpab_muon_tensor &t) const { return !joined && is_small(t.rows, t.columns); }
+};
+
 std::vector<Sequence> sequences(const cpab_muon_tensor *tensors, int count) {
+  const Split split(tensors, count);
   std::vector<Set> shapes;
   std::vector<std::vector<int>> members;
   for (int i = 0; i < count; ++i) {
     const cpab_muon_tensor &t = tensors[i];
-    if (t.rows == 0 || t.columns == 0 || is_small(t.rows, t.columns)) continue;
+    if (t.rows == 0 || t.columns == 0 || split.small(t)) continue;
     size_t k = 0;
     while (k < shapes.size() && !(shapes[k].rows == t.rows && shapes[k].cols == t.columns && shapes[k].dtype == t.dtype &&
                                   shapes[k].batch < kMatrices))
@@ -1252,6 +1272,7 @@ extern "C" int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double
     return (float)(adjust ? 0.2 * std::sqrt((double)std::max(rows, columns))
                           : std::sqrt(std::max(1.0, (double)rows / (double)columns)));
   };
+  const Split split(tensors, count);
   SmallArgs small = {};
   small.momentum = (float)momentum, small.lr = (float)lr, small.decay = (float)weight_decay, small.lr_device = lr_device;
   small.nesterov = nesterov, small.steps = steps, small.eps = eps;
@@ -1263,7 +1284,7 @@ extern "C" int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double
     }
     if (i == count) break;
     const cpab_muon_tensor &t = tensors[i];
-    if (t.rows > 0 && t.columns > 0 && is_small(t.rows, t.columns))
+    if (t.rows > 0 && t.columns > 0 && split.small(t))
       small.m[n++] = {t.grad, t.momentum, t.param, (int)t.rows, (int)t.columns, t.dtype, 1, rate(t.rows, t.columns)};
   }
   for (const Sequence &q : list) {

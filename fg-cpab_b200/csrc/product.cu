@@ -357,6 +357,10 @@ struct Product {
     const int in = i - band * 8 * a.tiles_n;
     return {(top + in % high) * 128 * CTAS, in / high * BN, a.steps, (i / (int)(gridDim.x / CTAS)) & 1};
   }
+  __device__ void warm(const Tile &) const {
+    if (threadIdx.x == 0) tc::prefetch_map(&a.a), tc::prefetch_map(&a.b);
+    tc::touch(a.sa.bytes), tc::touch(a.sb.bytes), tc::touch(a.y), tc::touch(a.bias), tc::touch(a.wide);
+  }
   __device__ void load(const Tile &t, int k, uint32_t sa, uint32_t sb, uint32_t bar, uint32_t rank) const {
     tc::tile_load<CTAS>(sa, &a.a, bar, k * 128, t.m0 + rank * 128, 0);
     tc::tile_load<CTAS>(sb, &a.b, bar, k * 128, t.n0 + rank * (BN / CTAS), 0);

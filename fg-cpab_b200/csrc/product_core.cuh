@@ -20,6 +20,7 @@
 //   Shared            what its epilogue keeps in shared memory
 //   int tiles()                     tiles of this launch
 //   Tile tile(int i)                {m0, n0, steps, ...}
+//   warm(tile)                      touches its arguments
 //   load(tile, step, a, b, bar, rank)    issues the copies of one stage; the second
 //                     parts lie kAHalf and kBHalf bytes behind the first
 //   scales_a / _b(tile, rank, row, group, words)  a row's scales of 8 steps, four to a word
@@ -118,9 +119,12 @@ __device__ __forceinline__ void core(const P &p) {
   fence_after();
   const uint32_t tmem = __shfl_sync(~0u, *reinterpret_cast<volatile uint32_t *>(&bars->tmem), 0);
   volatile int *gave_up = &bars->gave_up;
+  const int tiles = p.tiles(), first = blockIdx.x / C, stride = gridDim.x / C;
+  // What the launch itself brings (arguments, tensor maps) is fetched while the
+  // kernel before still runs.
+  p.warm(p.tile(first));
   dep_wait();
 
-  const int tiles = p.tiles(), first = blockIdx.x / C, stride = gridDim.x / C;
   // The pair's shared barriers are the first block's.
   const uint32_t full0 = C == 2 ? mapa(full, 0) : full;
 

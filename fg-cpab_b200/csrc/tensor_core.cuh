@@ -117,6 +117,13 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
+// Keeps a load whose value nothing needs.
+template <typename T>
+__device__ __forceinline__ void touch(const T &v) {
+  if constexpr (sizeof(T) == 8) asm volatile("" ::"l"(v));
+  else asm volatile("" ::"r"(v));
+}
+
 // ---- tensor memory -------------------------------------------------------------
 
 // (one whole warp; with CTAS == 2 one of each block of the pair)
