@@ -472,6 +472,182 @@ cudaError_t launch_product(ProductArgs &a, cudaStream_t s) {
   }
 }
 
+// ---- few rows ----------------------------------------------------------------------
+//
+// A product of at most 16 rows is a pass over the weight: its codes go from memory to
+// the registers of the warp that multiplies them (as halves, which hold them exactly),
+// without a tile of 128 rows that would be empty.  A warp takes 16 of the weight's rows
+// and an eighth of the sum, in blocks of 128; a block's eight warps are added in order.
+// Any order of the summed index will do as long as both operands have it: a lane's 16
+// neighbouring codes of a row are its share of four instructions.
+// One row by 4096 x 2048: 4.3 us, by tiles 7.9; by 8192 x 8192 25.9 and 20.3.
+
+constexpr int kFewMost = 16;
+constexpr int kFewWarps = 8;
+
+struct FewArgs {
+  const uint8_t *x, *w;
+  int64_t x_row, w_row;
+  Scales sx, sw;
+  const float *rx, *rw;  // float32 scales of rows, or null
+  const void *bias;
+  void *y;
+  int64_t y_row;
+  int M, N, K, blocks;
+};
+
+// 16 codes of a row from k on; 0 past its end.
+__device__ __forceinline__ uint4 sixteen(const uint8_t *row, int k, int K) {
+  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4 *>(row + k));
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (k + i < K) w[i >> 2] |= (uint32_t)__ldg(row + k + i) << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Two codes (the low or high half of a word) as halves.
+__device__ __forceinline__ uint32_t two_halves(uint32_t w, bool high) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(high ? w >> 16 : w & 0xFFFFu), __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+// The scale of an e8m0 byte (255: NaN; 2^-127 is subnormal).
+__device__ __forceinline__ float power(uint32_t e) {
+  return __uint_as_float(e == 255u ? 0x7FC00000u : e == 0u ? 0x00400000u : e << 23);
+}
+__device__ __forceinline__ float scale_of(const Scales &s, int64_t row, int block) {
+  return s.bytes == nullptr ? 1.f : power(__ldg(s.bytes + row * s.row + block));
+}
+
+template <typename T, typename TB, int TILES>
+__global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_constant__ FewArgs a) {
+  extern __shared__ __align__(16) uint8_t few_smem[];  // x as halves, [M, pitch]
+  __shared__ float part[kFewWarps][16][8 * TILES + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16, pitch = a.blocks * 128 + 8;
+  // (rows past the end are others' again, and not stored)
+  const int r0 = min(n0 + g, a.N - 1), r1 = min(n0 + g + 8, a.N - 1);
+  const uint8_t *w0 = a.w + r0 * a.w_row, *w1 = a.w + r1 * a.w_row;
+  const uint4 *x[TILES];
+#pragma unroll
+  for (int i = 0; i < TILES; ++i)
+    x[i] = reinterpret_cast<const uint4 *>(few_smem + (min(8 * i + g, a.M - 1) * pitch + 16 * t) * 2);
+  tc::dep_launch();
+  tc::dep_wait();
+  float sum[TILES][4] = {};
+  struct Block {
+    uint4 p[2], q[2];
+    uint32_t s0, s1;
+  };
+  auto fetch = [&](int b, Block &f) {
+    if (b * 128 + 128 <= a.K) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = b * 128 + 64 * h + 16 * t;
+        f.p[h] = __ldg(reinterpret_cast<const uint4 *>(w0 + k)), f.q[h] = __ldg(reinterpret_cast<const uint4 *>(w1 + k));
+      }
+    } else if (b < a.blocks) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = b * 128 + 64 * h + 16 * t;
+        f.p[h] = sixteen(w0, k, a.K), f.q[h] = sixteen(w1, k, a.K);
+      }
+    }
+    f.s0 = f.s1 = 127u;
+    if (a.sw.bytes != nullptr && b < a.blocks)
+      f.s0 = __ldg(a.sw.bytes + r0 * a.sw.row + b), f.s1 = __ldg(a.sw.bytes + r1 * a.sw.row + b);
+  };
+  auto multiply = [&](int b, const Block &f) {
+    const float s0 = power(f.s0), s1 = power(f.s1);
+    float acc[TILES][4] = {};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint4 u[TILES][2];
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) u[i][0] = x[i][b * 16 + 8 * h], u[i][1] = x[i][b * 16 + 8 * h + 1];
+      const uint32_t pw[4] = {f.p[h].x, f.p[h].y, f.p[h].z, f.p[h].w}, qw[4] = {f.q[h].x, f.q[h].y, f.q[h].z, f.q[h].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t m[4] = {two_halves(pw[k], false), two_halves(qw[k], false), two_halves(pw[k], true),
+                               two_halves(qw[k], true)};
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+          const uint4 &c = u[i][k >> 1];
+          const uint32_t c0 = k & 1 ? c.z : c.x, c1 = k & 1 ? c.w : c.y;
+          asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+              "{%8, %9}, {%0, %1, %2, %3};"
+              : "+f"(acc[i][0]), "+f"(acc[i][1]), "+f"(acc[i][2]), "+f"(acc[i][3])
+              : "r"(m[0]), "r"(m[1]), "r"(m[2]), "r"(m[3]), "r"(c0), "r"(c1));
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) {
+      const int c0 = min(8 * i + 2 * t, a.M - 1), c1 = min(8 * i + 2 * t + 1, a.M - 1);
+      const float x0 = scale_of(a.sx, c0, b), x1 = scale_of(a.sx, c1, b);
+      sum[i][0] = fmaf(acc[i][0] * s0, x0, sum[i][0]), sum[i][1] = fmaf(acc[i][1] * s0, x1, sum[i][1]);
+      sum[i][2] = fmaf(acc[i][2] * s1, x0, sum[i][2]), sum[i][3] = fmaf(acc[i][3] * s1, x1, sum[i][3]);
+    }
+  };
+  // Three blocks in flight.
+  const int per = (a.blocks + kFewWarps - 1) / kFewWarps, end = min(a.blocks, (warp + 1) * per);
+  int b = warp * per;
+  Block f0, f1, f2;
+  fetch(b, f0), fetch(b + 1, f1);
+  for (int i = threadIdx.x; i < a.M * a.blocks * 8; i += 32 * kFewWarps) {
+    const int row = i / (a.blocks * 8), k = i % (a.blocks * 8) * 16;
+    const uint4 c = sixteen(a.x + row * a.x_row, k, a.K);
+    uint4 *to = reinterpret_cast<uint4 *>(few_smem + (row * pitch + k) * 2);
+    to[0] = make_uint4(two_halves(c.x, false), two_halves(c.x, true), two_halves(c.y, false), two_halves(c.y, true));
+    to[1] = make_uint4(two_halves(c.z, false), two_halves(c.z, true), two_halves(c.w, false), two_halves(c.w, true));
+  }
+  __syncthreads();
+  for (; b < end; b += 3) {
+    fetch(b + 2, f2);
+    multiply(b, f0);
+    if (b + 1 >= end) break;
+    fetch(b + 3, f0);
+    multiply(b + 1, f1);
+    if (b + 2 >= end) break;
+    fetch(b + 4, f1);
+    multiply(b + 2, f2);
+  }
+#pragma unroll
+  for (int i = 0; i < TILES; ++i) {
+    part[warp][g][8 * i + 2 * t] = sum[i][0], part[warp][g][8 * i + 2 * t + 1] = sum[i][1];
+    part[warp][g + 8][8 * i + 2 * t] = sum[i][2], part[warp][g + 8][8 * i + 2 * t + 1] = sum[i][3];
+  }
+  __syncthreads();
+  const int r = threadIdx.x & 15, m = threadIdx.x >> 4;
+  if (m >= 8 * TILES || m >= a.M || n0 + r >= a.N) return;
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < kFewWarps; ++k) v += part[k][r][m];
+  if (a.rx != nullptr) v *= a.rx[m];
+  if (a.rw != nullptr) v *= a.rw[n0 + r];
+  if (a.bias != nullptr) v += to_f32(static_cast<const TB *>(a.bias)[n0 + r]);
+  static_cast<T *>(a.y)[m * a.y_row + n0 + r] = from_f32<T>(v);
+}
+
+// Bytes of x as halves; few rows whose x takes more are left to the tiles, and so are
+// large weights, whose codes this kernel's conversions are too many for (16 rows by
+// 4096 x 2048: 7.4 and 7.9 us).
+int64_t few_bytes(int64_t M, int64_t K) { return M * ((K + kBlock - 1) / kBlock * 128 + 8) * 2; }
+bool is_few(int64_t M, int64_t N, int64_t K) {
+  return M <= kFewMost && few_bytes(M, K) <= 72 * 1024 && N * K <= int64_t(1) << (M <= 8 ? 25 : 24);
+}
+
+template <typename T, typename TB, int TILES>
+cudaError_t launch_few_as(const FewArgs &a, cudaStream_t s) {
+  auto *kernel = k_few_rows<T, TB, TILES>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);
+  if (e != cudaSuccess) return e;
+  return tc::launch(kernel, (unsigned)((a.N + 15) / 16), 32 * kFewWarps, (size_t)few_bytes(a.M, a.K), 1, s, a);
+}
+template <typename T, typename TB>
+cudaError_t launch_few(const FewArgs &a, cudaStream_t s) {
+  return a.M <= 8 ? launch_few_as<T, TB, 1>(a, s) : launch_few_as<T, TB, 2>(a, s);
+}
+
 // What an operand lacks, or null; fills its scales.
 const char *operand(const cpab_quantized &o, int64_t K, Scales *blocks, const float **per_row) {
   if (o.codes == nullptr || o.scale == nullptr) return "null codes or scales";
@@ -559,7 +735,7 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   ProductArgs a = {};
   const char *why = operand(*x, K, &a.sa, &a.ra);
   if (why == nullptr) why = operand(*weight, K, &a.sb, &a.rb);
-  if (why == nullptr) {
+  if (why == nullptr && !is_few(M, N, K)) {
     const int columns = tile_of(M, N, (K + kBlock - 1) / kBlock) == 0 ? 64 : 128;  // of B a block loads
     if (!make_tile_map(&a.a, false, x->codes, K, M, 1, x->row, x->row * M, 128) ||
         !make_tile_map(&a.b, false, weight->codes, K, N, 1, weight->row, weight->row * N, columns))
@@ -570,6 +746,15 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   a.wide = aligned_to(y, y_row, dtype_size(dtype), 16);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
+  if (is_few(M, N, K)) {
+    const FewArgs f = {x->codes, weight->codes, x->row, weight->row, a.sa, a.sb, a.ra, a.rb, bias, y, y_row,
+                       (int)M, (int)N, (int)K, a.steps};
+    if (dtype == CPAB_F32) e = launch_few<float, float>(f, s);
+    else if (dtype == CPAB_F16) e = bias_dtype == CPAB_F32 ? launch_few<__half, float>(f, s) : launch_few<__half, __half>(f, s);
+    else e = bias_dtype == CPAB_F32 ? launch_few<__nv_bfloat16, float>(f, s)
+                                    : launch_few<__nv_bfloat16, __nv_bfloat16>(f, s);
+    return launch_status(e, "matmul_quantized");
+  }
   if (dtype == CPAB_F32) e = launch_product<float, float>(a, s);
   else if (dtype == CPAB_F16)
     e = bias_dtype == CPAB_F32 ? launch_product<__half, float>(a, s) : launch_product<__half, __half>(a, s);

@@ -43,30 +43,59 @@ void check_quantize(const Tensor &x) {
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x must be [..., K] with K > 0, got ", x.sizes());
 }
 
-// Codes of x's rows, of its transpose, and the sums of its columns, as asked for.
-struct Quantized {
-  Codes rows, turned;
-  Tensor sums;
+// Codes as the library takes them: a place in somebody's memory.
+struct Place {
+  uint8_t *q = nullptr, *scale = nullptr;
+  int64_t q_row = 0, scale_row = 0;
+};
+Place place_of(const Codes &c) {
+  return {static_cast<uint8_t *>(ptr_mut(c.q)), static_cast<uint8_t *>(ptr_mut(c.scale)), c.q_row, c.scale_row};
+}
+
+// Codes of several matrices in one tensor of bytes.
+class Slab {
+ public:
+  // A place for R rows of K codes, from a multiple of 256 bytes; filled in by allocate().
+  size_t add(int64_t R, int64_t K) {
+    Place p;
+    p.q_row = round_to(K, 16), p.scale_row = round_to((K + 127) / 128, 4);
+    starts_.push_back({bytes_, bytes_ + round_to(R * p.q_row, 256)});
+    places_.push_back(p);
+    bytes_ = starts_.back().second + round_to(R * p.scale_row, 256);
+    return places_.size() - 1;
+  }
+  void allocate(const Tensor &like) { place(at::empty({bytes_}, like.options().dtype(at::kByte))); }
+  void place(const Tensor &bytes) {
+    memory = bytes;
+    auto *base = static_cast<uint8_t *>(ptr_mut(memory));
+    for (size_t i = 0; i < places_.size(); ++i)
+      places_[i].q = base + starts_[i].first, places_[i].scale = base + starts_[i].second;
+  }
+  const Place &operator[](size_t i) const { return places_[i]; }
+  Tensor memory;
+
+ private:
+  std::vector<Place> places_;
+  std::vector<std::pair<int64_t, int64_t>> starts_;
+  int64_t bytes_ = 0;
 };
 
-Quantized quantize(const Tensor &x, bool rows, bool turned, const at::ScalarType *sum_type) {
-  Quantized o;
+// x's codes by rows and of its transpose (null: not wanted), and the sums of its columns.
+Tensor quantize(const Tensor &x, const Place *rows, const Place *turned, const at::ScalarType *sum_type) {
   const Tensor xr = rows_of(x);
   const int64_t R = xr.size(0), K = xr.size(1);
-  if (rows) o.rows = new_codes(x.sizes().slice(0, x.dim() - 1), K, x);
-  if (turned) o.turned = new_codes({K}, R, x);
+  Tensor sums;
   Tensor work;
   if (sum_type != nullptr) {
-    o.sums = at::empty({K}, x.options().dtype(*sum_type));
+    sums = at::empty({K}, x.options().dtype(*sum_type));
     work = at::empty({cpab_b200_quantize_blocks_workspace(R, K)}, x.options().dtype(at::kFloat));
   }
-  auto bytes = [](const Tensor &t) { return static_cast<uint8_t *>(ptr_mut(t)); };
-  check(cpab_b200_quantize_blocks(dtype_of(x, "x"), ptr(xr), xr.stride(0), R, K, bytes(o.rows.q), o.rows.q_row,
-                                  bytes(o.rows.scale), o.rows.scale_row, bytes(o.turned.q), o.turned.q_row,
-                                  bytes(o.turned.scale), o.turned.scale_row,
-                                  o.sums.defined() ? dtype_of(o.sums, "bias") : CPAB_F32, ptr_mut(o.sums),
-                                  fptr_mut(work), stream_of(x)));
-  return o;
+  const Place none;
+  const Place &r = rows != nullptr ? *rows : none, &t = turned != nullptr ? *turned : none;
+  check(cpab_b200_quantize_blocks(dtype_of(x, "x"), ptr(xr), xr.stride(0), R, K, r.q, r.q_row, r.scale, r.scale_row, t.q,
+                                  t.q_row, t.scale, t.scale_row, sums.defined() ? dtype_of(sums, "bias") : CPAB_F32,
+                                  ptr_mut(sums), fptr_mut(work), stream_of(x)));
+  return sums;
 }
 
 std::vector<Tensor> quantize_blocks(const Tensor &x, bool transposed) {
@@ -74,9 +103,16 @@ std::vector<Tensor> quantize_blocks(const Tensor &x, bool transposed) {
   TORCH_CHECK(!has_tangent({&x}), "quantize_blocks has no gradient, of forward mode neither");
   TORCH_CHECK_VALUE(!transposed || x.dim() == 2, "x must be [R, K] for its transpose, got ", x.sizes());
   const c10::cuda::CUDAGuard guard(x.device());
-  const Quantized o = quantize(x, true, transposed, nullptr);
-  if (transposed) return {o.rows.q, o.rows.scale, o.turned.q, o.turned.scale};
-  return {o.rows.q, o.rows.scale};
+  const Codes rows = new_codes(x.sizes().slice(0, x.dim() - 1), x.size(-1), x);
+  const Place r = place_of(rows);
+  if (!transposed) {
+    quantize(x, &r, nullptr, nullptr);
+    return {rows.q, rows.scale};
+  }
+  const Codes turned = new_codes({x.size(1)}, x.size(0), x);
+  const Place t = place_of(turned);
+  quantize(x, &r, &t, nullptr);
+  return {rows.q, rows.scale, turned.q, turned.scale};
 }
 
 // ---- products --------------------------------------------------------------------
@@ -123,10 +159,10 @@ Operand operand(const Tensor &q, const Tensor &scale, const char *name) {
   return o;
 }
 
-Operand operand(const Codes &c, int64_t rows, int64_t K) {
+Operand operand(const Place &p, int64_t rows, int64_t K) {
   Operand o;
   o.rows = rows, o.K = K;
-  o.c = {static_cast<const uint8_t *>(ptr(c.q)), c.q_row, ptr(c.scale), c.scale_row};
+  o.c = {p.q, p.q_row, p.scale, p.scale_row};
   return o;
 }
 
@@ -180,13 +216,29 @@ void check_linear(const Tensor &x, const Tensor &weight, const Tensor &bias) {
   }
 }
 
-Tensor linear_forward(const Tensor &x, const Tensor &weight, const Tensor &bias, bool keep_x, bool keep_w,
-                      Codes *turned_x, Codes *turned_w) {
-  const Quantized q = quantize(x, true, keep_x, nullptr), w = quantize(weight, true, keep_w, nullptr);
-  *turned_x = q.turned, *turned_w = w.turned;
-  const int64_t K = x.size(-1);
-  return product(operand(q.rows, x.numel() / K, K), operand(w.rows, weight.size(0), K),
-                 bias.defined() ? bias.contiguous() : bias, x.sizes().slice(0, x.dim() - 1), x.scalar_type(), x);
+// What the backward keeps, in one tensor: the codes of x's transpose (for the
+// weight's gradient) and of the weight's (for x's).
+struct Kept {
+  Slab slab;
+  size_t x = 0, w = 0;
+  Kept(int64_t M, int64_t N, int64_t K, bool keep_x, bool keep_w) {
+    if (keep_x) x = slab.add(K, M);
+    if (keep_w) w = slab.add(K, N);
+  }
+};
+
+Tensor linear_forward(const Tensor &x, const Tensor &weight, const Tensor &bias, bool keep_x, bool keep_w, Tensor *kept) {
+  const int64_t K = x.size(-1), N = weight.size(0), M = x.numel() / K;
+  Slab s;
+  const size_t xq = s.add(M, K), wq = s.add(N, K);
+  s.allocate(x);
+  Kept k(M, N, K, keep_x, keep_w);
+  if (keep_x || keep_w) k.slab.allocate(x);
+  *kept = k.slab.memory;
+  quantize(x, &s[xq], keep_x ? &k.slab[k.x] : nullptr, nullptr);
+  quantize(weight, &s[wq], keep_w ? &k.slab[k.w] : nullptr, nullptr);
+  return product(operand(s[xq], M, K), operand(s[wq], N, K), bias.defined() ? bias.contiguous() : bias,
+                 x.sizes().slice(0, x.dim() - 1), x.scalar_type(), x);
 }
 
 class LinearFunction : public torch::autograd::Function<LinearFunction> {
@@ -195,15 +247,12 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
     const Tensor bias = given(bias_);
     const c10::cuda::CUDAGuard guard(x.device());
     const bool want_x = x.requires_grad(), want_w = weight.requires_grad();
-    Codes xt, wt;
-    const Tensor y = linear_forward(x, weight, bias, want_w, want_x, &xt, &wt);
-    ctx->save_for_backward({xt.q, xt.scale, wt.q, wt.scale});
-    ctx->saved_data["want_x"] = want_x, ctx->saved_data["want_w"] = want_w;
-    ctx->saved_data["want_b"] = bias.defined() && bias.requires_grad();
-    ctx->saved_data["x_type"] = (int64_t)x.scalar_type();
-    ctx->saved_data["w_type"] = (int64_t)weight.scalar_type();
-    ctx->saved_data["b_type"] = (int64_t)(bias.defined() ? bias.scalar_type() : at::kFloat);
-    ctx->saved_data["K"] = x.size(-1);
+    Tensor kept;
+    const Tensor y = linear_forward(x, weight, bias, want_w, want_x, &kept);
+    ctx->save_for_backward({kept});
+    ctx->saved_data["facts"] = std::vector<int64_t>{
+        want_x, want_w, bias.defined() && bias.requires_grad(), (int64_t)x.scalar_type(), (int64_t)weight.scalar_type(),
+        (int64_t)(bias.defined() ? bias.scalar_type() : at::kFloat), x.size(-1)};
     return y;
   }
 
@@ -211,34 +260,34 @@ class LinearFunction : public torch::autograd::Function<LinearFunction> {
     once("linear_quantized");
     const Tensor &dy = grads[0];
     if (!dy.defined()) return {Tensor(), Tensor(), Tensor()};
-    const auto saved = ctx->get_saved_variables();
-    const bool want_x = ctx->saved_data["want_x"].toBool(), want_w = ctx->saved_data["want_w"].toBool();
-    const bool want_b = ctx->saved_data["want_b"].toBool();
-    auto type = [&](const char *k) { return static_cast<at::ScalarType>(ctx->saved_data[k].toInt()); };
-    const at::ScalarType b_type = type("b_type");
-    const int64_t K = ctx->saved_data["K"].toInt(), N = dy.size(-1), M = dy.numel() / std::max<int64_t>(N, 1);
+    const auto facts = ctx->saved_data["facts"].toIntVector();
+    const bool want_x = facts[0], want_w = facts[1], want_b = facts[2];
+    const auto x_type = (at::ScalarType)facts[3], w_type = (at::ScalarType)facts[4], b_type = (at::ScalarType)facts[5];
+    const int64_t K = facts[6], N = dy.size(-1), M = N > 0 ? dy.numel() / N : 0;
     const c10::cuda::CUDAGuard guard(dy.device());
     if (N == 0) {
       std::vector<int64_t> shape(dy.sizes().begin(), dy.sizes().end());
       shape.back() = K;
       return {want_x ? at::zeros(shape, dy.options()) : Tensor(),
-              want_w ? at::zeros({0, K}, dy.options().dtype(type("w_type"))) : Tensor(),
+              want_w ? at::zeros({0, K}, dy.options().dtype(w_type)) : Tensor(),
               want_b ? at::zeros({0}, dy.options().dtype(b_type)) : Tensor()};
     }
-    const Quantized q = quantize(dy, want_x, want_w, want_b ? &b_type : nullptr);
-    auto kept = [&](int i, int64_t codes) {
-      Codes c;
-      c.q = saved[i], c.scale = saved[i + 1], c.q_row = round_to(codes, 16), c.scale_row = round_to((codes + 127) / 128, 4);
-      return c;
-    };
+    Kept kept(M, N, K, want_w, want_x);
+    if (want_x || want_w) kept.slab.place(ctx->get_saved_variables()[0]);
+    Slab s;
+    size_t rows = 0, turned = 0;
+    if (want_x) rows = s.add(M, N);
+    if (want_w) turned = s.add(N, M);
+    if (want_x || want_w) s.allocate(dy);
+    const Tensor db = quantize(dy, want_x ? &s[rows] : nullptr, want_w ? &s[turned] : nullptr, want_b ? &b_type : nullptr);
     Tensor dx, dw;
     if (want_x)
-      dx = product(operand(q.rows, M, N), operand(kept(2, N), K, N), Tensor(), dy.sizes().slice(0, dy.dim() - 1),
-                   type("x_type"), dy);
+      dx = product(operand(s[rows], M, N), operand(kept.slab[kept.w], K, N), Tensor(), dy.sizes().slice(0, dy.dim() - 1),
+                   x_type, dy);
     if (want_w)
-      dw = M == 0 ? at::zeros({N, K}, dy.options().dtype(type("w_type")))
-                  : product(operand(q.turned, N, M), operand(kept(0, M), K, M), Tensor(), {N}, type("w_type"), dy);
-    return {dx, dw, q.sums};
+      dw = M == 0 ? at::zeros({N, K}, dy.options().dtype(w_type))
+                  : product(operand(s[turned], N, M), operand(kept.slab[kept.x], K, M), Tensor(), {N}, w_type, dy);
+    return {dx, dw, db};
   }
 };
 
@@ -247,8 +296,8 @@ Tensor linear_quantized(const Tensor &x, const Tensor &weight, const MaybeTensor
   check_linear(x, weight, bias);
   if (needs_grad({&x, &weight, &bias})) return LinearFunction::apply(x, weight, bias_);
   const c10::cuda::CUDAGuard guard(x.device());
-  Codes xt, wt;
-  return linear_forward(x, weight, bias, false, false, &xt, &wt);
+  Tensor kept;
+  return linear_forward(x, weight, bias, false, false, &kept);
 }
 
 // ---- orthogonalised steps ---------------------------------------------------------------

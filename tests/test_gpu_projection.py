@@ -156,7 +156,7 @@ def near(y, x, w, bias, floor=0.0):
     assert (d <= off).all(), (d / off).max().item()
 
 
-SIZES = [(1, 16, 16), (1, 4096, 128), (2, 40, 257), (16, 300, 1000), (100, 64, 129), (128, 128, 128),
+SIZES = [(1, 16, 16), (1, 4096, 128), (2, 40, 257), (16, 300, 1000), (8, 33, 3000), (9, 50, 127), (16, 20, 5000), (100, 64, 129), (128, 128, 128),
          (129, 65, 384), (257, 513, 640), (333, 1500, 1000), (515, 1003, 77), (1000, 260, 2049), (700, 1100, 1536)]
 
 
@@ -232,8 +232,12 @@ def test_products_of_any_layout(path):
         for b in (s, s.view(torch.uint8).contiguous().view(SCALES), ss.view(SCALES)):
             assert torch.equal(matmul_quantized(a, b, v, vs, dtype=F32), want)
             assert torch.equal(matmul_quantized(v, vs, a, b, dtype=F32).t(), want)
-    assert torch.equal(matmul_quantized(q[3], s[3], v, vs, dtype=F32), want[3])
-    assert torch.equal(matmul_quantized(q[3:4], s[3:4], v, vs, dtype=F32), want[3:4])
+    # (few rows are summed in another order)
+    one = matmul_quantized(q[3], s[3], v, vs, dtype=F32)
+    near(one[None], xv[3:4], wv, None)
+    assert torch.equal(matmul_quantized(q[3:4], s[3:4], v, vs, dtype=F32), one[None])
+    assert torch.equal(matmul_quantized(loose[3:4], s[3:4].clone(), v, vs, dtype=F32), one[None])
+    near(matmul_quantized(v[:, :K - 3], vs, q[:5, :K - 3].contiguous(), s[:5], dtype=F32).t(), xv[:5, :K - 3], wv[:, :K - 3], None)
     cube = matmul_quantized(q.view(7, 10, K), s.view(7, 10, -1), v, vs, dtype=F32)
     assert torch.equal(cube, want.view(7, 10, N))
     assert matmul_quantized(q[:0], s[:0], v, vs).shape == (0, N)
