@@ -118,28 +118,34 @@ struct Eight<float> {
 // A block takes a tile of 128 x 128; a thread 8 rows x 8 columns of it, so that a
 // row's block is 16 threads' (half a warp's) and a column's 8 codes are one word
 // pair of the transposed codes, which cross through shared memory.
-template <typename T, bool VEC, bool ROWS, bool COLUMNS, bool SUMS>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize(const QuantizeArgs a) {
+template <typename T, bool COLUMNS, bool SUMS>
+struct QuantizeShared {
+  uint2 turned[COLUMNS ? 128 * 16 : 1];
+  uint32_t most_of[COLUMNS ? 8 : 1][COLUMNS ? 16 * Eight<T>::kWords : 1];
+  float inverse[COLUMNS ? 128 : 1];
+  float sum_of[SUMS ? 8 : 1][SUMS ? 128 : 1];
+};
+
+// FULL: the tile lies inside the matrix (16384 x 4096 both ways without this form: 67 us).
+template <typename T, bool VEC, bool ROWS, bool COLUMNS, bool SUMS, bool FULL>
+__device__ __forceinline__ void quantize_tile(const QuantizeArgs &a, QuantizeShared<T, COLUMNS, SUMS> &sh, int64_t tx,
+                                              int64_t ty) {
   using E = Eight<T>;
   constexpr int W = E::kWords;
-  __shared__ uint32_t most_of[COLUMNS ? 8 : 1][COLUMNS ? 16 * W : 1];
-  __shared__ float inverse[COLUMNS ? 128 : 1];
-  __shared__ float sum_of[SUMS ? 8 : 1][SUMS ? 128 : 1];
-  __shared__ uint2 turned[COLUMNS ? 128 * 16 : 1];
+  auto &most_of = sh.most_of;
+  auto &inverse = sh.inverse;
+  auto &sum_of = sh.sum_of;
+  auto &turned = sh.turned;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane & 15, band = 2 * warp + (lane >> 4);  // this thread's columns 8 l.., rows 8 band..
-  const int64_t tiles_x = (a.columns + 127) / 128;
-  const int64_t ty = blockIdx.x / tiles_x, tx = blockIdx.x % tiles_x;
   const int64_t c0 = tx * 128 + 8 * l, r0 = ty * 128 + 8 * band;
   const T *x = static_cast<const T *>(a.x) + r0 * a.x_row + c0;
-  tc::dep_launch();
-  tc::dep_wait();
 
   E v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const bool in = r0 + i < a.rows;
-    if (VEC && in && c0 + 8 <= a.columns) {
+    const bool in = FULL || r0 + i < a.rows;
+    if (VEC && in && (FULL || c0 + 8 <= a.columns)) {
 #pragma unroll
       for (int k = 0; k < W; k += 4)
         *reinterpret_cast<uint4 *>(v[i].w + k) =
@@ -147,8 +153,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize(const 
     } else {  // (nothing is read past a row's end)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float e0 = in && c0 + 2 * k < a.columns ? to_f32(x[i * a.x_row + 2 * k]) : 0.f;
-        const float e1 = in && c0 + 2 * k + 1 < a.columns ? to_f32(x[i * a.x_row + 2 * k + 1]) : 0.f;
+        const float e0 = in && (FULL || c0 + 2 * k < a.columns) ? to_f32(x[i * a.x_row + 2 * k]) : 0.f;
+        const float e1 = in && (FULL || c0 + 2 * k + 1 < a.columns) ? to_f32(x[i * a.x_row + 2 * k + 1]) : 0.f;
         if constexpr (sizeof(T) == 2) v[i].w[k] = pack_pair<T>(e0, e1);
         else v[i].w[2 * k] = __float_as_uint(e0), v[i].w[2 * k + 1] = __float_as_uint(e1);
       }
@@ -186,9 +192,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize(const 
       uint2 w;
       w.x = codes_of(p0.x * r, p0.y * r, p1.x * r, p1.y * r);
       w.y = codes_of(p2.x * r, p2.y * r, p3.x * r, p3.y * r);
-      if (r0 + i < a.rows) {
+      if (FULL || r0 + i < a.rows) {
         // (rows are padded to multiples of 16 codes)
-        if (c0 < a.columns) *reinterpret_cast<uint2 *>(a.q + (r0 + i) * a.q_row + c0) = w;
+        if (FULL || c0 < a.columns) *reinterpret_cast<uint2 *>(a.q + (r0 + i) * a.q_row + c0) = w;
         if (l == 0) a.scale[(r0 + i) * a.scale_row + tx] = (uint8_t)e;
       }
     }
@@ -207,9 +213,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize(const 
       }
       const uint32_t e = scale_exponent(E::bits(most));
       inverse[c] = inverse_scale(e);
-      if (column < a.columns) a.scale_t[column * a.scale_t_row + ty] = (uint8_t)e;
+      if (FULL || column < a.columns) a.scale_t[column * a.scale_t_row + ty] = (uint8_t)e;
     }
-    if (SUMS && column < a.columns) {
+    if (SUMS && (FULL || column < a.columns)) {
       float s = 0.f;
 #pragma unroll
       for (int b = 0; b < 8; ++b) s += sum_of[b][c];
@@ -237,9 +243,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) k_quantize(const 
   for (int i = 0; i < 8; ++i) {
     const int c = i * 16 + (threadIdx.x >> 4), k = threadIdx.x & 15;
     const int64_t column = tx * 128 + c, row = ty * 128 + 8 * k;
-    if (column < a.columns && row < a.rows)
+    if (FULL || (column < a.columns && row < a.rows))
       *reinterpret_cast<uint2 *>(a.qt + column * a.qt_row + row) = turned[c * 16 + (k ^ (c >> 3))];
   }
+}
+
+template <typename T, bool VEC, bool ROWS, bool COLUMNS, bool SUMS>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && !SUMS ? 3 : 2) k_quantize(const QuantizeArgs a) {
+  __shared__ QuantizeShared<T, COLUMNS, SUMS> sh;
+  const int64_t tiles_x = (a.columns + 127) / 128;
+  const int64_t ty = blockIdx.x / tiles_x, tx = blockIdx.x - ty * tiles_x;
+  tc::dep_launch();
+  tc::dep_wait();
+  if (ty * 128 + 128 <= a.rows && tx * 128 + 128 <= a.columns)
+    quantize_tile<T, VEC, ROWS, COLUMNS, SUMS, true>(a, sh, tx, ty);
+  else
+    quantize_tile<T, VEC, ROWS, COLUMNS, SUMS, false>(a, sh, tx, ty);
 }
 
 // Columns' sums over the tiles, in a fixed order: 32 columns a block, each by 8
