@@ -353,14 +353,14 @@ struct Schulz {
   // (16-bit results: up to 1.5e-5 of the sum at 4096 summed, against 2^-12 of its operands)
   static constexpr int kSegment = PARTS == 2 ? 4 : 0;
   static constexpr bool kScaled = false, kBMn = PHASE >= kUpdate, kSymmetric = PHASE <= kSquare;
-  static constexpr int kBM = 128 * CTAS;
-  static_assert(kBM == BN, "symmetric results are computed by square tiles");
+  static constexpr int kBM = 128 * CTAS, kAcross = kBM / BN;
+  static_assert(kBM % BN == 0, "tiles of symmetric results begin on the diagonal");
   struct alignas(16) Shared {
     int unused;
   };
   struct Tile {
     int m0, n0, steps, z, g;
-    bool mirror;
+    bool mirror, edge;  // stored turned too; some of it on or under the diagonal
   };
   const PhaseArgs &p;
 
@@ -372,18 +372,17 @@ struct Schulz {
     i -= begin;
     Tile t;
     t.g = g, t.steps = q.steps;
-    if (kSymmetric) {
-      const int per = q.tiles_m * (q.tiles_m + 1) / 2;
+    if (kSymmetric) {  // rows of tiles, each from the diagonal on
+      const int per = q.tiles_m * q.tiles_n - kAcross * (q.tiles_m * (q.tiles_m - 1) / 2);
       t.z = i / per, i %= per;
-      int column = (int)((sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
-      while (column * (column + 1) / 2 > i) --column;
-      while ((column + 1) * (column + 2) / 2 <= i) ++column;
-      const int row = i - column * (column + 1) / 2;
-      t.m0 = row * kBM, t.n0 = column * BN, t.mirror = row != column;
+      int row = 0;
+      for (int n = q.tiles_n; i >= n; n -= kAcross) i -= n, ++row;
+      t.m0 = row * kBM, t.n0 = (row * kAcross + i) * BN;
+      t.mirror = kAcross > 1 || i > 0, t.edge = kAcross > 1 && i < kAcross;
     } else {
       const int per = q.tiles_m * q.tiles_n;
       t.z = i / per, i %= per;
-      t.m0 = i % q.tiles_m * kBM, t.n0 = i / q.tiles_m * BN, t.mirror = false;
+      t.m0 = i % q.tiles_m * kBM, t.n0 = i / q.tiles_m * BN, t.mirror = t.edge = false;
     }
     return t;
   }
@@ -400,11 +399,10 @@ struct Schulz {
     for (int h = 0; h < PARTS; ++h) {
       tc::tile_load<CTAS>(sa + h * tc::kAHalf, &q.a[h], bar, at, t.m0 + rank * 128, t.z);
       const uint32_t to = sb + h * (BN / CTAS * 128);
-      if constexpr (kBMn) {  // 64 summed rows of 64 columns, twice
-        tc::tile_load<CTAS>(to, &q.b[h], bar, n, at, t.z);
-        tc::tile_load<CTAS>(to + 8192, &q.b[h], bar, n + 64, at, t.z);
-      } else {
-        tc::tile_load<CTAS>(to, &q.b[h], bar, at, n, t.z);
+#pragma unroll
+      for (int c = 0; c < BN / CTAS; c += 64) {  // boxes of 64 rows
+        if constexpr (kBMn) tc::tile_load<CTAS>(to + c * 128, &q.b[h], bar, n + c, at, t.z);
+        else tc::tile_load<CTAS>(to + c * 128, &q.b[h], bar, at, n + c, t.z);
       }
     }
   }
@@ -459,6 +457,23 @@ struct Schulz {
         const float2 x = unpack_pair<__half>(h[j]);
         l[j] = pack_pair<__half>(a - x.x, b - x.y);
       }
+      // A value and its mirror image come from one sum: what lies under the diagonal is
+      // not stored from here.
+      const int rows0 = row - (int)(threadIdx.x & 31);
+      if (t.edge && col < rows0 + 32) {
+        if (col + 16 <= rows0) continue;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int column = col + j;
+          if (row >= q.m || column >= q.n || column < row) continue;
+          const __half x = __ushort_as_half((uint16_t)(h[j >> 1] >> (16 * (j & 1))));
+          const __half y = __ushort_as_half((uint16_t)(l[j >> 1] >> (16 * (j & 1))));
+          const int64_t at = row * q.write_pitch + column, to = column * q.write_pitch + row;
+          hi[at] = x, hi[to] = x;
+          if (q.write_lo) lo[at] = y, lo[to] = y;
+        }
+        continue;
+      }
       // (what lies past a row's end, up to the next multiple of 16, is never read as a value)
       if (row < q.m) {
         const int64_t at = row * q.write_pitch + col;
@@ -499,8 +514,10 @@ cudaError_t launch_phase_as(PhaseArgs &a, const int *batch, cudaStream_t s) {
   int64_t tiles = 0;
   for (int g = 0; g < a.groups; ++g) {
     PhaseGroup &q = a.g[g];
-    q.tiles_m = (q.m + BN - 1) / BN, q.tiles_n = (q.n + BN - 1) / BN;
-    const int64_t per = PHASE <= kSquare ? (int64_t)q.tiles_m * (q.tiles_m + 1) / 2 : (int64_t)q.tiles_m * q.tiles_n;
+    constexpr int kBM = 128 * CTAS;
+    q.tiles_m = (q.m + kBM - 1) / kBM, q.tiles_n = (q.n + BN - 1) / BN;
+    int64_t per = (int64_t)q.tiles_m * q.tiles_n;
+    if (PHASE <= kSquare) per -= kBM / BN * ((int64_t)q.tiles_m * (q.tiles_m - 1) / 2);
     tiles += per * batch[g];
     if (tiles >= int64_t(1) << 30) return cudaErrorInvalidValue;
     q.end = (int)tiles;
@@ -561,15 +578,35 @@ bool map_of(CUtensorMap *map, const __half *p, int columns, int rows, int batch,
   return make_tile_map(map, true, p, columns, rows, batch, pitch * 2, pitch * 2 * rows, box_rows);
 }
 
+// Tiles of 128 x 64 or 128 x 128, or 256 x 256 by a pair of blocks, by the time that the
+// waves of tiles should take (as tile_of in product.cu).
 template <int PHASE, int PARTS>
 cudaError_t launch_phase(PhaseArgs &a, const int *batch, cudaStream_t s) {
-  int64_t tiles = 0;
-  for (int g = 0; g < a.groups; ++g) {
-    const int64_t tm = (a.g[g].m + 255) / 256, tn = (a.g[g].n + 255) / 256;
-    tiles += (PHASE <= kSquare ? tm * (tm + 1) / 2 : tm * tn) * batch[g];
+  const int64_t sms = device_info().sm_count;
+  const int rows[3] = {128, 128, 256}, columns[3] = {64, 128, 256};
+  // (narrow tiles on the diagonal are stored element by element)
+  const float launch[3] = {PHASE <= kSquare ? 6.5f : 4.f, 5.f, 7.f}, wave[3] = {0.5f, 1.f, 2.f};
+  const float step[3] = {PARTS == 2 ? 0.36f : 0.2f, PARTS == 2 ? 0.5f : 0.25f, PARTS == 2 ? 0.85f : 0.33f};
+  int best = 0;
+  float least = 0.f;
+  for (int k = 0; k < 3; ++k) {
+    int64_t tiles = 0;
+    double work = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      const PhaseGroup &q = a.g[g];
+      const int64_t tm = (q.m + rows[k] - 1) / rows[k], tn = (q.n + columns[k] - 1) / columns[k];
+      const int64_t per = (tm * tn - (PHASE <= kSquare ? rows[k] / columns[k] * (tm * (tm - 1) / 2) : 0)) * batch[g];
+      tiles += per, work += (double)per * (wave[k] + step[k] * (float)q.steps);
+    }
+    const int64_t slots = std::max<int64_t>(1, k == 2 ? sms / 2 : sms), waves = (tiles + slots - 1) / slots;
+    const float t = launch[k] + (float)(work / (double)tiles * (double)waves);
+    if (k == 0 || t < least) best = k, least = t;
   }
-  return tiles * 2 >= device_info().sm_count / 2 ? launch_phase_as<PHASE, PARTS, 2, 256>(a, batch, s)
-                                                 : launch_phase_as<PHASE, PARTS, 1, 128>(a, batch, s);
+  switch (best) {
+    case 2: return launch_phase_as<PHASE, PARTS, 2, 256>(a, batch, s);
+    case 1: return launch_phase_as<PHASE, PARTS, 1, 128>(a, batch, s);
+    default: return launch_phase_as<PHASE, PARTS, 1, 64>(a, batch, s);
+  }
 }
 
 // The products of at most kGroups sets, all of one kind.
@@ -591,7 +628,7 @@ cudaError_t schulz_as(const std::vector<Set> &sets, const std::vector<Places> &p
       PhaseGroup &q = a.g[g];
       for (int h = 0; h < 2; ++h) {
         ok = ok && map_of(&q.a[h], w.x[now][h], t.n(), t.m(), t.batch, t.x_pitch(), 128);
-        q.b[h] = q.a[h];
+        ok = ok && map_of(&q.b[h], w.x[now][h], t.n(), t.m(), t.batch, t.x_pitch(), 64);
         q.read[h] = nullptr, q.write[h] = w.a[h];
       }
       q.terms = w.terms;
@@ -606,7 +643,7 @@ cudaError_t schulz_as(const std::vector<Set> &sets, const std::vector<Places> &p
       PhaseGroup &q = a.g[g];
       for (int h = 0; h < 2; ++h) {
         ok = ok && map_of(&q.a[h], w.a[h], t.m(), t.m(), t.batch, t.a_pitch(), 128);
-        q.b[h] = q.a[h];
+        ok = ok && map_of(&q.b[h], w.a[h], t.m(), t.m(), t.batch, t.a_pitch(), 64);
         q.read[h] = w.a[h], q.write[h] = w.b[h];
       }
       q.read_pitch = t.a_pitch(), q.read_plane = t.m() * t.a_pitch();
@@ -1240,6 +1277,12 @@ const char *check_tensors(const cpab_muon_tensor *tensors, int count) {
     if (t.rows > 0 && t.columns > 0 && (t.param == nullptr || t.grad == nullptr || t.momentum == nullptr))
       return "null parameter, gradient or momentum";
   }
+  // (steps of one matrix at a time would race)
+  std::vector<const void *> seen;
+  for (int i = 0; i < count; ++i)
+    if (tensors[i].rows > 0 && tensors[i].columns > 0) seen.push_back(tensors[i].param), seen.push_back(tensors[i].momentum);
+  std::sort(seen.begin(), seen.end());
+  if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) return "a parameter or momentum given twice";
   return nullptr;
 }
 

@@ -71,10 +71,7 @@ struct CoreBarriers {
   int gave_up;
 };
 
-// Counts kernels in which a wait ran out; their unfinished tiles are stored as NaN.
-static __device__ unsigned g_gave_up;
-
-// N columns from tensor memory, NaN where the tile was given up.
+// N columns from tensor memory; NaN where a wait ran out and the tile was given up.
 template <int N>
 __device__ __forceinline__ void read_accumulators(bool ok, uint32_t addr, float (&v)[N]) {
   if (ok) {
@@ -220,7 +217,7 @@ __device__ __forceinline__ void core(const P &p) {
               if (warp == 3) p.scales_b(t, 128 * c + lane + 32 * j, g, w[c][j]);
               else if (c == 0) p.scales_a(t, rank, lane + 32 * j, g, w[c][j]);
             }
-          ok = bar_wait(sempty + 8 * sc, sphase ^ 1);
+          ok = bar_wait_warp(sempty + 8 * sc, sphase ^ 1);
           uint8_t *to = scales + sc * S::kSlotBytes + 16 * lane + (warp == 3 ? 512 : 0);
 #pragma unroll
           for (int c = 0; c < kB; ++c) {
@@ -257,8 +254,7 @@ __device__ __forceinline__ void core(const P &p) {
       float v[kHold];
       typename P::Ahead now = p.ahead(t, row, half * kHalf);
       for (int g = 0; g < segments; ++g) {
-        ok = ok && bar_wait(afull + 8 * acc, aphase);
-        ok = __all_sync(~0u, ok);
+        ok = ok && bar_wait_warp(afull + 8 * acc, aphase);
         fence_after();
         const uint32_t d = tmem + acc * P::kBN + half * kHalf + ((uint32_t)(quarter * 32) << 16);
         if constexpr (kHold < kHalf) {
@@ -308,10 +304,8 @@ __device__ __forceinline__ void core(const P &p) {
   __syncthreads();
   if (*gave_up) {
     // Copies in flight land before the block ends.
-    if (threadIdx.x == 0) {
-      atomicAdd(&g_gave_up, 1u);
+    if (threadIdx.x == 0)
       for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-    }
     __syncthreads();
   }
   fence_before();

@@ -42,11 +42,15 @@ __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Waits for the phase of the given parity.  Every wait of these kernels ends: a
-// try suspends the thread for a bounded time, and after kTries of them (seconds;
-// the longest wait in earnest is a tile's product, under a millisecond) the
+// Waits for the phase of the given parity.  Every wait of these kernels ends: after
+// two seconds (the longest in earnest is a tile's product, under a millisecond) the
 // caller gives its work up.
-constexpr int kTries = 1 << 22;
+constexpr uint64_t kLongest = 2000000000ull;
+__device__ __forceinline__ uint64_t nanoseconds() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -57,11 +61,14 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  for (int i = 0; i < kTries; ++i)
+  for (int i = 0; i < 16; ++i)
     if (bar_try(bar, parity)) return true;
+  const uint64_t begin = nanoseconds();
+  do {
+    if (bar_try(bar, parity)) return true;
+  } while (nanoseconds() - begin < kLongest);
   return false;
 }
-
 // The same for a whole warp, with one answer.
 __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(~0u, bar_wait(bar, parity)); }
 

@@ -296,6 +296,8 @@ def test_refusals(path):
                 dict(params=[p[0]], grads=[g[0]], momenta=[m[0]])):
         with pytest.raises(ValueError):
             muon_(**{**dict(params=[p], grads=[g], momenta=[m]), **bad}, lr=0.1)
+    with pytest.raises(RuntimeError, match="twice"):
+        muon_([p, p], [g, g], [m, m.clone()], lr=0.1)
     with pytest.raises(RuntimeError, match="device"):
         muon_([p], [g.cpu()], [m], lr=0.1)
     with pytest.raises(ValueError, match="lr"):

@@ -97,7 +97,7 @@ def test_muon_entry_point_validates():
     t = (_native._MuonTensor * 1)()
 
     def one(count=1, coefficients=COEFFICIENTS, steps=5, eps=1e-7, adjust=0, work=P, **kw):
-        base = dict(param=4096, grad=4096, momentum=4096, rows=300, columns=400, dtype=0)
+        base = dict(param=4096, grad=4096, momentum=8192, rows=300, columns=400, dtype=0)
         for k, v in {**base, **kw}.items():
             setattr(t[0], k, v)
         return L.cpab_b200_muon(ctypes.byref(t), count, 0.1, None, 0.9, 1, 0.1, steps, coefficients, eps, adjust, work,
@@ -113,6 +113,10 @@ def test_muon_entry_point_validates():
     assert one(rows=0, work=None) == 0 and err() == ""
     assert L.cpab_b200_muon(None, 1, 0.1, None, 0.9, 1, 0.1, 5, COEFFICIENTS, 1e-7, 0, P, None) == -1
     one()
+    two = (_native._MuonTensor * 2)(t[0], t[0])
+    two[1].momentum = 16384
+    assert L.cpab_b200_muon(ctypes.byref(two), 2, 0.1, None, 0.9, 1, 0.1, 5, COEFFICIENTS, 1e-7, 0, P, None) == -1
+    assert "twice" in err()
     assert L.cpab_b200_muon_workspace(ctypes.byref(t), 1) > 0
     assert L.cpab_b200_muon_workspace(None, 1) == 0
 
