@@ -26,6 +26,7 @@
 // theta' = min(1, 2^ceil(log2 a) theta), until theta is 1.
 #include <algorithm>
 #include <cmath>
+#include <exception>
 #include <vector>
 
 #include "product_core.cuh"
@@ -1135,6 +1136,16 @@ cudaError_t launch_small(const SmallArgs &a, int shapes, int64_t count, cudaStre
 
 constexpr int64_t kMostRows = 1 << 20;
 
+// No exception leaves a C entry (the lists may ask for more memory than there is).
+template <typename F>
+int guarded(const char *what, F f) {
+  try {
+    return f();
+  } catch (const std::exception &e) {
+    return report_error(CPAB_ERR_SIZE, "%s: %s", what, e.what());
+  }
+}
+
 const char *check_steps(int steps, const double *c, double eps) {
   if (steps < 1 || steps > kMostSteps) return "steps must be 1 to 64";
   if (!(eps >= 0)) return "eps must not be negative";
@@ -1188,28 +1199,30 @@ extern "C" int cpab_b200_orthogonalize(int dtype, const void *x, int64_t batch, 
   }
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256)
     return report_error(CPAB_ERR_ARG, "%s", "orthogonalize: a null workspace, or one off 256 bytes");
-  const std::vector<Set> sets = {{(int)rows, (int)columns, dtype, (int)batch}};
-  std::vector<Places> places;
-  double *partials;
-  place(sets, batch, static_cast<char *>(workspace), &places, &partials);
-  std::vector<Prepared> list((size_t)batch);
-  const Set &t = sets[0];
-  for (int64_t z = 0; z < batch; ++z) {
-    const int64_t at = z * t.m() * t.x_pitch();
-    list[z] = {static_cast<const char *>(x) + z * rows * columns * dtype_size(dtype), nullptr, places[0].x[0][0] + at,
-               places[0].x[0][1] + at, partials + z * kPartials, places[0].terms + z * kTerms, t.x_pitch(), (int)rows, (int)columns, dtype, t.turned()};
-  }
-  cudaError_t e = prepare(list, 0.f, 0, steps, coefficients, eps, s);
-  if (e == cudaSuccess) e = schulz(sets, places, steps, s);
-  std::vector<Finished> results((size_t)batch);
-  for (int64_t z = 0; z < batch; ++z) {
-    const int64_t at = z * t.m() * t.x_pitch();
-    results[z] = {places[0].x[steps & 1][0] + at, places[0].x[steps & 1][1] + at, places[0].terms + z * kTerms,
-                  static_cast<char *>(out) + z * rows * columns * dtype_size(dtype), t.x_pitch(), 1.f, (int)rows,
-                  (int)columns, dtype, t.turned(), 0};
-  }
-  if (e == cudaSuccess) e = finish(results, 0.0, nullptr, 0.0, s);
-  return launch_status(e, "orthogonalize");
+  return guarded("orthogonalize", [&]() -> int {
+    const std::vector<Set> sets = {{(int)rows, (int)columns, dtype, (int)batch}};
+    std::vector<Places> places;
+    double *partials;
+    place(sets, batch, static_cast<char *>(workspace), &places, &partials);
+    std::vector<Prepared> list((size_t)batch);
+    const Set &t = sets[0];
+    for (int64_t z = 0; z < batch; ++z) {
+      const int64_t at = z * t.m() * t.x_pitch();
+      list[z] = {static_cast<const char *>(x) + z * rows * columns * dtype_size(dtype), nullptr, places[0].x[0][0] + at,
+                 places[0].x[0][1] + at, partials + z * kPartials, places[0].terms + z * kTerms, t.x_pitch(), (int)rows, (int)columns, dtype, t.turned()};
+    }
+    cudaError_t e = prepare(list, 0.f, 0, steps, coefficients, eps, s);
+    if (e == cudaSuccess) e = schulz(sets, places, steps, s);
+    std::vector<Finished> results((size_t)batch);
+    for (int64_t z = 0; z < batch; ++z) {
+      const int64_t at = z * t.m() * t.x_pitch();
+      results[z] = {places[0].x[steps & 1][0] + at, places[0].x[steps & 1][1] + at, places[0].terms + z * kTerms,
+                    static_cast<char *>(out) + z * rows * columns * dtype_size(dtype), t.x_pitch(), 1.f, (int)rows,
+                    (int)columns, dtype, t.turned(), 0};
+    }
+    if (e == cudaSuccess) e = finish(results, 0.0, nullptr, 0.0, s);
+    return launch_status(e, "orthogonalize");
+  });
 }
 
 namespace cpab {
@@ -1291,9 +1304,12 @@ const char *check_tensors(const cpab_muon_tensor *tensors, int count) {
 
 extern "C" int64_t cpab_b200_muon_workspace(const cpab_muon_tensor *tensors, int count) {
   int64_t most = 0;
-  if (check_tensors(tensors, count) != nullptr) return 0;
-  for (const Sequence &q : sequences(tensors, count))
-    most = std::max(most, place(q.sets, (int64_t)q.tensors.size(), nullptr, nullptr, nullptr));
+  guarded("muon", [&]() -> int {
+    if (check_tensors(tensors, count) != nullptr) return CPAB_ERR_ARG;
+    for (const Sequence &q : sequences(tensors, count))
+      most = std::max(most, place(q.sets, (int64_t)q.tensors.size(), nullptr, nullptr, nullptr));
+    return CPAB_OK;
+  });
   return most;
 }
 
@@ -1302,56 +1318,58 @@ extern "C" int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double
                               const double *coefficients, double eps, int adjust, void *workspace,
                               cpab_stream_t stream) {
   if (coefficients == nullptr) return report_error(CPAB_ERR_ARG, "%s", "muon: null coefficients");
-  const char *why = check_tensors(tensors, count);
-  if (why == nullptr) why = check_steps(steps, coefficients, eps);
-  if (why == nullptr && adjust != 0 && adjust != 1) why = "adjust must be 0 or 1";
-  if (why != nullptr) return report_error(CPAB_ERR_ARG, "muon: %s", why);
-  const std::vector<Sequence> list = sequences(tensors, count);
-  if (!list.empty() && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256))
-    return report_error(CPAB_ERR_ARG, "%s", "muon: null workspace, or one off 256 bytes");
-  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaSuccess;
-  auto rate = [&](int64_t rows, int64_t columns) {
-    return (float)(adjust ? 0.2 * std::sqrt((double)std::max(rows, columns))
-                          : std::sqrt(std::max(1.0, (double)rows / (double)columns)));
-  };
-  const Split split(tensors, count);
-  SmallArgs small = {};
-  small.momentum = (float)momentum, small.lr = (float)lr, small.decay = (float)weight_decay, small.lr_device = lr_device;
-  small.nesterov = nesterov, small.steps = steps, small.eps = eps;
-  small.a = coefficients[0], small.b = coefficients[1], small.c = coefficients[2];
-  for (int i = 0, n = 0; i <= count; ++i) {
-    if (n > 0 && (n == kMatrices || i == count)) {
-      if ((e = launch_small(small, n, n, s)) != cudaSuccess) return launch_status(e, "muon");
-      n = 0;
-    }
-    if (i == count) break;
-    const cpab_muon_tensor &t = tensors[i];
-    if (t.rows > 0 && t.columns > 0 && split.small(t))
-      small.m[n++] = {t.grad, t.momentum, t.param, (int)t.rows, (int)t.columns, t.dtype, 1, rate(t.rows, t.columns)};
-  }
-  for (const Sequence &q : list) {
-    std::vector<Places> places;
-    double *partials;
-    place(q.sets, (int64_t)q.tensors.size(), static_cast<char *>(workspace), &places, &partials);
-    std::vector<Prepared> in;
-    std::vector<Finished> out;
-    for (size_t g = 0; g < q.sets.size(); ++g) {
-      const Set &t = q.sets[g];
-      for (int z = 0; z < t.batch; ++z) {
-        const int k = (int)in.size();
-        const cpab_muon_tensor &m = tensors[q.tensors[k]];
-        const Places &w = places[g];
-        const int64_t at = z * t.m() * t.x_pitch();
-        in.push_back({m.grad, m.momentum, w.x[0][0] + at, w.x[0][1] + at, partials + k * kPartials, w.terms + z * kTerms,
-                      t.x_pitch(), t.rows, t.cols, t.dtype, t.turned()});
-        out.push_back({w.x[steps & 1][0] + at, w.x[steps & 1][1] + at, w.terms + z * kTerms, m.param, t.x_pitch(),
-                       rate(t.rows, t.cols), t.rows, t.cols, t.dtype, t.turned(), 1});
+  return guarded("muon", [&]() -> int {
+    const char *why = check_tensors(tensors, count);
+    if (why == nullptr) why = check_steps(steps, coefficients, eps);
+    if (why == nullptr && adjust != 0 && adjust != 1) why = "adjust must be 0 or 1";
+    if (why != nullptr) return report_error(CPAB_ERR_ARG, "muon: %s", why);
+    const std::vector<Sequence> list = sequences(tensors, count);
+    if (!list.empty() && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256))
+      return report_error(CPAB_ERR_ARG, "%s", "muon: null workspace, or one off 256 bytes");
+    const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaSuccess;
+    auto rate = [&](int64_t rows, int64_t columns) {
+      return (float)(adjust ? 0.2 * std::sqrt((double)std::max(rows, columns))
+                            : std::sqrt(std::max(1.0, (double)rows / (double)columns)));
+    };
+    const Split split(tensors, count);
+    SmallArgs small = {};
+    small.momentum = (float)momentum, small.lr = (float)lr, small.decay = (float)weight_decay, small.lr_device = lr_device;
+    small.nesterov = nesterov, small.steps = steps, small.eps = eps;
+    small.a = coefficients[0], small.b = coefficients[1], small.c = coefficients[2];
+    for (int i = 0, n = 0; i <= count; ++i) {
+      if (n > 0 && (n == kMatrices || i == count)) {
+        if ((e = launch_small(small, n, n, s)) != cudaSuccess) return launch_status(e, "muon");
+        n = 0;
       }
+      if (i == count) break;
+      const cpab_muon_tensor &t = tensors[i];
+      if (t.rows > 0 && t.columns > 0 && split.small(t))
+        small.m[n++] = {t.grad, t.momentum, t.param, (int)t.rows, (int)t.columns, t.dtype, 1, rate(t.rows, t.columns)};
     }
-    if ((e = prepare(in, (float)momentum, nesterov, steps, coefficients, eps, s)) != cudaSuccess) break;
-    if ((e = schulz(q.sets, places, steps, s)) != cudaSuccess) break;
-    if ((e = finish(out, lr, lr_device, weight_decay, s)) != cudaSuccess) break;
-  }
-  return launch_status(e, "muon");
+    for (const Sequence &q : list) {
+      std::vector<Places> places;
+      double *partials;
+      place(q.sets, (int64_t)q.tensors.size(), static_cast<char *>(workspace), &places, &partials);
+      std::vector<Prepared> in;
+      std::vector<Finished> out;
+      for (size_t g = 0; g < q.sets.size(); ++g) {
+        const Set &t = q.sets[g];
+        for (int z = 0; z < t.batch; ++z) {
+          const int k = (int)in.size();
+          const cpab_muon_tensor &m = tensors[q.tensors[k]];
+          const Places &w = places[g];
+          const int64_t at = z * t.m() * t.x_pitch();
+          in.push_back({m.grad, m.momentum, w.x[0][0] + at, w.x[0][1] + at, partials + k * kPartials, w.terms + z * kTerms,
+                        t.x_pitch(), t.rows, t.cols, t.dtype, t.turned()});
+          out.push_back({w.x[steps & 1][0] + at, w.x[steps & 1][1] + at, w.terms + z * kTerms, m.param, t.x_pitch(),
+                         rate(t.rows, t.cols), t.rows, t.cols, t.dtype, t.turned(), 1});
+        }
+      }
+      if ((e = prepare(in, (float)momentum, nesterov, steps, coefficients, eps, s)) != cudaSuccess) break;
+      if ((e = schulz(q.sets, places, steps, s)) != cudaSuccess) break;
+      if ((e = finish(out, lr, lr_device, weight_decay, s)) != cudaSuccess) break;
+    }
+    return launch_status(e, "muon");
+  });
 }

@@ -204,6 +204,41 @@ def test_many_matrices(path):
         assert (p.double() - wp).norm() <= most(F32, (1, 1)) * move.norm() + 2.0 ** -22 * (wp.norm() + move.norm())
 
 
+def test_many_larger_matrices_of_mixed_types(path):
+    """More shapes and matrices than a sequence of launches takes, float32 and 16-bit
+    ones, matrices of none, small ones among them."""
+    kinds = [((130 + 7 * (k % 10), 150), F32) for k in range(140)] + [((300, 260 + 8 * k), BF16) for k in range(3)] + \
+        [((0, 5), F32), ((20, 30), BF16), ((12, 200), F16), ((280, 280), F16)]
+    ps = [matrices(s, t, k, 0.05) if 0 not in s else torch.empty(s, device=DEV) for k, (s, t) in enumerate(kinds)]
+    gs = [matrices(s, t, 300 + k) if 0 not in s else torch.empty(s, device=DEV) for k, (s, t) in enumerate(kinds)]
+    ms = [torch.zeros(s, device=DEV) for s, _ in kinds]
+    want = [step64(p, g, m, 0.1, 0.9, True, 0.1, "original") if p.numel() else None for p, g, m in zip(ps, gs, ms)]
+    muon_(ps, gs, ms, lr=0.1, momentum=0.9, weight_decay=0.1)
+    for p, w in zip(ps, want):
+        if w is not None:
+            wp, _, move = w
+            assert (p.double() - wp).norm() <= most(p.dtype, p.shape) * move.norm() + \
+                (STEP[p.dtype] + 2.0 ** -22) * (wp.norm() + move.norm())
+
+
+@pytest.mark.parametrize("shape", [(70, 130, 140), (3000, 8, 9), (1, 70000)])
+def test_many_in_a_batch(shape, path):
+    x = matrices(shape, F32, 4)
+    y, want = orthogonalize(x), exact(x)
+    off_ = (y.double() - want).flatten(-2).norm(dim=-1) / want.flatten(-2).norm(dim=-1)
+    assert off_.max() <= most(F32, shape)
+
+
+def test_learning_rate_on_the_device_for_all_kinds(path):
+    shapes = [(300, 400), (400, 300), (20, 30)]
+    a = [matrices(s, F32, k, 0.05) for k, s in enumerate(shapes)]
+    b = [p.clone() for p in a]
+    gs = [matrices(s, F32, 9 + k) for k, s in enumerate(shapes)]
+    for ps, lr in ((a, torch.tensor(0.25, device=DEV)), (b, 0.25)):
+        muon_(ps, gs, [torch.zeros_like(p) for p in ps], lr=lr)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
 def net(dtype=F32, seed=0):
     torch.manual_seed(seed)
     return torch.nn.Sequential(torch.nn.Linear(20, 40, bias=False), torch.nn.Linear(40, 40, bias=False),

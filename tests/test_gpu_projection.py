@@ -431,3 +431,32 @@ def test_refusals(path):
         linear_quantized(x, w.to(BF16))
     with pytest.raises(ValueError, match="transpose"):
         quantize_blocks(x[None], transposed=True)
+
+
+def test_a_vector_through_a_projection(path):
+    x, w, b = features(1, 200, F32)[0].requires_grad_(True), features(30, 200, F32, 1).requires_grad_(True), torch.zeros(30, device=DEV)
+    y = linear_quantized(x, w, b)
+    assert y.shape == (30,)
+    dy = torch.randn(30, device=DEV)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    v = lambda t: valued(*encoded(t.detach()))  # noqa: E731
+    near(y[None], v(x[None]), v(w), None)
+    near(dx[None], v(dy[None]), v(w.t()), None)
+    near(dw, v(dy[:, None]), v(x[None].t()), None)
+
+
+def test_two_streams_at_once(path):
+    """Calls that overlap share nothing."""
+    xs = [features(700, 900, BF16, k) for k in range(4)]
+    w = features(800, 900, BF16, 9)
+    want = [linear_quantized(x, w) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = []
+    for _ in range(5):
+        got = []
+        for x, s in zip(xs, streams):
+            with torch.cuda.stream(s):
+                got.append(linear_quantized(x, w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
