@@ -926,9 +926,9 @@ def orthogonalize(x, steps, coefficients, eps):
     batch = x.numel() // (m * n) if x.numel() else 0
     out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     dt = _dtype(x, "x")
-    work = torch.empty(lib().cpab_b200_orthogonalize_workspace(dt, batch, m, n), device=x.device,
-                       dtype=torch.uint8)
     with _on(x.device):
+        work = torch.empty(lib().cpab_b200_orthogonalize_workspace(dt, batch, m, n), device=x.device,
+                           dtype=torch.uint8)
         _check(lib().cpab_b200_orthogonalize(dt, _ptr(xc), batch, m, n, steps, _doubles(coefficients), eps,
                                              _ptr(out), _ptr(work), _stream(x.device)))
     return out
@@ -967,9 +967,9 @@ def muon(params, grads, momenta, lr, lr_device, momentum, nesterov, weight_decay
             alive.append(g)
         table[k] = _MuonTensor(_ptr(p), _ptr(g), _ptr(m), p.shape[0], p.shape[1], _dtype(p, "a parameter"))
         _written(p, m)
-    work = torch.empty(lib().cpab_b200_muon_workspace(ctypes.byref(table), len(params)), device=device,
-                       dtype=torch.uint8)
     with _on(device):
+        work = torch.empty(lib().cpab_b200_muon_workspace(ctypes.byref(table), len(params)), device=device,
+                           dtype=torch.uint8)
         _check(lib().cpab_b200_muon(ctypes.byref(table), len(params), lr, _ptr(lr_device), momentum,
                                     int(nesterov), weight_decay, steps, _doubles(coefficients), eps, adjust,
                                     _ptr(work), _stream(device)))

@@ -341,6 +341,8 @@ struct PhaseGroup {
   int tiles_m, tiles_n, end;       // tiles of one matrix; end of the group's in the launch
   int write_lo;
   const float *terms;              // of the set's first matrix, kTerms apart
+  int splits, total;               // kGram: the sum over `total` stages in so many parts of `steps`,
+  float *parts;                    // whose results go here as float32 (null: one part)
 };
 struct PhaseArgs {
   PhaseGroup g[kGroups];
@@ -361,6 +363,7 @@ struct Schulz {
   };
   struct Tile {
     int m0, n0, steps, z, g;
+    int k0, part;         // first stage and place of a part of the sum
     bool mirror, edge;  // stored turned too; some of it on or under the diagonal
   };
   const PhaseArgs &p;
@@ -372,7 +375,7 @@ struct Schulz {
     const PhaseGroup &q = p.g[g];
     i -= begin;
     Tile t;
-    t.g = g, t.steps = q.steps;
+    t.g = g, t.steps = q.steps, t.k0 = 0, t.part = 0;
     if (kSymmetric) {  // rows of tiles, each from the diagonal on
       const int per = q.tiles_m * q.tiles_n - kAcross * (q.tiles_m * (q.tiles_m - 1) / 2);
       t.z = i / per, i %= per;
@@ -380,6 +383,10 @@ struct Schulz {
       for (int n = q.tiles_n; i >= n; n -= kAcross) i -= n, ++row;
       t.m0 = row * kBM, t.n0 = (row * kAcross + i) * BN;
       t.mirror = kAcross > 1 || i > 0, t.edge = kAcross > 1 && i < kAcross;
+      if (PHASE == kGram && q.splits > 1) {
+        t.part = t.z, t.z /= q.splits;
+        t.k0 = (t.part - t.z * q.splits) * q.steps, t.steps = min(q.steps, q.total - t.k0);
+      }
     } else {
       const int per = q.tiles_m * q.tiles_n;
       t.z = i / per, i %= per;
@@ -395,7 +402,7 @@ struct Schulz {
   }
   __device__ void load(const Tile &t, int k, uint32_t sa, uint32_t sb, uint32_t bar, uint32_t rank) const {
     const PhaseGroup &q = p.g[t.g];
-    const int at = k * 64, n = t.n0 + rank * (BN / CTAS);
+    const int at = (t.k0 + k) * 64, n = t.n0 + rank * (BN / CTAS);
 #pragma unroll
     for (int h = 0; h < PARTS; ++h) {
       tc::tile_load<CTAS>(sa + h * tc::kAHalf, &q.a[h], bar, at, t.m0 + rank * 128, t.z);
@@ -440,6 +447,17 @@ struct Schulz {
   }
   __device__ void store(const Tile &t, const Shared &, int row, int c, const float *acc, const Ahead &w) const {
     const PhaseGroup &q = p.g[t.g];
+    if (PHASE == kGram && q.splits > 1) {
+      float *to = q.parts + t.part * q.write_plane + row * q.write_pitch + t.n0 + c;
+#pragma unroll
+      for (int k = 0; k < kChunk; k += 8) {
+        uint32_t x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(acc[k + j] * w.product);
+        if (row < q.m && t.n0 + c + k < q.n) tc::store_sector(to + k, x);
+      }
+      return;
+    }
     __half *hi = q.write[0] + t.z * q.write_plane, *lo = q.write[1] + t.z * q.write_plane;
     const int odd = threadIdx.x & 1;
 #pragma unroll
@@ -519,12 +537,80 @@ cudaError_t launch_phase_as(PhaseArgs &a, const int *batch, cudaStream_t s) {
     q.tiles_m = (q.m + kBM - 1) / kBM, q.tiles_n = (q.n + BN - 1) / BN;
     int64_t per = (int64_t)q.tiles_m * q.tiles_n;
     if (PHASE <= kSquare) per -= kBM / BN * ((int64_t)q.tiles_m * (q.tiles_m - 1) / 2);
+    if (PHASE == kGram) per *= q.splits;
     tiles += per * batch[g];
     if (tiles >= int64_t(1) << 30) return cudaErrorInvalidValue;
     q.end = (int)tiles;
   }
   return tc::launch(kernel, (unsigned)(CTAS * std::min<int64_t>(tiles, device_info().sm_count / CTAS)), tc::kCoreThreads,
                     S::kBytes, CTAS, s, a);
+}
+
+// A of the parts of its sum, added in order: tiles of 64 x 64 on and above the
+// diagonal, each stored twice.
+__global__ void __launch_bounds__(256) k_join(const __grid_constant__ PhaseArgs a) {
+  int g = 0, z = blockIdx.y;
+  tc::dep_launch();
+  tc::dep_wait();
+  // (the groups' matrices one after another; `end` counts those of groups in parts)
+  while (z >= a.g[g].end) z -= a.g[g++].end;
+  const PhaseGroup &q = a.g[g];
+  const int side = (q.m + 63) / 64;
+  int row = 0, i = blockIdx.x;
+  if (i >= side * (side + 1) / 2) return;
+  for (int n = side; i >= n; --n) i -= n, ++row;
+  const int r0 = row * 64, c0 = (row + i) * 64;
+  __shared__ float tile[64][65];
+  const int x = (threadIdx.x & 7) * 8, y0 = threadIdx.x >> 3;
+#pragma unroll
+  for (int y = y0; y < 64; y += 32) {
+    float v[8] = {};
+    if (r0 + y < q.m && c0 + x < q.m) {  // (rows are padded to 16)
+      const float *from = q.parts + (int64_t)z * q.splits * q.write_plane + (r0 + y) * q.write_pitch + c0 + x;
+      float p[8][8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < q.splits) read_eight(from + k * q.write_plane, CPAB_F32, 0, p[k]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < q.splits) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] += p[k][j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) tile[y][x + j] = v[j];
+  }
+  __syncthreads();
+  __half *hi = q.write[0] + z * q.write_plane, *lo = q.write[1] + z * q.write_plane;
+#pragma unroll
+  for (int y = y0; y < 64; y += 32) {
+    float v[8];
+    if (r0 + y < q.m && c0 + x < q.m) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i == 0 && x + j < y ? tile[x + j][y] : tile[y][x + j];
+      store_eight(hi, lo, (r0 + y) * q.write_pitch + c0 + x, v);
+    }
+    if (i > 0 && c0 + y < q.m && r0 + x < q.m) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = tile[x + j][y];
+      store_eight(hi, lo, (c0 + y) * q.write_pitch + r0 + x, v);
+    }
+  }
+}
+
+// Joins what kGram left in parts (nothing, where it left none).
+cudaError_t launch_join(const PhaseArgs &grams, const int *batch, cudaStream_t s) {
+  PhaseArgs a = grams;
+  int matrices = 0, tiles = 0;
+  for (int g = 0; g < a.groups; ++g) {
+    a.g[g].end = a.g[g].splits > 1 ? batch[g] : 0;
+    if (a.g[g].splits == 1) continue;
+    const int side = (a.g[g].m + 63) / 64;
+    matrices += batch[g], tiles = std::max(tiles, side * (side + 1) / 2);
+  }
+  if (matrices == 0) return cudaSuccess;
+  return tc::launch(k_join, dim3((unsigned)tiles, (unsigned)matrices), 256, 0, 1, s, a);
 }
 
 // ---- a sequence of launches ---------------------------------------------------------
@@ -546,8 +632,24 @@ int64_t round_up(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct Places {
   __half *x[2][2], *a[2], *b[2];  // [buffer][half]
-  float *terms;
+  float *terms, *parts;
+  int splits;
 };
+// Parts that the sums of X X^T are cut into where tiles are few and the sums long: as
+// many as there are blocks for, of at least four stages.  Five steps of 256 x 4096: 169 us,
+// in one part 278; 100 x 4000 float32 144 and 249; 1024 x 1024 207 and 221.
+int splits_of(const std::vector<Set> &sets, const Set &set) {
+  int64_t tiles = 0;
+  for (const Set &s : sets) {
+    const int64_t t = (s.m() + 127) / 128;
+    tiles += t * (t + 1) / 2 * s.batch;
+  }
+  const int64_t stages = (set.n() + 63) / 64;
+  const int64_t parts = std::min<int64_t>({8, device_info().sm_count / std::max<int64_t>(1, tiles), stages / 4});
+  if (parts < 2) return 1;
+  const int64_t each = (stages + parts - 1) / parts;
+  return (int)((stages + each - 1) / each);
+}
 // Bytes of the sets' workspace; with `base`, the places too.
 int64_t place(const std::vector<Set> &sets, int64_t matrices, char *base, std::vector<Places> *places, double **partials) {
   int64_t at = 0;
@@ -562,7 +664,9 @@ int64_t place(const std::vector<Set> &sets, int64_t matrices, char *base, std::v
   for (size_t i = 0; i < sets.size(); ++i) {
     const Set &s = sets[i];
     float *terms = reinterpret_cast<float *>(take((int64_t)s.batch * kTerms * (int64_t)sizeof(float)));
-    if (places != nullptr) (*places)[i].terms = terms;
+    const int splits = splits_of(sets, s);
+    float *parts = splits > 1 ? reinterpret_cast<float *>(take(4 * splits * s.a_halves())) : nullptr;
+    if (places != nullptr) (*places)[i].terms = terms, (*places)[i].parts = parts, (*places)[i].splits = splits;
     for (int k = 0; k < 8; ++k) {
       __half *p = reinterpret_cast<__half *>(take(2 * (k < 4 ? s.x_halves() : s.a_halves())));
       if (places == nullptr) continue;
@@ -596,7 +700,7 @@ cudaError_t launch_phase(PhaseArgs &a, const int *batch, cudaStream_t s) {
     for (int g = 0; g < a.groups; ++g) {
       const PhaseGroup &q = a.g[g];
       const int64_t tm = (q.m + rows[k] - 1) / rows[k], tn = (q.n + columns[k] - 1) / columns[k];
-      const int64_t per = (tm * tn - (PHASE <= kSquare ? rows[k] / columns[k] * (tm * (tm - 1) / 2) : 0)) * batch[g];
+      const int64_t per = (tm * tn - (PHASE <= kSquare ? rows[k] / columns[k] * (tm * (tm - 1) / 2) : 0)) * batch[g] * (PHASE == kGram ? q.splits : 1);
       tiles += per, work += (double)per * (wave[k] + step[k] * (float)q.steps);
     }
     const int64_t slots = std::max<int64_t>(1, k == 2 ? sms / 2 : sms), waves = (tiles + slots - 1) / slots;
@@ -634,10 +738,12 @@ cudaError_t schulz_as(const std::vector<Set> &sets, const std::vector<Places> &p
       }
       q.terms = w.terms;
       q.write_pitch = t.a_pitch(), q.write_plane = t.m() * t.a_pitch();
-      q.m = q.n = t.m(), q.steps = (t.n() + 63) / 64, q.write_lo = 1;
+      q.m = q.n = t.m(), q.total = (t.n() + 63) / 64, q.write_lo = 1;
+      q.splits = w.splits, q.parts = w.parts, q.steps = (q.total + q.splits - 1) / q.splits;
     }
     if (!ok) return cudaErrorInvalidValue;
     if ((e = launch_phase<kGram, PARTS>(a, batch, s)) != cudaSuccess) return e;
+    if ((e = launch_join(a, batch, s)) != cudaSuccess) return e;
     for (int g = 0; g < groups; ++g) {
       const Set &t = sets[g];
       const Places &w = places[g];

@@ -536,8 +536,8 @@ int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, const cpab_qu
  * for each of `batch` contiguous matrices [rows, columns] of dtype; out is shaped
  * as x and may be x.  Matrices of 16 bits are multiplied as halves, float32 ones as
  * pairs of halves (22 bits).  coefficients must keep the singular values and the
- * products' within 60.  workspace: cpab_b200_orthogonalize_workspace bytes (0 for
- * small matrices), 256-byte aligned.
+ * products' within 60.  workspace: cpab_b200_orthogonalize_workspace bytes (for
+ * the current device; 0 for small matrices), 256-byte aligned.
  */
 int64_t cpab_b200_orthogonalize_workspace(int dtype, int64_t batch, int64_t rows, int64_t columns);
 int cpab_b200_orthogonalize(int dtype, const void *x, int64_t batch, int64_t rows, int64_t columns,
@@ -560,8 +560,8 @@ typedef struct {
  *   p = p (1 - lr weight_decay) - lr r O(u)
  * with O that of cpab_b200_orthogonalize, r = sqrt(max(1, rows / columns)) (adjust 0)
  * or 0.2 sqrt(max(rows, columns)) (adjust 1).  lr_device: the learning rate as one
- * float32 on the device, or NULL: lr.  workspace: cpab_b200_muon_workspace bytes,
- * 256-byte aligned.
+ * float32 on the device, or NULL: lr.  workspace: cpab_b200_muon_workspace bytes (for
+ * the current device), 256-byte aligned.
  */
 int64_t cpab_b200_muon_workspace(const cpab_muon_tensor *tensors, int count);
 int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double lr, const float *lr_device,

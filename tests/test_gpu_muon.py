@@ -63,7 +63,8 @@ def matrices(shape, dtype, seed=0, scale=1.0):
 
 
 SHAPES = [(1, 1), (1, 7), (5, 1), (3, 17), (16, 16), (49, 130), (130, 3), (128, 128), (130, 260), (260, 130),
-          (3, 130, 260), (193, 200), (257, 300), (640, 256), (2, 3, 65, 40), (500, 1000), (1000, 1003), (40, 3000)]
+          (3, 130, 260), (193, 200), (257, 300), (640, 256), (2, 3, 65, 40), (500, 1000), (1000, 1003), (40, 3000),
+          (129, 4097), (3, 150, 2000), (3000, 300)]
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
