@@ -11,13 +11,14 @@
 // rounded to a half and its remainder (22 bits together):
 //
 //   - parameters and matrices of 16 bits, of more than 256 rows, are multiplied by
-//     their first halves (11 bits, 2^-12 off); the remainder enters the terms a X and b A, which would
-//     otherwise drown small singular values beside large ones.  The result is
-//     1.5e-3 to 2.7e-3 off (relative 2-norm, normal matrices of up to 1500 rows),
-//     about a rounding to bfloat16 (1.7e-3).
-//   - float32 ones and small ones take three products, first x first + first x remainder +
-//     remainder x first (4e-7 to 3e-6 off): a float32 parameter keeps that many
-//     bits of its update.
+//     their first halves (11 bits, 2^-12 off); the remainder enters the terms a X and
+//     b A, which would otherwise drown small singular values beside large ones.  The
+//     result is 1.5e-3 to 2.7e-3 off (relative 2-norm, normal matrices of up to 1500
+//     rows), about a rounding to bfloat16 (1.7e-3); three products would take 2.2 times
+//     as long.
+//   - float32 ones and small ones take three products, first x first + first x
+//     remainder + remainder x first (up to 5e-6 off): a float32 parameter keeps that
+//     many bits of its update.
 //
 // 2^10 keeps values from 6e-8 in a half's normal range and leaves room to 64.  Where
 // eps is not small beside |G|_F, X is: it is kept as theta Y with theta a power of two
@@ -358,9 +359,7 @@ struct Schulz {
   static constexpr bool kScaled = false, kBMn = PHASE >= kUpdate, kSymmetric = PHASE <= kSquare;
   static constexpr int kBM = 128 * CTAS, kAcross = kBM / BN;
   static_assert(kBM % BN == 0, "tiles of symmetric results begin on the diagonal");
-  struct alignas(16) Shared {
-    int unused;
-  };
+  struct alignas(16) Shared {};
   struct Tile {
     int m0, n0, steps, z, g;
     int k0, part;         // first stage and place of a part of the sum

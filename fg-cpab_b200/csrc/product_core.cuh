@@ -1,12 +1,12 @@
 // The product kernel's skeleton: a persistent block (or pair of blocks that share
 // one tile of 256 rows) walks tiles of C = A B^T; one warp fetches operand tiles
-// into a ring of stages, one issues the matrix instructions, two bring scale words,
-// eight move the accumulators from tensor memory to registers (each a quarter of the
+// into a ring of stages, one issues the matrix instructions, two bring scale words (idle
+// without), eight move the accumulators from tensor memory to registers (each a quarter of the
 // block's rows and half of the columns), hand the accumulator back at once, and give
 // the values to the policy.
 //
 // The policy P says what is multiplied:
-//   kCtas, kBN        blocks to a tile (128 rows each), its columns
+//   kCtas, kBN        blocks to a tile (128 rows each; 1 or 2), its columns
 //   kScaled           e4m3 codes with e8m0 scales (128 codes a step), else halves (64)
 //   kParts            2: operands are sums of two halves; a stage holds both, and
 //                     takes part x part of all but the remainders' product
@@ -23,7 +23,8 @@
 //   warm(tile)                      touches its arguments
 //   load(tile, step, a, b, bar, rank)    issues the copies of one stage; the second
 //                     parts lie kAHalf and kBHalf bytes behind the first
-//   scales_a / _b(tile, rank, row, group, words)  a row's scales of 8 steps, four to a word
+//   scales_a(tile, rank, row, group, words), scales_b(tile, row, group, words)
+//                     a row's scales of 8 steps, four to a word (kScaled)
 //   begin(tile, shared, thread)     before a tile's accumulators are waited for
 //   Ahead, ahead(tile, row, column)  what store reads besides, asked for a chunk early
 //   store(tile, shared, row, column, values, ahead)  kChunk values of this thread's row;
