@@ -413,6 +413,7 @@ struct Schulz {
       }
     }
   }
+  __device__ uint32_t stage_bytes() const { return CTAS * tc::CoreShape<Schulz>::kStageBytes; }
   __device__ void begin(const Tile &, Shared &, int) const {}
 
   // A's or X's halves in the place of what is stored.  (Read when a chunk is stored and

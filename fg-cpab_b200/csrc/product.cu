@@ -324,6 +324,7 @@ struct ProductArgs {
   int M, N, steps;
   int tiles_m, tiles_n;
   int wide;              // y's rows begin on 16 bytes
+  int a_rows;            // of A that a block loads: what M leaves of 128
 };
 
 // A row's scales of 8 steps.  Rows outside hold no codes: any scale but NaN.
@@ -384,6 +385,9 @@ struct Product {
     tc::tile_load<CTAS>(sa, &a.a, bar, k * 128, t.m0 + rank * 128, 0);
     tc::tile_load<CTAS>(sb, &a.b, bar, k * 128, t.n0 + rank * (BN / CTAS), 0);
   }
+  // (Rows of A that are not loaded hold anything, and so do the sums that nobody
+  // stores.  With all 128 loaded, as zeros, a row by 8192 x 8192 took 31 us.)
+  __device__ uint32_t stage_bytes() const { return CTAS * 128 * (a.a_rows + BN / CTAS); }
   __device__ void scales_a(const Tile &t, uint32_t rank, int row, int g, uint32_t (&w)[2]) const {
     scale_words(a.sa, t.m0 + rank * 128 + row, a.M, g, a.steps, w);
   }
@@ -499,7 +503,8 @@ cudaError_t launch_product(ProductArgs &a, cudaStream_t s) {
 // and an eighth of the sum, in blocks of 128; a block's eight warps are added in order.
 // Any order of the summed index will do as long as both operands have it: a lane's 16
 // neighbouring codes of a row are its share of four instructions.
-// One row by 4096 x 2048: 4.3 us, by tiles 7.9; by 8192 x 8192 25.9 and 20.3.
+// One row by 4096 x 2048: 4.3 us, by tiles 6.9; by 5000 x 6000 18.7 and 15.5; 16 rows by
+// 4096 x 2048 7.5 and 6.9.
 
 constexpr int kFewMost = 16;
 constexpr int kFewWarps = 8;
@@ -648,11 +653,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
 }
 
 // Bytes of x as halves; few rows whose x takes more are left to the tiles, and so are
-// large weights, whose codes this kernel's conversions are too many for (16 rows by
-// 4096 x 2048: 7.4 and 7.9 us).
+// large weights, for whose codes this kernel's conversions are too many.
 int64_t few_bytes(int64_t M, int64_t K) { return M * ((K + kBlock - 1) / kBlock * 128 + 8) * 2; }
 bool is_few(int64_t M, int64_t N, int64_t K) {
-  return M <= kFewMost && few_bytes(M, K) <= 72 * 1024 && N * K <= int64_t(1) << (M <= 8 ? 25 : 24);
+  return M <= kFewMost && few_bytes(M, K) <= 72 * 1024 && N * K <= int64_t(1) << (M <= 8 ? 24 : 22);
 }
 
 template <typename T, typename TB, int TILES>
@@ -755,8 +759,9 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   const char *why = operand(*x, K, &a.sa, &a.ra);
   if (why == nullptr) why = operand(*weight, K, &a.sb, &a.rb);
   if (why == nullptr && !is_few(M, N, K)) {
-    const int columns = tile_of(M, N, (K + kBlock - 1) / kBlock) == 0 ? 64 : 128;  // of B a block loads
-    if (!make_tile_map(&a.a, false, x->codes, K, M, 1, x->row, x->row * M, 128) ||
+    const int tile = tile_of(M, N, (K + kBlock - 1) / kBlock), columns = tile == 0 ? 64 : 128;  // of B a block loads
+    a.a_rows = tile == 2 || M > 64 ? 128 : M > 32 ? 64 : M > 16 ? 32 : 16;
+    if (!make_tile_map(&a.a, false, x->codes, K, M, 1, x->row, x->row * M, a.a_rows) ||
         !make_tile_map(&a.b, false, weight->codes, K, N, 1, weight->row, weight->row * N, columns))
       why = "no tensor map for the codes";
   }

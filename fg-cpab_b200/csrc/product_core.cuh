@@ -23,6 +23,7 @@
 //   warm(tile)                      touches its arguments
 //   load(tile, step, a, b, bar, rank)    issues the copies of one stage; the second
 //                     parts lie kAHalf and kBHalf bytes behind the first
+//   stage_bytes()                   bytes that a stage's copies bring, to all blocks
 //   scales_a(tile, rank, row, group, words), scales_b(tile, row, group, words)
 //                     a row's scales of 8 steps, four to a word (kScaled)
 //   begin(tile, shared, thread)     before a tile's accumulators are waited for
@@ -120,7 +121,8 @@ __device__ __forceinline__ void core(const P &p) {
   const int tiles = p.tiles(), first = blockIdx.x / C, stride = gridDim.x / C;
   // What the launch itself brings (arguments, tensor maps) is fetched while the
   // kernel before still runs.
-  p.warm(p.tile(first));
+  const auto first_tile = p.tile(first);
+  p.warm(first_tile);
   dep_wait();
 
   // The pair's shared barriers are the first block's.
@@ -130,12 +132,12 @@ __device__ __forceinline__ void core(const P &p) {
     int s = 0, phase = 0;
     bool ok = true;
     for (int i = first; i < tiles && ok; i += stride) {
-      const auto t = p.tile(i);
+      const auto t = i == first ? first_tile : p.tile(i);
       for (int k = 0; k < t.steps; ++k) {
         ok = bar_wait_warp(empty + 8 * s, phase ^ 1);
         if (!ok) break;
         if (elect()) {
-          if (rank == 0) bar_expect(full + 8 * s, C * S::kStageBytes);
+          if (rank == 0) bar_expect(full + 8 * s, p.stage_bytes());
           const uint32_t a = stage0 + s * S::kStageBytes;
           p.load(t, k, a, a + P::kParts * kAHalf, full0 + 8 * s, rank);
         }
@@ -149,7 +151,7 @@ __device__ __forceinline__ void core(const P &p) {
       int s = 0, phase = 0, sc = 0, sphase = 0, acc = 0, aphase = 0;
       bool ok = true;
       for (int i = first; i < tiles && ok; i += stride) {
-        const auto t = p.tile(i);
+        const auto t = i == first ? first_tile : p.tile(i);
         for (int k = 0; k < t.steps; ++k) {
           const bool fresh = k % kLength == 0;
           if (fresh && !(ok = bar_wait_warp(aempty + 8 * acc, aphase ^ 1))) break;
@@ -208,7 +210,7 @@ __device__ __forceinline__ void core(const P &p) {
       int sc = 0, sphase = 0;
       bool ok = true;
       for (int i = first; i < tiles && ok; i += stride) {
-        const auto t = p.tile(i);
+        const auto t = i == first ? first_tile : p.tile(i);
         for (int g = 0; 8 * g < t.steps && ok; ++g) {
           uint32_t w[kB][4][2];  // [chunk][row lane + 32 j][word]
 #pragma unroll
@@ -248,7 +250,7 @@ __device__ __forceinline__ void core(const P &p) {
     int acc = 0, aphase = 0;
     bool ok = true;
     for (int i = first; i < tiles; i += stride) {
-      const auto t = p.tile(i);
+      const auto t = i == first ? first_tile : p.tile(i);
       p.begin(t, *shared, threadIdx.x - 128);
       const int row = t.m0 + (int)rank * 128 + quarter * 32 + lane;
       const int segments = P::kSegment > 0 ? (t.steps + kLength - 1) / kLength : 1;
