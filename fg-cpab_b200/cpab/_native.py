@@ -65,7 +65,7 @@ _SIGNATURES = {
     "cpab_b200_quantize_blocks": [_c_int, _p, _c_i64, _c_i64, _c_i64, _p, _c_i64, _p, _c_i64, _p,
                                   _c_i64, _p, _c_i64, _c_int, _p, _p, _p],
     "cpab_b200_matmul_quantized": [_c_int, _p, _p, _c_i64, _c_i64, _c_i64, _c_int, _p, _p, _c_i64,
-                                   _p],
+                                   _p, _p],
     "cpab_b200_orthogonalize": [_c_int, _p, _c_i64, _c_i64, _c_i64, _c_int, _p, ctypes.c_double, _p,
                                 _p, _p],
     "cpab_b200_muon": [_p, _c_int, ctypes.c_double, _p, ctypes.c_double, _c_int, ctypes.c_double,
@@ -81,6 +81,7 @@ _OTHERS = {
     "cpab_b200_gated_scan_workspace": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
     "cpab_b200_rms_norm_workspace": (_c_i64, [_c_int, _c_i64, _c_i64]),
     "cpab_b200_quantize_blocks_workspace": (_c_i64, [_c_i64, _c_i64]),
+    "cpab_b200_matmul_quantized_workspace": (_c_i64, [_c_i64, _c_i64, _c_i64]),
     "cpab_b200_orthogonalize_workspace": (_c_i64, [_c_int, _c_i64, _c_i64, _c_i64]),
     "cpab_b200_muon_workspace": (_c_i64, [_p, _c_int]),
 }
@@ -896,10 +897,12 @@ def matmul_quantized(q, scale, weight, weight_scale, bias, dtype):
         bias = bias.contiguous()
     y = torch.empty((*q.shape[:-1], N), device=q.device, dtype=dtype)
     with _on(q.device):
+        floats = lib().cpab_b200_matmul_quantized_workspace(M, N, K)
+        work = torch.empty(floats, device=q.device, dtype=torch.float32) if floats else None
         _check(lib().cpab_b200_matmul_quantized(
             _DTYPES[dtype], ctypes.byref(x), ctypes.byref(w), M, N, K,
             _DTYPES[bias.dtype] if bias is not None else _DTYPES[dtype], _ptr(bias), _ptr(y), N,
-            _stream(q.device)))
+            _ptr(work), _stream(q.device)))
     return y
 
 

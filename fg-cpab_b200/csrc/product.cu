@@ -46,6 +46,7 @@ bool make_tile_map(CUtensorMap *map, bool halves, const void *base, int64_t colu
 namespace {
 
 constexpr int kBlock = 128;  // codes to a scale
+constexpr int64_t kMostSize = (int64_t(1) << 31) - 512;
 
 // ---- codes -------------------------------------------------------------------
 
@@ -325,6 +326,9 @@ struct ProductArgs {
   int tiles_m, tiles_n;
   int wide;              // y's rows begin on 16 bytes
   int a_rows;            // of A that a block loads: what M leaves of 128
+  int splits, each;      // the sum in so many parts of `each` steps (a multiple of 8),
+  float *parts;          // float32 [splits, M, pitch], where they are not one
+  int64_t pitch;
 };
 
 // A row's scales of 8 steps.  Rows outside hold no codes: any scale but NaN.
@@ -365,37 +369,40 @@ struct Product {
     uint4 rows[8][32][5];
   };
   struct Tile {
-    int m0, n0, steps, slot;
+    int m0, n0, steps, slot, part;
   };
   const ProductArgs &a;
 
-  __device__ int tiles() const { return a.tiles_m * a.tiles_n; }
+  __device__ int tiles() const { return a.tiles_m * a.tiles_n * a.splits; }
   // Bands of 8 rows of tiles, column by column, so that tiles at work together
   // share operands in L2.
   __device__ Tile tile(int i) const {
+    const int slot = (i / (int)(gridDim.x / CTAS)) & 1, part = a.splits > 1 ? i / (a.tiles_m * a.tiles_n) : 0;
+    i -= part * a.tiles_m * a.tiles_n;
     const int band = i / (8 * a.tiles_n), top = band * 8, high = min(8, a.tiles_m - top);
     const int in = i - band * 8 * a.tiles_n;
-    return {(top + in % high) * 128 * CTAS, in / high * BN, a.steps, (i / (int)(gridDim.x / CTAS)) & 1};
+    return {(top + in % high) * 128 * CTAS, in / high * BN, min(a.each, a.steps - part * a.each), slot, part};
   }
   __device__ void warm(const Tile &) const {
     if (threadIdx.x == 0) tc::prefetch_map(&a.a), tc::prefetch_map(&a.b);
     tc::touch(a.sa.bytes), tc::touch(a.sb.bytes), tc::touch(a.y), tc::touch(a.bias), tc::touch(a.wide);
   }
   __device__ void load(const Tile &t, int k, uint32_t sa, uint32_t sb, uint32_t bar, uint32_t rank) const {
-    tc::tile_load<CTAS>(sa, &a.a, bar, k * 128, t.m0 + rank * 128, 0);
-    tc::tile_load<CTAS>(sb, &a.b, bar, k * 128, t.n0 + rank * (BN / CTAS), 0);
+    const int at = (t.part * a.each + k) * 128;
+    tc::tile_load<CTAS>(sa, &a.a, bar, at, t.m0 + rank * 128, 0);
+    tc::tile_load<CTAS>(sb, &a.b, bar, at, t.n0 + rank * (BN / CTAS), 0);
   }
   // (Rows of A that are not loaded hold anything, and so do the sums that nobody
   // stores.  With all 128 loaded, as zeros, a row by 8192 x 8192 took 31 us.)
   __device__ uint32_t stage_bytes() const { return CTAS * 128 * (a.a_rows + BN / CTAS); }
   __device__ void scales_a(const Tile &t, uint32_t rank, int row, int g, uint32_t (&w)[2]) const {
-    scale_words(a.sa, t.m0 + rank * 128 + row, a.M, g, a.steps, w);
+    scale_words(a.sa, t.m0 + rank * 128 + row, a.M, t.part * (a.each / 8) + g, a.steps, w);
   }
   __device__ void scales_b(const Tile &t, int row, int g, uint32_t (&w)[2]) const {
-    scale_words(a.sb, t.n0 + row, a.N, g, a.steps, w);
+    scale_words(a.sb, t.n0 + row, a.N, t.part * (a.each / 8) + g, a.steps, w);
   }
   __device__ void begin(const Tile &t, Shared &sh, int thread) const {
-    if (a.rb == nullptr && a.bias == nullptr) return;
+    if (a.splits > 1 || (a.rb == nullptr && a.bias == nullptr)) return;
     if (thread < BN) {
       const int n = t.n0 + thread;
       const bool in = n < a.N;
@@ -409,6 +416,18 @@ struct Product {
   __device__ void store(const Tile &t, Shared &sh, int row, int c, const float *acc, const Ahead &) const {
     const int col = t.n0 + c, lane = threadIdx.x & 31;
     if (col >= a.N) return;
+    if (a.splits > 1) {
+      if (row >= a.M) return;
+      float *to = a.parts + ((int64_t)t.part * a.M + row) * a.pitch + col;
+#pragma unroll
+      for (int k = 0; k < kChunk; k += 8) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(acc[k + j]);
+        if (col + k < a.N) tc::store_sector(to + k, w);  // (the pitch is a multiple of 8)
+      }
+      return;
+    }
     uint4(&rows)[32][5] = sh.rows[(threadIdx.x >> 5) - 4];
     const float ra = a.ra != nullptr && row < a.M ? a.ra[row] : 1.f;
     const bool columns = a.rb != nullptr || a.bias != nullptr;
@@ -450,6 +469,25 @@ struct Product {
   }
 };
 
+// The parts of a sum, in order.
+template <typename T, typename TB>
+__global__ void __launch_bounds__(256) k_join_product(const __grid_constant__ ProductArgs a) {
+  tc::dep_launch();
+  tc::dep_wait();
+  const int64_t count = (int64_t)a.M * a.N, plane = a.M * a.pitch;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / a.N, col = i - row * a.N;
+    const float *from = a.parts + row * a.pitch + col;
+    float v = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < a.splits; ++k) v += from[k * plane];
+    if (a.ra != nullptr) v *= a.ra[row];
+    if (a.rb != nullptr) v *= a.rb[col];
+    if (a.bias != nullptr) v += to_f32(static_cast<const TB *>(a.bias)[col]);
+    static_cast<T *>(a.y)[row * a.y_row + col] = from_f32<T>(v);
+  }
+}
+
 template <typename T, typename TB, int CTAS, int BN>
 __global__ void __launch_bounds__(tc::kCoreThreads, 1) k_product(const __grid_constant__ ProductArgs a) {
   tc::core(Product<T, TB, CTAS, BN>{a});
@@ -463,8 +501,11 @@ cudaError_t launch_product_as(ProductArgs &a, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   a.tiles_m = (a.M + 128 * CTAS - 1) / (128 * CTAS);
   a.tiles_n = (a.N + BN - 1) / BN;
-  const int tiles = a.tiles_m * a.tiles_n, groups = device_info().sm_count / CTAS;
-  return tc::launch(kernel, (unsigned)(CTAS * std::min(tiles, groups)), tc::kCoreThreads, S::kBytes, CTAS, s, a);
+  const int tiles = a.tiles_m * a.tiles_n * a.splits, groups = device_info().sm_count / CTAS;
+  e = tc::launch(kernel, (unsigned)(CTAS * std::min(tiles, groups)), tc::kCoreThreads, S::kBytes, CTAS, s, a);
+  if (e != cudaSuccess || a.splits == 1) return e;
+  const int64_t blocks = std::min<int64_t>(((int64_t)a.M * a.N + 255) / 256, 8 * device_info().sm_count);
+  return tc::launch(k_join_product<T, TB>, (unsigned)blocks, 256, 0, 1, s, a);
 }
 
 // The tile of the least time: 128 x 64, 128 x 128, or 256 x 256 by a pair of blocks.
@@ -484,6 +525,24 @@ int tile_of(int64_t M, int64_t N, int64_t steps) {
     if (k == 0 || t < least) best = k, least = t;
   }
   return best;
+}
+
+// Parts that a long sum of few tiles is cut into, and their steps: as many parts as
+// there are blocks for, of at least 16 steps (the joining launch costs 4 us, 16 steps).
+// 256 x 128 x 131072, a narrow network's weight gradient: 18 us, where one part's 1024
+// steps of 0.26 take 270; 16 x 361 x 6942 11 us, in one part 17.
+struct Split {
+  int splits, each;
+};
+Split split_of(int64_t M, int64_t N, int64_t steps) {
+  const int tile = tile_of(M, N, steps);
+  const int64_t rows = tile == 2 ? 256 : 128, columns = tile == 2 ? 256 : tile == 1 ? 128 : 64;
+  const int64_t tiles = (M + rows - 1) / rows * ((N + columns - 1) / columns);
+  const int64_t slots = tile == 2 ? device_info().sm_count / 2 : device_info().sm_count;
+  const int64_t parts = std::min<int64_t>({64, slots / tiles, steps / 16});
+  if (parts < 2) return {1, (int)steps};
+  const int64_t each = ((steps + parts - 1) / parts + 7) / 8 * 8;
+  return {(int)((steps + each - 1) / each), (int)each};
 }
 
 template <typename T, typename TB>
@@ -743,15 +802,20 @@ extern "C" int cpab_b200_quantize_blocks(int dtype, const void *x, int64_t x_row
   return launch_status(e, "quantize_blocks");
 }
 
+extern "C" int64_t cpab_b200_matmul_quantized_workspace(int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 1 || M > kMostSize || N > kMostSize || K > kMostSize || is_few(M, N, K)) return 0;
+  const Split split = split_of(M, N, (K + kBlock - 1) / kBlock);
+  return split.splits > 1 ? split.splits * M * ((N + 15) / 16 * 16) : 0;
+}
+
 extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, const cpab_quantized *weight, int64_t M,
                                           int64_t N, int64_t K, int bias_dtype, const void *bias, void *y,
-                                          int64_t y_row, cpab_stream_t stream) {
+                                          int64_t y_row, float *workspace, cpab_stream_t stream) {
   if (!dtype_ok(dtype) || (bias != nullptr && bias_dtype != CPAB_F32 && bias_dtype != dtype))
     return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: unknown element type, or a bias of neither y's nor float32");
   if (x == nullptr || weight == nullptr) return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: null operand");
   if (M < 0 || N < 0 || K < 1 || y_row < N) return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: sizes out of range");
-  constexpr int64_t kMost = (int64_t(1) << 31) - 512;
-  if (M > kMost || N > kMost || K > kMost || (M + 127) / 128 * ((N + 63) / 64) >= kMost)
+  if (M > kMostSize || N > kMostSize || K > kMostSize || (M + 127) / 128 * ((N + 63) / 64) >= kMostSize)
     return report_error(CPAB_ERR_SIZE, "%s", "matmul_quantized: sizes too large");
   if (M == 0 || N == 0) return report_error(CPAB_OK, "%s", "");
   if (y == nullptr) return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: null y");
@@ -768,6 +832,10 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   if (why != nullptr) return report_error(CPAB_ERR_ARG, "matmul_quantized: %s", why);
   a.bias = bias, a.y = y, a.y_row = y_row, a.M = (int)M, a.N = (int)N, a.steps = (int)((K + kBlock - 1) / kBlock);
   a.wide = aligned_to(y, y_row, dtype_size(dtype), 16);
+  const Split split = split_of(M, N, a.steps);
+  a.splits = split.splits, a.each = split.each, a.parts = workspace, a.pitch = (N + 15) / 16 * 16;
+  if (!is_few(M, N, K) && a.splits > 1 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 32))
+    return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: a null workspace, or one off 32 bytes");
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (is_few(M, N, K)) {

@@ -172,8 +172,10 @@ Tensor product(const Operand &x, const Operand &w, const Tensor &bias, at::IntAr
   shape.push_back(w.rows);
   const Tensor y = at::empty(shape, like.options().dtype(type));
   const int dt = dtype_of(y, "dtype");
+  const int64_t floats = cpab_b200_matmul_quantized_workspace(x.rows, w.rows, x.K);
+  const Tensor work = floats > 0 ? at::empty({floats}, like.options().dtype(at::kFloat)) : Tensor();
   check(cpab_b200_matmul_quantized(dt, &x.c, &w.c, x.rows, w.rows, x.K, bias.defined() ? dtype_of(bias, "bias") : dt,
-                                   ptr(bias), ptr_mut(y), w.rows, stream_of(like)));
+                                   ptr(bias), ptr_mut(y), w.rows, fptr_mut(work), stream_of(like)));
   return y;
 }
 

@@ -523,11 +523,13 @@ int cpab_b200_quantize_blocks(int dtype, const void *x, int64_t x_row, int64_t r
 /*
  * y[m, n] = sum_k x[m, k] weight[n, k] + bias[n] of quantized x [M, K] and weight
  * [N, K], summed in float32 and rounded once to dtype; bias [N] of dtype or
- * float32, or NULL; y's rows are y_row elements apart.
+ * float32, or NULL; y's rows are y_row elements apart.  workspace: 32-byte aligned,
+ * cpab_b200_matmul_quantized_workspace floats (for the current device; 0: may be NULL).
  */
+int64_t cpab_b200_matmul_quantized_workspace(int64_t M, int64_t N, int64_t K);
 int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, const cpab_quantized *weight,
                                int64_t M, int64_t N, int64_t K, int bias_dtype, const void *bias,
-                               void *y, int64_t y_row, cpab_stream_t stream);
+                               void *y, int64_t y_row, float *workspace, cpab_stream_t stream);
 
 /*
  * Moves matrices towards their orthogonal factor (all singular values towards 1)

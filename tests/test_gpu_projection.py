@@ -181,7 +181,8 @@ def test_products(size, dtype, path):
     near(matmul_quantized(q, rx, v, vs, dtype=dtype), q.double() * rx.double()[:, None], wv, None)
 
 
-@pytest.mark.parametrize("size", [(2048, 2304, 256), (256, 20000, 128), (40000, 300, 384), (300, 300, 20000)])
+@pytest.mark.parametrize("size", [(2048, 2304, 256), (256, 20000, 128), (40000, 300, 384), (300, 300, 20000),
+                                  (17, 361, 6942), (256, 128, 50001), (200, 70, 4097), (700, 650, 9000)])
 def test_large_products(size, path):
     """Many tiles, tall, wide and long ones; the last rows and columns too."""
     M, N, K = size
@@ -194,10 +195,28 @@ def test_large_products(size, path):
     near(y[:300], xv[:300], wv, None)
 
 
+def test_long_sums_in_parts_with_scales_of_rows_and_bias(path):
+    M, N, K = 40, 90, 9001
+    x, w = features(M, K, F32, 6), features(N, K, F32, 7)
+    b = torch.randn(N, device=DEV)
+    q, _ = quantize_blocks(x)
+    v, vs = quantize_blocks(w)
+    r, u = torch.rand(M, device=DEV) + 0.1, torch.rand(N, device=DEV) + 0.1
+    for dtype in (F32, BF16):
+        near(matmul_quantized(q, r, v, u, bias=b, dtype=dtype), q.double() * r.double()[:, None],
+             v.double() * u.double()[:, None], b)
+        near(matmul_quantized(q, r, v, vs, bias=b, dtype=dtype), q.double() * r.double()[:, None],
+             valued(*encoded(w)), b)
+
+
 def test_product_of_every_block_of_scales():
     """A scale that belongs to another block, row or column would show: one code
     of 1 in one block of one row, its scale a power of its own."""
-    M, N, K = 260, 300, 1500
+    for M, N, K in ((260, 300, 1500), (100, 60, 5000)):
+        blocks_of_scales(M, N, K)
+
+
+def blocks_of_scales(M, N, K):
     nb = -(-K // 128)
     s = (120 + torch.randint(0, 16, (M, nb), generator=torch.Generator().manual_seed(1))).to(DEV, torch.uint8)
     vs = (120 + torch.randint(0, 16, (N, nb), generator=torch.Generator().manual_seed(2))).to(DEV, torch.uint8)

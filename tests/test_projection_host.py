@@ -55,7 +55,7 @@ def test_product_entry_point_validates():
     def one(x=None, w=None, dtype=0, M=8, N=8, K=200, bias_dtype=0, bias=None, y=P, y_row=8):
         x, w = x or operand(), w or operand()
         return L.cpab_b200_matmul_quantized(dtype, ctypes.byref(x), ctypes.byref(w), M, N, K, bias_dtype, bias, y,
-                                            y_row, None)
+                                            y_row, P, None)
 
     assert one(dtype=4) == -1 and "type" in err()
     assert one(dtype=2, bias_dtype=1, bias=P) == -1 and "bias" in err()
@@ -68,7 +68,9 @@ def test_product_entry_point_validates():
     assert one(w=operand(scale_row=1)) == -1 and "scales" in err()
     assert one(w=operand(scale=4098, scale_row=0)) == -1 and "float32" in err()
     assert one(M=0) == 0 and one(N=0) == 0 and err() == ""
-    assert L.cpab_b200_matmul_quantized(0, None, None, 8, 8, 8, 0, None, P, 8, None) == -1
+    assert L.cpab_b200_matmul_quantized(0, None, None, 8, 8, 8, 0, None, P, 8, None, None) == -1
+    w = L.cpab_b200_matmul_quantized_workspace
+    assert w(0, 8, 8) == 0 and w(8, 8, 0) == 0 and w(4096, 4096, 512) == 0
 
 
 COEFFICIENTS = (ctypes.c_double * 3)(3.4445, -4.775, 2.0315)
