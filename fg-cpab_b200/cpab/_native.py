@@ -66,6 +66,7 @@ _SIGNATURES = {
                                   _c_i64, _p, _c_i64, _c_int, _p, _p, _p],
     "cpab_b200_matmul_quantized": [_c_int, _p, _p, _c_i64, _c_i64, _c_i64, _c_int, _p, _p, _c_i64,
                                    _p, _p],
+    "cpab_b200_lay_out_codes": [_c_int, _p, _p, _p, _p, _c_i64, _p],
     "cpab_b200_orthogonalize": [_c_int, _p, _c_i64, _c_i64, _c_i64, _c_int, _p, ctypes.c_double, _p,
                                 _p, _p],
     "cpab_b200_muon": [_p, _c_int, ctypes.c_double, _p, ctypes.c_double, _c_int, ctypes.c_double,
@@ -860,9 +861,14 @@ def _quantized(q, scale, name):
         raise ValueError("%s's scale must have shape %s, got %s" % (name, want, tuple(scale.shape)))
     qr = q if q.dim() == 2 else q.reshape(-1, K)
     rows = qr.shape[0]
-    if (K > 1 and qr.stride(1) != 1) or (rows > 1 and (qr.stride(0) % 16 or qr.stride(0) < K)) or \
-            qr.data_ptr() % 16:
+    if K > 1 and qr.stride(1) != 1:
         qr = _codes((rows,), K, q.device)[0].copy_(qr)
+    if (rows > 1 and (qr.stride(0) % 16 or qr.stride(0) < K)) or qr.data_ptr() % 16:
+        src, qr = qr, _codes((rows,), K, q.device)[0]
+        with _on(q.device):
+            _check(lib().cpab_b200_lay_out_codes(
+                1, (_p * 1)(_ptr(src)), (_c_i64 * 1)(src.stride(0)), (_c_i64 * 1)(rows), (_p * 1)(_ptr(qr)), K,
+                _stream(q.device)))
     if per_row:
         sr = scale.reshape(-1).contiguous()
         scale_row = 0

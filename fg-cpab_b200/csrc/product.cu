@@ -307,6 +307,44 @@ cudaError_t launch_quantize(const QuantizeArgs &a, unsigned grid, cudaStream_t s
                                                  : launch_quantize_as<T, false>(a, grid, s);
 }
 
+// ---- codes that lie otherwise ---------------------------------------------------
+
+struct LayoutArgs {
+  const uint8_t *src[2];
+  uint8_t *dst[2];
+  int64_t src_row[2], rows[2];
+  int64_t K, groups;  // 16 codes to a group
+};
+
+// Rows of codes that begin anywhere, to rows that begin on 16 bytes; the codes of up
+// to two matrices at once, 16 a thread.  (A product of 100 x 2000 x 1003 such codes takes
+// 16 us, with torch's copies of both 23.)
+__global__ void __launch_bounds__(256) k_lay_out(const __grid_constant__ LayoutArgs a) {
+  tc::dep_launch();
+  tc::dep_wait();
+  const int m = blockIdx.y;
+  const int64_t count = a.rows[m] * a.groups;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / a.groups, k = (i - row * a.groups) * 16;
+    const uint8_t *from = a.src[m] + row * a.src_row[m] + k;
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (k >= 4 && k + 20 <= a.K) {  // whole words around them lie in the row
+      const uint32_t shift = 8 * (uint32_t)(reinterpret_cast<uintptr_t>(from) & 3);
+      const uint32_t *words = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t(3));
+      uint32_t v[5];
+#pragma unroll
+      for (int j = 0; j < 5; ++j) v[j] = __ldg(words + j);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(v[j], v[j + 1], shift);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (k + j < a.K) w[j >> 2] |= (uint32_t)__ldg(from + j) << (8 * (j & 3));
+    }
+    *reinterpret_cast<uint4 *>(a.dst[m] + row * a.groups * 16 + k) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 // ---- products ------------------------------------------------------------------
 
 struct Scales {
@@ -800,6 +838,28 @@ extern "C" int cpab_b200_quantize_blocks(int dtype, const void *x, int64_t x_row
     else e = tc::launch(k_sum_tiles<__nv_bfloat16>, grid, 256, 0, 1, s, static_cast<const float *>(workspace), n, columns, static_cast<__nv_bfloat16 *>(column_sum));
   }
   return launch_status(e, "quantize_blocks");
+}
+
+extern "C" int cpab_b200_lay_out_codes(int count, const uint8_t *const *src, const int64_t *src_row,
+                                       const int64_t *rows, uint8_t *const *dst, int64_t K, cpab_stream_t stream) {
+  if (count < 0 || count > 2 || K < 1 || (count > 0 && (src == nullptr || src_row == nullptr || rows == nullptr || dst == nullptr)))
+    return report_error(CPAB_ERR_ARG, "%s", "lay_out_codes: one or two matrices of rows of codes");
+  LayoutArgs a = {};
+  a.K = K, a.groups = (K + 15) / 16;
+  int64_t most = 0;
+  for (int i = 0; i < count; ++i) {
+    if (rows[i] < 0 || src_row[i] < 0 || (rows[i] > 0 && (src[i] == nullptr || dst[i] == nullptr)) ||
+        reinterpret_cast<uintptr_t>(dst[i]) % 16)
+      return report_error(CPAB_ERR_ARG, "%s", "lay_out_codes: null codes, negative sizes, or a destination off 16 bytes");
+    if (rows[i] > kMostSize || K > kMostSize) return report_error(CPAB_ERR_SIZE, "%s", "lay_out_codes: sizes too large");
+    a.src[i] = src[i], a.dst[i] = dst[i], a.src_row[i] = src_row[i], a.rows[i] = rows[i];
+    most = std::max(most, rows[i] * a.groups);
+  }
+  if (most == 0) return report_error(CPAB_OK, "%s", "");
+  const int64_t blocks = std::min<int64_t>((most + 255) / 256, 16 * device_info().sm_count);
+  return launch_status(tc::launch(k_lay_out, dim3((unsigned)blocks, (unsigned)count), 256, 0, 1,
+                                  reinterpret_cast<cudaStream_t>(stream), a),
+                       "lay_out_codes");
 }
 
 extern "C" int64_t cpab_b200_matmul_quantized_workspace(int64_t M, int64_t N, int64_t K) {

@@ -122,6 +122,7 @@ struct Operand {
   Tensor q, scale;
   int64_t rows, K;
   cpab_quantized c;
+  bool loose = false;  // codes whose rows do not begin on multiples of 16 bytes
 };
 
 Operand operand(const Tensor &q, const Tensor &scale, const char *name) {
@@ -140,12 +141,13 @@ Operand operand(const Tensor &q, const Tensor &scale, const char *name) {
                     scale.sizes());
   o.q = q.dim() == 2 ? q : q.reshape({-1, o.K});
   o.rows = o.q.size(0);
-  if ((o.K > 1 && o.q.stride(1) != 1) || (o.rows > 1 && (o.q.stride(0) % 16 != 0 || o.q.stride(0) < o.K)) ||
-      reinterpret_cast<uintptr_t>(o.q.const_data_ptr()) % 16 != 0) {
+  if (o.K > 1 && o.q.stride(1) != 1) {
     const Tensor copy = padded({o.rows}, o.K, round_to(o.K, 16), kCodes, q);
     copy.copy_(o.q);
     o.q = copy;
   }
+  o.loose = (o.rows > 1 && (o.q.stride(0) % 16 != 0 || o.q.stride(0) < o.K)) ||
+            reinterpret_cast<uintptr_t>(o.q.const_data_ptr()) % 16 != 0;
   int64_t scale_row = 0;
   if (per_row) {
     o.scale = scale.reshape({-1}).contiguous();
@@ -157,6 +159,26 @@ Operand operand(const Tensor &q, const Tensor &scale, const char *name) {
   }
   o.c = {static_cast<const uint8_t *>(ptr(o.q)), o.rows > 1 ? o.q.stride(0) : round_to(o.K, 16), ptr(o.scale), scale_row};
   return o;
+}
+
+// Copies loose codes to where the products can read them, both operands' at once.
+void lay_out(Operand &x, Operand &w) {
+  const uint8_t *src[2];
+  uint8_t *dst[2];
+  int64_t row[2], rows[2], bytes = 0;
+  Operand *which[2];
+  int n = 0;
+  const int64_t pitch = round_to(x.K, 16);
+  for (Operand *o : {&x, &w})
+    if (o->loose) which[n] = o, src[n] = o->c.codes, row[n] = o->q.stride(0), rows[n] = o->rows, bytes += pitch * o->rows, ++n;
+  if (n == 0) return;
+  const Tensor copy = at::empty({bytes}, x.q.options().dtype(at::kByte));
+  auto *at = static_cast<uint8_t *>(ptr_mut(copy));
+  for (int i = 0; i < n; ++i) {
+    dst[i] = at, which[i]->c.codes = at, which[i]->c.row = pitch, which[i]->q = copy;
+    at += pitch * rows[i];
+  }
+  check(cpab_b200_lay_out_codes(n, src, row, rows, dst, x.K, stream_of(x.q)));
 }
 
 Operand operand(const Place &p, int64_t rows, int64_t K) {
@@ -191,7 +213,7 @@ Tensor matmul_quantized(const Tensor &q, const Tensor &scale, const Tensor &weig
     TORCH_CHECK(t->device() == q.device(), "a scale is on ", t->device(), ", the codes on ", q.device());
   TORCH_CHECK(!has_tangent({&bias}), "matmul_quantized has no gradient, of forward mode neither");
   const c10::cuda::CUDAGuard guard(q.device());
-  const Operand x = operand(q, scale, "q"), w = operand(weight, weight_scale, "weight");
+  Operand x = operand(q, scale, "q"), w = operand(weight, weight_scale, "weight");
   TORCH_CHECK_VALUE(w.K == x.K, "weight must be [N, ", x.K, "], got ", weight.sizes());
   Tensor b;
   if (bias.defined()) {
@@ -200,6 +222,8 @@ Tensor matmul_quantized(const Tensor &q, const Tensor &scale, const Tensor &weig
     require(bias, q, bias.scalar_type(), {w.rows}, "bias");
     b = bias.contiguous();
   }
+  const Tensor kept_q = x.q, kept_w = w.q;  // (until their copies are asked for)
+  lay_out(x, w);
   return product(x, w, b, q.sizes().slice(0, q.dim() - 1), type, q);
 }
 

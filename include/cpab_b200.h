@@ -521,6 +521,16 @@ int cpab_b200_quantize_blocks(int dtype, const void *x, int64_t x_row, int64_t r
                               cpab_stream_t stream);
 
 /*
+ * Rows of codes that begin anywhere, for cpab_b200_matmul_quantized: matrix i of
+ * `count` (1 or 2; arrays in host memory) has rows[i] rows of K codes, src_row[i]
+ * bytes apart, and is copied to dst[i] (16-byte aligned), whose rows are K rounded up
+ * to 16 bytes apart (filled with 0).
+ */
+int cpab_b200_lay_out_codes(int count, const uint8_t *const *src, const int64_t *src_row,
+                            const int64_t *rows, uint8_t *const *dst, int64_t K,
+                            cpab_stream_t stream);
+
+/*
  * y[m, n] = sum_k x[m, k] weight[n, k] + bias[n] of quantized x [M, K] and weight
  * [N, K], summed in float32 and rounded once to dtype; bias [N] of dtype or
  * float32, or NULL; y's rows are y_row elements apart.  workspace: 32-byte aligned,

@@ -263,6 +263,24 @@ def test_products_of_any_layout(path):
     assert matmul_quantized(q, s, v[:0], vs[:0]).shape == (M, 0)
 
 
+@pytest.mark.parametrize("K", [1, 15, 19, 20, 35, 129, 1001, 4099])
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_codes_whose_rows_begin_anywhere(rows, K, path):
+    """From every offset in a word; the bytes before and behind are NaN codes."""
+    x, w = features(rows, K, F32, 6), features(37, K, F32, 7)
+    q, s = quantize_blocks(x)
+    v, vs = quantize_blocks(w)
+    want = matmul_quantized(q, s, v, vs, dtype=F32)
+    for lead in range(5):
+        loose = []
+        for c in (q, v):
+            t = torch.full((c.shape[0], K + 2 * lead + 1), 0x7F, device=DEV, dtype=torch.uint8).view(CODES)[:, lead:lead + K]
+            loose.append(t.copy_(c))
+        assert torch.equal(matmul_quantized(loose[0], s, loose[1], vs, dtype=F32), want)
+        assert torch.equal(matmul_quantized(q, s, loose[1], vs, dtype=F32), want)
+        assert torch.equal(matmul_quantized(loose[0], s, v, vs, dtype=F32), want)
+
+
 def test_a_block_of_nan_reaches_its_row_alone(path):
     x, w = features(300, 500, F32, 8), features(200, 500, F32, 9)
     x[17, 130] = float("inf")

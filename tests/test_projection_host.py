@@ -73,6 +73,19 @@ def test_product_entry_point_validates():
     assert w(0, 8, 8) == 0 and w(8, 8, 0) == 0 and w(4096, 4096, 512) == 0
 
 
+def test_layout_entry_point_validates():
+    L = _native.lib()
+    one = lambda v: (ctypes.c_void_p * 1)(v)  # noqa: E731
+    size = lambda v: (ctypes.c_int64 * 1)(v)  # noqa: E731
+    ok = [1, one(4097), size(33), size(5), one(4096), 33, None]
+    f = L.cpab_b200_lay_out_codes
+    assert call(f, ok, a0=3) == -1 and call(f, ok, a5=0) == -1 and call(f, ok, a1=None) == -1
+    assert call(f, ok, a4=one(4100)) == -1 and "16" in err()
+    assert call(f, ok, a1=one(None)) == -1 and call(f, ok, a3=size(-1)) == -1
+    assert call(f, ok, a3=size(1 << 31)) == -4
+    assert call(f, ok, a3=size(0)) == 0 and call(f, ok, a0=0) == 0 and err() == ""
+
+
 COEFFICIENTS = (ctypes.c_double * 3)(3.4445, -4.775, 2.0315)
 
 
