@@ -286,6 +286,18 @@ def test_a_block_of_nan_reaches_its_row_alone(path):
     x[17, 130] = float("inf")
     y = matmul_quantized(*quantize_blocks(x), *quantize_blocks(w))
     assert y[17].isnan().all() and y.isnan().sum() == 200
+    for rows in (slice(17, 18), slice(14, 20), slice(5, 18)):       # (few rows)
+        y = matmul_quantized(*quantize_blocks(x[rows]), *quantize_blocks(w))
+        assert y.isnan().sum() == 200 and y.isnan().all(1).sum() == 1
+        y = matmul_quantized(*quantize_blocks(w), *quantize_blocks(x[rows]))
+        assert y.isnan().sum() == 200 and y.isnan().all(0).sum() == 1
+    # a NaN in the gradient reaches its row of dx, its column of the transposed product
+    x[17, 130] = 0.0
+    x.requires_grad_(True)
+    dy = torch.ones(300, 200, device=DEV)
+    dy[3, 7] = float("nan")
+    (dx,) = torch.autograd.grad(linear_quantized(x, w), x, dy)
+    assert dx[3].isnan().all() and dx.isnan().sum() == 500
 
 
 def test_an_8_bit_norm_feeds_a_product(path):
