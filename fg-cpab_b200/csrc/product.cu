@@ -333,13 +333,13 @@ __global__ void __launch_bounds__(256) k_lay_out(const __grid_constant__ LayoutA
       const uint32_t *words = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(from) & ~uintptr_t(3));
       uint32_t v[5];
 #pragma unroll
-      for (int j = 0; j < 5; ++j) v[j] = __ldg(words + j);
+      for (int j = 0; j < 5; ++j) v[j] = words[j];
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(v[j], v[j + 1], shift);
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        if (k + j < a.K) w[j >> 2] |= (uint32_t)__ldg(from + j) << (8 * (j & 3));
+        if (k + j < a.K) w[j >> 2] |= (uint32_t)from[j] << (8 * (j & 3));
     }
     *reinterpret_cast<uint4 *>(a.dst[m] + row * a.groups * 16 + k) = make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -382,11 +382,11 @@ __device__ __forceinline__ void scale_words(const Scales &s, int row, int rows, 
   for (int q = 0; q < 2; ++q) {
     w[q] = 0;
     if (s.words && first + 4 * q + 4 <= blocks) {
-      w[q] = __ldg(reinterpret_cast<const uint32_t *>(p) + q);
+      w[q] = reinterpret_cast<const uint32_t *>(p)[q];
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (first + 4 * q + i < blocks) w[q] |= (uint32_t)__ldg(p + 4 * q + i) << (8 * i);
+        if (first + 4 * q + i < blocks) w[q] |= (uint32_t)p[4 * q + i] << (8 * i);
     }
   }
 }
@@ -619,11 +619,11 @@ struct FewArgs {
 
 // 16 codes of a row from k on; 0 past its end.
 __device__ __forceinline__ uint4 sixteen(const uint8_t *row, int k, int K) {
-  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4 *>(row + k));
+  if (k + 16 <= K) return *reinterpret_cast<const uint4 *>(row + k);
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    if (k + i < K) w[i >> 2] |= (uint32_t)__ldg(row + k + i) << (8 * (i & 3));
+    if (k + i < K) w[i >> 2] |= (uint32_t)row[k + i] << (8 * (i & 3));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 // Two codes (the low or high half of a word) as halves.
@@ -636,7 +636,7 @@ __device__ __forceinline__ float power(uint32_t e) {
   return __uint_as_float(e == 255u ? 0x7FC00000u : e == 0u ? 0x00400000u : e << 23);
 }
 __device__ __forceinline__ float scale_of(const Scales &s, int64_t row, int block) {
-  return s.bytes == nullptr ? 1.f : power(__ldg(s.bytes + row * s.row + block));
+  return s.bytes == nullptr ? 1.f : power(s.bytes[row * s.row + block]);
 }
 
 template <typename T, typename TB, int TILES>
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = b * 128 + 64 * h + 16 * t;
-        f.p[h] = __ldg(reinterpret_cast<const uint4 *>(w0 + k)), f.q[h] = __ldg(reinterpret_cast<const uint4 *>(w1 + k));
+        f.p[h] = *reinterpret_cast<const uint4 *>(w0 + k), f.q[h] = *reinterpret_cast<const uint4 *>(w1 + k);
       }
     } else if (b < a.blocks) {
 #pragma unroll
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
     }
     f.s0 = f.s1 = 127u;
     if (a.sw.bytes != nullptr && b < a.blocks)
-      f.s0 = __ldg(a.sw.bytes + r0 * a.sw.row + b), f.s1 = __ldg(a.sw.bytes + r1 * a.sw.row + b);
+      f.s0 = a.sw.bytes[r0 * a.sw.row + b], f.s1 = a.sw.bytes[r1 * a.sw.row + b];
   };
   auto multiply = [&](int b, const Block &f) {
     const float s0 = power(f.s0), s1 = power(f.s1);

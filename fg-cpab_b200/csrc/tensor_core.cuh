@@ -99,7 +99,9 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Programmatic launch: the next kernel of the stream may begin while this one
-// ends; what it reads of this one's results it reads after dep_wait.
+// ends; what it reads of this one's results it reads after dep_wait, and with ordinary
+// loads: read-only ones (__ldg, ld.global.nc) are for memory that nothing writes while
+// the kernel runs, and it runs while this one writes.
 __device__ __forceinline__ void dep_launch() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ void dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
