@@ -347,16 +347,35 @@ __global__ void __launch_bounds__(256) k_lay_out(const __grid_constant__ LayoutA
 
 // ---- products ------------------------------------------------------------------
 
+// An operand's scales: of blocks, or of rows.  A row's float32 scale is taken apart: its
+// power of two goes to each of its blocks, so that the sums are within a factor 4 of the
+// results and leave float32's range only where those do, and the rest (1 to 2) to the
+// sum.  (As one factor of the sum, 1e30 and the other operand's 1e-33 came to infinity; a
+// choice of the order for each element made 8192 x 8192 x 8192 547 us.)
 struct Scales {
-  const uint8_t *bytes;  // e8m0 [rows, row], or null: all 1
+  const uint8_t *bytes;  // e8m0 [rows, row], or null
   int64_t row;
   int words;             // rows begin on multiples of 4 bytes
+  const float *rows;     // float32 [rows], or null
 };
+
+// A row's scale as a byte's power of two (an infinity and a NaN have none), and the rest.
+__device__ __forceinline__ uint32_t row_power(float r) {
+  const uint32_t e = __float_as_uint(r) >> 23 & 255u;
+  return e == 255u ? 127u : max(e, 1u);
+}
+__device__ __forceinline__ float row_rest(float r) {
+  const uint32_t bits = __float_as_uint(r), e = bits & 0x7F800000u;
+  if (e == 0u) return r * 0x1p126f;
+  return e == 0x7F800000u ? r : __uint_as_float((bits & 0x807FFFFFu) | 0x3F800000u);
+}
+__device__ __forceinline__ float row_rest(const Scales &s, int64_t row) {
+  return s.rows != nullptr ? row_rest(s.rows[row]) : 1.f;
+}
 
 struct ProductArgs {
   CUtensorMap a, b;
   Scales sa, sb;
-  const float *ra, *rb;  // float32 scales of rows of A, of B, or null
   const void *bias;
   void *y;
   int64_t y_row;
@@ -369,9 +388,14 @@ struct ProductArgs {
   int64_t pitch;
 };
 
-// A row's scales of 8 steps.  Rows outside hold no codes: any scale but NaN.
+// A row's scales of 8 steps (of a row's one scale its bits, until all are asked for).
+// Rows outside hold no codes: any scale but NaN.
 __device__ __forceinline__ void scale_words(const Scales &s, int row, int rows, int group, int blocks, uint32_t (&w)[2]) {
-  if (s.bytes == nullptr || row >= rows) {
+  if (s.rows != nullptr) {
+    w[0] = row < rows ? __float_as_uint(s.rows[row]) : 0x3F800000u;
+    return;
+  }
+  if (row >= rows) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) w[q] = 0x7F7F7F7Fu;
     return;
@@ -439,12 +463,15 @@ struct Product {
   __device__ void scales_b(const Tile &t, int row, int g, uint32_t (&w)[2]) const {
     scale_words(a.sb, t.n0 + row, a.N, t.part * (a.each / 8) + g, a.steps, w);
   }
+  __device__ bool one_a() const { return a.sa.rows != nullptr; }
+  __device__ bool one_b() const { return a.sb.rows != nullptr; }
+  __device__ void words_of_one(uint32_t (&w)[2]) const { w[0] = w[1] = 0x01010101u * row_power(__uint_as_float(w[0])); }
   __device__ void begin(const Tile &t, Shared &sh, int thread) const {
-    if (a.splits > 1 || (a.rb == nullptr && a.bias == nullptr)) return;
+    if (a.splits > 1 || (a.sb.rows == nullptr && a.bias == nullptr)) return;
     if (thread < BN) {
       const int n = t.n0 + thread;
       const bool in = n < a.N;
-      sh.scale[t.slot][thread] = in && a.rb != nullptr ? a.rb[n] : 1.f;
+      sh.scale[t.slot][thread] = in ? row_rest(a.sb, n) : 1.f;
       sh.bias[t.slot][thread] = in && a.bias != nullptr ? to_f32(static_cast<const TB *>(a.bias)[n]) : 0.f;
     }
     tc::epilogue_sync();
@@ -467,8 +494,8 @@ struct Product {
       return;
     }
     uint4(&rows)[32][5] = sh.rows[(threadIdx.x >> 5) - 4];
-    const float ra = a.ra != nullptr && row < a.M ? a.ra[row] : 1.f;
-    const bool columns = a.rb != nullptr || a.bias != nullptr;
+    const float ra = row < a.M ? row_rest(a.sa, row) : 1.f;
+    const bool columns = a.sb.rows != nullptr || a.bias != nullptr;
     __syncwarp();
 #pragma unroll
     for (int h = 0; h < 4; ++h) {  // 16 bytes
@@ -516,11 +543,11 @@ __global__ void __launch_bounds__(256) k_join_product(const __grid_constant__ Pr
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / a.N, col = i - row * a.N;
     const float *from = a.parts + row * a.pitch + col;
+    const float ra = row_rest(a.sa, row), rb = row_rest(a.sb, col);
     float v = 0.f;
 #pragma unroll 8
     for (int k = 0; k < a.splits; ++k) v += from[k * plane];
-    if (a.ra != nullptr) v *= a.ra[row];
-    if (a.rb != nullptr) v *= a.rb[col];
+    v *= ra, v *= rb;
     if (a.bias != nullptr) v += to_f32(static_cast<const TB *>(a.bias)[col]);
     static_cast<T *>(a.y)[row * a.y_row + col] = from_f32<T>(v);
   }
@@ -610,7 +637,9 @@ struct FewArgs {
   const uint8_t *x, *w;
   int64_t x_row, w_row;
   Scales sx, sw;
-  const float *rx, *rw;  // float32 scales of rows, or null
+  // A row's scale beside the other operand's blocks: its power of two is that of each of
+  // its blocks.  (Where both have rows' the sums are of codes alone.)
+  const float *x_one, *w_one;
   const void *bias;
   void *y;
   int64_t y_row;
@@ -635,8 +664,16 @@ __device__ __forceinline__ uint32_t two_halves(uint32_t w, bool high) {
 __device__ __forceinline__ float power(uint32_t e) {
   return __uint_as_float(e == 255u ? 0x7FC00000u : e == 0u ? 0x00400000u : e << 23);
 }
-__device__ __forceinline__ float scale_of(const Scales &s, int64_t row, int block) {
-  return s.bytes == nullptr ? 1.f : power(s.bytes[row * s.row + block]);
+// Whether one is so far from 1 that a block's sum of products of codes (a multiple of
+// 2^-18, at most 2^25) times it alone can leave float32's normal range.
+__device__ __forceinline__ bool is_far(uint32_t e) { return e - 67u > 120u; }
+// Such a sum times two of them, the smaller first (which is exact, down to 2^-145).
+__device__ __forceinline__ float by_powers(float v, float a, float b) { return a < b ? v * a * b : v * b * a; }
+// v (2^-18 to 2^51 or 0) times two rows' powers, half of their sum's at a time: only what
+// ends as 0 or an infinity leaves float32's range between.
+__device__ __forceinline__ float by_rows(float v, float a, float b) {
+  const int e = (int)(row_power(a) + row_power(b)) - 254, p = e >> 1;
+  return v * __uint_as_float((uint32_t)(p + 127) << 23) * __uint_as_float((uint32_t)(e - p + 127) << 23);
 }
 
 template <typename T, typename TB, int TILES>
@@ -678,7 +715,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
       f.s0 = a.sw.bytes[r0 * a.sw.row + b], f.s1 = a.sw.bytes[r1 * a.sw.row + b];
   };
   auto multiply = [&](int b, const Block &f) {
-    const float s0 = power(f.s0), s1 = power(f.s1);
+    uint32_t u0 = f.s0, u1 = f.s1;
+    if (a.w_one != nullptr) u0 = row_power(a.w_one[r0]), u1 = row_power(a.w_one[r1]);
+    const bool far = is_far(u0) || is_far(u1);
+    const float s0 = power(u0), s1 = power(u1);
     float acc[TILES][4] = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -704,9 +744,17 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int c0 = min(8 * i + 2 * t, a.M - 1), c1 = min(8 * i + 2 * t + 1, a.M - 1);
-      const float x0 = scale_of(a.sx, c0, b), x1 = scale_of(a.sx, c1, b);
-      sum[i][0] = fmaf(acc[i][0] * s0, x0, sum[i][0]), sum[i][1] = fmaf(acc[i][1] * s0, x1, sum[i][1]);
-      sum[i][2] = fmaf(acc[i][2] * s1, x0, sum[i][2]), sum[i][3] = fmaf(acc[i][3] * s1, x1, sum[i][3]);
+      uint32_t e0 = 127u, e1 = 127u;
+      if (a.sx.bytes != nullptr) e0 = a.sx.bytes[c0 * a.sx.row + b], e1 = a.sx.bytes[c1 * a.sx.row + b];
+      if (a.x_one != nullptr) e0 = row_power(a.x_one[c0]), e1 = row_power(a.x_one[c1]);
+      const float x0 = power(e0), x1 = power(e1);
+      if (!far) {
+        sum[i][0] = fmaf(acc[i][0] * s0, x0, sum[i][0]), sum[i][1] = fmaf(acc[i][1] * s0, x1, sum[i][1]);
+        sum[i][2] = fmaf(acc[i][2] * s1, x0, sum[i][2]), sum[i][3] = fmaf(acc[i][3] * s1, x1, sum[i][3]);
+      } else {
+        sum[i][0] += by_powers(acc[i][0], s0, x0), sum[i][1] += by_powers(acc[i][1], s0, x1);
+        sum[i][2] += by_powers(acc[i][2], s1, x0), sum[i][3] += by_powers(acc[i][3], s1, x1);
+      }
     }
   };
   // Three blocks in flight.
@@ -737,14 +785,16 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
     part[warp][g][8 * i + 2 * t] = sum[i][0], part[warp][g][8 * i + 2 * t + 1] = sum[i][1];
     part[warp][g + 8][8 * i + 2 * t] = sum[i][2], part[warp][g + 8][8 * i + 2 * t + 1] = sum[i][3];
   }
-  __syncthreads();
   const int r = threadIdx.x & 15, m = threadIdx.x >> 4;
+  const float rx = a.sx.rows != nullptr ? a.sx.rows[min(m, a.M - 1)] : 1.f;
+  const float rw = a.sw.rows != nullptr ? a.sw.rows[min(n0 + r, a.N - 1)] : 1.f;
+  __syncthreads();
   if (m >= 8 * TILES || m >= a.M || n0 + r >= a.N) return;
   float v = 0.f;
 #pragma unroll
   for (int k = 0; k < kFewWarps; ++k) v += part[k][r][m];
-  if (a.rx != nullptr) v *= a.rx[m];
-  if (a.rw != nullptr) v *= a.rw[n0 + r];
+  v = v * row_rest(rx) * row_rest(rw);
+  if (a.sx.rows != nullptr && a.sw.rows != nullptr) v = by_rows(v, rx, rw);
   if (a.bias != nullptr) v += to_f32(static_cast<const TB *>(a.bias)[n0 + r]);
   static_cast<T *>(a.y)[m * a.y_row + n0 + r] = from_f32<T>(v);
 }
@@ -769,19 +819,19 @@ cudaError_t launch_few(const FewArgs &a, cudaStream_t s) {
 }
 
 // What an operand lacks, or null; fills its scales.
-const char *operand(const cpab_quantized &o, int64_t K, Scales *blocks, const float **per_row) {
+const char *operand(const cpab_quantized &o, int64_t K, Scales *scales) {
   if (o.codes == nullptr || o.scale == nullptr) return "null codes or scales";
   if (reinterpret_cast<uintptr_t>(o.codes) % 16 || o.row % 16 || o.row < K)
     return "codes must begin on 16 bytes, each row on a multiple of 16 that holds it";
-  *per_row = nullptr, *blocks = {nullptr, 0, 0};
+  *scales = {};
   if (o.scale_row == 0) {
     if (reinterpret_cast<uintptr_t>(o.scale) % 4) return "float32 scales must begin on 4 bytes";
-    *per_row = static_cast<const float *>(o.scale);
+    scales->rows = static_cast<const float *>(o.scale);
   } else {
     const int64_t n = (K + kBlock - 1) / kBlock;
     if (o.scale_row < n) return "a row of scales must hold one for each 128 codes";
     const bool words = reinterpret_cast<uintptr_t>(o.scale) % 4 == 0 && o.scale_row % 4 == 0;
-    *blocks = {static_cast<const uint8_t *>(o.scale), o.scale_row, words};
+    *scales = {static_cast<const uint8_t *>(o.scale), o.scale_row, words, nullptr};
   }
   return nullptr;
 }
@@ -880,8 +930,8 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   if (M == 0 || N == 0) return report_error(CPAB_OK, "%s", "");
   if (y == nullptr) return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: null y");
   ProductArgs a = {};
-  const char *why = operand(*x, K, &a.sa, &a.ra);
-  if (why == nullptr) why = operand(*weight, K, &a.sb, &a.rb);
+  const char *why = operand(*x, K, &a.sa);
+  if (why == nullptr) why = operand(*weight, K, &a.sb);
   if (why == nullptr && !is_few(M, N, K)) {
     const int tile = tile_of(M, N, (K + kBlock - 1) / kBlock), columns = tile == 0 ? 64 : 128;  // of B a block loads
     a.a_rows = tile == 2 || M > 64 ? 128 : M > 32 ? 64 : M > 16 ? 32 : 16;
@@ -899,7 +949,8 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (is_few(M, N, K)) {
-    const FewArgs f = {x->codes, weight->codes, x->row, weight->row, a.sa, a.sb, a.ra, a.rb, bias, y, y_row,
+    const FewArgs f = {x->codes, weight->codes, x->row, weight->row, a.sa, a.sb, a.sb.rows == nullptr ? a.sa.rows : nullptr,
+                       a.sa.rows == nullptr ? a.sb.rows : nullptr, bias, y, y_row,
                        (int)M, (int)N, (int)K, a.steps};
     if (dtype == CPAB_F32) e = launch_few<float, float>(f, s);
     else if (dtype == CPAB_F16) e = bias_dtype == CPAB_F32 ? launch_few<__half, float>(f, s) : launch_few<__half, __half>(f, s);

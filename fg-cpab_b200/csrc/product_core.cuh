@@ -25,7 +25,9 @@
 //                     parts lie kAHalf and kBHalf bytes behind the first
 //   stage_bytes()                   bytes that a stage's copies bring, to all blocks
 //   scales_a(tile, rank, row, group, words), scales_b(tile, row, group, words)
-//                     a row's scales of 8 steps, four to a word (kScaled)
+//                     asks for a row's scales of 8 steps, four to a word (kScaled);
+//   one_a(), one_b(), words_of_one(words)  whether a row has one scale, and the words of
+//                     that one, once all rows' are asked for
 //   begin(tile, shared, thread)     before a tile's accumulators are waited for
 //   Ahead, ahead(tile, row, column)  what store reads besides, asked for a chunk early
 //   store(tile, shared, row, column, values, ahead)  kChunk values of this thread's row;
@@ -220,6 +222,12 @@ __device__ __forceinline__ void core(const P &p) {
               if (warp == 3) p.scales_b(t, 128 * c + lane + 32 * j, g, w[c][j]);
               else if (c == 0) p.scales_a(t, rank, lane + 32 * j, g, w[c][j]);
             }
+          if (warp == 3 ? p.one_b() : p.one_a()) {
+#pragma unroll
+            for (int c = 0; c < kB; ++c)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) p.words_of_one(w[c][j]);
+          }
           ok = bar_wait_warp(sempty + 8 * sc, sphase ^ 1);
           uint8_t *to = scales + sc * S::kSlotBytes + 16 * lane + (warp == 3 ? 512 : 0);
 #pragma unroll

@@ -8,6 +8,7 @@ import torch
 
 from cpab import _ext, _native
 from cpab.pytorch.projection import matmul_quantized, quantize_blocks
+from test_gpu_projection import near, valued
 
 pytestmark = [pytest.mark.gpu,
               pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA GPU")]
@@ -59,3 +60,88 @@ def test_codes_made_anew_in_one_buffer(M):
             one = quantize_blocks(xs[k])
             torch.cuda.synchronize()
             assert torch.equal(ys[k], matmul_quantized(*one, w, ws, dtype=F32)), (turn, k)
+
+
+# Rows that take each of the kernels: one pass (8 and 16 rows at a time), tiles, tiles
+# whose sum is cut into parts, pairs of tiles.
+ROWS = [(1, 70, 300), (8, 70, 300), (9, 70, 300), (16, 70, 300), (17, 70, 300), (40, 90, 9001), (300, 200, 500)]
+
+
+def codes(R, K, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(R, K, generator=g) * 20).to(DEV).to(CODES)
+
+
+def powers(R, K, near_, seed):
+    """Scales of blocks, as bytes, within 8 times of 2^near_."""
+    g = torch.Generator().manual_seed(seed)
+    return (127 + near_ + torch.randint(-3, 4, (R, -(-K // 128)), generator=g)).to(torch.uint8).to(DEV)
+
+
+def by_blocks(q, s):
+    return valued(q, s.long() - 127)
+
+
+def by_rows(q, r):
+    return q.double() * r.double()[:, None]
+
+
+@pytest.mark.parametrize("far", [(115, -108), (-108, 115), (-120, 110), (124, -124)])
+@pytest.mark.parametrize("size", ROWS)
+def test_scales_of_blocks_far_apart(size, far, path):
+    """One scale near float32's end, the other near its beginning: the result is
+    neither, whichever kernel the number of rows takes."""
+    M, N, K = size
+    q, v = codes(M, K, 1), codes(N, K, 2)
+    s, vs = powers(M, K, far[0], 3), powers(N, K, far[1], 4)
+    y = matmul_quantized(q, s.view(SCALES), v, vs.view(SCALES), dtype=F32)
+    near(y, by_blocks(q, s), by_blocks(v, vs), None)
+    if M > 1:                       # a row alone is what it is among others
+        one = matmul_quantized(q[:1], s[:1].view(SCALES), v, vs.view(SCALES), dtype=F32)
+        near(one, by_blocks(q[:1], s[:1]), by_blocks(v, vs), None)
+
+
+@pytest.mark.parametrize("far", [(1e30, 1e-33), (1e-37, 1e36), (3e38, 1e-38), (1e-44, 1e38)])
+@pytest.mark.parametrize("size", ROWS)
+def test_scales_of_rows_far_apart(size, far, path):
+    M, N, K = size
+    q, v = codes(M, K, 1), codes(N, K, 2)
+    g = torch.Generator().manual_seed(5)
+    r, u = (((0.5 + torch.rand(n, generator=g) / 2) * f).to(DEV) for n, f in zip((M, N), far))
+    b = torch.randn(N, generator=g).to(DEV) * (far[0] * far[1])
+    for bias in (None, b):
+        near(matmul_quantized(q, r, v, u, bias=bias, dtype=F32), by_rows(q, r), by_rows(v, u), bias)
+
+
+@pytest.mark.parametrize("far", [(1e-33, 110), (1e30, -105), (2e-38, 124), (1e-44, 119)])
+@pytest.mark.parametrize("size", ROWS)
+def test_a_scale_of_rows_far_from_those_of_blocks(size, far, path):
+    M, N, K = size
+    g = torch.Generator().manual_seed(6)
+    for rows_first in (True, False):
+        q, v = codes(M, K, 1), codes(N, K, 2)
+        R, B = (M, N) if rows_first else (N, M)
+        r = ((0.5 + torch.rand(R, generator=g) / 2) * far[0]).to(DEV)
+        s = powers(B, K, far[1], 7)
+        if rows_first:
+            y, x, w = matmul_quantized(q, r, v, s.view(SCALES), dtype=F32), by_rows(q, r), by_blocks(v, s)
+        else:
+            y, x, w = matmul_quantized(q, s.view(SCALES), v, r, dtype=F32), by_blocks(q, s), by_rows(v, r)
+        near(y, x, w, None)
+
+
+def test_scales_of_nothing_and_of_no_number(path):
+    """A row's scale of 0, an infinity or a NaN is what it is beside any other's."""
+    q, v = codes(20, 200, 1), codes(30, 200, 2)
+    u = torch.full((30,), 1e-30, device=DEV)
+    s = powers(30, 200, -100, 3)
+    r = torch.ones(20, device=DEV)
+    r[3], r[5], r[7], r[9] = 0.0, float("inf"), float("nan"), -2e30
+    for rows in (slice(0, 20), slice(0, 10), slice(3, 4), slice(5, 6)):
+        for scale, value in ((u, by_rows(v, u)), (s.view(SCALES), by_blocks(v, s))):
+            y = matmul_quantized(q[rows], r[rows], v, scale, dtype=F32)
+            want = (q[rows].double() @ value.t()) * r[rows].double()[:, None]
+            assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.isinf(), want.isinf())
+            ok = want.isfinite()
+            assert (y.double() - want)[ok].abs().max() <= 1e-5 * want[ok].abs().max() if ok.any() else True
+            assert torch.equal(y[want.isinf()].sign(), want[want.isinf()].sign().float())
