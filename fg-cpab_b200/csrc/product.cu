@@ -415,10 +415,23 @@ __device__ __forceinline__ void scale_words(const Scales &s, int row, int rows, 
   }
 }
 
-// y = A B^T in tiles of 128 CTAS x BN.
-template <typename T, typename TB, int CTAS, int BN>
+// Longer sums are cut into segments of so many steps, which are added in registers: what
+// an accumulator cuts off has one sign, in the mean 2.2e-8 of the sum for each 32 codes
+// of like signs.  Float32 results are at most 5.6e-6 off by it (in one piece 3.9e-5 at
+// 32768 codes and 2.8e-4 at 131072), 16-bit ones 1.1e-5 (2^20 codes: 4e-3, a whole
+// rounding to bfloat16).  A segment's end costs 1 us of its 26 (2048 x 2048 x 32768 in
+// float32: 104 -> 108 us), segments of 16 steps 19% of the whole.
+template <typename T>
+constexpr int longest_sum() {
+  return sizeof(T) == 4 ? 64 : 128;
+}
+
+// y = A B^T in tiles of 128 CTAS x BN.  LONG: with segments (kernels of their own: their
+// registers made 16384 x 4096 x 2048 in float32 162 us, without 128).
+template <typename T, typename TB, int CTAS, int BN, bool LONG>
 struct Product {
-  static constexpr int kCtas = CTAS, kBN = BN, kAcc = BN * 2 + 16 <= 512 ? 2 : 1, kParts = 1, kSegment = 0;
+  static constexpr int kCtas = CTAS, kBN = BN, kAcc = BN * 2 + 16 <= 512 ? 2 : 1, kParts = 1;
+  static constexpr int kSegment = LONG ? longest_sum<T>() : 0;
   static constexpr int kChunk = 64 / sizeof(T);  // 64 bytes of a row at a time
   static constexpr bool kScaled = true, kBMn = false;
   // A tile's columns' scales and bias; the next tile's are written while slow warps
@@ -553,15 +566,15 @@ __global__ void __launch_bounds__(256) k_join_product(const __grid_constant__ Pr
   }
 }
 
-template <typename T, typename TB, int CTAS, int BN>
+template <typename T, typename TB, int CTAS, int BN, bool LONG>
 __global__ void __launch_bounds__(tc::kCoreThreads, 1) k_product(const __grid_constant__ ProductArgs a) {
-  tc::core(Product<T, TB, CTAS, BN>{a});
+  tc::core(Product<T, TB, CTAS, BN, LONG>{a});
 }
 
 template <typename T, typename TB, int CTAS, int BN>
 cudaError_t launch_product_as(ProductArgs &a, cudaStream_t s) {
-  using S = tc::CoreShape<Product<T, TB, CTAS, BN>>;
-  auto *kernel = k_product<T, TB, CTAS, BN>;
+  using S = tc::CoreShape<Product<T, TB, CTAS, BN, false>>;  // (as large with segments)
+  auto *kernel = a.each > longest_sum<T>() ? k_product<T, TB, CTAS, BN, true> : k_product<T, TB, CTAS, BN, false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
   if (e != cudaSuccess) return e;
   a.tiles_m = (a.M + 128 * CTAS - 1) / (128 * CTAS);

@@ -145,3 +145,34 @@ def test_scales_of_nothing_and_of_no_number(path):
             ok = want.isfinite()
             assert (y.double() - want)[ok].abs().max() <= 1e-5 * want[ok].abs().max() if ok.any() else True
             assert torch.equal(y[want.isinf()].sign(), want[want.isinf()].sign().float())
+
+
+def drift(M, N, K, dtype):
+    """The mean relative error of sums of like signs, of 16 x 64 results (rows of other
+    sizes, so that their roundings differ)."""
+    g = torch.Generator(DEV).manual_seed(1)
+    # codes of 2^-5 to 3.75, whose products are multiples of 2^-16
+    q, v = (torch.randint(0x10, 0x48, (n, K), device=DEV, dtype=torch.uint8, generator=g).view(CODES) for n in (M, N))
+    r, u = (torch.rand(n, device=DEV, generator=g) * f + f for n, f in ((M, 1.0), (N, 2.0 ** -30)))
+    y = matmul_quantized(q, r, v, u, dtype=dtype)
+    rows, columns = torch.arange(0, M, max(1, M // 16)), torch.arange(0, N, max(1, N // 64))
+    want = sum(q[rows, k:k + 32768].double() @ v[columns, k:k + 32768].double().t() for k in range(0, K, 32768))
+    want = want * r[rows].double()[:, None] * u[columns].double()
+    return ((y[rows][:, columns].double() - want) / want).mean().item()
+
+
+@pytest.mark.parametrize("size", [(2048, 2048, 32768), (2048, 2048, 131072), (1000, 1000, 65536), (128, 2048, 65536),
+                                  (64, 64, 262144)])
+def test_long_sums_of_like_signs_do_not_drift(size):
+    """What an instruction of 32 codes cuts off its sum is less than 2^-23 of it and has
+    one sign, evenly spread.  A sum that grows evenly is cut, in the mean over its course,
+    by half of half of that: n instructions' errors come to n / 4 2^-23 of it (the sum is
+    at a power of two's end at worst).  Float32 sums begin anew every 256 instructions,
+    and are then added with roundings, which have both signs."""
+    assert abs(drift(*size, F32)) <= (256 + 1) / 4 * 2.0 ** -23 + 2.0 ** -24
+
+
+def test_very_long_sums_of_like_signs_do_not_drift_in_16_bits():
+    """As above with 512 instructions; a rounding to bfloat16, 2^-8 at most, has both
+    signs: the mean of 1024 of them is within 5 sqrt(1 / 3 / 1024) 2^-8."""
+    assert abs(drift(1600, 1600, 1 << 20, BF16)) <= (512 + 1) / 4 * 2.0 ** -23 + 5 * (1 / 3 / 1024) ** 0.5 * 2.0 ** -8
