@@ -350,12 +350,17 @@ struct PhaseArgs {
   int groups, step;
 };
 
-template <int PHASE, int PARTS, int CTAS, int BN>
+// What the tensor cores cut off a sum has one sign.  16-bit matrices: 1.5e-5 of the sum at
+// 4096 summed, beside 2^-12 of its operands, but 2^20 summed halves in 8 parts took the
+// result of 300 x 2^20 from 2.2e-3 to 3.9e-3 off.  X X^T of over kLongest stages (LONG,
+// kernels of their own) therefore adds segments of as many in registers.
+constexpr int kLongest = 128;
+
+template <int PHASE, int PARTS, int CTAS, int BN, bool LONG>
 struct Schulz {
   static constexpr int kCtas = CTAS, kBN = BN, kAcc = 2, kParts = PARTS;
   static constexpr int kChunk = PARTS == 2 && BN == 256 ? 16 : 32;
-  // (16-bit results: up to 1.5e-5 of the sum at 4096 summed, against 2^-12 of its operands)
-  static constexpr int kSegment = PARTS == 2 ? 4 : 0;
+  static constexpr int kSegment = PARTS == 2 ? 4 : LONG ? kLongest : 0;
   static constexpr bool kScaled = false, kBMn = PHASE >= kUpdate, kSymmetric = PHASE <= kSquare;
   static constexpr int kBM = 128 * CTAS, kAcross = kBM / BN;
   static_assert(kBM % BN == 0, "tiles of symmetric results begin on the diagonal");
@@ -518,16 +523,20 @@ struct Schulz {
   }
 };
 
-template <int PHASE, int PARTS, int CTAS, int BN>
+template <int PHASE, int PARTS, int CTAS, int BN, bool LONG>
 __global__ void __launch_bounds__(tc::kCoreThreads, 1)
     k_schulz(const __grid_constant__ PhaseArgs a) {
-  tc::core(Schulz<PHASE, PARTS, CTAS, BN>{a});
+  tc::core(Schulz<PHASE, PARTS, CTAS, BN, LONG>{a});
 }
 
 template <int PHASE, int PARTS, int CTAS, int BN>
 cudaError_t launch_phase_as(PhaseArgs &a, const int *batch, cudaStream_t s) {
-  using S = tc::CoreShape<Schulz<PHASE, PARTS, CTAS, BN>>;
-  auto *kernel = k_schulz<PHASE, PARTS, CTAS, BN>;
+  using S = tc::CoreShape<Schulz<PHASE, PARTS, CTAS, BN, false>>;  // (as large with segments)
+  auto *kernel = k_schulz<PHASE, PARTS, CTAS, BN, false>;
+  if constexpr (PHASE == kGram && PARTS == 1) {
+    for (int g = 0; g < a.groups; ++g)
+      if (a.g[g].steps > kLongest) kernel = k_schulz<PHASE, PARTS, CTAS, BN, true>;
+  }
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
   if (e != cudaSuccess) return e;
   int64_t tiles = 0;

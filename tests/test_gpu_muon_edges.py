@@ -1,0 +1,34 @@
+"""orthogonalize, muon_ and Muon at the edges of what they take."""
+import contextlib
+
+import pytest
+import torch
+
+from cpab import _ext
+from cpab.optim import orthogonalize
+from test_gpu_muon import exact, matrices, most, off
+
+pytestmark = [pytest.mark.gpu,
+              pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA GPU")]
+DEV = "cuda"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(params=["ext", "python"])
+def path(request):
+    with _ext.python_path() if request.param == "python" else contextlib.nullcontext():
+        yield request.param
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_long_sums_do_not_drift(dtype):
+    """64 copies of a matrix side by side: their X X^T is the same as one's (64 and its
+    root are powers of two), their result an eighth of one's, with the same roundings.  Only
+    the sums are longer.  What an instruction cuts off them is a quarter of 2^-23 of the
+    whole in the mean, which over the 512 of a segment comes to 1.5e-5 of A; the polynomial's
+    slopes (1.2 of a change of A, 1.5 from step to step) make that 16 times as much."""
+    g = torch.Generator(DEV).manual_seed(0)
+    x = torch.randn(1700, 4096, device=DEV, generator=g).to(dtype)
+    one = orthogonalize(x).double()
+    many = orthogonalize(x.repeat(1, 64))[:, 4096 * 21:4096 * 22].double() * 8
+    assert abs((one * many).sum() / (one * one).sum() - 1) <= 16 * 512 / 4 * 2.0 ** -23
