@@ -73,7 +73,7 @@ struct Prepared {
 };
 struct PrepareArgs {
   Prepared m[kPrepared];
-  float momentum;
+  float momentum, rest;  // rest: 1 - momentum, of which the rounded momentum has fewer bits
   int nesterov, steps;
   double eps, a, b, c;
 };
@@ -131,8 +131,8 @@ __global__ void __launch_bounds__(256) k_direction(const __grid_constant__ Prepa
   auto one = [&](float g, float m, float *next) {
     float u = g;
     if (moving) {
-      m = k * m + (1.f - k) * g;
-      u = a.nesterov ? (1.f - k) * g + k * m : m;
+      m = k * m + a.rest * g;
+      u = a.nesterov ? a.rest * g + k * m : m;
     }
     *next = m;
     sum += (double)u * (double)u;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(256) k_normalise(const __grid_constant__ Prepa
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float u = !moving ? g[j] : a.nesterov ? (1.f - a.momentum) * g[j] + a.momentum * m[j] : m[j];
+        const float u = !moving ? g[j] : a.nesterov ? a.rest * g[j] + a.momentum * m[j] : m[j];
         g[j] = (float)((double)u * scale);
         if (p.turned) tile[y][x + j] = g[j];
       }
@@ -791,7 +791,7 @@ cudaError_t schulz(const std::vector<Set> &sets, const std::vector<Places> &plac
 }
 
 // Launches what reads the matrices in.
-cudaError_t prepare(const std::vector<Prepared> &list, float momentum, int nesterov, int steps, const double *c,
+cudaError_t prepare(const std::vector<Prepared> &list, double momentum, int nesterov, int steps, const double *c,
                     double eps, cudaStream_t s) {
   for (size_t first = 0; first < list.size(); first += kPrepared) {
     const int n = (int)std::min<size_t>(kPrepared, list.size() - first);
@@ -804,7 +804,7 @@ cudaError_t prepare(const std::vector<Prepared> &list, float momentum, int neste
       most = std::max(most, (int64_t)a.m[i].rows * a.m[i].cols);
       tiles = std::max(tiles, (int64_t)((a.m[i].rows + 63) / 64) * ((a.m[i].cols + 63) / 64));
     }
-    a.momentum = momentum, a.nesterov = nesterov, a.steps = steps, a.eps = eps, a.a = c[0], a.b = c[1], a.c = c[2];
+    a.momentum = (float)momentum, a.rest = (float)(1.0 - momentum), a.nesterov = nesterov, a.steps = steps, a.eps = eps, a.a = c[0], a.b = c[1], a.c = c[2];
     const int partials = (int)std::min<int64_t>(kPartials, (most + 2047) / 2048);
     cudaError_t e = tc::launch(k_direction, dim3(partials, n), 256, 0, 1, s, a);
     if (e == cudaSuccess)
@@ -856,7 +856,7 @@ struct Small {
 struct SmallArgs {
   Small m[kMatrices];
   int64_t stride;        // > 0: matrix z is m[0]'s, z * stride elements on
-  float momentum, lr, decay;
+  float momentum, rest, lr, decay;
   const float *lr_device;
   int nesterov, steps;
   double eps, a, b, c;
@@ -1010,7 +1010,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_schulz_small(const __grid_
   };
   auto direction_of = [&](int64_t i, float m) {
     const float g = read_as(p.grad, p.dtype, i);
-    return p.momentum == nullptr ? g : a.nesterov ? (1.f - a.momentum) * g + a.momentum * m : m;
+    return p.momentum == nullptr ? g : a.nesterov ? a.rest * g + a.momentum * m : m;
   };
   double sum = 0;
   for (int e = threadIdx.x; e < count; e += kSmallThreads) {
@@ -1018,7 +1018,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) k_schulz_small(const __grid_
     const int64_t i = place(e, &row, &column);
     float m = 0.f;
     if (p.momentum != nullptr) {
-      m = a.momentum * p.momentum[i] + (1.f - a.momentum) * read_as(p.grad, p.dtype, i);
+      m = a.momentum * p.momentum[i] + a.rest * read_as(p.grad, p.dtype, i);
       p.momentum[i] = m;
     }
     const double u = direction_of(i, m);
@@ -1326,7 +1326,7 @@ extern "C" int cpab_b200_orthogonalize(int dtype, const void *x, int64_t batch, 
       list[z] = {static_cast<const char *>(x) + z * rows * columns * dtype_size(dtype), nullptr, places[0].x[0][0] + at,
                  places[0].x[0][1] + at, partials + z * kPartials, places[0].terms + z * kTerms, t.x_pitch(), (int)rows, (int)columns, dtype, t.turned()};
     }
-    cudaError_t e = prepare(list, 0.f, 0, steps, coefficients, eps, s);
+    cudaError_t e = prepare(list, 0.0, 0, steps, coefficients, eps, s);
     if (e == cudaSuccess) e = schulz(sets, places, steps, s);
     std::vector<Finished> results((size_t)batch);
     for (int64_t z = 0; z < batch; ++z) {
@@ -1449,7 +1449,7 @@ extern "C" int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double
     };
     const Split split(tensors, count);
     SmallArgs small = {};
-    small.momentum = (float)momentum, small.lr = (float)lr, small.decay = (float)weight_decay, small.lr_device = lr_device;
+    small.momentum = (float)momentum, small.rest = (float)(1.0 - momentum), small.lr = (float)lr, small.decay = (float)weight_decay, small.lr_device = lr_device;
     small.nesterov = nesterov, small.steps = steps, small.eps = eps;
     small.a = coefficients[0], small.b = coefficients[1], small.c = coefficients[2];
     for (int i = 0, n = 0; i <= count; ++i) {
@@ -1481,7 +1481,7 @@ extern "C" int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double
                          rate(t.rows, t.cols), t.rows, t.cols, t.dtype, t.turned(), 1});
         }
       }
-      if ((e = prepare(in, (float)momentum, nesterov, steps, coefficients, eps, s)) != cudaSuccess) break;
+      if ((e = prepare(in, momentum, nesterov, steps, coefficients, eps, s)) != cudaSuccess) break;
       if ((e = schulz(q.sets, places, steps, s)) != cudaSuccess) break;
       if ((e = finish(out, lr, lr_device, weight_decay, s)) != cudaSuccess) break;
     }

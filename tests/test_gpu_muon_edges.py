@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from cpab import _ext
-from cpab.optim import orthogonalize
+from cpab.optim import muon_, orthogonalize
 from test_gpu_muon import exact, matrices, most, off
 
 pytestmark = [pytest.mark.gpu,
@@ -32,3 +32,24 @@ def test_long_sums_do_not_drift(dtype):
     one = orthogonalize(x).double()
     many = orthogonalize(x.repeat(1, 64))[:, 4096 * 21:4096 * 22].double() * 8
     assert abs((one * many).sum() / (one * one).sum() - 1) <= 16 * 512 / 4 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("eps", [1e-3, 0.3, 1.0, 30.0, 1e6])
+@pytest.mark.parametrize("shape", [(40, 70), (130, 260), (400, 300)])
+def test_eps_near_and_above_the_norm(shape, eps, path):
+    for dtype in (F32, BF16):
+        x = matrices(shape, F32, 6)
+        x = (x / x.norm()).to(dtype)
+        assert off(orthogonalize(x, eps=eps), exact(x, eps=eps)) <= most(dtype, shape) + 2.0 ** -8 * (dtype == BF16)
+
+
+@pytest.mark.parametrize("momentum", [0.95, 0.999, 0.99999, 1 - 2.0 ** -20])
+@pytest.mark.parametrize("shape", [(20, 30), (130, 260), (131, 257)])
+def test_momenta_keep_their_precision_near_1(shape, momentum, path):
+    """1 - momentum is not the rounded momentum's: the new momentum is off by two
+    products' and a sum's roundings and those of the two factors."""
+    g, m = matrices(shape, F32, 1), matrices(shape, F32, 2) * 1e-3
+    want = momentum * m.double() + (1 - momentum) * g.double()
+    size = momentum * m.double().abs() + (1 - momentum) * g.double().abs()
+    muon_([matrices(shape, F32, 3)], [g], [m], lr=0.1, momentum=momentum)
+    assert ((m.double() - want).abs() <= 4 * 2.0 ** -24 * size).all()
