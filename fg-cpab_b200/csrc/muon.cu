@@ -24,7 +24,8 @@
 // eps is not small beside |G|_F, X is: it is kept as theta Y with theta a power of two
 // and |Y|_F in (1/2, 1], and the steps are taken in Y with
 //   Y <- r (a + theta^2 b Y Y^T + theta^4 c (Y Y^T)^2) Y,   r = theta / theta',
-// theta' = min(1, 2^ceil(log2 a) theta), until theta is 1.
+// theta' the least power of two that keeps |Y| at 1 (by the coefficients' magnitudes), until
+// theta is 1.
 #include <algorithm>
 #include <cmath>
 #include <exception>
@@ -88,9 +89,12 @@ __device__ __forceinline__ double first_theta(double norm, double eps) {
   return exp2(ceil(log2(x)));
 }
 __device__ __forceinline__ void write_terms(float *to, double theta, double a, double b, double c, int steps) {
-  const double growth = exp2(ceil(log2(fmax(1.0, fabs(a)))));
+  double most = 1.0;  // |Y| is no more
   for (int k = 0; k < steps; ++k) {
-    const double next = fmin(1.0, growth * theta), r = theta / next, q = theta * theta;
+    const double q = theta * theta, x = q * most * most;
+    most *= fabs(a) + x * (fabs(b) + x * fabs(c));
+    const double next = fmin(1.0, theta * exp2(ceil(log2(fmax(1.0, most))))), r = theta / next;
+    most *= r;
     to[3 * k] = (float)(a * r), to[3 * k + 1] = (float)(b * q * r), to[3 * k + 2] = (float)(c * q * q * r);
     theta = next;
   }

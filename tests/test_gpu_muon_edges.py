@@ -53,3 +53,27 @@ def test_momenta_keep_their_precision_near_1(shape, momentum, path):
     size = momentum * m.double().abs() + (1 - momentum) * g.double().abs()
     muon_([matrices(shape, F32, 3)], [g], [m], lr=0.1, momentum=momentum)
     assert ((m.double() - want).abs() <= 4 * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.parametrize("shape", [(1, 7), (1, 70000), (300, 1)])
+def test_values_on_their_way_from_far_below_eps_stay_in_range(shape, path):
+    """A norm well under eps, and coefficients that let it grow by its cube's part alone
+    and then move without rest, to 1.7 at most: 14 times the power of two that it began
+    at, whose square is more than what is kept can be."""
+    x = torch.zeros(shape, device=DEV)
+    x.view(-1)[0] = 1.0
+    for steps in (40, 56, 64):
+        y = orthogonalize(x, steps, (1.0, 1.0, -0.5), 1 / 0.12 - 1)
+        assert y.isfinite().all() and 0.1 < y.abs().max() <= 1.7
+
+
+@pytest.mark.parametrize("shape", [(40, 70), (130, 260), (300, 280)])
+def test_steps_from_far_below_eps(shape, path):
+    """Steps that do not grow, or grow slowly, do not lose the bits of what is small."""
+    x = matrices(shape, F32, 5)
+    x = x / x.norm()
+    for coefficients in ((1.0, 0.0, 0.0), (1.0, 1.0, -0.5), (1.5, -0.5, 0.0)):
+        for eps in (4.0, 1e4, 1e9):
+            for steps in (1, 6):
+                y, want = orthogonalize(x, steps, coefficients, eps), exact(x, steps, coefficients, eps)
+                assert off(y, want) <= 2 * most(F32, shape)
