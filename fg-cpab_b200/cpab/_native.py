@@ -890,7 +890,7 @@ def matmul_quantized(q, scale, weight, weight_scale, bias, dtype):
         raise ValueError("weight must be [N, K], got %s" % (tuple(weight.shape),))
     if weight.device != q.device:
         raise RuntimeError("weight is on %s, q on %s" % (weight.device, q.device))
-    if has_tangent(bias):
+    if has_tangent(scale, weight_scale, bias):
         raise RuntimeError("matmul_quantized has no gradient, of forward mode neither")
     alive, M, K, x = _quantized(q, scale, "q")
     alive_w, N, Kw, w = _quantized(weight, weight_scale, "weight")

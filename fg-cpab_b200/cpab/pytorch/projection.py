@@ -39,8 +39,10 @@ def matmul_quantized(q, scale, weight, weight_scale, bias=None, dtype=torch.bflo
     dtype (float32, float16 or bfloat16).  A scale is float8_e8m0fnu
     [..., ceil(K / 128)] (of quantize_blocks) or float32 [...], one for each row
     (of rms_norm_quantized); bias [N] is float32 or of dtype.  Codes whose rows
-    do not begin on multiples of 16 bytes are copied.  No gradient."""
-    if torch.is_grad_enabled() and bias is not None and bias.requires_grad:
+    do not begin on multiples of 16 bytes are copied.  No gradient (scales,
+    codes or a bias that want one are refused)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
+                                       (q, scale, weight, weight_scale, bias)):
         raise RuntimeError("matmul_quantized has no gradient; call it under torch.no_grad(), or use "
                            "linear_quantized")
     ext = _ext.module()

@@ -211,7 +211,7 @@ Tensor matmul_quantized(const Tensor &q, const Tensor &scale, const Tensor &weig
   TORCH_CHECK(weight.device() == q.device(), "weight is on ", weight.device(), ", q on ", q.device());
   for (const Tensor *t : {&scale, &weight_scale})
     TORCH_CHECK(t->device() == q.device(), "a scale is on ", t->device(), ", the codes on ", q.device());
-  TORCH_CHECK(!has_tangent({&bias}), "matmul_quantized has no gradient, of forward mode neither");
+  TORCH_CHECK(!has_tangent({&scale, &weight_scale, &bias}), "matmul_quantized has no gradient, of forward mode neither");
   const c10::cuda::CUDAGuard guard(q.device());
   Operand x = operand(q, scale, "q"), w = operand(weight, weight_scale, "weight");
   TORCH_CHECK_VALUE(w.K == x.K, "weight must be [N, ", x.K, "], got ", weight.sizes());

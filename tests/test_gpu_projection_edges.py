@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from cpab import _ext, _native
-from cpab.pytorch.projection import matmul_quantized, quantize_blocks
+from cpab.pytorch.projection import linear_quantized, matmul_quantized, quantize_blocks
 from test_gpu_projection import near, valued
 
 pytestmark = [pytest.mark.gpu,
@@ -176,3 +176,12 @@ def test_very_long_sums_of_like_signs_do_not_drift_in_16_bits():
     """As above with 512 instructions; a rounding to bfloat16, 2^-8 at most, has both
     signs: the mean of 1024 of them is within 5 sqrt(1 / 3 / 1024) 2^-8."""
     assert abs(drift(1600, 1600, 1 << 20, BF16)) <= (512 + 1) / 4 * 2.0 ** -23 + 5 * (1 / 3 / 1024) ** 0.5 * 2.0 ** -8
+
+
+def test_a_product_refuses_forward_derivatives_of_its_scales(path):
+    q, s = codes(4, 32, 1), torch.ones(4, device=DEV)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(s, s)
+        for args in ((q, dual, q, s), (q, s, q, dual)):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
+                matmul_quantized(*args)

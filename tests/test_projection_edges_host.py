@@ -4,6 +4,10 @@ import os
 import re
 
 import pytest
+import torch
+
+from cpab import _ext
+from cpab.pytorch.projection import matmul_quantized
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fg-cpab_b200", "csrc")
 
@@ -22,3 +26,27 @@ def test_kernels_that_begin_early_read_with_ordinary_loads(name):
     if not re.search(r"griddepcontrol\.wait|\bdep_wait\b", code):
         pytest.skip("no kernel of this file begins early")
     assert not re.findall(r"__ldg|ld\.global(?:\.\w+)*\.nc|__restrict__", code)
+
+
+@pytest.fixture(params=["ext", "python"])
+def path(request):
+    if request.param == "python":
+        with _ext.python_path():
+            yield
+    else:
+        assert _ext.module() is not None
+        yield
+
+
+def test_a_product_refuses_scales_and_codes_that_want_a_gradient(path):
+    """A row's float32 scale is an ordinary tensor of a graph: its gradient would be lost."""
+    q, s = torch.zeros(4, 32).to(torch.float8_e4m3fn), torch.ones(4)
+    wanting = torch.ones(4, requires_grad=True)
+    for args in ((q, wanting, q, s), (q, s, q, wanting), (q, wanting * 2, q, s),
+                 (q.clone().requires_grad_(True), s, q, s), (q, s, q.clone().requires_grad_(True), s)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            matmul_quantized(*args)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            matmul_quantized(*args)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        matmul_quantized(q, s, q, s, bias=wanting)
