@@ -7,6 +7,8 @@ made of them.
 
 No counterpart in the reference.
 """
+import functools
+
 import torch
 
 from .. import _ext, _native
@@ -76,6 +78,7 @@ class _LinearQuantized(torch.autograd.Function):
         q, s, qt, st, _ = _native.quantize_blocks(x, True, want_w)
         w, ws, wt, wst, _ = _native.quantize_blocks(weight, True, want_x)
         ctx.save_for_backward(qt, st, wt, wst)
+        ctx.K = x.shape[-1]
         ctx.types = x.dtype, weight.dtype, bias.dtype if bias is not None else None
         return _native.matmul_quantized(q, s, w, ws, bias, x.dtype)
 
@@ -86,6 +89,11 @@ class _LinearQuantized(torch.autograd.Function):
         qt, st, wt, wst = ctx.saved_tensors
         x_type, w_type, b_type = ctx.types
         want_x, want_w, want_b = ctx.needs_input_grad
+        if dy.shape[-1] == 0:
+            zeros = functools.partial(torch.zeros, device=dy.device)
+            return (zeros((*dy.shape[:-1], ctx.K), dtype=x_type) if want_x else None,
+                    zeros((0, ctx.K), dtype=w_type) if want_w else None,
+                    zeros(0, dtype=b_type) if want_b else None)
         q, s, dt, dst, db = _native.quantize_blocks(dy, want_x, want_w, b_type if want_b else None)
         dx = _native.matmul_quantized(q, s, wt, wst, None, x_type) if want_x else None
         dw = None

@@ -185,3 +185,19 @@ def test_a_product_refuses_forward_derivatives_of_its_scales(path):
         for args in ((q, dual, q, s), (q, s, q, dual)):
             with torch.no_grad(), pytest.raises(RuntimeError, match="no gradient"):
                 matmul_quantized(*args)
+
+
+@pytest.mark.parametrize("lead", [(5,), (2, 3), (), (0,)])
+def test_a_projection_without_outputs(lead, path):
+    """A weight of no rows: a gradient of zeros for x, empty ones for the others."""
+    x = torch.randn(*lead, 40, device=DEV, requires_grad=True)
+    w, b = (torch.empty(s, device=DEV, requires_grad=True) for s in ((0, 40), (0,)))
+    for bias in (None, b):
+        y = linear_quantized(x, w, bias)
+        assert y.shape == (*lead, 0)
+        leaves = [x, w] + ([b] if bias is not None else [])
+        dx, *others = torch.autograd.grad(y.sum(), leaves)
+        assert dx.shape == x.shape and not dx.any()
+        assert [g.shape for g in others] == [t.shape for t in leaves[1:]]
+    (gw,) = torch.autograd.grad(linear_quantized(x.detach(), w).sum(), w)
+    assert gw.shape == (0, 40)
