@@ -66,6 +66,7 @@ _SIGNATURES = {
                                   _c_i64, _p, _c_i64, _c_int, _p, _p, _p],
     "cpab_b200_matmul_quantized": [_c_int, _p, _p, _c_i64, _c_i64, _c_i64, _c_int, _p, _p, _c_i64,
                                    _p, _p],
+    "cpab_b200_set_wait_limit": [_c_i64],
     "cpab_b200_lay_out_codes": [_c_int, _p, _p, _p, _p, _c_i64, _p],
     "cpab_b200_orthogonalize": [_c_int, _p, _c_i64, _c_i64, _c_i64, _c_int, _p, ctypes.c_double, _p,
                                 _p, _p],

@@ -352,6 +352,7 @@ struct PhaseGroup {
 struct PhaseArgs {
   PhaseGroup g[kGroups];
   int groups, step;
+  tc::Waits waits;
 };
 
 // What the tensor cores cut off a sum has one sign.  16-bit matrices: 1.5e-5 of the sum at
@@ -376,6 +377,7 @@ struct Schulz {
   };
   const PhaseArgs &p;
 
+  __device__ const tc::Waits &waits() const { return p.waits; }
   __device__ int tiles() const { return p.g[p.groups - 1].end; }
   __device__ Tile tile(int i) const {
     int g = 0, begin = 0;
@@ -733,7 +735,7 @@ cudaError_t schulz_as(const std::vector<Set> &sets, const std::vector<Places> &p
   int batch[kGroups];
   PhaseArgs a;
   const int groups = (int)sets.size();
-  a.groups = groups;
+  a.groups = groups, a.waits = tc::waits();
   for (int g = 0; g < groups; ++g) batch[g] = sets[g].batch;
   for (int step = 0; step < steps; ++step) {
     const int now = step & 1;
@@ -1308,6 +1310,7 @@ extern "C" int cpab_b200_orthogonalize(int dtype, const void *x, int64_t batch, 
   if (batch > 65536 || rows > kMostRows || columns > kMostRows)
     return report_error(CPAB_ERR_SIZE, "%s", "orthogonalize: at most 65536 matrices of 2^20 rows and columns");
   if (x == nullptr || out == nullptr) return report_error(CPAB_ERR_ARG, "%s", "orthogonalize: null pointer");
+  if (tc::gave_up()) return tc::report_gave_up("orthogonalize");
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (is_small(rows, columns)) {
     SmallArgs a = {};
@@ -1445,6 +1448,7 @@ extern "C" int cpab_b200_muon(const cpab_muon_tensor *tensors, int count, double
     const std::vector<Sequence> list = sequences(tensors, count);
     if (!list.empty() && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256))
       return report_error(CPAB_ERR_ARG, "%s", "muon: null workspace, or one off 256 bytes");
+    if (tc::gave_up()) return tc::report_gave_up("muon");
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
     auto rate = [&](int64_t rows, int64_t columns) {

@@ -10,6 +10,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -17,6 +18,52 @@
 #include "sequence.cuh"
 
 namespace cpab {
+
+namespace {
+
+constexpr int kDevices = 64;
+std::atomic<int64_t> g_longest{2000000000};
+std::atomic<int *> g_words[kDevices];  // a page that host and device share, for each device
+std::mutex g_words_mutex;
+
+std::atomic<int *> *word_of_device() {
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess && device >= 0 && device < kDevices ? &g_words[device] : nullptr;
+}
+
+}  // namespace
+
+tc::Waits tc::waits() {
+  std::atomic<int *> *word = word_of_device();
+  if (word != nullptr && word->load() == nullptr) {
+    std::lock_guard<std::mutex> lock(g_words_mutex);
+    if (word->load() == nullptr) {
+      // (the first call may be one of a capture)
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      void *p = nullptr;
+      if (cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess) {
+        *static_cast<int *>(p) = 0;
+        word->store(static_cast<int *>(p));
+      } else {
+        (void)cudaGetLastError();
+      }
+      cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+  }
+  return {(uint64_t)g_longest.load(), word != nullptr ? word->load() : nullptr};
+}
+bool tc::gave_up() {
+  std::atomic<int *> *word = word_of_device();
+  volatile int *p = word != nullptr ? word->load() : nullptr;
+  if (p == nullptr || *p == 0) return false;
+  *p = 0;
+  return true;
+}
+int tc::report_gave_up(const char *what) {
+  return report_error(CPAB_ERR_WAIT, "%s: not begun: a matrix product before it gave up waiting, and its results are NaN",
+                      what);
+}
 
 bool make_tile_map(CUtensorMap *map, bool halves, const void *base, int64_t columns, int64_t rows, int64_t batch,
                    int64_t pitch, int64_t plane, int box_rows) {
@@ -386,6 +433,7 @@ struct ProductArgs {
   int splits, each;      // the sum in so many parts of `each` steps (a multiple of 8),
   float *parts;          // float32 [splits, M, pitch], where they are not one
   int64_t pitch;
+  tc::Waits waits;
 };
 
 // A row's scales of 8 steps (of a row's one scale its bits, until all are asked for).
@@ -448,6 +496,7 @@ struct Product {
   };
   const ProductArgs &a;
 
+  __device__ const tc::Waits &waits() const { return a.waits; }
   __device__ int tiles() const { return a.tiles_m * a.tiles_n * a.splits; }
   // Bands of 8 rows of tiles, column by column, so that tiles at work together
   // share operands in L2.
@@ -854,6 +903,12 @@ const char *operand(const cpab_quantized &o, int64_t K, Scales *scales) {
 
 using namespace cpab;
 
+extern "C" int cpab_b200_set_wait_limit(int64_t nanoseconds) {
+  if (nanoseconds < 0) return report_error(CPAB_ERR_ARG, "%s", "set_wait_limit: negative time");
+  g_longest.store(nanoseconds);
+  return report_error(CPAB_OK, "%s", "");
+}
+
 extern "C" int64_t cpab_b200_quantize_blocks_workspace(int64_t rows, int64_t columns) {
   return rows < 0 || columns < 0 ? 0 : (rows + 127) / 128 * columns;
 }
@@ -959,6 +1014,7 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   a.splits = split.splits, a.each = split.each, a.parts = workspace, a.pitch = (N + 15) / 16 * 16;
   if (!is_few(M, N, K) && a.splits > 1 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 32))
     return report_error(CPAB_ERR_ARG, "%s", "matmul_quantized: a null workspace, or one off 32 bytes");
+  if (tc::gave_up()) return tc::report_gave_up("matmul_quantized");
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (is_few(M, N, K)) {
@@ -971,6 +1027,7 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
                                     : launch_few<__nv_bfloat16, __nv_bfloat16>(f, s);
     return launch_status(e, "matmul_quantized");
   }
+  a.waits = tc::waits();
   if (dtype == CPAB_F32) e = launch_product<float, float>(a, s);
   else if (dtype == CPAB_F16)
     e = bias_dtype == CPAB_F32 ? launch_product<__half, float>(a, s) : launch_product<__half, __half>(a, s);

@@ -18,6 +18,7 @@
 //                     what a float32 sum cannot hold, so an error of up to 2^-24 of
 //                     the sum a step piles up where a tile has hundreds of steps
 //   Shared            what its epilogue keeps in shared memory
+//   const Waits &waits()            how long a wait may last, and whom to tell
 //   int tiles()                     tiles of this launch
 //   Tile tile(int i)                {m0, n0, steps, ...}
 //   warm(tile)                      touches its arguments
@@ -132,11 +133,11 @@ __device__ __forceinline__ void core(const P &p) {
 
   if (warp == 0) {
     int s = 0, phase = 0;
-    bool ok = true;
+    bool ok = p.waits().longest > 0;
     for (int i = first; i < tiles && ok; i += stride) {
       const auto t = i == first ? first_tile : p.tile(i);
       for (int k = 0; k < t.steps; ++k) {
-        ok = bar_wait_warp(empty + 8 * s, phase ^ 1);
+        ok = bar_wait_warp(empty + 8 * s, phase ^ 1, p.waits());
         if (!ok) break;
         if (elect()) {
           if (rank == 0) bar_expect(full + 8 * s, p.stage_bytes());
@@ -151,16 +152,16 @@ __device__ __forceinline__ void core(const P &p) {
   } else if (warp == 1) {
     if (rank == 0) {
       int s = 0, phase = 0, sc = 0, sphase = 0, acc = 0, aphase = 0;
-      bool ok = true;
+      bool ok = p.waits().longest > 0;
       for (int i = first; i < tiles && ok; i += stride) {
         const auto t = i == first ? first_tile : p.tile(i);
         for (int k = 0; k < t.steps; ++k) {
           const bool fresh = k % kLength == 0;
-          if (fresh && !(ok = bar_wait_warp(aempty + 8 * acc, aphase ^ 1))) break;
+          if (fresh && !(ok = bar_wait_warp(aempty + 8 * acc, aphase ^ 1, p.waits()))) break;
           if constexpr (P::kScaled) {
             if ((k & 7) == 0) {
               if ((k > 0 || i != first) && ++sc == S::kScaleSlots) sc = 0, sphase ^= 1;
-              if (!(ok = bar_wait_warp(sfull + 8 * sc, sphase))) break;
+              if (!(ok = bar_wait_warp(sfull + 8 * sc, sphase, p.waits()))) break;
               fence_after();
               const uint32_t from = scale0 + sc * S::kSlotBytes, to = tmem + S::kScaleColumn + sc * S::kSlotColumns;
               const int chunks = min(2, (t.steps - k + 3) >> 2) * S::kScaleChunks;
@@ -171,7 +172,7 @@ __device__ __forceinline__ void core(const P &p) {
               __syncwarp();
             }
           }
-          if (!(ok = bar_wait_warp(full + 8 * s, phase))) break;
+          if (!(ok = bar_wait_warp(full + 8 * s, phase, p.waits()))) break;
           fence_after();
           const bool last = k + 1 == t.steps || (k + 1) % kLength == 0;
           const uint32_t d = tmem + acc * P::kBN;
@@ -210,7 +211,7 @@ __device__ __forceinline__ void core(const P &p) {
       // Warp 2 brings A's words (the first chunk of each four steps), warp 3 B's.
       constexpr int kB = S::kScaleChunks - 1;
       int sc = 0, sphase = 0;
-      bool ok = true;
+      bool ok = p.waits().longest > 0;
       for (int i = first; i < tiles && ok; i += stride) {
         const auto t = i == first ? first_tile : p.tile(i);
         for (int g = 0; 8 * g < t.steps && ok; ++g) {
@@ -228,11 +229,11 @@ __device__ __forceinline__ void core(const P &p) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) p.words_of_one(w[c][j]);
           }
-          ok = bar_wait_warp(sempty + 8 * sc, sphase ^ 1);
+          ok = bar_wait_warp(sempty + 8 * sc, sphase ^ 1, p.waits());
           uint8_t *to = scales + sc * S::kSlotBytes + 16 * lane + (warp == 3 ? 512 : 0);
 #pragma unroll
           for (int c = 0; c < kB; ++c) {
-            if (warp == 2 && c > 0) break;
+            if ((warp == 2 && c > 0) || !ok) break;  // (a slot that is not free may still be read)
 #pragma unroll
             for (int q = 0; q < 2; ++q)
               *reinterpret_cast<uint4 *>(to + 512 * (q * S::kScaleChunks + c)) =
@@ -256,7 +257,7 @@ __device__ __forceinline__ void core(const P &p) {
     constexpr int kHold = P::kSegment > 0 || P::kAcc == 1 ? kHalf : 32;
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     int acc = 0, aphase = 0;
-    bool ok = true;
+    bool ok = p.waits().longest > 0;
     for (int i = first; i < tiles; i += stride) {
       const auto t = i == first ? first_tile : p.tile(i);
       p.begin(t, *shared, threadIdx.x - 128);
@@ -265,7 +266,7 @@ __device__ __forceinline__ void core(const P &p) {
       float v[kHold];
       typename P::Ahead now = p.ahead(t, row, half * kHalf);
       for (int g = 0; g < segments; ++g) {
-        ok = ok && bar_wait_warp(afull + 8 * acc, aphase);
+        ok = ok && bar_wait_warp(afull + 8 * acc, aphase, p.waits());
         fence_after();
         const uint32_t d = tmem + acc * P::kBN + half * kHalf + ((uint32_t)(quarter * 32) << 16);
         if constexpr (kHold < kHalf) {
@@ -315,6 +316,10 @@ __device__ __forceinline__ void core(const P &p) {
   __syncthreads();
   if (*gave_up) {
     // Copies in flight land before the block ends.
+    if (threadIdx.x == 0 && p.waits().gave_up != nullptr) {
+      *static_cast<volatile int *>(p.waits().gave_up) = 1;
+      __threadfence_system();
+    }
     if (threadIdx.x == 0)
       for (int i = 0; i < 2000; ++i) __nanosleep(1000);
     __syncthreads();

@@ -42,10 +42,16 @@ __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// How long a wait of these kernels may last (nanoseconds; 0: what waits gives up at once)
+// and the word that is set where one ran out, in memory that the host reads too (or null).
+struct Waits {
+  uint64_t longest;
+  int *gave_up;
+};
+
 // Waits for the phase of the given parity.  Every wait of these kernels ends: after
-// two seconds (the longest in earnest is a tile's product, under a millisecond) the
-// caller gives its work up.
-constexpr uint64_t kLongest = 2000000000ull;
+// `longest` (two seconds by default; a tile's whole sum, the longest in earnest, takes 0.4
+// us for each 128 codes or 64 halves, milliseconds at most) the caller gives its work up.
 __device__ __forceinline__ uint64_t nanoseconds() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -60,17 +66,19 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const Waits &waits) {
   for (int i = 0; i < 16; ++i)
     if (bar_try(bar, parity)) return true;
   const uint64_t begin = nanoseconds();
   do {
     if (bar_try(bar, parity)) return true;
-  } while (nanoseconds() - begin < kLongest);
+  } while (nanoseconds() - begin < waits.longest);
   return false;
 }
 // The same for a whole warp, with one answer.
-__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(~0u, bar_wait(bar, parity)); }
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, const Waits &waits) {
+  return __all_sync(~0u, bar_wait(bar, parity, waits));
+}
 
 // One lane of a whole warp.  (Copies and matrix instructions take their operands from
 // the warp's uniform registers: warps that issue them run their loops whole and elect
@@ -264,6 +272,13 @@ cudaError_t launch(void (*kernel)(P...), dim3 grid, unsigned block, size_t share
   cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
+
+// What a launch on the current device passes on, and whether a kernel of an earlier one
+// gave up waiting there (once for each time; the answer to the call is then reported as
+// CPAB_ERR_WAIT).  Defined in product.cu.
+Waits waits();
+bool gave_up();
+int report_gave_up(const char *what);
 
 }  // namespace tc
 

@@ -55,7 +55,8 @@ typedef enum {
   CPAB_ERR_ARG = -1,    /* invalid shape / pointer / flag                 */
   CPAB_ERR_STEPS = -2,  /* nstepsolver outside [1, cpab_b200_max_steps()] */
   CPAB_ERR_CUDA = -3,   /* a CUDA launch or runtime call failed           */
-  CPAB_ERR_SIZE = -4    /* a size exceeds a documented limit              */
+  CPAB_ERR_SIZE = -4,   /* a size exceeds a documented limit              */
+  CPAB_ERR_WAIT = -5    /* a kernel of an earlier call gave up waiting    */
 } cpab_status;
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -499,6 +500,15 @@ typedef struct {
                              the next one's; scale_row 0: float32, one for each row   */
   int64_t scale_row;
 } cpab_quantized;
+
+/*
+ * The kernels of the products below (of cpab_b200_orthogonalize and cpab_b200_muon too)
+ * hand tiles from warp to warp; a wait inside them that lasts longer than this many
+ * nanoseconds (2 * 10^9 unless set here, for all later launches of the process; 0: all
+ * work is given up at once) ends with the tile's results NaN.  The next call of one of
+ * them on that device that sees it returns CPAB_ERR_WAIT and does nothing else.
+ */
+int cpab_b200_set_wait_limit(int64_t nanoseconds);
 
 /* Floats of the workspace of cpab_b200_quantize_blocks. */
 int64_t cpab_b200_quantize_blocks_workspace(int64_t rows, int64_t columns);

@@ -6,7 +6,7 @@ import re
 import pytest
 import torch
 
-from cpab import _ext
+from cpab import _ext, _native
 from cpab.pytorch.projection import matmul_quantized
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fg-cpab_b200", "csrc")
@@ -50,3 +50,9 @@ def test_a_product_refuses_scales_and_codes_that_want_a_gradient(path):
             matmul_quantized(*args)
     with pytest.raises(RuntimeError, match="no gradient"):
         matmul_quantized(q, s, q, s, bias=wanting)
+
+
+def test_a_wait_limit_is_a_time():
+    L = _native.lib()
+    assert L.cpab_b200_set_wait_limit(-1) == -1 and b"negative" in L.cpab_b200_last_error()
+    assert L.cpab_b200_set_wait_limit(0) == 0 and L.cpab_b200_set_wait_limit(2 * 10 ** 9) == 0
