@@ -91,10 +91,16 @@ __device__ __forceinline__ double first_theta(double norm, double eps) {
 __device__ __forceinline__ void write_terms(float *to, double theta, double a, double b, double c, int steps) {
   double most = 1.0;  // |Y| is no more
   for (int k = 0; k < steps; ++k) {
-    const double q = theta * theta, x = q * most * most;
-    most *= fabs(a) + x * (fabs(b) + x * fabs(c));
-    const double next = fmin(1.0, theta * exp2(ceil(log2(fmax(1.0, most))))), r = theta / next;
-    most *= r;
+    const double q = theta * theta;
+    double next = 1.0, r = 1.0;
+    if (theta < 1.0) {
+      const double x = q * most * most;
+      most *= fabs(a) + x * (fabs(b) + x * fabs(c));
+      int e;
+      if (frexp(fmax(1.0, most), &e) == 0.5) --e;  // (powers of two themselves)
+      next = fmin(1.0, ldexp(theta, e)), r = theta / next;
+      most *= r;
+    }
     to[3 * k] = (float)(a * r), to[3 * k + 1] = (float)(b * q * r), to[3 * k + 2] = (float)(c * q * q * r);
     theta = next;
   }

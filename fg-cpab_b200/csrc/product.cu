@@ -510,6 +510,7 @@ struct Product {
   __device__ void warm(const Tile &) const {
     if (threadIdx.x == 0) tc::prefetch_map(&a.a), tc::prefetch_map(&a.b);
     tc::touch(a.sa.bytes), tc::touch(a.sb.bytes), tc::touch(a.y), tc::touch(a.bias), tc::touch(a.wide);
+    tc::touch(a.sa.rows), tc::touch(a.sb.rows);
   }
   __device__ void load(const Tile &t, int k, uint32_t sa, uint32_t sb, uint32_t bar, uint32_t rank) const {
     const int at = (t.part * a.each + k) * 128;

@@ -126,6 +126,7 @@ __device__ __forceinline__ void core(const P &p) {
   // kernel before still runs.
   const auto first_tile = p.tile(first);
   p.warm(first_tile);
+  const bool go = p.waits().longest > 0;
   dep_wait();
 
   // The pair's shared barriers are the first block's.
@@ -133,7 +134,7 @@ __device__ __forceinline__ void core(const P &p) {
 
   if (warp == 0) {
     int s = 0, phase = 0;
-    bool ok = p.waits().longest > 0;
+    bool ok = go;
     for (int i = first; i < tiles && ok; i += stride) {
       const auto t = i == first ? first_tile : p.tile(i);
       for (int k = 0; k < t.steps; ++k) {
@@ -152,7 +153,7 @@ __device__ __forceinline__ void core(const P &p) {
   } else if (warp == 1) {
     if (rank == 0) {
       int s = 0, phase = 0, sc = 0, sphase = 0, acc = 0, aphase = 0;
-      bool ok = p.waits().longest > 0;
+      bool ok = go;
       for (int i = first; i < tiles && ok; i += stride) {
         const auto t = i == first ? first_tile : p.tile(i);
         for (int k = 0; k < t.steps; ++k) {
@@ -211,7 +212,7 @@ __device__ __forceinline__ void core(const P &p) {
       // Warp 2 brings A's words (the first chunk of each four steps), warp 3 B's.
       constexpr int kB = S::kScaleChunks - 1;
       int sc = 0, sphase = 0;
-      bool ok = p.waits().longest > 0;
+      bool ok = go;
       for (int i = first; i < tiles && ok; i += stride) {
         const auto t = i == first ? first_tile : p.tile(i);
         for (int g = 0; 8 * g < t.steps && ok; ++g) {
@@ -257,7 +258,7 @@ __device__ __forceinline__ void core(const P &p) {
     constexpr int kHold = P::kSegment > 0 || P::kAcc == 1 ? kHalf : 32;
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     int acc = 0, aphase = 0;
-    bool ok = p.waits().longest > 0;
+    bool ok = go;
     for (int i = first; i < tiles; i += stride) {
       const auto t = i == first ? first_tile : p.tile(i);
       p.begin(t, *shared, threadIdx.x - 128);
