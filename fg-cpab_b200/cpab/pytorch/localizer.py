@@ -13,7 +13,6 @@ counterpart in the reference, whose localisation networks read images.
 """
 import torch
 import torch.nn as nn
-import torch.nn.functional as F
 
 from .norm import rms_norm, rms_norm_quantized
 from .projection import linear_quantized, matmul_quantized
@@ -110,9 +109,12 @@ class SeriesLocalizer(nn.Module):
         """One sample of each of B streams: samples [B, channels], states from
         new_states, updated in place, slots [B] the streams' rows of it (None:
         row b; -1: no sample now, whose theta means nothing).  Returns theta
-        [B, theta_dim] of the streams so far.  quantized: norms and input
-        projections in 8 bits (see quantize), whose products are rounded to
-        16 bits."""
+        [B, theta_dim] of the streams so far, as forward gives for them (with
+        projection_bits=8 the projections are its 8-bit ones, whose weights are
+        quantized at every step).  quantized, whatever projection_bits is: norms
+        and input projections in 8 bits with the weights that quantize keeps,
+        whose products are rounded to 16 bits; output projections in the
+        weights' type."""
         s = self.embed(samples)
         update = None
         for k, block in enumerate(self.blocks):
@@ -128,7 +130,7 @@ class SeriesLocalizer(nn.Module):
                     y = rms_norm(s, block.norm, eps=self.eps)
                 else:
                     y, s = rms_norm(update, block.norm, residual=s, eps=self.eps)
-                z = block.in_proj(y)
-            update = F.linear(gated_scan_step(z, None, states[k], slots), block.out_proj.weight,
-                              block.out_proj.bias)
+                z = self._project(block.in_proj, y)
+            h = gated_scan_step(z, None, states[k], slots)
+            update = block.out_proj(h) if quantized else self._project(block.out_proj, h)
         return self._theta(update, s)
