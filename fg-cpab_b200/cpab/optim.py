@@ -273,10 +273,15 @@ class Muon(torch.optim.Optimizer):
     float32 whatever the parameters' type.  adjust_lr_fn: None or "original",
     or "match_rms_adamw", with which lr and weight_decay of AdamW can be kept.
     step() can be captured in a CUDA graph once the parameters have states, that
-    is after one step; lr may then be a float32 tensor on the device."""
+    is after one step; lr may then be a float32 tensor on the device (a step reads
+    the value of one on the CPU, a captured one that of its capture).  Refused,
+    other than by torch.optim.Muon: parameters that are not contiguous, and a
+    momentum of 1 or more."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
                  ns_coefficients=COEFFICIENTS, eps=1e-7, ns_steps=5, adjust_lr_fn=None):
+        if torch.is_tensor(lr) and lr.numel() != 1:
+            raise ValueError("lr must be a number or a tensor of one element, got one of shape %s" % (tuple(lr.shape),))
         if not torch.is_tensor(lr) and not lr >= 0:
             raise ValueError("lr must not be negative, got %r" % (lr,))
         if not 0.0 <= momentum < 1.0:
@@ -325,6 +330,8 @@ class Muon(torch.optim.Optimizer):
                 to[2].append(state["momentum_buffer"])
             for device, to in lists.items():
                 lr = group["lr"]
+                if torch.is_tensor(lr) and not lr.is_cuda:
+                    lr = float(lr)
                 if torch.is_tensor(lr) and lr.is_cuda and lr.device != device:
                     lr = lr.to(device, non_blocking=True)
                 muon_(*to, lr=lr, momentum=group["momentum"], nesterov=group["nesterov"],

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from cpab import _ext
-from cpab.optim import muon_, orthogonalize
+from cpab.optim import Muon, muon_, orthogonalize
 from test_gpu_muon import exact, matrices, most, off
 
 pytestmark = [pytest.mark.gpu,
@@ -77,3 +77,26 @@ def test_steps_from_far_below_eps(shape, path):
             for steps in (1, 6):
                 y, want = orthogonalize(x, steps, coefficients, eps), exact(x, steps, coefficients, eps)
                 assert off(y, want) <= 2 * most(F32, shape)
+
+
+@pytest.mark.parametrize("dtype", [F32, torch.float64])
+def test_a_learning_rate_on_the_cpu(dtype, path):
+    """As torch's optimizer and its state dicts may have one; schedulers write into it."""
+    a, b = (torch.nn.Parameter(matrices((20, 30), F32, 1)) for _ in range(2))
+    lr = torch.tensor(0.25, dtype=dtype)
+    ours, same = Muon([a], lr=lr), Muon([b], lr=0.25)
+    for rate in (0.25, 0.5):
+        lr.fill_(rate)
+        same.param_groups[0]["lr"] = rate
+        a.grad = matrices((20, 30), F32, 2)
+        b.grad = a.grad.clone()
+        ours.step()
+        same.step()
+        assert torch.equal(a, b)
+    theirs = torch.optim.Muon([torch.nn.Parameter(a.detach().clone())], lr=torch.tensor(0.5))
+    theirs.param_groups[0]["params"][0].grad = a.grad.clone()
+    theirs.step()
+    ours.load_state_dict(theirs.state_dict())
+    ours.step()
+    with pytest.raises(ValueError, match="one element"):
+        Muon([a], lr=torch.zeros(2))
