@@ -1424,6 +1424,14 @@ const char *check_tensors(const cpab_muon_tensor *tensors, int count) {
     if (tensors[i].rows > 0 && tensors[i].columns > 0) seen.push_back(tensors[i].param), seen.push_back(tensors[i].momentum);
   std::sort(seen.begin(), seen.end());
   if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) return "a parameter or momentum given twice";
+  // (the momentum is written before the gradient is read for the second time)
+  std::vector<const void *> momenta;
+  for (int i = 0; i < count; ++i)
+    if (tensors[i].rows > 0 && tensors[i].columns > 0) momenta.push_back(tensors[i].momentum);
+  std::sort(momenta.begin(), momenta.end());
+  for (int i = 0; i < count; ++i)
+    if (tensors[i].rows > 0 && tensors[i].columns > 0 && std::binary_search(momenta.begin(), momenta.end(), tensors[i].grad))
+      return "a gradient that is a momentum";
   return nullptr;
 }
 

@@ -581,7 +581,8 @@ typedef struct {
  *   m = momentum m + (1 - momentum) g,   u = nesterov ? (1 - momentum) g + momentum m : m,
  *   p = p (1 - lr weight_decay) - lr r O(u)
  * with O that of cpab_b200_orthogonalize, r = sqrt(max(1, rows / columns)) (adjust 0)
- * or 0.2 sqrt(max(rows, columns)) (adjust 1).  lr_device: the learning rate as one
+ * or 0.2 sqrt(max(rows, columns)) (adjust 1).  No parameter or momentum may be given twice,
+ * nor a momentum as a gradient.  lr_device: the learning rate as one
  * float32 on the device, or NULL: lr.  workspace: cpab_b200_muon_workspace bytes (for
  * the current device), 256-byte aligned.
  */

@@ -1,5 +1,6 @@
 """Host-side checks at the edges of the 8-bit projections and the orthogonalised
 steps (no GPU needed)."""
+import ctypes
 import os
 import re
 
@@ -56,3 +57,17 @@ def test_a_wait_limit_is_a_time():
     L = _native.lib()
     assert L.cpab_b200_set_wait_limit(-1) == -1 and b"negative" in L.cpab_b200_last_error()
     assert L.cpab_b200_set_wait_limit(0) == 0 and L.cpab_b200_set_wait_limit(2 * 10 ** 9) == 0
+
+
+def test_muon_refuses_a_gradient_that_is_a_momentum():
+    """The momentum is written before the gradient is read the second time."""
+    L = _native.lib()
+    coefficients = (ctypes.c_double * 3)(3.4445, -4.775, 2.0315)
+    for rows in (300, 20):
+        for grads in ((8192, 4096), (4096, 65536), (65536, 8192)):
+            t = (_native._MuonTensor * 2)()
+            for k in range(2):
+                t[k] = _native._MuonTensor(1 << 20 << k, grads[k], (8192, 65536)[k], rows, 20, 0)
+            assert L.cpab_b200_muon(ctypes.byref(t), 2, 0.1, None, 0.9, 1, 0.1, 5, coefficients, 1e-7, 0,
+                                    ctypes.c_void_p(4096), None) == -1
+            assert b"momentum" in L.cpab_b200_last_error()
