@@ -100,3 +100,32 @@ def test_a_learning_rate_on_the_cpu(dtype, path):
     ours.step()
     with pytest.raises(ValueError, match="one element"):
         Muon([a], lr=torch.zeros(2))
+
+
+def in_a_bucket(tensors, lead):
+    """The tensors as views into one flat buffer, `lead` elements from its beginning."""
+    flat = torch.zeros(lead + sum(t.numel() + 1 for t in tensors), device=DEV, dtype=tensors[0].dtype)
+    views, at = [], lead
+    for t in tensors:
+        views.append(flat[at:at + t.numel()].view(t.shape).copy_(t))
+        at += t.numel() + 1
+    return views
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lead", [0, 1, 3])
+def test_views_into_a_flat_bucket(lead, dtype, path):
+    """Parameters, gradients and momenta off 16 bytes whose rows are whole vectors, as
+    data-parallel training makes them: the same step as of tensors of their own."""
+    shapes = [(130, 264), (264, 130), (304, 296), (296, 304), (16, 24), (136, 8), (1, 40)]
+    ps, gs = ([matrices(s, dtype, k + at, 0.05) for k, s in enumerate(shapes)] for at in (0, 20))
+    ms = [matrices(s, F32, k + 40) for k, s in enumerate(shapes)]
+    views = [in_a_bucket(ts, lead) for ts in (ps, gs, ms)]
+    for lists in ((ps, gs, ms), views):
+        for _ in range(2):
+            muon_(*lists, lr=0.1, momentum=0.9)
+    for own, seen in zip((ps, gs, ms), views):
+        assert all(torch.equal(a, b) for a, b in zip(own, seen))
+    for x in ps:
+        (view,) = in_a_bucket([x], lead + 1)
+        assert torch.equal(orthogonalize(view), orthogonalize(x))

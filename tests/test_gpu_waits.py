@@ -2,6 +2,9 @@
 kernels return, and the next call says so.  (With a limit of 0 the roles of a block
 give up before they hand one another anything, so nothing is left to wait for.)"""
 import contextlib
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -115,3 +118,27 @@ def test_captured_products_report_to_the_next_call():
     torch.cuda.synchronize()
     assert z.isnan().all()
     assert torch.equal(reported(lambda: orthogonalize(x)), want)
+
+
+FIRST = """
+import torch
+from cpab.optim import orthogonalize
+from cpab.pytorch.projection import matmul_quantized, quantize_blocks
+x = torch.randn(300, 500, device="cuda")
+q = quantize_blocks(x)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y, z = matmul_quantized(*q, *q), orthogonalize(x)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, matmul_quantized(*q, *q)) and torch.equal(z, orthogonalize(x))
+print("captured")
+"""
+
+
+def test_the_first_product_of_a_process_is_captured():
+    """What is set up at a device's first product may be set up in a capture."""
+    env = {**os.environ, "PYTHONPATH": os.pathsep.join(p for p in sys.path if p)}
+    run = subprocess.run([sys.executable, "-c", FIRST], env=env, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
