@@ -700,9 +700,7 @@ struct FewArgs {
   const uint8_t *x, *w;
   int64_t x_row, w_row;
   Scales sx, sw;
-  // A row's scale beside the other operand's blocks: its power of two is that of each of
-  // its blocks.  (Where both have rows' the sums are of codes alone.)
-  const float *x_one, *w_one;
+  int mixed;
   const void *bias;
   void *y;
   int64_t y_row;
@@ -739,7 +737,11 @@ __device__ __forceinline__ float by_rows(float v, float a, float b) {
   return v * __uint_as_float((uint32_t)(p + 127) << 23) * __uint_as_float((uint32_t)(e - p + 127) << 23);
 }
 
-template <typename T, typename TB, int TILES>
+// MIXED: one operand has rows' scales and the other blocks'; a row's power of two is then
+// that of each of its blocks (kernels of their own: a row by 4096 x 2048 of other scales
+// 5.3 us with that choice in the loop, without 4.9 to 5.1).  Where both have rows' the
+// sums are of codes alone.
+template <typename T, typename TB, int TILES, bool MIXED>
 __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_constant__ FewArgs a) {
   extern __shared__ __align__(16) uint8_t few_smem[];  // x as halves, [M, pitch]
   __shared__ float part[kFewWarps][16][8 * TILES + 1];
@@ -779,7 +781,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
   };
   auto multiply = [&](int b, const Block &f) {
     uint32_t u0 = f.s0, u1 = f.s1;
-    if (a.w_one != nullptr) u0 = row_power(a.w_one[r0]), u1 = row_power(a.w_one[r1]);
+    if (MIXED && a.sw.rows != nullptr) u0 = row_power(a.sw.rows[r0]), u1 = row_power(a.sw.rows[r1]);
     const bool far = is_far(u0) || is_far(u1);
     const float s0 = power(u0), s1 = power(u1);
     float acc[TILES][4] = {};
@@ -809,7 +811,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
       const int c0 = min(8 * i + 2 * t, a.M - 1), c1 = min(8 * i + 2 * t + 1, a.M - 1);
       uint32_t e0 = 127u, e1 = 127u;
       if (a.sx.bytes != nullptr) e0 = a.sx.bytes[c0 * a.sx.row + b], e1 = a.sx.bytes[c1 * a.sx.row + b];
-      if (a.x_one != nullptr) e0 = row_power(a.x_one[c0]), e1 = row_power(a.x_one[c1]);
+      if (MIXED && a.sx.rows != nullptr) e0 = row_power(a.sx.rows[c0]), e1 = row_power(a.sx.rows[c1]);
       const float x0 = power(e0), x1 = power(e1);
       if (!far) {
         sum[i][0] = fmaf(acc[i][0] * s0, x0, sum[i][0]), sum[i][1] = fmaf(acc[i][1] * s0, x1, sum[i][1]);
@@ -856,8 +858,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
   float v = 0.f;
 #pragma unroll
   for (int k = 0; k < kFewWarps; ++k) v += part[k][r][m];
-  v = v * row_rest(rx) * row_rest(rw);
-  if (a.sx.rows != nullptr && a.sw.rows != nullptr) v = by_rows(v, rx, rw);
+  if (MIXED) v = v * row_rest(rx) * row_rest(rw);
+  else if (a.sx.rows != nullptr) v = by_rows(v * row_rest(rx) * row_rest(rw), rx, rw);
   if (a.bias != nullptr) v += to_f32(static_cast<const TB *>(a.bias)[n0 + r]);
   static_cast<T *>(a.y)[m * a.y_row + n0 + r] = from_f32<T>(v);
 }
@@ -869,16 +871,17 @@ bool is_few(int64_t M, int64_t N, int64_t K) {
   return M <= kFewMost && few_bytes(M, K) <= 72 * 1024 && N * K <= int64_t(1) << (M <= 8 ? 24 : 22);
 }
 
-template <typename T, typename TB, int TILES>
+template <typename T, typename TB, int TILES, bool MIXED>
 cudaError_t launch_few_as(const FewArgs &a, cudaStream_t s) {
-  auto *kernel = k_few_rows<T, TB, TILES>;
+  auto *kernel = k_few_rows<T, TB, TILES, MIXED>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);
   if (e != cudaSuccess) return e;
   return tc::launch(kernel, (unsigned)((a.N + 15) / 16), 32 * kFewWarps, (size_t)few_bytes(a.M, a.K), 1, s, a);
 }
 template <typename T, typename TB>
 cudaError_t launch_few(const FewArgs &a, cudaStream_t s) {
-  return a.M <= 8 ? launch_few_as<T, TB, 1>(a, s) : launch_few_as<T, TB, 2>(a, s);
+  if (a.mixed) return a.M <= 8 ? launch_few_as<T, TB, 1, true>(a, s) : launch_few_as<T, TB, 2, true>(a, s);
+  return a.M <= 8 ? launch_few_as<T, TB, 1, false>(a, s) : launch_few_as<T, TB, 2, false>(a, s);
 }
 
 // What an operand lacks, or null; fills its scales.
@@ -1019,8 +1022,7 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (is_few(M, N, K)) {
-    const FewArgs f = {x->codes, weight->codes, x->row, weight->row, a.sa, a.sb, a.sb.rows == nullptr ? a.sa.rows : nullptr,
-                       a.sa.rows == nullptr ? a.sb.rows : nullptr, bias, y, y_row,
+    const FewArgs f = {x->codes, weight->codes, x->row, weight->row, a.sa, a.sb, (a.sa.rows == nullptr) != (a.sb.rows == nullptr), bias, y, y_row,
                        (int)M, (int)N, (int)K, a.steps};
     if (dtype == CPAB_F32) e = launch_few<float, float>(f, s);
     else if (dtype == CPAB_F16) e = bias_dtype == CPAB_F32 ? launch_few<__half, float>(f, s) : launch_few<__half, __half>(f, s);
