@@ -43,8 +43,8 @@ def matmul_quantized(q, scale, weight, weight_scale, bias=None, dtype=torch.bflo
     (of rms_norm_quantized); bias [N] is float32 or of dtype.  Codes whose rows
     do not begin on multiples of 16 bytes are copied.  No gradient (scales,
     codes or a bias that want one are refused)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
-                                       (q, scale, weight, weight_scale, bias)):
+    if torch.is_grad_enabled() and (scale.requires_grad or weight_scale.requires_grad or q.requires_grad or
+                                    weight.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("matmul_quantized has no gradient; call it under torch.no_grad(), or use "
                            "linear_quantized")
     ext = _ext.module()
