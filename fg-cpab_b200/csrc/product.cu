@@ -700,7 +700,6 @@ struct FewArgs {
   const uint8_t *x, *w;
   int64_t x_row, w_row;
   Scales sx, sw;
-  int mixed;
   const void *bias;
   void *y;
   int64_t y_row;
@@ -737,11 +736,11 @@ __device__ __forceinline__ float by_rows(float v, float a, float b) {
   return v * __uint_as_float((uint32_t)(p + 127) << 23) * __uint_as_float((uint32_t)(e - p + 127) << 23);
 }
 
-// MIXED: one operand has rows' scales and the other blocks'; a row's power of two is then
-// that of each of its blocks (kernels of their own: a row by 4096 x 2048 of other scales
-// 5.3 us with that choice in the loop, without 4.9 to 5.1).  Where both have rows' the
-// sums are of codes alone.
-template <typename T, typename TB, int TILES, bool MIXED>
+// KIND: both operands have scales of blocks; both of rows, whose sums are of codes alone;
+// or one of each, where a row's power of two is that of each of its blocks.  (A row by
+// 4096 x 2048, weights out of L2: 5.0, 4.4 and 5.3 us; with all of it in one kernel 5.3.)
+enum FewScales { kBlocks, kRows, kMixed };
+template <typename T, typename TB, int TILES, FewScales KIND>
 __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_constant__ FewArgs a) {
   extern __shared__ __align__(16) uint8_t few_smem[];  // x as halves, [M, pitch]
   __shared__ float part[kFewWarps][16][8 * TILES + 1];
@@ -759,8 +758,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
   float sum[TILES][4] = {};
   struct Block {
     uint4 p[2], q[2];
-    uint32_t s0, s1;
+    uint32_t s0, s1, e0, e1;  // (e0, e1: x's of the first eight rows)
   };
+  const int c0 = min(2 * t, a.M - 1), c1 = min(2 * t + 1, a.M - 1);
+  const uint8_t *x0 = a.sx.bytes + c0 * a.sx.row, *x1 = a.sx.bytes + c1 * a.sx.row;
   auto fetch = [&](int b, Block &f) {
     if (b * 128 + 128 <= a.K) {
 #pragma unroll
@@ -775,15 +776,14 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
         f.p[h] = sixteen(w0, k, a.K), f.q[h] = sixteen(w1, k, a.K);
       }
     }
-    f.s0 = f.s1 = 127u;
-    if (a.sw.bytes != nullptr && b < a.blocks)
-      f.s0 = a.sw.bytes[r0 * a.sw.row + b], f.s1 = a.sw.bytes[r1 * a.sw.row + b];
+    if constexpr (KIND != kRows) {
+      f.s0 = f.s1 = f.e0 = f.e1 = 127u;
+      if ((KIND == kBlocks || a.sw.bytes != nullptr) && b < a.blocks)
+        f.s0 = a.sw.bytes[r0 * a.sw.row + b], f.s1 = a.sw.bytes[r1 * a.sw.row + b];
+      if ((KIND == kBlocks || a.sx.bytes != nullptr) && b < a.blocks) f.e0 = x0[b], f.e1 = x1[b];
+    }
   };
   auto multiply = [&](int b, const Block &f) {
-    uint32_t u0 = f.s0, u1 = f.s1;
-    if (MIXED && a.sw.rows != nullptr) u0 = row_power(a.sw.rows[r0]), u1 = row_power(a.sw.rows[r1]);
-    const bool far = is_far(u0) || is_far(u1);
-    const float s0 = power(u0), s1 = power(u1);
     float acc[TILES][4] = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -806,19 +806,31 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
         }
       }
     }
+    if constexpr (KIND == kRows) {
 #pragma unroll
-    for (int i = 0; i < TILES; ++i) {
-      const int c0 = min(8 * i + 2 * t, a.M - 1), c1 = min(8 * i + 2 * t + 1, a.M - 1);
-      uint32_t e0 = 127u, e1 = 127u;
-      if (a.sx.bytes != nullptr) e0 = a.sx.bytes[c0 * a.sx.row + b], e1 = a.sx.bytes[c1 * a.sx.row + b];
-      if (MIXED && a.sx.rows != nullptr) e0 = row_power(a.sx.rows[c0]), e1 = row_power(a.sx.rows[c1]);
-      const float x0 = power(e0), x1 = power(e1);
-      if (!far) {
-        sum[i][0] = fmaf(acc[i][0] * s0, x0, sum[i][0]), sum[i][1] = fmaf(acc[i][1] * s0, x1, sum[i][1]);
-        sum[i][2] = fmaf(acc[i][2] * s1, x0, sum[i][2]), sum[i][3] = fmaf(acc[i][3] * s1, x1, sum[i][3]);
-      } else {
-        sum[i][0] += by_powers(acc[i][0], s0, x0), sum[i][1] += by_powers(acc[i][1], s0, x1);
-        sum[i][2] += by_powers(acc[i][2], s1, x0), sum[i][3] += by_powers(acc[i][3], s1, x1);
+      for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[i][j] += acc[i][j];
+    } else {
+      uint32_t u0 = f.s0, u1 = f.s1;
+      if (KIND == kMixed && a.sw.rows != nullptr) u0 = row_power(a.sw.rows[r0]), u1 = row_power(a.sw.rows[r1]);
+      const bool far = is_far(u0) || is_far(u1);
+      const float s0 = power(u0), s1 = power(u1);
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) {
+        const int c0 = min(8 * i + 2 * t, a.M - 1), c1 = min(8 * i + 2 * t + 1, a.M - 1);
+        uint32_t e0 = f.e0, e1 = f.e1;
+        if (i > 0 && (KIND == kBlocks || a.sx.bytes != nullptr))
+          e0 = a.sx.bytes[c0 * a.sx.row + b], e1 = a.sx.bytes[c1 * a.sx.row + b];
+        if (KIND == kMixed && a.sx.rows != nullptr) e0 = row_power(a.sx.rows[c0]), e1 = row_power(a.sx.rows[c1]);
+        const float y0 = power(e0), y1 = power(e1);
+        if (!far) {
+          sum[i][0] = fmaf(acc[i][0] * s0, y0, sum[i][0]), sum[i][1] = fmaf(acc[i][1] * s0, y1, sum[i][1]);
+          sum[i][2] = fmaf(acc[i][2] * s1, y0, sum[i][2]), sum[i][3] = fmaf(acc[i][3] * s1, y1, sum[i][3]);
+        } else {
+          sum[i][0] += by_powers(acc[i][0], s0, y0), sum[i][1] += by_powers(acc[i][1], s0, y1);
+          sum[i][2] += by_powers(acc[i][2], s1, y0), sum[i][3] += by_powers(acc[i][3], s1, y1);
+        }
       }
     }
   };
@@ -851,15 +863,16 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(const __grid_consta
     part[warp][g + 8][8 * i + 2 * t] = sum[i][2], part[warp][g + 8][8 * i + 2 * t + 1] = sum[i][3];
   }
   const int r = threadIdx.x & 15, m = threadIdx.x >> 4;
-  const float rx = a.sx.rows != nullptr ? a.sx.rows[min(m, a.M - 1)] : 1.f;
-  const float rw = a.sw.rows != nullptr ? a.sw.rows[min(n0 + r, a.N - 1)] : 1.f;
+  float rx = 1.f, rw = 1.f;
+  if (KIND == kRows || (KIND == kMixed && a.sx.rows != nullptr)) rx = a.sx.rows[min(m, a.M - 1)];
+  if (KIND == kRows || (KIND == kMixed && a.sw.rows != nullptr)) rw = a.sw.rows[min(n0 + r, a.N - 1)];
   __syncthreads();
   if (m >= 8 * TILES || m >= a.M || n0 + r >= a.N) return;
   float v = 0.f;
 #pragma unroll
   for (int k = 0; k < kFewWarps; ++k) v += part[k][r][m];
-  if (MIXED) v = v * row_rest(rx) * row_rest(rw);
-  else if (a.sx.rows != nullptr) v = by_rows(v * row_rest(rx) * row_rest(rw), rx, rw);
+  if constexpr (KIND != kBlocks) v = v * row_rest(rx) * row_rest(rw);
+  if constexpr (KIND == kRows) v = by_rows(v, rx, rw);
   if (a.bias != nullptr) v += to_f32(static_cast<const TB *>(a.bias)[n0 + r]);
   static_cast<T *>(a.y)[m * a.y_row + n0 + r] = from_f32<T>(v);
 }
@@ -871,17 +884,21 @@ bool is_few(int64_t M, int64_t N, int64_t K) {
   return M <= kFewMost && few_bytes(M, K) <= 72 * 1024 && N * K <= int64_t(1) << (M <= 8 ? 24 : 22);
 }
 
-template <typename T, typename TB, int TILES, bool MIXED>
+template <typename T, typename TB, int TILES, FewScales KIND>
 cudaError_t launch_few_as(const FewArgs &a, cudaStream_t s) {
-  auto *kernel = k_few_rows<T, TB, TILES, MIXED>;
+  auto *kernel = k_few_rows<T, TB, TILES, KIND>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);
   if (e != cudaSuccess) return e;
   return tc::launch(kernel, (unsigned)((a.N + 15) / 16), 32 * kFewWarps, (size_t)few_bytes(a.M, a.K), 1, s, a);
 }
 template <typename T, typename TB>
 cudaError_t launch_few(const FewArgs &a, cudaStream_t s) {
-  if (a.mixed) return a.M <= 8 ? launch_few_as<T, TB, 1, true>(a, s) : launch_few_as<T, TB, 2, true>(a, s);
-  return a.M <= 8 ? launch_few_as<T, TB, 1, false>(a, s) : launch_few_as<T, TB, 2, false>(a, s);
+  const bool one = a.M <= 8;
+  if (a.sx.rows == nullptr && a.sw.rows == nullptr)
+    return one ? launch_few_as<T, TB, 1, kBlocks>(a, s) : launch_few_as<T, TB, 2, kBlocks>(a, s);
+  if (a.sx.rows != nullptr && a.sw.rows != nullptr)
+    return one ? launch_few_as<T, TB, 1, kRows>(a, s) : launch_few_as<T, TB, 2, kRows>(a, s);
+  return one ? launch_few_as<T, TB, 1, kMixed>(a, s) : launch_few_as<T, TB, 2, kMixed>(a, s);
 }
 
 // What an operand lacks, or null; fills its scales.
@@ -1022,7 +1039,7 @@ extern "C" int cpab_b200_matmul_quantized(int dtype, const cpab_quantized *x, co
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (is_few(M, N, K)) {
-    const FewArgs f = {x->codes, weight->codes, x->row, weight->row, a.sa, a.sb, (a.sa.rows == nullptr) != (a.sb.rows == nullptr), bias, y, y_row,
+    const FewArgs f = {x->codes, weight->codes, x->row, weight->row, a.sa, a.sb, bias, y, y_row,
                        (int)M, (int)N, (int)K, a.steps};
     if (dtype == CPAB_F32) e = launch_few<float, float>(f, s);
     else if (dtype == CPAB_F16) e = bias_dtype == CPAB_F32 ? launch_few<__half, float>(f, s) : launch_few<__half, __half>(f, s);
