@@ -34,7 +34,10 @@ class RecurrentBlock(nn.Module):
 class SeriesLocalizer(nn.Module):
     """SeriesLocalizer(channels, theta_dim, width, depth)(series, lengths) ->
     theta; theta starts at 0 (the identity warp).  projection_bits=8: the blocks'
-    projections and their gradients are 8-bit products (linear_quantized)."""
+    projections and their gradients are 8-bit products (linear_quantized).  A training
+    step on 32 series of 512 samples, 16 and 8 bits (us): width 128 in bfloat16 987 and
+    899, 2048 2442 and 2105; in float32, whose library products take no tensor cores
+    unless told to, 1001 and 889, 42004 and 2753."""
 
     def __init__(self, channels, theta_dim, width=128, depth=2, eps=1e-6, projection_bits=16):
         super().__init__()
